@@ -15,6 +15,11 @@
  *   ws_lse_merge                      combine the GPU partial with the host
  *                                     partial (any of the reference's partial
  *                                     formats) and normalise
+ *   ws_pages_extend / ws_pages_release   page tables and slots from the lengths
+ *   ws_rope / ws_rope_append          rotary positions, with the write of k and v
+ *                                     into the pages (bf16 or 8-bit)
+ *   ws_gqa8_decode_partial            decode attention over 8-bit pages
+ *   ws_gqa_prompt                     prompt attention over the pages
  *
  * Conventions
  *   - bf16 tensors are passed as uint16_t bit patterns; fp32 as float.
@@ -474,6 +479,134 @@ int ws_gqa_append_decode_partial_noalloc(const uint16_t* q, const uint16_t* k_ne
                                          int page_size, int max_pages, int num_pages,
                                          int max_len, int n_splits, float scale,
                                          float* out, float* lse, void* stream);
+
+/*
+ * Pages and slots of a ragged batch from its lengths, on the GPU.
+ *
+ * The free pages are a stack: stack[0 .. free_in[0]) of stack_size entries, the
+ * top first to go.  Sequence b holds len_in[b] tokens in the first
+ * ceil(len_in[b] / page_size) pages of its row of page_table [B][max_pages] and
+ * brings n_new[b] more (0 allowed).  With need_b = ceil((len + n) / page_size) -
+ * ceil(len / page_size) and pre_b = need_0 + ... + need_b, the sequence succeeds iff
+ * 0 <= len, 0 <= n, len + n <= page_size * max_pages, its tokens end within the
+ * n_tokens of the call, and need_b = 0 or pre_b <= free_in[0].  Its j-th new page
+ * is stack[free_in[0] - 1 - (pre_b - need_b + j)], written into its row.  The order
+ * is the sequences', so the result depends on the inputs alone.
+ *   len_out   [B]      len_in + n_new, or -1 where the sequence did not succeed
+ *   cu_new    [B + 1]  sequence b's tokens are cu_new[b] .. cu_new[b + 1] of the
+ *                      packed batch (a failed sequence keeps its places)
+ *   positions [n_tokens]  len_in[b] + i (+ pos_base[b]: tokens of the sequence that
+ *                      are not in this partition; NULL for none)
+ *   slots     [n_tokens]  page * page_size + offset of the token's place in the pools
+ *   free_out  [1]      free pages left: free_in less the last success's pre_b
+ * Tokens of a failed sequence, or past the last one, get position 0 and slot -1 (no
+ * place), and so does a token whose page id lies outside [0, num_pages).  len_out
+ * and free_out must not alias len_in, n_new and free_in.
+ * The reference has no counterpart: its caches are dense per-sequence buffers
+ * (system/deepseek.py:144-209, system/mixoffload.py:51-144).
+ */
+int ws_pages_extend(int32_t* page_table, const int32_t* len_in, const int32_t* n_new,
+                    const int32_t* stack, const int32_t* free_in, const int32_t* pos_base,
+                    int32_t* len_out, int32_t* cu_new, int32_t* positions, int32_t* slots,
+                    int32_t* free_out, int B, int max_pages, int num_pages, int stack_size,
+                    int page_size, int n_tokens, void* stream);
+
+/*
+ * Pages of ended sequences (done[b] != 0) back on the stack, in the order of the
+ * sequences, each row's pages in order; len_out[b] = 0 for them and len_in[b] for the
+ * others; free_out = free_in + the pages given back (at most stack_size: what does
+ * not fit is dropped).  The rows keep their entries, which a length of 0 never reads.
+ */
+int ws_pages_release(const int32_t* page_table, const int32_t* len_in, const uint8_t* done,
+                     int32_t* stack, const int32_t* free_in, int32_t* len_out,
+                     int32_t* free_out, int B, int max_pages, int stack_size, int page_size,
+                     void* stream);
+
+/*
+ * Rotary positions of q [N][Hq][D] and k [N][Hkv][D] (bf16; token strides in
+ * elements, multiples of 8: views of a fused projection's rows).  Pair i of the
+ * rot / 2 pairs turns by positions[pair_axis[i]][token] * inv_freq[i]:
+ *   (x, y) -> factor * (x cos - y sin, y cos + x sin)
+ * of columns (i, i + rot / 2), or (2 i, 2 i + 1) with adjacent != 0; columns >= rot
+ * pass.  positions [axes][N] int32, up to 4 axes; pair_axis (host memory) rot / 2
+ * values < axes, or NULL for axis 0.  D and rot: multiples of 16, rot <= D <= 256.
+ * q_out / k_out contiguous; they may be q / k themselves where those are contiguous.
+ * The reference has no counterpart: its keys come rotated from the model library,
+ * before the cache append.
+ */
+int ws_rope(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
+            const int32_t* positions, int axes, const float* inv_freq,
+            const uint8_t* pair_axis, int adjacent, float factor, uint16_t* q_out,
+            uint16_t* k_out, int N, int Hq, int Hkv, int D, int rot, void* stream);
+
+/*
+ * ws_rope of q into q_out and of k into the pages, with v beside it: token t goes to
+ * slot slots[t] = page * page_size + offset of the pools [num_pages][Hkv][page_size][D]
+ * (ws_pages_extend); a slot outside [0, num_pages * page_size) writes nothing.  Slots
+ * must differ.  k_scale == NULL: bf16 pools.  Otherwise 8-bit pools: e4m3 values, and
+ * for each token and KV head one e8m0 byte (k_scale, v_scale [num_pages][Hkv][page_size])
+ * for 2^(byte - 127), the least power of two with max|x| <= 448 times it, not below
+ * 2^-126 (byte 127 for a row of zeros); the rotated key is rounded once.  A row with
+ * an infinity or a NaN becomes NaN whole (byte 255).
+ */
+int ws_rope_append(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
+                   const uint16_t* v, int64_t v_stride, const int32_t* positions, int axes,
+                   const float* inv_freq, const uint8_t* pair_axis, int adjacent, float factor,
+                   const int32_t* slots, uint16_t* q_out, void* k_pages, void* v_pages,
+                   uint8_t* k_scale, uint8_t* v_scale, int N, int Hq, int Hkv, int D, int rot,
+                   int page_size, int num_pages, void* stream);
+
+/*
+ * ws_gqa_decode_partial over 8-bit pools (ws_rope_append's): k_pages, v_pages
+ * [num_pages][Hkv][page_size][D] e4m3, k_scale, v_scale [num_pages][Hkv][page_size] e8m0.
+ * D: a multiple of 32 up to 256; page_size a multiple of 32; group size 1 to 16.
+ * Bad page ids and lengths, empty sequences and the limits are the bf16 call's.
+ * Pieces of rows that several splits share are fp32 (workspace from
+ * ws_gqa8_decode_plan).  ws_gqa8_decode_full also writes the output in bf16.
+ */
+int ws_gqa8_decode_plan(int rows_kv, int heads, int D, int max_len, int n_splits,
+                        int* n_splits_out, size_t* workspace_bytes_out);
+int ws_gqa8_decode_partial(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pages,
+                           const uint8_t* k_scale, const uint8_t* v_scale,
+                           const int32_t* page_table, const int32_t* gpu_len, int B, int Hq,
+                           int Hkv, int D, int page_size, int max_pages, int num_pages,
+                           int max_len, int n_splits, float scale, float* out, float* lse,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int ws_gqa8_decode_full(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pages,
+                        const uint8_t* k_scale, const uint8_t* v_scale,
+                        const int32_t* page_table, const int32_t* gpu_len, int B, int Hq,
+                        int Hkv, int D, int page_size, int max_pages, int num_pages,
+                        int max_len, int n_splits, float scale, uint16_t* out_bf16, float* out,
+                        float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Prompt attention: the new tokens of every sequence over the pages, causal.
+ * q [N][Hq][D] bf16, packed: sequence b's n = cu_new[b + 1] - cu_new[b] queries are
+ * rows cu_new[b] .. (non-decreasing, within [0, N]); query i stands at position
+ * kv_len[b] - n + i of the kv_len[b] tokens in the pages (the new ones among them) and
+ * sees positions 0 .. its own, so one at a negative position (its tokens are not in
+ * this partition) sees nothing: out 0, lse -inf.  Pools as ws_gqa_decode_partial's
+ * (k_scale == NULL) or ws_gqa8_decode_partial's; D a multiple of 32 up to 256,
+ * page_size a multiple of 32, any group size Hq / Hkv.
+ * Outputs: any of out_bf16 / out_f32 [N][Hq][D] (not both NULL) and lse [N][Hq] (may be
+ * NULL), mergeable with a host partial (ws_lse_merge).  Rows outside [cu_new[0],
+ * cu_new[B]) are not written.  A row that sees a token in a page with an id outside the
+ * pool is NaN, and so is every row of a sequence whose length is outside [0, capacity].
+ * An infinity or a NaN in a token changes only the rows that see it.
+ * max_len bounds kv_len (it sizes the splits); n_splits: workgroups that share a tile's
+ * tokens (0: the library's choice, up to 64), with the workspace of ws_gqa_prompt_plan
+ * (none for one split).
+ * The reference runs prompts through its framework's attention (chunks:
+ * system/deepseek.py:279-322) on dense buffers.
+ */
+int ws_gqa_prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len, int n_splits,
+                       int* n_splits_out, size_t* workspace_bytes_out);
+int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void* v_pages,
+                  const uint8_t* k_scale, const uint8_t* v_scale, const int32_t* page_table,
+                  const int32_t* kv_len, const int32_t* cu_new, int N, int B, int Hq, int Hkv,
+                  int D, int page_size, int max_pages, int num_pages, int max_len,
+                  int n_splits, float scale, uint16_t* out_bf16, float* out_f32, float* lse,
+                  void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -293,14 +293,23 @@ merge_split_kernel(const MergeSplitParams p) {
   }
 }
 
-// Launches merge_split_kernel<FMT> over rows plan rows.  (fp32 pieces come with
-// at least 1024 output rows of 512 columns, mla_layout: 2048 column groups, so
-// one wave each.)
+// Launches merge_split_kernel<FMT> over rows plan rows.  (With a host partial fp32
+// pieces come with at least 1024 output rows of 512 columns, mla_layout: 2048
+// column groups, so one wave each; without one also from the 8-bit GQA kernel, of
+// any row count.)
 template <int FMT>
 static void launch_merge(const MergeSplitParams& p, long long rows, hipStream_t s) {
   const int groups = merge_groups(p.heads, p.Dv / 4);
   const int PS = merge_streams(p.grid, rows, groups);
-  if (PS == kMergeMaxStreams) {
+  if (FMT < 0 && p.f32_pieces && PS > 1) {
+    if constexpr (FMT < 0) {
+      const dim3 grid((unsigned)rows, groups), block(64 * PS);
+      if (PS == kMergeMaxStreams)
+        hipLaunchKernelGGL((merge_split_kernel<FMT, kMergeMaxStreams, float4>), grid, block, 0, s, p);
+      else
+        hipLaunchKernelGGL((merge_split_kernel<FMT, 4, float4>), grid, block, 0, s, p);
+    }
+  } else if (PS == kMergeMaxStreams) {
     hipLaunchKernelGGL((merge_split_kernel<FMT, kMergeMaxStreams, uint2>),
                        dim3((unsigned)rows, groups), dim3(64 * kMergeMaxStreams), 0, s, p);
   } else if (PS == 4) {

@@ -10,11 +10,16 @@ Tensor conventions (all CUDA/HIP tensors, contiguous):
   MLA pool    latent_pages      [num_pages, page_size, 576]    bfloat16
   page_table  [B, max_pages] int32, gpu_len [B] int32
   partials    (out fp32 normalised, lse fp32 natural log); empty = (0, -inf)
+  8-bit pools k_pages, v_pages  [num_pages, Hkv, page_size, D] float8_e4m3fn with
+              k_scale, v_scale  [num_pages, Hkv, page_size]    float8_e8m0fnu
+              (one power of two per token and KV head)
 """
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -48,6 +53,15 @@ EXPORTS = (
     "ws_copy_pages",
     "ws_noalloc_scratch_bytes",
     "ws_gqa_append_decode_partial_noalloc",
+    "ws_pages_extend",
+    "ws_pages_release",
+    "ws_rope",
+    "ws_rope_append",
+    "ws_gqa8_decode_plan",
+    "ws_gqa8_decode_partial",
+    "ws_gqa8_decode_full",
+    "ws_gqa_prompt_plan",
+    "ws_gqa_prompt",
 )
 
 # Formats of the second operand of lse_merge (include/wsgpu.h).
@@ -148,6 +162,26 @@ def lib() -> ctypes.CDLL:
         L.ws_lse_merge.restype = i32
         L.ws_lse_merge.argtypes = [vp, vp, vp, vp, vp, i32, vp, vp, vp, i32,
                                    i32, vp]
+        L.ws_pages_extend.restype = i32
+        L.ws_pages_extend.argtypes = [vp] * 11 + [i32] * 6 + [vp]
+        L.ws_pages_release.restype = i32
+        L.ws_pages_release.argtypes = [vp] * 7 + [i32] * 4 + [vp]
+        L.ws_rope.restype = i32
+        L.ws_rope.argtypes = [vp, i64, vp, i64, vp, i32, vp, ctypes.c_char_p, i32, f32, vp, vp] + \
+            [i32] * 5 + [vp]
+        L.ws_rope_append.restype = i32
+        L.ws_rope_append.argtypes = [vp, i64, vp, i64, vp, i64, vp, i32, vp, ctypes.c_char_p, i32,
+                                     f32, vp, vp, vp, vp, vp, vp] + [i32] * 7 + [vp]
+        L.ws_gqa8_decode_plan.restype = i32
+        L.ws_gqa8_decode_plan.argtypes = [i32] * 5 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
+        L.ws_gqa8_decode_partial.restype = i32
+        L.ws_gqa8_decode_partial.argtypes = [vp] * 7 + [i32] * 9 + [f32, vp, vp, vp, sz, vp]
+        L.ws_gqa8_decode_full.restype = i32
+        L.ws_gqa8_decode_full.argtypes = [vp] * 7 + [i32] * 9 + [f32, vp, vp, vp, vp, sz, vp]
+        L.ws_gqa_prompt_plan.restype = i32
+        L.ws_gqa_prompt_plan.argtypes = [i32] * 7 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
+        L.ws_gqa_prompt.restype = i32
+        L.ws_gqa_prompt.argtypes = [vp] * 8 + [i32] * 10 + [f32, vp, vp, vp, vp, sz, vp]
         _lib = L
     return _lib
 
@@ -969,3 +1003,353 @@ def lse_merge(out_g, lse_g, b, fmt=PARTIAL_LSE_F32, out_dtype=torch.bfloat16,
                               _ptr(lse_out if want_lse else None), rows, Dv,
                               _stream(dev)), "ws_lse_merge")
     return out, (lse_out if want_lse else None)
+
+
+# ---------------------------------------------------------------------------
+# a request's path into the pages: pages and slots, rotary positions with the
+# write, decode over 8-bit pages, prompt attention
+
+E4M3 = torch.float8_e4m3fn
+E8M0 = torch.float8_e8m0fnu
+
+
+def _run(name: str, dev: torch.device, *args) -> None:
+    """The entry point `name` on the current stream of `dev`, with `dev` the
+    current device for the launch (the operands may live on another one than
+    the caller's current)."""
+    fn = getattr(lib(), name)
+    if torch._C._cuda_getDevice() == dev.index:
+        _check(fn(*args, _stream(dev)), name)
+    else:
+        with torch.cuda.device(dev):
+            _check(fn(*args, _stream(dev)), name)
+
+
+def _gpu(t, name: str) -> torch.device:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a GPU (got {t.device})")
+    return t.device
+
+
+class PageStep(NamedTuple):
+    """What pages_extend hands out (all int32 on the GPU)."""
+
+    len_out: torch.Tensor    # [B] lengths with the new tokens; -1 where they got no place
+    cu_new: torch.Tensor     # [B + 1] each sequence's first token of the packed batch
+    positions: torch.Tensor  # [n_tokens]
+    slots: torch.Tensor      # [n_tokens] page * page_size + offset, or -1
+    free_out: torch.Tensor   # [1] free pages left on the stack
+
+
+def pages_extend(page_table, len_in, n_new, stack, free_in, page_size, num_pages, n_tokens,
+                 pos_base=None) -> PageStep:
+    """Pages and slots for n_new[b] more tokens of every sequence, from the
+    stack of free pages stack[:free_in] (ws_pages_extend): new page ids go into
+    page_table in place, everything else into new tensors, so a call that is
+    not wanted is undone by keeping len_in and free_in.  n_tokens: the packed
+    batch's tokens, sum(n_new) or more (the rest is padding: slot -1).
+    pos_base [B]: what a position counts beside the partition's tokens."""
+    dev = _gpu(page_table, "page_table")
+    _require(page_table, "page_table", torch.int32, dev, 2)
+    _require(len_in, "len_in", torch.int32, dev, 1)
+    _require(n_new, "n_new", torch.int32, dev, 1)
+    _require(stack, "stack", torch.int32, dev, 1)
+    _require(free_in, "free_in", torch.int32, dev, 1)
+    B, max_pages = page_table.shape
+    N = int(n_tokens)
+    if len_in.shape[0] != B or n_new.shape[0] != B or free_in.shape[0] != 1:
+        raise ValueError("len_in and n_new must be [B] and free_in [1]")
+    if pos_base is not None:
+        _require(pos_base, "pos_base", torch.int32, dev, 1)
+        if pos_base.shape[0] != B:
+            raise ValueError("pos_base must be [B]")
+    if N < 0:
+        raise ValueError(f"n_tokens {N} < 0")
+    step = PageStep(*torch.empty(2 * B + 2 + 2 * N, dtype=torch.int32, device=dev).split_with_sizes(
+        (B, B + 1, N, N, 1)))
+    _run("ws_pages_extend", dev, _ptr(page_table), _ptr(len_in), _ptr(n_new), _ptr(stack),
+         _ptr(free_in), _ptr(pos_base), step.len_out.data_ptr(), step.cu_new.data_ptr(),
+         step.positions.data_ptr(), step.slots.data_ptr(), step.free_out.data_ptr(), B, max_pages,
+         int(num_pages), stack.shape[0], int(page_size), N)
+    return step
+
+
+def pages_release(page_table, len_in, done, stack, free_in, page_size):
+    """The pages of the sequences with done[b] (bool [B]) back on the stack, in
+    place (ws_pages_release).  Returns (lengths: 0 for those, free pages)."""
+    dev = _gpu(page_table, "page_table")
+    _require(page_table, "page_table", torch.int32, dev, 2)
+    _require(len_in, "len_in", torch.int32, dev, 1)
+    _require(done, "done", torch.bool, dev, 1)
+    _require(stack, "stack", torch.int32, dev, 1)
+    _require(free_in, "free_in", torch.int32, dev, 1)
+    B, max_pages = page_table.shape
+    if len_in.shape[0] != B or done.shape[0] != B or free_in.shape[0] != 1:
+        raise ValueError("len_in and done must be [B] and free_in [1]")
+    len_out, free_out = torch.empty(B + 1, dtype=torch.int32, device=dev).split_with_sizes((B, 1))
+    _run("ws_pages_release", dev, _ptr(page_table), _ptr(len_in), _ptr(done), _ptr(stack),
+         _ptr(free_in), len_out.data_ptr(), free_out.data_ptr(), B, max_pages, stack.shape[0],
+         int(page_size))
+    return len_out, free_out
+
+
+@functools.lru_cache(maxsize=256)
+def _axis_bytes(pair_axis: tuple) -> bytes:
+    if any(a != int(a) or not 0 <= a < 4 for a in pair_axis):
+        raise ValueError("pair_axis must hold axis numbers from 0 to 3")
+    return bytes(int(a) for a in pair_axis)
+
+
+def rope_sections(sections, interleaved=False) -> list:
+    """pair_axis of sections[a] pairs on axis a: one axis after the other, or
+    interleaved (0 1 2 0 1 2 ..., an axis dropping out once its pairs are used)."""
+    if not interleaved:
+        return [a for a, n in enumerate(sections) for _ in range(n)]
+    left, out = list(sections), []
+    while any(left):
+        for a in range(len(left)):
+            if left[a] > 0:
+                left[a] -= 1
+                out.append(a)
+    return out
+
+
+def _rope_rows(t, name, dev, N=None, D=None):
+    """(heads, token stride) of a [N, heads, D] bf16 operand whose tokens may be
+    strided (a slice of a fused projection's rows)."""
+    _require(t, name, torch.bfloat16, dev, 3, contiguous=False)
+    n, heads, d = t.shape
+    if (N is not None and n != N) or (D is not None and d != D):
+        raise ValueError(f"{name} must be [{N}, heads, {D}] (got {tuple(t.shape)})")
+    if heads == 0 or (n > 0 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != d))):
+        raise ValueError(f"{name} must have contiguous [heads, D] rows (strides {t.stride()})")
+    return heads, (t.stride(0) if n > 1 else heads * d)
+
+
+def _rope_args(q, k, positions, inv_freq, pair_axis, dev):
+    Hq, q_stride = _rope_rows(q, "q", dev)
+    N, _, D = q.shape
+    Hkv, k_stride = _rope_rows(k, "k", dev, N, D)
+    _require(positions, "positions", torch.int32, dev)
+    _require(inv_freq, "inv_freq", torch.float32, dev, 1)
+    if positions.dim() not in (1, 2) or positions.shape[-1] != N:
+        raise ValueError(f"positions must be [N] or [axes, N], N = {N} (got {tuple(positions.shape)})")
+    axes = positions.shape[0] if positions.dim() == 2 else 1
+    half = inv_freq.shape[0]
+    axis = None
+    if pair_axis is not None:
+        axis = _axis_bytes(tuple(pair_axis))
+        if len(axis) != half:
+            raise ValueError(f"pair_axis has {len(axis)} pairs, inv_freq {half}")
+    return N, Hq, Hkv, D, q_stride, k_stride, axes, axis, 2 * half
+
+
+def rope(q, k, positions, inv_freq, pair_axis=None, adjacent=False, factor=1.0, q_out=None,
+         k_out=None):
+    """Rotary positions of q [N, Hq, D] and k [N, Hkv, D] (ws_rope; tokens may be
+    strided).  positions [N] or [axes, N] int32; inv_freq [rot / 2] fp32, the
+    radians a position turns each pair; pair_axis: the axis of each pair
+    (rope_sections; None: axis 0); adjacent: pairs (2 i, 2 i + 1) instead of
+    (i, i + rot / 2); factor scales the rotated columns.  Returns contiguous
+    (q_out, k_out)."""
+    dev = _gpu(q, "q")
+    N, Hq, Hkv, D, qs, ks, axes, axis, rot = _rope_args(q, k, positions, inv_freq, pair_axis, dev)
+    if q_out is None:
+        q_out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=dev)
+    if k_out is None:
+        k_out = torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=dev)
+    _require(q_out, "q_out", torch.bfloat16, dev, 3)
+    _require(k_out, "k_out", torch.bfloat16, dev, 3)
+    if q_out.shape != q.shape or k_out.shape != k.shape:
+        raise ValueError("q_out and k_out must have q's and k's shapes")
+    if N == 0:
+        return q_out, k_out
+    _run("ws_rope", dev, _ptr(q), qs, _ptr(k), ks, _ptr(positions), axes, _ptr(inv_freq), axis,
+         int(bool(adjacent)), float(factor), _ptr(q_out), _ptr(k_out), N, Hq, Hkv, D, rot)
+    return q_out, k_out
+
+
+def _pools(k_pages, v_pages, k_scale, v_scale, dev):
+    """(num_pages, Hkv, page_size, D) of bf16 pools, or of 8-bit ones with scales."""
+    dt = torch.bfloat16 if k_scale is None else E4M3
+    _require(k_pages, "k_pages", dt, dev, 4)
+    _require(v_pages, "v_pages", dt, dev, 4)
+    if k_pages.shape != v_pages.shape:
+        raise ValueError("k/v page pools differ in shape")
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("8-bit pools take both k_scale and v_scale")
+    if k_scale is not None:
+        _require(k_scale, "k_scale", E8M0, dev, 3)
+        _require(v_scale, "v_scale", E8M0, dev, 3)
+        if k_scale.shape != k_pages.shape[:3] or v_scale.shape != k_pages.shape[:3]:
+            raise ValueError("k_scale and v_scale must be [num_pages, Hkv, page_size]")
+    return k_pages.shape
+
+
+def rope_append(q, k, v, positions, inv_freq, slots, k_pages, v_pages, k_scale=None, v_scale=None,
+                pair_axis=None, adjacent=False, factor=1.0, q_out=None):
+    """rope() of q, and of k into the pages with v beside it (ws_rope_append):
+    token t's keys and values go to slot slots[t] (pages_extend) of the pools,
+    bf16, or e4m3 with k_scale and v_scale (one power of two per token and KV
+    head).  A slot outside the pools (-1) writes nothing; slots must differ.
+    Returns q_out [N, Hq, D]."""
+    dev = _gpu(q, "q")
+    N, Hq, Hkv, D, qs, ks, axes, axis, rot = _rope_args(q, k, positions, inv_freq, pair_axis, dev)
+    Hv, vs = _rope_rows(v, "v", dev, N, D)
+    _require(slots, "slots", torch.int32, dev, 1)
+    P, Hp, PS, Dp = _pools(k_pages, v_pages, k_scale, v_scale, dev)
+    if Hv != Hkv or Hp != Hkv or Dp != D or slots.shape[0] != N:
+        raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)}, slots {tuple(slots.shape)} and pools "
+                         f"{tuple(k_pages.shape)} do not match")
+    if q_out is None:
+        q_out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=dev)
+    _require(q_out, "q_out", torch.bfloat16, dev, 3)
+    if q_out.shape != q.shape:
+        raise ValueError("q_out must have q's shape")
+    if N == 0:
+        return q_out
+    _run("ws_rope_append", dev, _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(positions), axes,
+         _ptr(inv_freq), axis, int(bool(adjacent)), float(factor), _ptr(slots), _ptr(q_out),
+         _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), N, Hq, Hkv, D, rot, PS, P)
+    return q_out
+
+
+def gqa8_plan(rows_kv: int, heads: int, D: int, max_len: int, n_workgroups: int = 0):
+    """(n_splits, workspace_bytes) of a decode call over 8-bit pages."""
+    key = ("gqa8", rows_kv, heads, D, max_len, n_workgroups,
+           torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1)
+    hit = _plans.get(key)
+    if hit is not None:
+        return hit
+    n, wsb = ctypes.c_int(0), ctypes.c_size_t(0)
+    _check(lib().ws_gqa8_decode_plan(rows_kv, heads, D, max_len, n_workgroups, ctypes.byref(n),
+                                     ctypes.byref(wsb)), "ws_gqa8_decode_plan")
+    if len(_plans) > 4096:
+        _plans.clear()
+    _plans[key] = (n.value, wsb.value)
+    return n.value, wsb.value
+
+
+def _gqa8_decode(name, q, k_pages, v_pages, k_scale, v_scale, page_table, gpu_len, scale, max_len,
+                 n_workgroups, out_bf16, out, lse):
+    dev = _gpu(k_pages, "k_pages")
+    if k_scale is None or v_scale is None:
+        raise ValueError("8-bit pools take both k_scale and v_scale")
+    P, Hkv, PS, D = _pools(k_pages, v_pages, k_scale, v_scale, dev)
+    _require(q, "q", torch.bfloat16, dev, 3)
+    _require(page_table, "page_table", torch.int32, dev, 2)
+    _require(gpu_len, "gpu_len", torch.int32, dev, 1)
+    B, Hq, Dq = q.shape
+    if Dq != D or Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"q {tuple(q.shape)} does not match the pools {tuple(k_pages.shape)}")
+    if page_table.shape[0] != B or gpu_len.shape[0] != B:
+        raise ValueError("page_table/gpu_len batch mismatch")
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=torch.float32, device=dev)
+    if lse is None:
+        lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
+    _require(out, "out", torch.float32, dev, 3)
+    _require(lse, "lse", torch.float32, dev, 2)
+    if out.shape != q.shape or lse.shape != (B, Hq):
+        raise ValueError("out must be [B, Hq, D] and lse [B, Hq]")
+    if B == 0:
+        return out, lse
+    nwg, wsb = gqa8_plan(B * Hkv, Hq // Hkv, D, int(max_len), int(n_workgroups))
+    # the call's own: a buffer kept between calls would be shared by graphs that
+    # were captured one after the other and replay together
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    outs = (_ptr(out), _ptr(lse)) if out_bf16 is None else (_ptr(out_bf16), _ptr(out), _ptr(lse))
+    _run(name, dev, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
+         _ptr(page_table), _ptr(gpu_len), B, Hq, Hkv, D, PS, page_table.shape[1], P, int(max_len),
+         nwg, float(scale), *outs, _ptr(ws), wsb)
+    return out, lse
+
+
+def gqa8_decode_partial(q, k_pages, v_pages, k_scale, v_scale, page_table, gpu_len, scale, max_len,
+                        n_workgroups=0, out=None, lse=None):
+    """gqa_decode_partial over 8-bit pages (ws_gqa8_decode_partial): q [B, Hq, D]
+    bf16, pools [P, Hkv, PS, D] float8_e4m3fn with scales [P, Hkv, PS]
+    float8_e8m0fnu -> (out [B, Hq, D] fp32 normalised, lse [B, Hq] fp32).
+    max_len must bound every gpu_len[b]."""
+    return _gqa8_decode("ws_gqa8_decode_partial", q, k_pages, v_pages, k_scale, v_scale, page_table,
+                        gpu_len, scale, max_len, n_workgroups, None, out, lse)
+
+
+def gqa8_decode_full(q, k_pages, v_pages, k_scale, v_scale, page_table, gpu_len, scale, max_len,
+                     n_workgroups=0, out_bf16=None, lse=None):
+    """gqa8_decode_partial for a partition that holds every token: returns
+    (out [B, Hq, D] bf16, lse [B, Hq] fp32)."""
+    dev = _gpu(q, "q")
+    if out_bf16 is None:
+        out_bf16 = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    _require(out_bf16, "out_bf16", torch.bfloat16, dev, 3)
+    if out_bf16.shape != q.shape:
+        raise ValueError("out_bf16 must have q's shape")
+    _, lse = _gqa8_decode("ws_gqa8_decode_full", q, k_pages, v_pages, k_scale, v_scale, page_table,
+                          gpu_len, scale, max_len, n_workgroups, out_bf16, None, lse)
+    return out_bf16, lse
+
+
+def gqa_prompt_plan(n_tokens: int, batch: int, Hq: int, Hkv: int, D: int, max_len: int,
+                    n_splits: int = 0):
+    """(n_splits, workspace_bytes) of a prompt call."""
+    key = ("prompt", n_tokens, batch, Hq, Hkv, D, max_len, n_splits,
+           torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1)
+    hit = _plans.get(key)
+    if hit is not None:
+        return hit
+    n, wsb = ctypes.c_int(0), ctypes.c_size_t(0)
+    _check(lib().ws_gqa_prompt_plan(n_tokens, batch, Hq, Hkv, D, max_len, n_splits, ctypes.byref(n),
+                                    ctypes.byref(wsb)), "ws_gqa_prompt_plan")
+    if len(_plans) > 4096:
+        _plans.clear()
+    _plans[key] = (n.value, wsb.value)
+    return n.value, wsb.value
+
+
+def gqa_prompt(q, k_pages, v_pages, page_table, kv_len, cu_new, scale, max_len, k_scale=None,
+               v_scale=None, n_splits=0, out_dtype=torch.bfloat16, want_lse=True, out=None, lse=None):
+    """Causal attention of the new tokens of every sequence over the pages
+    (ws_gqa_prompt): q [N, Hq, D] bf16, packed; sequence b's queries are rows
+    cu_new[b] .. cu_new[b + 1] and the last of its kv_len[b] tokens in the pages.
+    Pools bf16, or 8-bit with k_scale and v_scale.  Returns (out [N, Hq, D] in
+    out_dtype (bf16 or fp32), lse [N, Hq] fp32 or None); rows outside
+    [cu_new[0], cu_new[B]) are not written.  max_len must bound every kv_len[b]."""
+    dev = _gpu(k_pages, "k_pages")
+    P, Hkv, PS, D = _pools(k_pages, v_pages, k_scale, v_scale, dev)
+    _require(q, "q", torch.bfloat16, dev, 3)
+    _require(page_table, "page_table", torch.int32, dev, 2)
+    _require(kv_len, "kv_len", torch.int32, dev, 1)
+    _require(cu_new, "cu_new", torch.int32, dev, 1)
+    N, Hq, Dq = q.shape
+    B = page_table.shape[0]
+    if Dq != D or Hkv == 0 or Hq % Hkv or Hq == 0:
+        raise ValueError(f"q {tuple(q.shape)} does not match the pools {tuple(k_pages.shape)}")
+    if kv_len.shape[0] != B or cu_new.shape[0] != B + 1:
+        raise ValueError("kv_len must be [B] and cu_new [B + 1] for page_table's B rows")
+    if out is None:
+        if out_dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError("out_dtype must be bfloat16 or float32")
+        out = torch.empty((N, Hq, D), dtype=out_dtype, device=dev)
+    if want_lse and lse is None:
+        lse = torch.empty((N, Hq), dtype=torch.float32, device=dev)
+    if out.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("out must be bfloat16 or float32")
+    _require(out, "out", out.dtype, dev, 3)
+    if out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    if lse is not None:
+        _require(lse, "lse", torch.float32, dev, 2)
+        if lse.shape != (N, Hq):
+            raise ValueError("lse must be [N, Hq]")
+    if N == 0 or B == 0:
+        return out, lse
+    n, wsb = gqa_prompt_plan(N, B, Hq, Hkv, D, int(max_len), int(n_splits))
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    o16, o32 = (out, None) if out.dtype == torch.bfloat16 else (None, out)
+    _run("ws_gqa_prompt", dev, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
+         _ptr(page_table), _ptr(kv_len), _ptr(cu_new), N, B, Hq, Hkv, D, PS, page_table.shape[1], P,
+         int(max_len), n, float(scale), _ptr(o16), _ptr(o32), _ptr(lse), _ptr(ws), wsb)
+    return out, lse
