@@ -6,8 +6,8 @@
 // len - n + i of the len tokens in the pages and sees positions 0 .. its own.
 // The query rows of a KV head are (token, head of the group) pairs, row = i G + g,
 // so the G heads that share K and V share their loads: a workgroup takes a tile of
-// 32 RB NW consecutive rows, a wave 32 RB of them, and walks the tokens in blocks
-// of 64 through LDS with a running maximum and sum (one pass over K and V).
+// 32 RB NW consecutive rows, a wave 32 RB of them, and walks the tokens in tiles
+// of 32 through LDS with a running maximum and sum (one pass over K and V).
 //
 //   S^T[token, row] = K Q^T   A = K from LDS (16 bytes a lane), B = Q in registers
 //   O^T[col, row] += V^T P^T  A = V^T read transposed from LDS, B = P as it comes out
@@ -19,12 +19,13 @@
 //
 // A row sees nothing of the tokens past its position: their scores are masked, and
 // so are their values, which P = 0 alone would not do for an infinity or a NaN
-// (0 * inf): where a block that some row masks holds one, its products are added
-// token by token (pv_masked).
+// (0 * inf): where a tile that some row masks holds one, values_masked adds it to the rows
+// that see it.
 //
 // With few rows the tokens are split over n_splits workgroups per tile, whose pieces
 // (fp32, with their lse) prompt_join_kernel combines.
 #include <algorithm>
+#include <type_traits>
 
 #include "ws_attn.h"
 #include "ws_plan.h"
@@ -35,10 +36,12 @@ namespace ws {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kPromptMaxD = 256;
-constexpr int kPromptBlock = 64;   // tokens of a block
-constexpr int kPromptPad = 32;     // bytes of padding of an LDS row: an odd multiple of 32
-                                   // bytes from row to row, so that 8 rows' 16-byte loads
-                                   // and 4 rows' transposed 32-byte reads meet no bank twice
+constexpr int kPromptTile = 32;    // tokens of a tile
+// Bytes from row to row of a tile in LDS (256 bytes of banks).  K: an odd multiple of
+// 16, so that 16 rows' 16-byte loads meet no bank twice; V: an odd multiple of 64, so
+// that the transposed reads of 4 rows' 64 bytes do not.
+__host__ __device__ constexpr int prompt_k_stride(int D) { return 2 * D + 16; }
+__host__ __device__ constexpr int prompt_v_stride(int D) { return 2 * D + (D % 64 ? 0 : 64); }
 constexpr int kPromptMaxSplits = 64;
 
 struct PromptParams {
@@ -82,6 +85,18 @@ __device__ __forceinline__ bool any_nonfinite(const u32x4& w) {
   return bad;
 }
 
+// Two bf16 values without their infinities and NaN (0 there), and 1 where they are
+// +inf or NaN (pos), -inf or NaN (neg).
+__device__ __forceinline__ void split_nonfinite(uint32_t& w, uint32_t& pos, uint32_t& neg) {
+  // the exponent bits of each half all set: a carry out of them into the sign's place
+  const uint32_t lo = (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15;  // 1 per half
+  const uint32_t man = (((w & 0x007f007fu) + 0x007f007fu) & 0x00800080u) >> 7;  // a NaN's
+  const uint32_t sign = (w >> 15) & 0x00010001u;
+  pos = (lo & (man | ~sign)) * 0x3f80u;
+  neg = (lo & (man | sign)) * 0x3f80u;
+  w &= ~(lo * 0xffffu);
+}
+
 struct PromptTile {
   int b, tile;  // sequence and tile of its rows (b < 0: none)
   int c0, n;    // the sequence's first row of q and its tokens
@@ -121,29 +136,42 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int t, 
   return r;
 }
 
-template <int D, bool F8, int RB, int NW>
+template <int D, bool F8, int NW>
 struct PromptShape {
-  static constexpr int kRows = 32 * RB * NW;
-  static constexpr int kStride = 2 * D + kPromptPad;  // bytes of an LDS row
-  static constexpr int kTile = kPromptBlock * kStride;
-  static constexpr int kBufs = NW > 1 ? 2 : 1;
-  static constexpr int kLds = kBufs * 2 * kTile;
-  // 16-byte pieces (bf16 columns: 8; 8-bit: 16) of a block's K or V, and of a thread's
-  static constexpr int kPieces = kPromptBlock * D / (F8 ? 16 : 8);
+  static constexpr int kKStride = prompt_k_stride(D);
+  static constexpr int kVStride = prompt_v_stride(D);
+  static constexpr int kKTile = kPromptTile * kKStride;
+  static constexpr int kVTile = kPromptTile * kVStride;
+  // 16-byte pieces (bf16: 8 columns; 8-bit: 16) of a tile's K or V, and of a thread's
+  static constexpr int kRowPieces = F8 ? D / 16 : D / 8;
+  static constexpr int kPieces = kPromptTile * kRowPieces;
   static constexpr int kThreads = 64 * NW;
   static constexpr int kLoads = (kPieces + kThreads - 1) / kThreads;
 };
 
+// The loop is a pipeline over 32-token tiles: step t takes the softmax of tile t,
+// whose scores the step before computed, the scores of tile t + 1 and the values'
+// product of tile t - 1, three independent strands, so that the matrix cores run
+// under the softmax's vector work (which costs about as many cycles: 32 rows x 32
+// tokens take 512 cycles of products at D = 128, and 16 exponentials of 16 cycles and
+// some 50 other instructions of 4).  A row whose maximum moved rescales its sums after
+// the step's products, which still are relative to the old one.
+//
+// K and V go through LDS in two slots each: step t reads K of tile t + 1 and V of
+// tile t - 1, both in slot (t + 1) & 1, and writes K of tile t + 2 and V of tile t
+// to the other, from registers requested two steps before.  One barrier a step.
 template <int D, bool F8, int RB, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void prompt_kernel(const PromptParams p) {
+__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const PromptParams p) {
   static_assert(D % 32 == 0 && D <= kPromptMaxD, "head width: a multiple of 32 up to 256");
-  using Sh = PromptShape<D, F8, RB, NW>;
-  constexpr int KS = D / 16;           // k-steps of the scores
-  constexpr int DT = D / 32;           // 32-column tiles of the output
-  constexpr int CH = F8 ? D / 16 : D / 8;  // 16-byte pieces of a token's row
+  using Sh = PromptShape<D, F8, NW>;
+  constexpr int KS = D / 16;  // k-steps of the scores
+  constexpr int DT = D / 32;  // 32-column tiles of the output
+  constexpr int CH = Sh::kRowPieces;
   constexpr int LD = Sh::kLoads;
-  __shared__ __attribute__((aligned(256))) char s_kv[Sh::kLds];
-  __shared__ int s_bad[2];  // a block's values hold an infinity or a NaN (masked blocks only)
+  constexpr int kRows = 32 * RB * NW;
+  __shared__ __attribute__((aligned(256))) char s_k[2 * Sh::kKTile];
+  __shared__ __attribute__((aligned(256))) char s_v[2 * Sh::kVTile];
+  __shared__ int s_bad[2];  // a slot's values held an infinity or a NaN (masked tiles only)
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -154,25 +182,25 @@ __global__ __launch_bounds__(64 * NW, 1) void prompt_kernel(const PromptParams p
   const int kvh = id % p.Hkv;
   const int rest = id / p.Hkv;
   const int split = rest % p.n_splits;
-  const PromptTile tl = prompt_tile(p, rest / p.n_splits, Sh::kRows);
+  const PromptTile tl = prompt_tile(p, rest / p.n_splits, kRows);
   if (tl.b < 0) return;
   const int G = p.G;
   const int R = tl.n * G;  // rows of the sequence and KV head
   const int len = uniform(p.kv_len[tl.b]);
   const bool len_good = len_ok(len, 0, p.cap);
   const int first_pos = len - tl.n;  // position of the sequence's first query
-  const int row0 = tl.tile * Sh::kRows;
-  const int rows_here = min(Sh::kRows, R - row0);
-  // visible tokens of the tile's first and last row
+  const int row0 = tl.tile * kRows;
+  const int rows_here = min(kRows, R - row0);
+  // visible tokens of the workgroup's first and last row
   const int lim_lo = first_pos + row0 / G + 1;
   const int lim_hi = len_good ? max(first_pos + (row0 + rows_here - 1) / G + 1, 0) : 0;
-  const int nb = (lim_hi + kPromptBlock - 1) / kPromptBlock;
+  const int nb = (lim_hi + kPromptTile - 1) / kPromptTile;
   const int blk0 = (int)((long long)split * nb / p.n_splits);
   const int blk1 = (int)((long long)(split + 1) * nb / p.n_splits);
 
   // the wave's rows
-  int lim[RB];        // visible tokens of the lane's row
-  size_t out_row[RB]; // its row of out / lse
+  int lim[RB];         // visible tokens of the lane's row
+  size_t out_row[RB];  // its row of out / lse
   bool live[RB];
   u32x4 qb[RB][KS];
 #pragma unroll
@@ -202,71 +230,79 @@ __global__ __launch_bounds__(64 * NW, 1) void prompt_kernel(const PromptParams p
     for (int d = 0; d < DT; ++d) acc[rb][d] = f32x16{};
   }
 
-  // A block's two 32-token halves: pool token index of the half's first token, its last
-  // row that holds a token (later rows repeat it), and whether the page id was bad.
-  struct Half {
+  // A tile's place: pool token index of its first token, its last row that holds a
+  // token (later rows repeat it), and whether the page id was bad.
+  struct Place {
     uint32_t tok;
     int last;
     bool bad;
   };
-  auto half_of = [&](int blk, int hf) __attribute__((always_inline)) {
-    const int t = min(blk * kPromptBlock + 32 * hf, len - 1) & ~31;
+  auto place_of = [&](int blk) __attribute__((always_inline)) {
+    const int t = min(blk, blk1 - 1) * kPromptTile;  // (< len)
     const int page = t / p.page_size;
     const int raw = p.page_table[(size_t)tl.b * p.max_pages + page];
     const int pid = clamp_page(raw, p.num_pages);
-    Half x;
+    Place x;
     x.tok = ((uint32_t)pid * (uint32_t)p.Hkv + (uint32_t)kvh) * (uint32_t)p.page_size +
             (uint32_t)(t - page * p.page_size);
     x.last = min(31, len - 1 - t);
     x.bad = raw != pid;
     return x;
   };
-  // Registers of the block under way: pieces tid, tid + threads, ... of K and V.
-  u32x4 kr[LD], vr[LD];
-  uint32_t ksr[F8 ? LD : 1], vsr[F8 ? LD : 1];
-  auto load_block = [&](const Half (&hv)[2]) __attribute__((always_inline)) {
+  // Pieces tid, tid + threads, ... of a tile of K or V: the tile's address is uniform, a
+  // lane's offset in it the same for every tile.
+  struct Regs {
+    u32x4 w[LD];
+    uint32_t s[F8 ? LD : 1];
+  };
+  uint32_t off[LD], off_s[F8 ? LD : 1];
+#pragma unroll
+  for (int u = 0; u < LD; ++u) {
+    const int piece = min(tid + u * Sh::kThreads, Sh::kPieces - 1);
+    off[u] = 16 * piece;
+    if (F8) off_s[u] = piece / CH;
+  }
+  auto load_tile = [&](const void* pages, const uint8_t* scale, const Place& x, Regs& g)
+                       __attribute__((always_inline)) {
+    const char* base = (const char*)pages + (size_t)x.tok * (16 * CH);
 #pragma unroll
     for (int u = 0; u < LD; ++u) {
-      const int piece = tid + u * Sh::kThreads;
-      if (Sh::kPieces % Sh::kThreads != 0 && piece >= Sh::kPieces) continue;
-      const int t = piece / CH;
-      const int c = piece - t * CH;
-      const Half& x = t < 32 ? hv[0] : hv[1];
-      const size_t row = (size_t)x.tok + min(t & 31, x.last);
-      kr[u] = ((const u32x4*)p.k_pages)[row * CH + c];
-      vr[u] = ((const u32x4*)p.v_pages)[row * CH + c];
-      if (F8) {
-        ksr[u] = p.k_scale[row];
-        vsr[u] = p.v_scale[row];
-      }
+      g.w[u] = *(const u32x4*)(base + off[u]);
+      if (F8) g.s[u] = *(scale + x.tok + off_s[u]);
     }
   };
-  // Writes them to LDS buffer `buf`; with `check`, notes an infinity or a NaN in V.
-  auto store_block = [&](int buf, bool check) __attribute__((always_inline)) {
-    char* kb = s_kv + buf * 2 * Sh::kTile;
-    char* vb = kb + Sh::kTile;
+  // The same of a tile that may hold fewer tokens: rows past the last repeat it.
+  auto load_last = [&](const void* pages, const uint8_t* scale, const Place& x, Regs& g)
+                       __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < LD; ++u) {
+      const int piece = min(tid + u * Sh::kThreads, Sh::kPieces - 1);
+      const int t = piece / CH;
+      const size_t row = (size_t)x.tok + min(t, x.last);
+      g.w[u] = ((const u32x4*)pages)[row * CH + (piece - t * CH)];
+      if (F8) g.s[u] = scale[row];
+    }
+  };
+  // Writes them to an LDS slot; with `bad`, notes an infinity or a NaN there.
+  auto store_tile = [&](char* slot, int stride, const Regs& g, int* bad)
+                        __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < LD; ++u) {
       const int piece = tid + u * Sh::kThreads;
       if (Sh::kPieces % Sh::kThreads != 0 && piece >= Sh::kPieces) continue;
       const int t = piece / CH;
       const int c = piece - t * CH;
-      if (F8) {
-        const int at = t * Sh::kStride + 32 * c;
-        const float ks = __builtin_bit_cast(float, ksr[u] << 23);
-        const float vs = __builtin_bit_cast(float, vsr[u] << 23);
-        *(u32x4*)(kb + at) = cvt8_fp8(kr[u][0], kr[u][1], ks);
-        *(u32x4*)(kb + at + 16) = cvt8_fp8(kr[u][2], kr[u][3], ks);
-        const u32x4 v0 = cvt8_fp8(vr[u][0], vr[u][1], vs);
-        const u32x4 v1 = cvt8_fp8(vr[u][2], vr[u][3], vs);
-        *(u32x4*)(vb + at) = v0;
-        *(u32x4*)(vb + at + 16) = v1;
-        if (check && (any_nonfinite(v0) || any_nonfinite(v1))) s_bad[buf] = 1;
+      if constexpr (F8) {
+        char* at = slot + t * stride + 32 * c;
+        const float sc = __builtin_bit_cast(float, g.s[u] << 23);
+        const u32x4 a = cvt8_fp8(g.w[u][0], g.w[u][1], sc);
+        const u32x4 b = cvt8_fp8(g.w[u][2], g.w[u][3], sc);
+        *(u32x4*)at = a;
+        *(u32x4*)(at + 16) = b;
+        if (bad && (any_nonfinite(a) || any_nonfinite(b))) *bad = 1;
       } else {
-        const int at = t * Sh::kStride + 16 * c;
-        *(u32x4*)(kb + at) = kr[u];
-        *(u32x4*)(vb + at) = vr[u];
-        if (check && any_nonfinite(vr[u])) s_bad[buf] = 1;
+        *(u32x4*)(slot + t * stride + 16 * c) = g.w[u];
+        if (bad && any_nonfinite(g.w[u])) *bad = 1;
       }
     }
   };
@@ -275,151 +311,214 @@ __global__ __launch_bounds__(64 * NW, 1) void prompt_kernel(const PromptParams p
   auto ref = [&](float m) __attribute__((always_inline)) {
     return m == neg_inf() ? 0.f : m * p.scale_log2;
   };
-  auto compute = [&](int blk, int buf, bool masked, bool bad0, bool bad1)
-                     __attribute__((always_inline)) {
-    const char* kb = s_kv + buf * 2 * Sh::kTile;
-    const uint32_t vb = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(
-        s_kv + buf * 2 * Sh::kTile + Sh::kTile);
-    f32x16 s[RB][2];
+  // S^T of a K slot
+  auto scores = [&](int slot, f32x16 (&s)[RB]) __attribute__((always_inline)) {
+    const char* kb = s_k + slot * Sh::kKTile + n32 * Sh::kKStride + 16 * h;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) s[rb][0] = s[rb][1] = f32x16{};
+    for (int rb = 0; rb < RB; ++rb) s[rb] = f32x16{};
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
+    for (int ks = 0; ks < KS; ++ks) {
+      const u32x4 a = *(const u32x4*)(kb + 32 * ks);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 a = *(const u32x4*)(kb + (32 * tt + n32) * Sh::kStride + 32 * ks + 16 * h);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) s[rb][tt] = mfma32x32x16(a, qb[rb][ks], s[rb][tt]);
-      }
-    const int t0 = blk * kPromptBlock;
-    u32x4 pb[RB][4];
+      for (int rb = 0; rb < RB; ++rb) s[rb] = mfma32x32x16(a, qb[rb][ks], s[rb]);
+    }
+  };
+  // P of tile blk from its scores; alpha: the factor of the sums so far (1: none)
+  auto softmax = [&](auto mask, int blk, bool bad, f32x16 (&s)[RB], u32x4 (&pb)[RB][2],
+                     float (&alpha)[RB]) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(mask)::value;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int seen = lim[rb] - t0;  // tokens of the block that the row sees
-      if (masked) {
+      const int seen = lim[rb] - blk * kPromptTile;  // tokens of the tile that the row sees
+      if (MASKED) {
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int t = 32 * tt + 8 * (i >> 2) + 4 * h + (i & 3);
-            float x = s[rb][tt][i];
-            if (tt ? bad1 : bad0) x = qnan();
-            s[rb][tt][i] = t < seen ? x : neg_inf();
-          }
+        for (int i = 0; i < 16; ++i) {
+          const float x = bad ? qnan() : s[rb][i];
+          s[rb][i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? x : neg_inf();
+        }
       }
-      float bm = s[rb][0][0];
+      float bm = s[rb][0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) bm = fmaxf(bm, s[rb][0][i]);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) bm = fmaxf(bm, s[rb][1][i]);
+      for (int i = 1; i < 16; ++i) bm = fmaxf(bm, s[rb][i]);
       float lo, hi;
       pair_xor32(bm, lo, hi);
       bm = fmaxf(lo, hi);
       // (-inf - -inf is NaN, and no reason to move)
       const bool move = (bm - m_run[rb]) * p.scale_log2 > kLazyRescaleLog2;
-      if (__builtin_amdgcn_ballot_w64(move) != 0) {
-        const float m_new = fmaxf(m_run[rb], bm);
-        const float alpha =
-            m_new == neg_inf() ? 1.f
-                               : __builtin_amdgcn_exp2f((m_run[rb] - m_new) * p.scale_log2);
-        m_run[rb] = m_new;
-        l_run[rb] *= alpha;
+      const float m_new = move ? bm : m_run[rb];
+      alpha[rb] = move ? __builtin_amdgcn_exp2f((m_run[rb] - m_new) * p.scale_log2) : 1.f;
+      m_run[rb] = m_new;
+      const float mc = ref(m_new);
+      float ps = 0.f, e[16];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[rb][d] = acc[rb][d] * alpha;
+      for (int i = 0; i < 16; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(fmaf(s[rb][i], p.scale_log2, -mc));
+        if (MASKED) e[i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? e[i] : 0.f;
+        ps += e[i];
       }
-      const float mc = ref(m_run[rb]);
-      float ps = 0.f;
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        float e[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(fmaf(s[rb][tt][i], p.scale_log2, -mc));
-          if (masked) {
-            const int t = 32 * tt + 8 * (i >> 2) + 4 * h + (i & 3);
-            e[i] = t < seen ? e[i] : 0.f;
-          }
-          ps += e[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) pb[rb][2 * tt + (i >> 3)][(i >> 1) & 3] = pack_bf16x2(e[i], e[i + 1]);
-      }
-      l_run[rb] += ps;
+      for (int i = 0; i < 16; i += 2) pb[rb][i >> 3][(i >> 1) & 3] = pack_bf16x2(e[i], e[i + 1]);
+      l_run[rb] = l_run[rb] * alpha[rb] + ps;
     }
-    if (masked && uniform(s_bad[buf])) {
-      // pv_masked: token by token, only where the row sees the token
-#pragma unroll 1
-      for (int t = 0; t < kPromptBlock; ++t) {
-        const int idx = 16 * (t >> 5) + 4 * ((t >> 3) & 3) + (t & 3);  // register of the owner half
-        const char* vrow = s_kv + buf * 2 * Sh::kTile + Sh::kTile + t * Sh::kStride;
+  };
+  // O^T += V^T P^T of a V slot: lane group g4 of 16 lanes reads 4 tokens x 16 columns
+  // transposed
+  const int g4 = lane >> 4;
+  const int l16 = lane & 15;
+  const uint32_t va = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_v +
+                      (4 * (g4 >> 1) + (l16 >> 2)) * Sh::kVStride + 32 * (g4 & 1) + 8 * (l16 & 3);
+  auto values = [&](int slot, const u32x4 (&pb)[RB][2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          uint32_t w = 0;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) w = k == (idx >> 1) ? pb[rb][k >> 2][k & 3] : w;
-          w = (uint32_t)__shfl((int)w, n32 + 32 * ((t >> 2) & 1));
-          const float pt = __builtin_bit_cast(float, (idx & 1) ? w & 0xffff0000u : w << 16);
-          const bool vis = t0 + t < lim[rb];
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int col = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
-              const float v = bf16_to_f32(*(const uint16_t*)(vrow + 2 * col));
-              if (vis) acc[rb][d][i] += pt * v;
-            }
-        }
-      }
-      return;
-    }
-    // V^T: lane group g4 of 16 lanes reads 4 tokens x 16 columns transposed
-    const int g4 = lane >> 4;
-    const int l16 = lane & 15;
-    const uint32_t va = vb + (4 * (g4 >> 1) + (l16 >> 2)) * Sh::kStride + 32 * (g4 & 1) +
-                        8 * (l16 & 3);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
+    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const uint2 x = lds_read_tr_b64(va + 16 * ks * Sh::kStride + 64 * d);
-        const uint2 y = lds_read_tr_b64(va + (16 * ks + 8) * Sh::kStride + 64 * d);
+        const uint32_t at = va + slot * Sh::kVTile + 16 * ks * Sh::kVStride + 64 * d;
+        const uint2 x = lds_read_tr_b64(at);
+        const uint2 y = lds_read_tr_b64(at + 8 * Sh::kVStride);
         const u32x4 a = {x.x, x.y, y.x, y.y};
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) acc[rb][d] = mfma32x32x16(a, pb[rb][ks], acc[rb][d]);
       }
   };
+  // The same where the slot holds an infinity or a NaN that some rows do not see: the
+  // finite values' product, and from two products of 0 and 1 whether a row sees an
+  // infinity of either sign (a NaN counts as both) in a column.
+  auto values_masked = [&](int slot, int blk, const u32x4 (&pb)[RB][2])
+                           __attribute__((always_inline)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        f32x16 pos{}, neg{};
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const uint32_t at = va + slot * Sh::kVTile + 16 * ks * Sh::kVStride + 64 * d;
+          const uint2 x = lds_read_tr_b64(at);
+          const uint2 y = lds_read_tr_b64(at + 8 * Sh::kVStride);
+          u32x4 fin = {x.x, x.y, y.x, y.y}, ap, an, vis;
+          // vis: 1 for the k slots (tokens 0 .. 3 and 8 .. 11 past 16 ks + 4 h) that are seen
+          const int seen = lim[rb] - blk * kPromptTile - 16 * ks - 4 * h;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t f = fin[e], u, w;
+            split_nonfinite(f, u, w);
+            fin[e] = f;
+            ap[e] = u;
+            an[e] = w;
+            const int t = 8 * (e >> 1) + 2 * (e & 1);
+            vis[e] = (t < seen ? 0x3f80u : 0u) | (t + 1 < seen ? 0x3f800000u : 0u);
+          }
+          acc[rb][d] = mfma32x32x16(fin, pb[rb][ks], acc[rb][d]);
+          pos = mfma32x32x16(ap, vis, pos);
+          neg = mfma32x32x16(an, vis, neg);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (pos[i] > 0.f) acc[rb][d][i] -= neg_inf();
+          if (neg[i] > 0.f) acc[rb][d][i] += neg_inf();
+        }
+      }
+    }
+  };
+  // acc times alpha, where some row's maximum moved
+  auto rescale = [&](const float (&alpha)[RB]) __attribute__((always_inline)) {
+    bool moved = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) moved |= alpha[rb] != 1.f;
+    if (__builtin_amdgcn_ballot_w64(moved) == 0) return;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[rb][d] = acc[rb][d] * alpha[rb];
+  };
 
-  if (blk0 < blk1) {
-    // a block some row of the tile masks a token of
-    auto is_masked = [&](int blk) { return (blk + 1) * kPromptBlock > lim_lo; };
-    Half cur[2] = {half_of(blk0, 0), half_of(blk0, 1)};
-    load_block(cur);
-    if (tid < 2) s_bad[tid] = 0;
+  // Tiles that every row sees whole, in the pipeline: [blk0, blkm).
+  const int blkm = max(blk0, min(blk1, max(lim_lo, 0) / kPromptTile));
+  bool bad_page = false;  // one of them lies in a bad page: every row is NaN
+  if (blk0 < blkm) {
+    const int T = blkm - blk0;
+    f32x16 s[2][RB];
+    u32x4 pb[2][RB][2];
+    Regs kg[2], vg[2];
+    // places of tiles t .. t + 3 (a page id is requested four steps before its use)
+    Place pl[4] = {place_of(blk0), place_of(blk0 + 1), place_of(blk0 + 2), place_of(blk0 + 3)};
+    load_tile(p.k_pages, p.k_scale, pl[0], kg[0]);
+    load_tile(p.k_pages, p.k_scale, pl[1], kg[1]);
+    // the values of "tile -1", which step 0 adds with weights of 0
+    for (int i = tid; i < Sh::kVTile / 16; i += Sh::kThreads)
+      ((u32x4*)(s_v + Sh::kVTile))[i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) pb[1][rb][0] = pb[1][rb][1] = u32x4{0, 0, 0, 0};
+    store_tile(s_k, Sh::kKStride, kg[0], nullptr);
+    store_tile(s_k + Sh::kKTile, Sh::kKStride, kg[1], nullptr);
+    load_tile(p.k_pages, p.k_scale, pl[2], kg[0]);
+    load_tile(p.v_pages, p.v_scale, pl[0], vg[0]);
+    load_tile(p.k_pages, p.k_scale, pl[3], kg[1]);
+    load_tile(p.v_pages, p.v_scale, pl[1], vg[1]);
     __syncthreads();
-    store_block(0, is_masked(blk0));
-    Half nxt[2] = {half_of(min(blk0 + 1, blk1 - 1), 0), half_of(min(blk0 + 1, blk1 - 1), 1)};
-    load_block(nxt);
+    scores(0, s[0]);
     __syncthreads();
-#pragma unroll 1
-    for (int blk = blk0; blk < blk1; ++blk) {
-      const int buf = Sh::kBufs == 2 ? (blk - blk0) & 1 : 0;
-      const bool bad0 = cur[0].bad, bad1 = cur[1].bad;
-      if (is_masked(blk) || bad0 || bad1)
-        compute(blk, buf, true, bad0, bad1);
-      else
-        compute(blk, buf, false, false, false);
-      if (blk + 1 == blk1) break;
-      if (Sh::kBufs == 1) __syncthreads();
-      // (s_bad stays set once a masked block held a bad value: the blocks after it take
-      // the slow sum too, which is right for any block)
-      store_block(Sh::kBufs == 2 ? buf ^ 1 : 0, is_masked(blk + 1));
-      cur[0] = nxt[0];
-      cur[1] = nxt[1];
-      const int want = min(blk + 2, blk1 - 1);
-      nxt[0] = half_of(want, 0);
-      nxt[1] = half_of(want, 1);
-      load_block(nxt);
+    auto step = [&](auto par, int t) __attribute__((always_inline)) {
+      constexpr int c = decltype(par)::value;  // t & 1
+      bad_page |= pl[0].bad;
+      store_tile(s_k + c * Sh::kKTile, Sh::kKStride, kg[c], nullptr);
+      store_tile(s_v + c * Sh::kVTile, Sh::kVStride, vg[c], nullptr);
+      pl[0] = pl[1];
+      pl[1] = pl[2];
+      pl[2] = pl[3];
+      pl[3] = place_of(blk0 + t + 4);
+      load_tile(p.k_pages, p.k_scale, pl[3], kg[c]);
+      load_tile(p.v_pages, p.v_scale, pl[1], vg[c]);
+      float alpha[RB];
+      scores(c ^ 1, s[c ^ 1]);
+      softmax(std::false_type{}, 0, false, s[c], pb[c], alpha);
+      values(c ^ 1, pb[c ^ 1]);
+      rescale(alpha);
       __syncthreads();
+    };
+    int t = 0;
+#pragma unroll 1
+    for (; t + 2 <= T; t += 2) {
+      step(std::integral_constant<int, 0>{}, t);
+      step(std::integral_constant<int, 1>{}, t + 1);
+    }
+    if (t < T) {
+      step(std::integral_constant<int, 0>{}, t);
+      values(0, pb[0]);
+    } else {
+      values(1, pb[1]);
+    }
+  }
+  // The others, masked, one after the other.
+  if (blkm < blk1) {
+    if (tid < 2) s_bad[tid] = 0;
+    Regs kg, vg;
+    Place nx = place_of(blkm);
+    load_last(p.k_pages, p.k_scale, nx, kg);
+    load_last(p.v_pages, p.v_scale, nx, vg);
+    __syncthreads();
+    int c = 0;
+#pragma unroll 1
+    for (int blk = blkm; blk < blk1; ++blk) {
+      const bool bad = nx.bad;
+      store_tile(s_k + c * Sh::kKTile, Sh::kKStride, kg, nullptr);
+      // (s_bad stays set: the slow sum is right for any tile)
+      store_tile(s_v + c * Sh::kVTile, Sh::kVStride, vg, &s_bad[c]);
+      nx = place_of(blk + 1);
+      load_last(p.k_pages, p.k_scale, nx, kg);
+      load_last(p.v_pages, p.v_scale, nx, vg);
+      __syncthreads();
+      f32x16 s[RB];
+      u32x4 pb[RB][2];
+      float alpha[RB];
+      scores(c, s);
+      softmax(std::true_type{}, blk, bad, s, pb, alpha);
+      rescale(alpha);
+      if (uniform(s_bad[c]))
+        values_masked(c, blk, pb);
+      else
+        values(c, pb);
+      c ^= 1;
     }
   }
 
@@ -431,8 +530,8 @@ __global__ __launch_bounds__(64 * NW, 1) void prompt_kernel(const PromptParams p
     const float l = lo + hi;
     if (!live[rb]) continue;
     const bool none = l == 0.f;
-    const float inv = !len_good ? qnan() : none ? 0.f : 1.f / l;
-    const float lse_v = !len_good ? qnan()
+    const float inv = !len_good || bad_page ? qnan() : none ? 0.f : 1.f / l;
+    const float lse_v = !len_good || bad_page ? qnan()
                         : none    ? neg_inf()
                                   : (ref(m_run[rb]) + __log2f(l)) * kLn2;
     const size_t rows = (size_t)p.N * p.Hq;
@@ -502,18 +601,21 @@ struct PromptPlan {
   bool wide;  // four waves a workgroup
   int rows, tiles, splits;
 };
-static PromptPlan prompt_plan(int N, int B, int Hq, int Hkv, int max_len, int n_splits) {
+// 32-row blocks of a wave: two share a tile's LDS reads (K and V operands) while
+// their sums and queries fit the 512 registers of one wave per SIMD.
+__host__ __device__ constexpr int prompt_row_blocks(int D) { return 1; }
+static PromptPlan prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len, int n_splits) {
   const int G = Hq / Hkv;
   PromptPlan r;
   r.wide = (long long)N * G > 64LL * B;
-  r.rows = r.wide ? 128 : 32;
+  r.rows = r.wide ? 128 * prompt_row_blocks(D) : 32;
   r.tiles = (int)(((long long)N * G + r.rows - 1) / r.rows) + B;
   r.splits = n_splits;
   if (n_splits == 0) {
-    // enough workgroups for the chip, of at least 4 blocks each
-    const int most = std::max(1, max_len / (4 * kPromptBlock));
+    // enough workgroups for the chip, of at least 8 tiles each
+    const int most = std::max(1, max_len / (8 * kPromptTile));
     const long long wgs = (long long)((N * (long long)G + r.rows - 1) / r.rows) * Hkv;
-    const int want = choose_workgroups(0, r.wide ? 2 : 4, 1LL << 30, 1);
+    const int want = choose_workgroups(0, r.wide ? 1 : 4, 1LL << 30, 1);
     r.splits = (int)std::min<long long>(std::max<long long>(want / std::max(wgs, 1LL), 1),
                                         std::min(most, kPromptMaxSplits));
   }
@@ -531,7 +633,7 @@ static void prompt_launch(const PromptParams& p, const PromptPlan& pl, int D, hi
 #define WS_PROMPT_CASE(DD)                                                              \
   case DD:                                                                              \
     if (pl.wide)                                                                        \
-      hipLaunchKernelGGL((prompt_kernel<DD, F8, 1, 4>), grid, dim3(256), 0, s, p);      \
+      hipLaunchKernelGGL((prompt_kernel<DD, F8, prompt_row_blocks(DD), 4>), grid, dim3(256), 0, s, p);      \
     else                                                                                \
       hipLaunchKernelGGL((prompt_kernel<DD, F8, 1, 1>), grid, dim3(64), 0, s, p);       \
     break;
@@ -552,9 +654,9 @@ static int prompt_sizes(const char* name, int N, int B, int Hq, int Hkv, int D, 
                      name, N, B, Hq, Hkv, max_len, n_splits, kMaxSeqs, kPromptMaxSplits);
   if (!prompt_width_ok(D))
     return set_error(WS_EINVAL, "%s: head_dim %d unsupported (multiples of 32 up to 256)", name, D);
-  if ((long long)N * (Hq / Hkv) + 128LL * B >= (1LL << 31) || max_len > (1 << 30))
+  if ((long long)N * (Hq / Hkv) + 256LL * B >= (1LL << 31) || max_len > (1 << 30))
     return set_error(WS_EINVAL, "%s: %d tokens of %d heads exceed the row index range", name, N, Hq);
-  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, max_len, n_splits);
+  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, max_len, n_splits);
   if ((long long)pl.tiles * Hkv * pl.splits * 256 >= (1LL << 32))
     return set_error(WS_EINVAL, "%s: %d tokens of %d heads exceed the launch grid", name, N, Hq);
   return WS_OK;
@@ -567,7 +669,7 @@ using namespace ws;
 extern "C" int ws_gqa_prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len, int n_splits,
                                   int* n_splits_out, size_t* workspace_bytes_out) {
   if (int rc = prompt_sizes("ws_gqa_prompt_plan", N, B, Hq, Hkv, D, max_len, n_splits)) return rc;
-  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, max_len, n_splits);
+  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, max_len, n_splits);
   if (n_splits_out) *n_splits_out = pl.splits;
   if (workspace_bytes_out) *workspace_bytes_out = prompt_bytes(N, Hq, D, pl.splits);
   return WS_OK;
@@ -599,7 +701,7 @@ extern "C" int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void*
     return set_error(WS_EINVAL, "%s: buffers must be 16-byte aligned", name);
   if (!(scale - scale == 0.f)) return set_error(WS_EINVAL, "%s: scale must be finite", name);
   if (N == 0 || B == 0) return WS_OK;
-  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, max_len, n_splits);
+  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, max_len, n_splits);
   const size_t need = prompt_bytes(N, Hq, D, pl.splits);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(WS_EWORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
