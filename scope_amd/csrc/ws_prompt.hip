@@ -34,14 +34,28 @@
 namespace ws {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef const int32_t __attribute__((address_space(4))) ConstInt;
 
 constexpr int kPromptMaxD = 256;
 constexpr int kPromptTile = 32;    // tokens of a tile
-// Bytes from row to row of a tile in LDS (256 bytes of banks).  K: an odd multiple of
-// 16, so that 16 rows' 16-byte loads meet no bank twice; V: an odd multiple of 64, so
-// that the transposed reads of 4 rows' 64 bytes do not.
-__host__ __device__ constexpr int prompt_k_stride(int D) { return 2 * D + 16; }
-__host__ __device__ constexpr int prompt_v_stride(int D) { return 2 * D + (D % 64 ? 0 : 64); }
+constexpr int kPromptSlots = 4;    // LDS slots of K and of V
+// 16-byte chunks of a tile's row lie in LDS in an order of their own, chunk ^ f(row), so
+// that no two of a read meet in a bank (256 bytes of banks): 16 rows' 16-byte loads of
+// one K chunk, 4 rows' transposed reads of 64 bytes of V.  f keeps a chunk in its group
+// of the row's largest power of two of chunks, p; 16 / p rows apart lies the next row
+// that begins at the same bank.
+__host__ __device__ constexpr int prompt_pow2(int D) {
+  const int ch = D / 8, p = ch & -ch;
+  return p < 16 ? p : 16;
+}
+__host__ __device__ constexpr int prompt_k_swap(int D, int row) {
+  return (row / (16 / prompt_pow2(D))) & (prompt_pow2(D) - 1);
+}
+__host__ __device__ constexpr int prompt_v_swap(int D, int row) {
+  return prompt_pow2(D) == 16  ? (row & 3) << 2
+         : prompt_pow2(D) == 8 ? (row >> 1 & 1) << 2
+                               : 0;
+}
 constexpr int kPromptMaxSplits = 64;
 
 struct PromptParams {
@@ -63,6 +77,9 @@ struct PromptParams {
   uint32_t q_sign;   // 0x80008000 where the caller's scale is negative
 };
 
+__device__ __forceinline__ u32x4 lds_read_b128(uint32_t addr) {
+  return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)addr;
+}
 __device__ __forceinline__ f32x16 mfma32x32x16(const u32x4& a, const u32x4& b, const f32x16& c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -138,16 +155,28 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int t, 
 
 template <int D, bool F8, int NW>
 struct PromptShape {
-  static constexpr int kKStride = prompt_k_stride(D);
-  static constexpr int kVStride = prompt_v_stride(D);
-  static constexpr int kKTile = kPromptTile * kKStride;
-  static constexpr int kVTile = kPromptTile * kVStride;
+  static constexpr int kRow = 2 * D;               // bytes of a row in LDS
+  static constexpr int kTile = kPromptTile * kRow;  // and of a slot
   // 16-byte pieces (bf16: 8 columns; 8-bit: 16) of a tile's K or V, and of a thread's
   static constexpr int kRowPieces = F8 ? D / 16 : D / 8;
   static constexpr int kPieces = kPromptTile * kRowPieces;
   static constexpr int kThreads = 64 * NW;
   static constexpr int kLoads = (kPieces + kThreads - 1) / kThreads;
 };
+
+// 16 bytes a lane from `base` + off to LDS at `lds` + 16 * lane, with no register between
+// (counted by vmcnt; the caller waits, then passes a barrier).  In assembly because the
+// compiler would wait for every one of them ahead of any LDS read.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base), "s"(lds)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N < 63 ? N : 63) : "memory");
+}
 
 // The loop is a pipeline over 32-token tiles: step t takes the softmax of tile t,
 // whose scores the step before computed, the scores of tile t + 1 and the values'
@@ -157,9 +186,11 @@ struct PromptShape {
 // some 50 other instructions of 4).  A row whose maximum moved rescales its sums after
 // the step's products, which still are relative to the old one.
 //
-// K and V go through LDS in two slots each: step t reads K of tile t + 1 and V of
-// tile t - 1, both in slot (t + 1) & 1, and writes K of tile t + 2 and V of tile t
-// to the other, from registers requested two steps before.  One barrier a step.
+// K and V go through LDS in four slots each: step t reads K of tile t + 1 and V of
+// tile t - 1.  bf16 tiles are loaded straight to LDS, three steps ahead (K of tile t + 4
+// and V of t + 2 in step t, to the slots the step before has left); 8-bit ones through
+// registers, requested two steps before they are converted and written.  One barrier a
+// step.
 template <int D, bool F8, int RB, int NW>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const PromptParams p) {
   static_assert(D % 32 == 0 && D <= kPromptMaxD, "head width: a multiple of 32 up to 256");
@@ -169,8 +200,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   constexpr int CH = Sh::kRowPieces;
   constexpr int LD = Sh::kLoads;
   constexpr int kRows = 32 * RB * NW;
-  __shared__ __attribute__((aligned(256))) char s_k[2 * Sh::kKTile];
-  __shared__ __attribute__((aligned(256))) char s_v[2 * Sh::kVTile];
+  __shared__ __attribute__((aligned(256))) char s_k[kPromptSlots * Sh::kTile];
+  __shared__ __attribute__((aligned(256))) char s_v[kPromptSlots * Sh::kTile];
   __shared__ int s_bad[2];  // a slot's values held an infinity or a NaN (masked tiles only)
 
   const int tid = threadIdx.x;
@@ -240,7 +271,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   auto place_of = [&](int blk) __attribute__((always_inline)) {
     const int t = min(blk, blk1 - 1) * kPromptTile;  // (< len)
     const int page = t / p.page_size;
-    const int raw = p.page_table[(size_t)tl.b * p.max_pages + page];
+    // a scalar load (the constant address space): a vector load's result would be
+    // waited for together with the tiles under way
+    const int raw = ((const ConstInt*)p.page_table)[(size_t)tl.b * p.max_pages + page];
     const int pid = clamp_page(raw, p.num_pages);
     Place x;
     x.tok = ((uint32_t)pid * (uint32_t)p.Hkv + (uint32_t)kvh) * (uint32_t)p.page_size +
@@ -249,26 +282,42 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     x.bad = raw != pid;
     return x;
   };
-  // Pieces tid, tid + threads, ... of a tile of K or V: the tile's address is uniform, a
-  // lane's offset in it the same for every tile.
+  const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_k;
+  const uint32_t lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_v;
+  // Straight to LDS: chunks of 1 KB, NW of them at a time, one a wave.  A lane's chunk of
+  // the row is the one that belongs at its place; the offsets are the same for every tile.
+  constexpr int kDma = Sh::kTile / 1024;
+  constexpr int LQ = (kDma + NW - 1) / NW;  // a wave's (the last one twice where NW is too many)
+  uint32_t dma_k[LQ], dma_v[LQ], dma_at[LQ];
+#pragma unroll
+  for (int u = 0; u < LQ; ++u) {
+    const int q = min(wave + u * NW, kDma - 1);
+    const int at = 64 * q + lane;
+    const int row = at / (D / 8);
+    const int c = at - row * (D / 8);
+    dma_at[u] = 1024 * q;
+    dma_k[u] = row * Sh::kRow + 16 * (c ^ prompt_k_swap(D, row));
+    dma_v[u] = row * Sh::kRow + 16 * (c ^ prompt_v_swap(D, row));
+  }
+  auto dma_tile = [&](const void* pages, const Place& x, const uint32_t (&off)[LQ], uint32_t slot)
+                      __attribute__((always_inline)) {
+    const char* base = (const char*)pages + (size_t)x.tok * Sh::kRow;
+#pragma unroll
+    for (int u = 0; u < LQ; ++u) load_to_lds(base, off[u], slot + dma_at[u]);
+  };
+  // Through registers: pieces tid, tid + threads, ... of a tile.
   struct Regs {
     u32x4 w[LD];
     uint32_t s[F8 ? LD : 1];
   };
-  uint32_t off[LD], off_s[F8 ? LD : 1];
-#pragma unroll
-  for (int u = 0; u < LD; ++u) {
-    const int piece = min(tid + u * Sh::kThreads, Sh::kPieces - 1);
-    off[u] = 16 * piece;
-    if (F8) off_s[u] = piece / CH;
-  }
   auto load_tile = [&](const void* pages, const uint8_t* scale, const Place& x, Regs& g)
                        __attribute__((always_inline)) {
     const char* base = (const char*)pages + (size_t)x.tok * (16 * CH);
 #pragma unroll
     for (int u = 0; u < LD; ++u) {
-      g.w[u] = *(const u32x4*)(base + off[u]);
-      if (F8) g.s[u] = *(scale + x.tok + off_s[u]);
+      const uint32_t piece = min(tid + u * Sh::kThreads, Sh::kPieces - 1);
+      g.w[u] = *(const u32x4*)(base + 16 * piece);
+      if (F8) g.s[u] = *(scale + x.tok + piece / CH);
     }
   };
   // The same of a tile that may hold fewer tokens: rows past the last repeat it.
@@ -283,25 +332,26 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       if (F8) g.s[u] = scale[row];
     }
   };
-  // Writes them to an LDS slot; with `bad`, notes an infinity or a NaN there.
-  auto store_tile = [&](char* slot, int stride, const Regs& g, int* bad)
+  // Writes them to an LDS slot of K or V; with `bad`, notes an infinity or a NaN there.
+  auto store_tile = [&](bool is_v, int slot, const Regs& g, int* bad)
                         __attribute__((always_inline)) {
+    char* to = (is_v ? s_v : s_k) + slot * Sh::kTile;
 #pragma unroll
     for (int u = 0; u < LD; ++u) {
       const int piece = tid + u * Sh::kThreads;
       if (Sh::kPieces % Sh::kThreads != 0 && piece >= Sh::kPieces) continue;
       const int t = piece / CH;
       const int c = piece - t * CH;
+      const int sw = is_v ? prompt_v_swap(D, t) : prompt_k_swap(D, t);
       if constexpr (F8) {
-        char* at = slot + t * stride + 32 * c;
         const float sc = __builtin_bit_cast(float, g.s[u] << 23);
         const u32x4 a = cvt8_fp8(g.w[u][0], g.w[u][1], sc);
         const u32x4 b = cvt8_fp8(g.w[u][2], g.w[u][3], sc);
-        *(u32x4*)at = a;
-        *(u32x4*)(at + 16) = b;
+        *(u32x4*)(to + t * Sh::kRow + 16 * ((2 * c) ^ sw)) = a;
+        *(u32x4*)(to + t * Sh::kRow + 16 * ((2 * c + 1) ^ sw)) = b;
         if (bad && (any_nonfinite(a) || any_nonfinite(b))) *bad = 1;
       } else {
-        *(u32x4*)(slot + t * stride + 16 * c) = g.w[u];
+        *(u32x4*)(to + t * Sh::kRow + 16 * (c ^ sw)) = g.w[u];
         if (bad && any_nonfinite(g.w[u])) *bad = 1;
       }
     }
@@ -312,16 +362,20 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     return m == neg_inf() ? 0.f : m * p.scale_log2;
   };
   // S^T of a K slot
+  uint32_t ka[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+    ka[ks] = lds_k + n32 * Sh::kRow + 16 * ((2 * ks + h) ^ prompt_k_swap(D, n32));
   auto scores = [&](int slot, f32x16 (&s)[RB]) __attribute__((always_inline)) {
-    const char* kb = s_k + slot * Sh::kKTile + n32 * Sh::kKStride + 16 * h;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) s[rb] = f32x16{};
+    u32x4 a[KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const u32x4 a = *(const u32x4*)(kb + 32 * ks);
+    for (int ks = 0; ks < KS; ++ks) a[ks] = lds_read_b128(ka[ks] + slot * Sh::kTile);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) s[rb] = mfma32x32x16(a, qb[rb][ks], s[rb]);
-    }
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) s[rb] = mfma32x32x16(a[ks], qb[rb][ks], s[rb]);
   };
   // P of tile blk from its scores; alpha: the factor of the sums so far (1: none)
   auto softmax = [&](auto mask, int blk, bool bad, f32x16 (&s)[RB], u32x4 (&pb)[RB][2],
@@ -365,17 +419,25 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   // transposed
   const int g4 = lane >> 4;
   const int l16 = lane & 15;
-  const uint32_t va = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_v +
-                      (4 * (g4 >> 1) + (l16 >> 2)) * Sh::kVStride + 32 * (g4 & 1) + 8 * (l16 & 3);
+  uint32_t va[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    const int row = 4 * (g4 >> 1) + (l16 >> 2);  // (its swap is that of rows 8 k away)
+    va[d] = lds_v + row * Sh::kRow + 8 * (l16 & 1) +
+            16 * ((4 * d + 2 * (g4 & 1) + ((l16 & 3) >> 1)) ^ prompt_v_swap(D, row));
+  }
+  auto values_operand = [&](int slot, int ks, int d) __attribute__((always_inline)) {
+    const uint32_t at = va[d] + slot * Sh::kTile + 16 * ks * Sh::kRow;
+    const uint2 x = lds_read_tr_b64(at);
+    const uint2 y = lds_read_tr_b64(at + 8 * Sh::kRow);
+    return u32x4{x.x, x.y, y.x, y.y};
+  };
   auto values = [&](int slot, const u32x4 (&pb)[RB][2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const uint32_t at = va + slot * Sh::kVTile + 16 * ks * Sh::kVStride + 64 * d;
-        const uint2 x = lds_read_tr_b64(at);
-        const uint2 y = lds_read_tr_b64(at + 8 * Sh::kVStride);
-        const u32x4 a = {x.x, x.y, y.x, y.y};
+        const u32x4 a = values_operand(slot, ks, d);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) acc[rb][d] = mfma32x32x16(a, pb[rb][ks], acc[rb][d]);
       }
@@ -392,10 +454,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
         f32x16 pos{}, neg{};
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          const uint32_t at = va + slot * Sh::kVTile + 16 * ks * Sh::kVStride + 64 * d;
-          const uint2 x = lds_read_tr_b64(at);
-          const uint2 y = lds_read_tr_b64(at + 8 * Sh::kVStride);
-          u32x4 fin = {x.x, x.y, y.x, y.y}, ap, an, vis;
+          u32x4 fin = values_operand(slot, ks, d), ap, an, vis;
           // vis: 1 for the k slots (tokens 0 .. 3 and 8 .. 11 past 16 ks + 4 h) that are seen
           const int seen = lim[rb] - blk * kPromptTile - 16 * ks - 4 * h;
 #pragma unroll
@@ -425,11 +484,14 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     bool moved = false;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) moved |= alpha[rb] != 1.f;
-    if (__builtin_amdgcn_ballot_w64(moved) == 0) return;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(moved) == 0, 1)) return;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int rb = 0; rb < RB; ++rb) {
+      float f = alpha[rb];
+      asm("" : "+v"(f));  // (else the products are taken every step, ahead of the test)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) acc[rb][d] = acc[rb][d] * alpha[rb];
+      for (int d = 0; d < DT; ++d) acc[rb][d] = acc[rb][d] * f;
+    }
   };
 
   // Tiles that every row sees whole, in the pipeline: [blk0, blkm).
@@ -439,55 +501,78 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     const int T = blkm - blk0;
     f32x16 s[2][RB];
     u32x4 pb[2][RB][2];
-    Regs kg[2], vg[2];
-    // places of tiles t .. t + 3 (a page id is requested four steps before its use)
-    Place pl[4] = {place_of(blk0), place_of(blk0 + 1), place_of(blk0 + 2), place_of(blk0 + 3)};
-    load_tile(p.k_pages, p.k_scale, pl[0], kg[0]);
-    load_tile(p.k_pages, p.k_scale, pl[1], kg[1]);
+    Regs kg[2], vg[2];  // (8-bit)
+    // places of tiles t .. t + 4 (a page id is requested a step before its use)
+    Place pl[5] = {place_of(blk0), place_of(blk0 + 1), place_of(blk0 + 2), place_of(blk0 + 3),
+                   place_of(blk0 + 4)};
+    // tile t of K (V) into slot t & 3, in the order of the steps that read them
+    if constexpr (F8) {
+      load_tile(p.k_pages, p.k_scale, pl[0], kg[0]);
+      load_tile(p.k_pages, p.k_scale, pl[1], kg[1]);
+      store_tile(false, 0, kg[0], nullptr);
+      store_tile(false, 1, kg[1], nullptr);
+      load_tile(p.k_pages, p.k_scale, pl[2], kg[0]);
+      load_tile(p.v_pages, p.v_scale, pl[0], vg[0]);
+      load_tile(p.k_pages, p.k_scale, pl[3], kg[1]);
+      load_tile(p.v_pages, p.v_scale, pl[1], vg[1]);
+    } else {
+      dma_tile(p.k_pages, pl[0], dma_k, lds_k);
+      dma_tile(p.k_pages, pl[1], dma_k, lds_k + Sh::kTile);
+      dma_tile(p.k_pages, pl[2], dma_k, lds_k + 2 * Sh::kTile);
+      dma_tile(p.v_pages, pl[0], dma_v, lds_v);
+      dma_tile(p.k_pages, pl[3], dma_k, lds_k + 3 * Sh::kTile);
+      dma_tile(p.v_pages, pl[1], dma_v, lds_v + Sh::kTile);
+    }
     // the values of "tile -1", which step 0 adds with weights of 0
-    for (int i = tid; i < Sh::kVTile / 16; i += Sh::kThreads)
-      ((u32x4*)(s_v + Sh::kVTile))[i] = u32x4{0, 0, 0, 0};
+    for (int i = tid; i < Sh::kTile / 16; i += Sh::kThreads)
+      ((u32x4*)(s_v + 3 * Sh::kTile))[i] = u32x4{0, 0, 0, 0};
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) pb[1][rb][0] = pb[1][rb][1] = u32x4{0, 0, 0, 0};
-    store_tile(s_k, Sh::kKStride, kg[0], nullptr);
-    store_tile(s_k + Sh::kKTile, Sh::kKStride, kg[1], nullptr);
-    load_tile(p.k_pages, p.k_scale, pl[2], kg[0]);
-    load_tile(p.v_pages, p.v_scale, pl[0], vg[0]);
-    load_tile(p.k_pages, p.k_scale, pl[3], kg[1]);
-    load_tile(p.v_pages, p.v_scale, pl[1], vg[1]);
+    if (!F8) wait_loads<4 * LQ>();
     __syncthreads();
     scores(0, s[0]);
     __syncthreads();
-    auto step = [&](auto par, int t) __attribute__((always_inline)) {
-      constexpr int c = decltype(par)::value;  // t & 1
+    auto step = [&](auto slot, int t) __attribute__((always_inline)) {
+      constexpr int c = decltype(slot)::value;  // t & 3
+      constexpr int u = c & 1;
       bad_page |= pl[0].bad;
-      store_tile(s_k + c * Sh::kKTile, Sh::kKStride, kg[c], nullptr);
-      store_tile(s_v + c * Sh::kVTile, Sh::kVStride, vg[c], nullptr);
-      pl[0] = pl[1];
-      pl[1] = pl[2];
-      pl[2] = pl[3];
-      pl[3] = place_of(blk0 + t + 4);
-      load_tile(p.k_pages, p.k_scale, pl[3], kg[c]);
-      load_tile(p.v_pages, p.v_scale, pl[1], vg[c]);
+      if constexpr (F8) {  // K of tile t + 2 and V of t; K of t + 4 and V of t + 2 requested
+        store_tile(false, c ^ 2, kg[u], nullptr);
+        store_tile(true, c, vg[u], nullptr);
+        load_tile(p.k_pages, p.k_scale, pl[4], kg[u]);
+        load_tile(p.v_pages, p.v_scale, pl[2], vg[u]);
+      } else {
+        dma_tile(p.k_pages, pl[4], dma_k, lds_k + c * Sh::kTile);
+        dma_tile(p.v_pages, pl[2], dma_v, lds_v + (c ^ 2) * Sh::kTile);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pl[i] = pl[i + 1];
+      pl[4] = place_of(blk0 + t + 5);
       float alpha[RB];
-      scores(c ^ 1, s[c ^ 1]);
-      softmax(std::false_type{}, 0, false, s[c], pb[c], alpha);
-      values(c ^ 1, pb[c ^ 1]);
+      scores((c + 1) & 3, s[u ^ 1]);
+      softmax(std::false_type{}, 0, false, s[u], pb[u], alpha);
+      values((c + 3) & 3, pb[u ^ 1]);
       rescale(alpha);
+      if (!F8) wait_loads<4 * LQ>();  // those of this step and the one before may go on
       __syncthreads();
     };
     int t = 0;
 #pragma unroll 1
-    for (; t + 2 <= T; t += 2) {
+    for (; t + 4 <= T; t += 4) {
       step(std::integral_constant<int, 0>{}, t);
       step(std::integral_constant<int, 1>{}, t + 1);
+      step(std::integral_constant<int, 2>{}, t + 2);
+      step(std::integral_constant<int, 3>{}, t + 3);
     }
-    if (t < T) {
-      step(std::integral_constant<int, 0>{}, t);
-      values(0, pb[0]);
-    } else {
-      values(1, pb[1]);
-    }
+    if (t < T) step(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < T) step(std::integral_constant<int, 1>{}, t + 1);
+    if (t + 2 < T) step(std::integral_constant<int, 2>{}, t + 2);
+    const int last = (T - 1) & 3;
+    if (last & 1)
+      values(last, pb[1]);
+    else
+      values(last, pb[0]);
+    if (!F8) wait_loads<0>();  // the tiles past the last, which nothing reads
   }
   // The others, masked, one after the other.
   if (blkm < blk1) {
@@ -501,9 +586,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
 #pragma unroll 1
     for (int blk = blkm; blk < blk1; ++blk) {
       const bool bad = nx.bad;
-      store_tile(s_k + c * Sh::kKTile, Sh::kKStride, kg, nullptr);
+      store_tile(false, c, kg, nullptr);
       // (s_bad stays set: the slow sum is right for any tile)
-      store_tile(s_v + c * Sh::kVTile, Sh::kVStride, vg, &s_bad[c]);
+      store_tile(true, c, vg, &s_bad[c]);
       nx = place_of(blk + 1);
       load_last(p.k_pages, p.k_scale, nx, kg);
       load_last(p.v_pages, p.v_scale, nx, vg);
