@@ -77,6 +77,21 @@ struct PromptParams {
   uint32_t q_sign;   // 0x80008000 where the caller's scale is negative
 };
 
+// Holds a value's computation between the sched_barriers around it: values that no
+// memory access needs are otherwise placed by the compiler.
+template <class T>
+__device__ __forceinline__ void pin(T& x) {
+  asm volatile("" : "+v"(x));
+}
+// The same of an output's sums, which lie in the accumulation registers in the kernels
+// that take more than 256 registers.
+template <bool ACC>
+__device__ __forceinline__ void pin_sum(f32x16& x) {
+  if constexpr (ACC)
+    asm volatile("" : "+a"(x));
+  else
+    asm volatile("" : "+v"(x));
+}
 __device__ __forceinline__ u32x4 lds_read_b128(uint32_t addr) {
   return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)addr;
 }
@@ -200,6 +215,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   constexpr int CH = Sh::kRowPieces;
   constexpr int LD = Sh::kLoads;
   constexpr int kRows = 32 * RB * NW;
+  constexpr bool kAcc = D > 128 || NW == 1;  // more than 256 registers
   __shared__ __attribute__((aligned(256))) char s_k[kPromptSlots * Sh::kTile];
   __shared__ __attribute__((aligned(256))) char s_v[kPromptSlots * Sh::kTile];
   __shared__ int s_bad[2];  // a slot's values held an infinity or a NaN (masked tiles only)
@@ -258,7 +274,10 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     m_run[rb] = neg_inf();
     l_run[rb] = 0.f;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) acc[rb][d] = f32x16{};
+    for (int d = 0; d < DT; ++d) {
+      acc[rb][d] = f32x16{};
+      pin_sum<kAcc>(acc[rb][d]);
+    }
   }
 
   // A tile's place: pool token index of its first token, its last row that holds a
@@ -268,18 +287,40 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     int last;
     bool bad;
   };
-  auto place_of = [&](int blk) __attribute__((always_inline)) {
-    const int t = min(blk, blk1 - 1) * kPromptTile;  // (< len)
-    const int page = t / p.page_size;
+  // The page id is requested (next_page) a step before it is used (place): tiles are asked
+  // for one after the other, the page and the place in it carried along; past the last
+  // tile it is the last one again.
+  struct PageRef {
+    int raw, off, t;
+  };
+  int at_blk, at_page, at_off;
+  auto seek = [&](int blk) __attribute__((always_inline)) {
+    at_blk = blk;
+    at_page = blk * kPromptTile / p.page_size;
+    at_off = blk * kPromptTile - at_page * p.page_size;
+  };
+  auto next_page = [&]() __attribute__((always_inline)) {
+    PageRef r;
     // a scalar load (the constant address space): a vector load's result would be
     // waited for together with the tiles under way
-    const int raw = ((const ConstInt*)p.page_table)[(size_t)tl.b * p.max_pages + page];
-    const int pid = clamp_page(raw, p.num_pages);
+    r.raw = ((const ConstInt*)p.page_table)[(size_t)tl.b * p.max_pages + at_page];
+    r.off = at_off;
+    r.t = at_blk * kPromptTile;  // (< len)
+    const int more = at_blk + 1 < blk1 ? 1 : 0;
+    at_blk += more;
+    at_off += more * kPromptTile;
+    const int wrap = at_off == p.page_size ? 1 : 0;
+    at_off = wrap ? 0 : at_off;
+    at_page += wrap;
+    return r;
+  };
+  auto place = [&](const PageRef& r) __attribute__((always_inline)) {
+    const int pid = clamp_page(r.raw, p.num_pages);
     Place x;
     x.tok = ((uint32_t)pid * (uint32_t)p.Hkv + (uint32_t)kvh) * (uint32_t)p.page_size +
-            (uint32_t)(t - page * p.page_size);
-    x.last = min(31, len - 1 - t);
-    x.bad = raw != pid;
+            (uint32_t)r.off;
+    x.last = min(31, len - 1 - r.t);
+    x.bad = r.raw != pid;
     return x;
   };
   const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_k;
@@ -377,37 +418,43 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) s[rb] = mfma32x32x16(a[ks], qb[rb][ks], s[rb]);
   };
-  // P of tile blk from its scores; alpha: the factor of the sums so far (1: none)
-  auto softmax = [&](auto mask, int blk, bool bad, f32x16 (&s)[RB], u32x4 (&pb)[RB][2],
+  // a lane's largest score of a tile
+  auto row_max = [&](const f32x16& s) __attribute__((always_inline)) {
+    float bm = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) bm = fmaxf(bm, s[i]);
+    return bm;
+  };
+  // moves the row's running maximum; the factor of the sums so far (1: it stays)
+  auto new_max = [&](int rb, float bm) __attribute__((always_inline)) {
+    float lo, hi;
+    pair_xor32(bm, lo, hi);
+    bm = fmaxf(lo, hi);
+    // (-inf - -inf is NaN, and no reason to move)
+    const bool move = (bm - m_run[rb]) * p.scale_log2 > kLazyRescaleLog2;
+    const float m_new = move ? bm : m_run[rb];
+    const float f = move ? __builtin_amdgcn_exp2f((m_run[rb] - m_new) * p.scale_log2) : 1.f;
+    m_run[rb] = m_new;
+    return f;
+  };
+  // P of the masked tile blk from its scores; alpha: the factor of the sums so far
+  auto softmax_masked = [&](int blk, bool bad, f32x16 (&s)[RB], u32x4 (&pb)[RB][2],
                      float (&alpha)[RB]) __attribute__((always_inline)) {
-    constexpr bool MASKED = decltype(mask)::value;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const int seen = lim[rb] - blk * kPromptTile;  // tokens of the tile that the row sees
-      if (MASKED) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = bad ? qnan() : s[rb][i];
-          s[rb][i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? x : neg_inf();
-        }
+      for (int i = 0; i < 16; ++i) {
+        const float x = bad ? qnan() : s[rb][i];
+        s[rb][i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? x : neg_inf();
       }
-      float bm = s[rb][0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) bm = fmaxf(bm, s[rb][i]);
-      float lo, hi;
-      pair_xor32(bm, lo, hi);
-      bm = fmaxf(lo, hi);
-      // (-inf - -inf is NaN, and no reason to move)
-      const bool move = (bm - m_run[rb]) * p.scale_log2 > kLazyRescaleLog2;
-      const float m_new = move ? bm : m_run[rb];
-      alpha[rb] = move ? __builtin_amdgcn_exp2f((m_run[rb] - m_new) * p.scale_log2) : 1.f;
-      m_run[rb] = m_new;
-      const float mc = ref(m_new);
+      alpha[rb] = new_max(rb, row_max(s[rb]));
+      const float mc = ref(m_run[rb]);
       float ps = 0.f, e[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         e[i] = __builtin_amdgcn_exp2f(fmaf(s[rb][i], p.scale_log2, -mc));
-        if (MASKED) e[i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? e[i] : 0.f;
+        e[i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? e[i] : 0.f;
         ps += e[i];
       }
 #pragma unroll
@@ -490,7 +537,10 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       float f = alpha[rb];
       asm("" : "+v"(f));  // (else the products are taken every step, ahead of the test)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) acc[rb][d] = acc[rb][d] * f;
+      for (int d = 0; d < DT; ++d) {
+        acc[rb][d] = acc[rb][d] * f;
+        pin_sum<kAcc>(acc[rb][d]);
+      }
     }
   };
 
@@ -502,9 +552,15 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     f32x16 s[2][RB];
     u32x4 pb[2][RB][2];
     Regs kg[2], vg[2];  // (8-bit)
-    // places of tiles t .. t + 4 (a page id is requested a step before its use)
-    Place pl[5] = {place_of(blk0), place_of(blk0 + 1), place_of(blk0 + 2), place_of(blk0 + 3),
-                   place_of(blk0 + 4)};
+    // places of tiles t .. t + 4, and the page of t + 5
+    seek(blk0);
+    PageRef ahead[6];
+    Place pl[5];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) ahead[i] = next_page();
+#pragma unroll
+    for (int i = 0; i < 5; ++i) pl[i] = place(ahead[i]);
+    PageRef nx = ahead[5];
     // tile t of K (V) into slot t & 3, in the order of the steps that read them
     if constexpr (F8) {
       load_tile(p.k_pages, p.k_scale, pl[0], kg[0]);
@@ -531,6 +587,10 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     if (!F8) wait_loads<4 * LQ>();
     __syncthreads();
     scores(0, s[0]);
+    float alpha[RB];   // of the tile whose softmax is next
+    float m_kept[RB];  // the maximum without that tile's
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) alpha[rb] = new_max(rb, row_max(s[0][rb]));
     __syncthreads();
     auto step = [&](auto slot, int t) __attribute__((always_inline)) {
       constexpr int c = decltype(slot)::value;  // t & 3
@@ -547,12 +607,84 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) pl[i] = pl[i + 1];
-      pl[4] = place_of(blk0 + t + 5);
-      float alpha[RB];
-      scores((c + 1) & 3, s[u ^ 1]);
-      softmax(std::false_type{}, 0, false, s[u], pb[u], alpha);
-      values((c + 3) & 3, pb[u ^ 1]);
+      pl[4] = place(nx);
+      nx = next_page();
+      // The scores of tile t + 1 under the exponentials of tile t, then the values of
+      // tile t - 1 under its sums and the next tile's maximum: one product and its share
+      // of the vector work at a time (sched_barrier keeps the order; the compiler's own
+      // runs the exponentials after the products).
+      constexpr int kExp = 16 * RB / KS > 0 ? (16 * RB + KS - 1) / KS : 1;
+      constexpr int kAhead = DT > 1 ? 3 : 2;  // V operands under way
+      u32x4 a[KS], av[2 * DT];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) a[ks] = lds_read_b128(ka[ks] + ((c + 1) & 3) * Sh::kTile);
+      float mc[RB], ps[RB], bm[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        mc[rb] = ref(m_run[rb]);
+        ps[rb] = 0.f;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          s[u ^ 1][rb] = mfma32x32x16(a[ks], qb[rb][ks], ks == 0 ? f32x16{} : s[u ^ 1][rb]);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) pin_sum<kAcc>(s[u ^ 1][rb]);
+#pragma unroll
+        for (int e = ks * kExp; e < (ks + 1) * kExp && e < 16 * RB; ++e) {
+          float x = s[u][e >> 4][e & 15];
+          pin(x);
+          x = __builtin_amdgcn_exp2f(fmaf(x, p.scale_log2, -mc[e >> 4]));
+          pin(x);
+          s[u][e >> 4][e & 15] = x;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+          if (ks == (KS > kAhead ? KS - kAhead + j : 0))
+            av[j] = values_operand((c + 3) & 3, j / DT, j % DT);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      constexpr int kSum = 8 * RB / (2 * DT) > 0 ? (8 * RB + 2 * DT - 1) / (2 * DT) : 1;
+      float next_alpha[RB];
+#pragma unroll
+      for (int j = 0; j < 2 * DT; ++j) {
+        const int f = j + kAhead;
+        if (f < 2 * DT) av[f] = values_operand((c + 3) & 3, f / DT, f % DT);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          acc[rb][j % DT] = mfma32x32x16(av[j], pb[u ^ 1][rb][j / DT], acc[rb][j % DT]);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) pin_sum<kAcc>(acc[rb][j % DT]);
+#pragma unroll
+        for (int e = j * kSum; e < (j + 1) * kSum && e < 8 * RB; ++e) {
+          const int rb = e >> 3, i = 2 * (e & 7);
+          const float x = s[u][rb][i], y = s[u][rb][i + 1];
+          pin(ps[rb]);
+          ps[rb] += x + y;
+          pin(ps[rb]);
+          uint32_t w = pack_bf16x2(x, y);
+          pin(w);
+          pb[u][rb][i >> 3][(i >> 1) & 3] = w;
+        }
+        if (j == DT) {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) bm[rb] = row_max(s[u ^ 1][rb]);
+        }
+        if (j == 2 * DT - 1) {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            l_run[rb] = l_run[rb] * alpha[rb] + ps[rb];
+            m_kept[rb] = m_run[rb];
+            next_alpha[rb] = new_max(rb, bm[rb]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
       rescale(alpha);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) alpha[rb] = next_alpha[rb];
       if (!F8) wait_loads<4 * LQ>();  // those of this step and the one before may go on
       __syncthreads();
     };
@@ -572,13 +704,17 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       values(last, pb[1]);
     else
       values(last, pb[0]);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) m_run[rb] = m_kept[rb];  // (tile T may hold tokens not seen)
     if (!F8) wait_loads<0>();  // the tiles past the last, which nothing reads
   }
   // The others, masked, one after the other.
   if (blkm < blk1) {
     if (tid < 2) s_bad[tid] = 0;
     Regs kg, vg;
-    Place nx = place_of(blkm);
+    seek(blkm);
+    Place nx = place(next_page());
+    PageRef far = next_page();
     load_last(p.k_pages, p.k_scale, nx, kg);
     load_last(p.v_pages, p.v_scale, nx, vg);
     __syncthreads();
@@ -589,7 +725,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       store_tile(false, c, kg, nullptr);
       // (s_bad stays set: the slow sum is right for any tile)
       store_tile(true, c, vg, &s_bad[c]);
-      nx = place_of(blk + 1);
+      nx = place(far);
+      far = next_page();
       load_last(p.k_pages, p.k_scale, nx, kg);
       load_last(p.v_pages, p.v_scale, nx, vg);
       __syncthreads();
@@ -597,7 +734,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       u32x4 pb[RB][2];
       float alpha[RB];
       scores(c, s);
-      softmax(std::true_type{}, blk, bad, s, pb, alpha);
+      softmax_masked(blk, bad, s, pb, alpha);
       rescale(alpha);
       if (uniform(s_bad[c]))
         values_masked(c, blk, pb);
