@@ -582,7 +582,7 @@ int ws_gqa8_decode_full(const uint16_t* q, const uint8_t* k_pages, const uint8_t
 /*
  * Prompt attention: the new tokens of every sequence over the pages, causal.
  * q [N][Hq][D] bf16, packed: sequence b's n = cu_new[b + 1] - cu_new[b] queries are
- * rows cu_new[b] .. (non-decreasing, within [0, N]); query i stands at position
+ * rows cu_new[b] .. (non-decreasing from 0 to N at the most); query i stands at position
  * kv_len[b] - n + i of the kv_len[b] tokens in the pages (the new ones among them) and
  * sees positions 0 .. its own, so one at a negative position (its tokens are not in
  * this partition) sees nothing: out 0, lse -inf.  Pools as ws_gqa_decode_partial's
@@ -593,14 +593,15 @@ int ws_gqa8_decode_full(const uint16_t* q, const uint8_t* k_pages, const uint8_t
  * cu_new[B]) are not written.  A row that sees a token in a page with an id outside the
  * pool is NaN, and so is every row of a sequence whose length is outside [0, capacity].
  * An infinity or a NaN in a token changes only the rows that see it.
- * max_len bounds kv_len (it sizes the splits); n_splits: workgroups that share a tile's
- * tokens (0: the library's choice, up to 64), with the workspace of ws_gqa_prompt_plan
- * (none for one split).
+ * n_splits: workgroups that share the tokens of a tile of rows (1 to 64; 0: the
+ * library's choice, which splits where the tiles do not fill the device, by the
+ * lengths).  max_len bounds kv_len.  Workspace: ws_gqa_prompt_plan's bytes for the same
+ * sizes (0: none); pieces_out: how many pieces the split tiles can leave.
  * The reference runs prompts through its framework's attention (chunks:
  * system/deepseek.py:279-322) on dense buffers.
  */
 int ws_gqa_prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len, int n_splits,
-                       int* n_splits_out, size_t* workspace_bytes_out);
+                       int* pieces_out, size_t* workspace_bytes_out);
 int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void* v_pages,
                   const uint8_t* k_scale, const uint8_t* v_scale, const int32_t* page_table,
                   const int32_t* kv_len, const int32_t* cu_new, int N, int B, int Hq, int Hkv,

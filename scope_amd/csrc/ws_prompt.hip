@@ -22,8 +22,9 @@
 // (0 * inf): where a tile that some row masks holds one, values_masked adds it to the rows
 // that see it.
 //
-// With few rows the tokens are split over n_splits workgroups per tile, whose pieces
-// (fp32, with their lse) prompt_join_kernel combines.
+// With few rows the tokens are split over several workgroups of a tile, so that all
+// take about as many, whatever the sequences' lengths; prompt_join_kernel combines
+// their pieces (fp32, with their lse).
 #include <algorithm>
 #include <type_traits>
 
@@ -70,9 +71,12 @@ struct PromptParams {
   uint16_t* out_bf16;
   float* out_f32;
   float* lse;
-  float* part_out;  // [n_splits][N * Hq][D], with part_lse when n_splits > 1
+  float* part_out;  // [pieces][rows of a tile][D], with part_lse [pieces][rows]
   float* part_lse;
-  int N, B, Hq, Hkv, G, page_size, max_pages, num_pages, cap, n_splits, tiles;
+  int N, B, Hq, Hkv, G, page_size, max_pages, num_pages, cap;
+  int n_splits;  // of every tile; 0: by the lengths, `share` workgroups in all (0: one a tile)
+  int share;
+  long long pieces;  // room for them
   float scale_log2;  // >= 0
   uint32_t q_sign;   // 0x80008000 where the caller's scale is negative
 };
@@ -129,41 +133,105 @@ __device__ __forceinline__ void split_nonfinite(uint32_t& w, uint32_t& pos, uint
   w &= ~(lo * 0xffffu);
 }
 
-struct PromptTile {
-  int b, tile;  // sequence and tile of its rows (b < 0: none)
-  int c0, n;    // the sequence's first row of q and its tokens
+// A workgroup's place in the list of all sequences' tiles of `rows` rows (of the tiles
+// alone, or of every tile's splits).
+struct PromptPlace {
+  int b;              // the sequence (< 0: past the list's end)
+  int tile;           // tile of its rows
+  int split, splits;  // and which of the tile's splits
+  int piece;          // the split's piece, less the KV head: (piece * Hkv + kvh)
+  int c0, n;          // the sequence's first row of q and its tokens
+  int len;
 };
-
-// Tile `t` of the list of all sequences' tiles of `rows` rows.  Every lane must
-// call it; the result is uniform.
-__device__ __forceinline__ int prompt_tokens(const PromptParams& p, int b, int& c0) {
-  c0 = min(max(p.cu_new[b], 0), p.N);
-  return min(max(p.cu_new[b + 1], c0), p.N) - c0;
+// What the list needs of a sequence.
+struct PromptSeq {
+  int c0, n, len, tiles, blocks;
+};
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b, int rows) {
+  PromptSeq s;
+  s.c0 = min(max(p.cu_new[b], 0), p.N);
+  s.n = min(max(p.cu_new[b + 1], s.c0), p.N) - s.c0;
+  s.len = p.kv_len[b];
+  s.tiles = (s.n * p.G + rows - 1) / rows;
+  s.blocks = len_ok(s.len, 0, p.cap) ? (s.len + kPromptTile - 1) / kPromptTile : 0;
+  return s;
 }
-__device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int t, int rows) {
+constexpr int kPromptMinShare = 8;  // tiles of tokens of a split, at the least
+
+// Item `at` of the list: longest sequences first (up to 64 of them), their last tile
+// first, since it walks the most tokens: the short ones fill the chip's end.  The splits
+// of a sequence's tiles: as many as give each `per_split` tiles of tokens, the batch's
+// total over `share` workgroups (computed alike by every caller).  Every lane must call
+// it; the result is uniform.
+template <bool TILES>
+__device__ __forceinline__ PromptPlace prompt_place(const PromptParams& p, int at, int rows) {
   const int lane = threadIdx.x & 63;
   const int per = (p.B + 63) >> 6;
   const int b0 = lane * per;
-  int sum = 0, c0;
-  for (int k = 0; k < per; ++k)
-    if (b0 + k < p.B) sum += (prompt_tokens(p, b0 + k, c0) * p.G + rows - 1) / rows;
-  const int incl = __ockl_wfscan_add_i32(sum, true);
-  const uint64_t past = __builtin_amdgcn_ballot_w64(incl > t);
-  PromptTile r{-1, 0, 0, 0};
+  int per_split = 0;
+  if (p.share > 0) {
+    float total = 0.f;
+    for (int k = 0; k < per && b0 + k < p.B; ++k) {
+      const PromptSeq s = prompt_seq(p, b0 + k, rows);
+      total += (float)s.tiles * (float)s.blocks;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+    per_split = max((int)min(total * (float)p.Hkv / (float)p.share, 1e9f) + 1, kPromptMinShare);
+  }
+  auto splits_of = [&](const PromptSeq& s) {
+    if (p.share == 0) return max(p.n_splits, 1);
+    return max(min((s.blocks + per_split - 1) / per_split, kPromptMaxSplits), 1);
+  };
+  // a lane's items, and the pieces before its first sequence in the batch's order
+  int items = 0, units = 0, key = -1;
+  for (int k = 0; k < per && b0 + k < p.B; ++k) {
+    const PromptSeq s = prompt_seq(p, b0 + k, rows);
+    units += s.tiles * splits_of(s);
+    items += TILES ? s.tiles : s.tiles * splits_of(s);
+    key = s.blocks;
+  }
+  const int before = __ockl_wfscan_add_i32(units, true) - units;
+  int from = lane;  // the lane whose sequences stand at this lane's place in the list
+  if (!TILES && per == 1 && p.B > 1) {
+    int rank = 0;
+    for (int j = 0; j < p.B; ++j) {
+      const int other = __builtin_amdgcn_readlane(key, j);
+      rank += other > key || (other == key && j < lane) ? 1 : 0;
+    }
+    if (lane >= p.B) rank = lane;
+    from = __builtin_amdgcn_ds_permute(4 * rank, lane);
+    items = __builtin_amdgcn_ds_permute(4 * rank, items);
+  }
+  const int incl = __ockl_wfscan_add_i32(items, true);
+  const uint64_t past = __builtin_amdgcn_ballot_w64(incl > at);
+  PromptPlace r{-1, 0, 0, 1, 0, 0, 0, 0};
   if (past == 0) return r;
-  const int at = __builtin_ctzll(past);
-  int left = t - __builtin_amdgcn_readlane(incl - sum, at);
+  const int slot = __builtin_ctzll(past);
+  int left = at - __builtin_amdgcn_readlane(incl - items, slot);
+  const int owner = __builtin_amdgcn_readlane(from, slot);
+  int piece = __builtin_amdgcn_readlane(before, owner);
   for (int k = 0; k < per; ++k) {
-    const int b = uniform(at * per + k);
+    const int b = uniform(owner * per + k);
     if (b >= p.B) break;
-    const int n = uniform(prompt_tokens(p, b, c0));
-    const int tiles = (n * p.G + rows - 1) / rows;
-    if (left < tiles) {
-      // the last tile first: it walks the most tokens
-      r = PromptTile{b, tiles - 1 - left, uniform(c0), n};
+    const PromptSeq s = prompt_seq(p, b, rows);
+    const int splits = uniform(splits_of(s));
+    const int here = uniform(TILES ? s.tiles : s.tiles * splits);
+    if (left < 0) break;  // (sums past 2^31: cu_new is not non-decreasing)
+    if (left < here) {
+      const int t = TILES ? left : left / splits;
+      r.b = b;
+      r.tile = TILES ? t : uniform(s.tiles) - 1 - t;
+      r.split = TILES ? 0 : left - t * splits;
+      r.splits = splits;
+      r.piece = piece + r.tile * splits + r.split;
+      r.c0 = uniform(s.c0);
+      r.n = uniform(s.n);
+      r.len = uniform(s.len);
       break;
     }
-    left -= tiles;
+    left -= here;
+    piece += uniform(s.tiles) * splits;
   }
   return r;
 }
@@ -206,7 +274,7 @@ __device__ __forceinline__ void wait_loads() {
 // and V of t + 2 in step t, to the slots the step before has left); 8-bit ones through
 // registers, requested two steps before they are converted and written.  One barrier a
 // step.
-template <int D, bool F8, int RB, int NW>
+template <int D, bool F8, int NW>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const PromptParams p) {
   static_assert(D % 32 == 0 && D <= kPromptMaxD, "head width: a multiple of 32 up to 256");
   using Sh = PromptShape<D, F8, NW>;
@@ -214,7 +282,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   constexpr int DT = D / 32;  // 32-column tiles of the output
   constexpr int CH = Sh::kRowPieces;
   constexpr int LD = Sh::kLoads;
-  constexpr int kRows = 32 * RB * NW;
+  constexpr int kRows = 32 * NW;
   constexpr bool kAcc = D > 128 || NW == 1;  // more than 256 registers
   __shared__ __attribute__((aligned(256))) char s_k[kPromptSlots * Sh::kTile];
   __shared__ __attribute__((aligned(256))) char s_v[kPromptSlots * Sh::kTile];
@@ -227,13 +295,13 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   const int h = lane >> 5;
   const int id = blockIdx.x;
   const int kvh = id % p.Hkv;
-  const int rest = id / p.Hkv;
-  const int split = rest % p.n_splits;
-  const PromptTile tl = prompt_tile(p, rest / p.n_splits, kRows);
-  if (tl.b < 0) return;
+  const PromptPlace tl = prompt_place<false>(p, id / p.Hkv, kRows);
+  const bool piece = tl.splits > 1;
+  const long long piece_at = (long long)tl.piece * p.Hkv + kvh;
+  if (tl.b < 0 || (piece && (piece_at < 0 || piece_at >= p.pieces))) return;
   const int G = p.G;
   const int R = tl.n * G;  // rows of the sequence and KV head
-  const int len = uniform(p.kv_len[tl.b]);
+  const int len = tl.len;
   const bool len_good = len_ok(len, 0, p.cap);
   const int first_pos = len - tl.n;  // position of the sequence's first query
   const int row0 = tl.tile * kRows;
@@ -242,42 +310,33 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   const int lim_lo = first_pos + row0 / G + 1;
   const int lim_hi = len_good ? max(first_pos + (row0 + rows_here - 1) / G + 1, 0) : 0;
   const int nb = (lim_hi + kPromptTile - 1) / kPromptTile;
-  const int blk0 = (int)((long long)split * nb / p.n_splits);
-  const int blk1 = (int)((long long)(split + 1) * nb / p.n_splits);
+  const int blk0 = (int)((long long)tl.split * nb / tl.splits);
+  const int blk1 = (int)((long long)(tl.split + 1) * nb / tl.splits);
 
-  // the wave's rows
-  int lim[RB];         // visible tokens of the lane's row
-  size_t out_row[RB];  // its row of out / lse
-  bool live[RB];
-  u32x4 qb[RB][KS];
+  // the lane's row, the tokens it sees, and its row of out / lse
+  const int tile_row = wave * 32 + n32;
+  const bool live = row0 + tile_row < R;
+  const int r = min(row0 + tile_row, R - 1);
+  const int i = r / G;
+  const int lim = first_pos + i + 1;
+  const size_t out_row = (size_t)(tl.c0 + i) * p.Hq + kvh * G + (r - i * G);
+  u32x4 qb[KS];
+  const u32x4* qp = (const u32x4*)(p.q + out_row * D);
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int r = row0 + (wave * RB + rb) * 32 + n32;
-    live[rb] = r < R;
-    const int rr = min(r, R - 1);
-    const int i = rr / G;
-    lim[rb] = first_pos + i + 1;
-    out_row[rb] = (size_t)(tl.c0 + i) * p.Hq + kvh * G + (rr - i * G);
-    const u32x4* qp = (const u32x4*)(p.q + out_row[rb] * D);
+  for (int s = 0; s < KS; ++s) {
+    qb[s] = qp[2 * s + h];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      qb[rb][s] = qp[2 * s + h];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) qb[rb][s][e] ^= p.q_sign;
-    }
+    for (int e = 0; e < 4; ++e) qb[s][e] ^= p.q_sign;
   }
 
-  f32x16 acc[RB][DT];
-  float m_run[RB], l_run[RB];
+  f32x16 acc[DT];
+  float m_run, l_run;
+  m_run = neg_inf();
+  l_run = 0.f;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    m_run[rb] = neg_inf();
-    l_run[rb] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      acc[rb][d] = f32x16{};
-      pin_sum<kAcc>(acc[rb][d]);
-    }
+  for (int d = 0; d < DT; ++d) {
+    acc[d] = f32x16{};
+    pin_sum<kAcc>(acc[d]);
   }
 
   // A tile's place: pool token index of its first token, its last row that holds a
@@ -407,16 +466,14 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks)
     ka[ks] = lds_k + n32 * Sh::kRow + 16 * ((2 * ks + h) ^ prompt_k_swap(D, n32));
-  auto scores = [&](int slot, f32x16 (&s)[RB]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) s[rb] = f32x16{};
+  auto scores = [&](int slot, f32x16& s) __attribute__((always_inline)) {
+    s = f32x16{};
     u32x4 a[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) a[ks] = lds_read_b128(ka[ks] + slot * Sh::kTile);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) s[rb] = mfma32x32x16(a[ks], qb[rb][ks], s[rb]);
+      s = mfma32x32x16(a[ks], qb[ks], s);
   };
   // a lane's largest score of a tile
   auto row_max = [&](const f32x16& s) __attribute__((always_inline)) {
@@ -426,41 +483,38 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     return bm;
   };
   // moves the row's running maximum; the factor of the sums so far (1: it stays)
-  auto new_max = [&](int rb, float bm) __attribute__((always_inline)) {
+  auto new_max = [&](float bm) __attribute__((always_inline)) {
     float lo, hi;
     pair_xor32(bm, lo, hi);
     bm = fmaxf(lo, hi);
     // (-inf - -inf is NaN, and no reason to move)
-    const bool move = (bm - m_run[rb]) * p.scale_log2 > kLazyRescaleLog2;
-    const float m_new = move ? bm : m_run[rb];
-    const float f = move ? __builtin_amdgcn_exp2f((m_run[rb] - m_new) * p.scale_log2) : 1.f;
-    m_run[rb] = m_new;
+    const bool move = (bm - m_run) * p.scale_log2 > kLazyRescaleLog2;
+    const float m_new = move ? bm : m_run;
+    const float f = move ? __builtin_amdgcn_exp2f((m_run - m_new) * p.scale_log2) : 1.f;
+    m_run = m_new;
     return f;
   };
   // P of the masked tile blk from its scores; alpha: the factor of the sums so far
-  auto softmax_masked = [&](int blk, bool bad, f32x16 (&s)[RB], u32x4 (&pb)[RB][2],
-                     float (&alpha)[RB]) __attribute__((always_inline)) {
+  auto softmax_masked = [&](int blk, bool bad, f32x16& s, u32x4 (&pb)[2],
+                     float& alpha) __attribute__((always_inline)) {
+    const int seen = lim - blk * kPromptTile;  // tokens of the tile that the row sees
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const int seen = lim[rb] - blk * kPromptTile;  // tokens of the tile that the row sees
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float x = bad ? qnan() : s[rb][i];
-        s[rb][i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? x : neg_inf();
-      }
-      alpha[rb] = new_max(rb, row_max(s[rb]));
-      const float mc = ref(m_run[rb]);
-      float ps = 0.f, e[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(fmaf(s[rb][i], p.scale_log2, -mc));
-        e[i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? e[i] : 0.f;
-        ps += e[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) pb[rb][i >> 3][(i >> 1) & 3] = pack_bf16x2(e[i], e[i + 1]);
-      l_run[rb] = l_run[rb] * alpha[rb] + ps;
+    for (int i = 0; i < 16; ++i) {
+      const float x = bad ? qnan() : s[i];
+      s[i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? x : neg_inf();
     }
+    alpha = new_max(row_max(s));
+    const float mc = ref(m_run);
+    float ps = 0.f, e[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale_log2, -mc));
+      e[i] = 8 * (i >> 2) + 4 * h + (i & 3) < seen ? e[i] : 0.f;
+      ps += e[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) pb[i >> 3][(i >> 1) & 3] = pack_bf16x2(e[i], e[i + 1]);
+    l_run = l_run * alpha + ps;
   };
   // O^T += V^T P^T of a V slot: lane group g4 of 16 lanes reads 4 tokens x 16 columns
   // transposed
@@ -479,68 +533,59 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     const uint2 y = lds_read_tr_b64(at + 8 * Sh::kRow);
     return u32x4{x.x, x.y, y.x, y.y};
   };
-  auto values = [&](int slot, const u32x4 (&pb)[RB][2]) __attribute__((always_inline)) {
+  auto values = [&](int slot, const u32x4 (&pb)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const u32x4 a = values_operand(slot, ks, d);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) acc[rb][d] = mfma32x32x16(a, pb[rb][ks], acc[rb][d]);
+        acc[d] = mfma32x32x16(a, pb[ks], acc[d]);
       }
   };
   // The same where the slot holds an infinity or a NaN that some rows do not see: the
   // finite values' product, and from two products of 0 and 1 whether a row sees an
   // infinity of either sign (a NaN counts as both) in a column.
-  auto values_masked = [&](int slot, int blk, const u32x4 (&pb)[RB][2])
+  auto values_masked = [&](int slot, int blk, const u32x4 (&pb)[2])
                            __attribute__((always_inline)) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
+    for (int d = 0; d < DT; ++d) {
+      f32x16 pos{}, neg{};
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        f32x16 pos{}, neg{};
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x4 fin = values_operand(slot, ks, d), ap, an, vis;
+        // vis: 1 for the k slots (tokens 0 .. 3 and 8 .. 11 past 16 ks + 4 h) that are seen
+        const int seen = lim - blk * kPromptTile - 16 * ks - 4 * h;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          u32x4 fin = values_operand(slot, ks, d), ap, an, vis;
-          // vis: 1 for the k slots (tokens 0 .. 3 and 8 .. 11 past 16 ks + 4 h) that are seen
-          const int seen = lim[rb] - blk * kPromptTile - 16 * ks - 4 * h;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t f = fin[e], u, w;
-            split_nonfinite(f, u, w);
-            fin[e] = f;
-            ap[e] = u;
-            an[e] = w;
-            const int t = 8 * (e >> 1) + 2 * (e & 1);
-            vis[e] = (t < seen ? 0x3f80u : 0u) | (t + 1 < seen ? 0x3f800000u : 0u);
-          }
-          acc[rb][d] = mfma32x32x16(fin, pb[rb][ks], acc[rb][d]);
-          pos = mfma32x32x16(ap, vis, pos);
-          neg = mfma32x32x16(an, vis, neg);
+        for (int e = 0; e < 4; ++e) {
+          uint32_t f = fin[e], u, w;
+          split_nonfinite(f, u, w);
+          fin[e] = f;
+          ap[e] = u;
+          an[e] = w;
+          const int t = 8 * (e >> 1) + 2 * (e & 1);
+          vis[e] = (t < seen ? 0x3f80u : 0u) | (t + 1 < seen ? 0x3f800000u : 0u);
         }
+        acc[d] = mfma32x32x16(fin, pb[ks], acc[d]);
+        pos = mfma32x32x16(ap, vis, pos);
+        neg = mfma32x32x16(an, vis, neg);
+      }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (pos[i] > 0.f) acc[rb][d][i] -= neg_inf();
-          if (neg[i] > 0.f) acc[rb][d][i] += neg_inf();
-        }
+      for (int i = 0; i < 16; ++i) {
+        if (pos[i] > 0.f) acc[d][i] -= neg_inf();
+        if (neg[i] > 0.f) acc[d][i] += neg_inf();
       }
     }
   };
   // acc times alpha, where some row's maximum moved
-  auto rescale = [&](const float (&alpha)[RB]) __attribute__((always_inline)) {
-    bool moved = false;
+  auto rescale = [&](const float& alpha) __attribute__((always_inline)) {
+    
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(alpha != 1.f) == 0, 1)) return;
+    float f = alpha;
+    asm("" : "+v"(f));  // (else the products are taken every step, ahead of the test)
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) moved |= alpha[rb] != 1.f;
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(moved) == 0, 1)) return;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      float f = alpha[rb];
-      asm("" : "+v"(f));  // (else the products are taken every step, ahead of the test)
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        acc[rb][d] = acc[rb][d] * f;
-        pin_sum<kAcc>(acc[rb][d]);
-      }
+    for (int d = 0; d < DT; ++d) {
+      acc[d] = acc[d] * f;
+      pin_sum<kAcc>(acc[d]);
     }
   };
 
@@ -549,8 +594,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   bool bad_page = false;  // one of them lies in a bad page: every row is NaN
   if (blk0 < blkm) {
     const int T = blkm - blk0;
-    f32x16 s[2][RB];
-    u32x4 pb[2][RB][2];
+    f32x16 s[2];
+    u32x4 pb[2][2];
     Regs kg[2], vg[2];  // (8-bit)
     // places of tiles t .. t + 4, and the page of t + 5
     seek(blk0);
@@ -582,15 +627,13 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     // the values of "tile -1", which step 0 adds with weights of 0
     for (int i = tid; i < Sh::kTile / 16; i += Sh::kThreads)
       ((u32x4*)(s_v + 3 * Sh::kTile))[i] = u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) pb[1][rb][0] = pb[1][rb][1] = u32x4{0, 0, 0, 0};
+    pb[1][0] = pb[1][1] = u32x4{0, 0, 0, 0};
     if (!F8) wait_loads<4 * LQ>();
     __syncthreads();
     scores(0, s[0]);
-    float alpha[RB];   // of the tile whose softmax is next
-    float m_kept[RB];  // the maximum without that tile's
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) alpha[rb] = new_max(rb, row_max(s[0][rb]));
+    float alpha;   // of the tile whose softmax is next
+    float m_kept;  // the maximum without that tile's
+    alpha = new_max(row_max(s[0]));
     __syncthreads();
     auto step = [&](auto slot, int t) __attribute__((always_inline)) {
       constexpr int c = decltype(slot)::value;  // t & 3
@@ -613,32 +656,26 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       // tile t - 1 under its sums and the next tile's maximum: one product and its share
       // of the vector work at a time (sched_barrier keeps the order; the compiler's own
       // runs the exponentials after the products).
-      constexpr int kExp = 16 * RB / KS > 0 ? (16 * RB + KS - 1) / KS : 1;
+      constexpr int kExp = 16 / KS > 0 ? (16 + KS - 1) / KS : 1;
       constexpr int kAhead = DT > 1 ? 3 : 2;  // V operands under way
       u32x4 a[KS], av[2 * DT];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) a[ks] = lds_read_b128(ka[ks] + ((c + 1) & 3) * Sh::kTile);
-      float mc[RB], ps[RB], bm[RB];
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        mc[rb] = ref(m_run[rb]);
-        ps[rb] = 0.f;
-      }
+      float mc, ps, bm;
+      mc = ref(m_run);
+      ps = 0.f;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
+        s[u ^ 1] = mfma32x32x16(a[ks], qb[ks], ks == 0 ? f32x16{} : s[u ^ 1]);
+        pin_sum<kAcc>(s[u ^ 1]);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-          s[u ^ 1][rb] = mfma32x32x16(a[ks], qb[rb][ks], ks == 0 ? f32x16{} : s[u ^ 1][rb]);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) pin_sum<kAcc>(s[u ^ 1][rb]);
-#pragma unroll
-        for (int e = ks * kExp; e < (ks + 1) * kExp && e < 16 * RB; ++e) {
-          float x = s[u][e >> 4][e & 15];
+        for (int e = ks * kExp; e < (ks + 1) * kExp && e < 16; ++e) {
+          float x = s[u][e];
           pin(x);
-          x = __builtin_amdgcn_exp2f(fmaf(x, p.scale_log2, -mc[e >> 4]));
+          x = __builtin_amdgcn_exp2f(fmaf(x, p.scale_log2, -mc));
           pin(x);
-          s[u][e >> 4][e & 15] = x;
+          s[u][e] = x;
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
@@ -646,45 +683,37 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
             av[j] = values_operand((c + 3) & 3, j / DT, j % DT);
         __builtin_amdgcn_sched_barrier(0);
       }
-      constexpr int kSum = 8 * RB / (2 * DT) > 0 ? (8 * RB + 2 * DT - 1) / (2 * DT) : 1;
-      float next_alpha[RB];
+      constexpr int kSum = 8 / (2 * DT) > 0 ? (8 + 2 * DT - 1) / (2 * DT) : 1;
+      float next_alpha;
 #pragma unroll
       for (int j = 0; j < 2 * DT; ++j) {
         const int f = j + kAhead;
         if (f < 2 * DT) av[f] = values_operand((c + 3) & 3, f / DT, f % DT);
+        acc[j % DT] = mfma32x32x16(av[j], pb[u ^ 1][j / DT], acc[j % DT]);
+        pin_sum<kAcc>(acc[j % DT]);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-          acc[rb][j % DT] = mfma32x32x16(av[j], pb[u ^ 1][rb][j / DT], acc[rb][j % DT]);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) pin_sum<kAcc>(acc[rb][j % DT]);
-#pragma unroll
-        for (int e = j * kSum; e < (j + 1) * kSum && e < 8 * RB; ++e) {
-          const int rb = e >> 3, i = 2 * (e & 7);
-          const float x = s[u][rb][i], y = s[u][rb][i + 1];
-          pin(ps[rb]);
-          ps[rb] += x + y;
-          pin(ps[rb]);
+        for (int e = j * kSum; e < (j + 1) * kSum && e < 8; ++e) {
+          const int i = 2 * e;
+          const float x = s[u][i], y = s[u][i + 1];
+          pin(ps);
+          ps += x + y;
+          pin(ps);
           uint32_t w = pack_bf16x2(x, y);
           pin(w);
-          pb[u][rb][i >> 3][(i >> 1) & 3] = w;
+          pb[u][i >> 3][(i >> 1) & 3] = w;
         }
         if (j == DT) {
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb) bm[rb] = row_max(s[u ^ 1][rb]);
+          bm = row_max(s[u ^ 1]);
         }
         if (j == 2 * DT - 1) {
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb) {
-            l_run[rb] = l_run[rb] * alpha[rb] + ps[rb];
-            m_kept[rb] = m_run[rb];
-            next_alpha[rb] = new_max(rb, bm[rb]);
-          }
+          l_run = l_run * alpha + ps;
+          m_kept = m_run;
+          next_alpha = new_max(bm);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
       rescale(alpha);
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) alpha[rb] = next_alpha[rb];
+      alpha = next_alpha;
       if (!F8) wait_loads<4 * LQ>();  // those of this step and the one before may go on
       __syncthreads();
     };
@@ -704,8 +733,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       values(last, pb[1]);
     else
       values(last, pb[0]);
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) m_run[rb] = m_kept[rb];  // (tile T may hold tokens not seen)
+    m_run = m_kept;  // (tile T may hold tokens not seen)
     if (!F8) wait_loads<0>();  // the tiles past the last, which nothing reads
   }
   // The others, masked, one after the other.
@@ -730,9 +758,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       load_last(p.k_pages, p.k_scale, nx, kg);
       load_last(p.v_pages, p.v_scale, nx, vg);
       __syncthreads();
-      f32x16 s[RB];
-      u32x4 pb[RB][2];
-      float alpha[RB];
+      f32x16 s;
+      u32x4 pb[2];
+      float alpha;
       scores(c, s);
       softmax_masked(blk, bad, s, pb, alpha);
       rescale(alpha);
@@ -745,119 +773,123 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   }
 
   // Outputs: lane half h of a row holds columns 32 d + 8 a + 4 h + b.
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    float lo, hi;
-    pair_xor32(l_run[rb], lo, hi);
-    const float l = lo + hi;
-    if (!live[rb]) continue;
-    const bool none = l == 0.f;
-    const float inv = !len_good || bad_page ? qnan() : none ? 0.f : 1.f / l;
-    const float lse_v = !len_good || bad_page ? qnan()
-                        : none    ? neg_inf()
-                                  : (ref(m_run[rb]) + __log2f(l)) * kLn2;
-    const size_t rows = (size_t)p.N * p.Hq;
-    const bool piece = p.n_splits > 1;
-    const size_t at = piece ? split * rows + out_row[rb] : out_row[rb];
-    if (h == 0) {
-      if (piece) p.part_lse[at] = lse_v;
-      else if (p.lse) p.lse[at] = lse_v;
-    }
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const int col = 32 * d + 8 * a + 4 * h;
-        const float4 o = make_float4(acc[rb][d][4 * a] * inv, acc[rb][d][4 * a + 1] * inv,
-                                     acc[rb][d][4 * a + 2] * inv, acc[rb][d][4 * a + 3] * inv);
-        if (piece) {
-          *(float4*)(p.part_out + at * D + col) = o;
-        } else {
-          if (p.out_f32) *(float4*)(p.out_f32 + at * D + col) = o;
-          if (p.out_bf16)
-            *(uint2*)(p.out_bf16 + at * D + col) =
-                make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
-        }
-      }
+  float l_lo, l_hi;
+  pair_xor32(l_run, l_lo, l_hi);
+  const float l = l_lo + l_hi;
+  if (!live) return;
+  const bool none = l == 0.f;
+  const bool gone = !len_good || bad_page;
+  const float inv = gone ? qnan() : none ? 0.f : 1.f / l;
+  const float lse_v = gone ? qnan() : none ? neg_inf() : (ref(m_run) + __log2f(l)) * kLn2;
+  const size_t at = piece ? (size_t)piece_at * kRows + tile_row : out_row;
+  if (h == 0) {
+    if (piece) p.part_lse[at] = lse_v;
+    else if (p.lse) p.lse[at] = lse_v;
   }
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int col = 32 * d + 8 * a + 4 * h;
+      const float4 o = make_float4(acc[d][4 * a] * inv, acc[d][4 * a + 1] * inv,
+                                   acc[d][4 * a + 2] * inv, acc[d][4 * a + 3] * inv);
+      if (piece) {
+        *(float4*)(p.part_out + at * D + col) = o;
+      } else {
+        if (p.out_f32) *(float4*)(p.out_f32 + at * D + col) = o;
+        if (p.out_bf16)
+          *(uint2*)(p.out_bf16 + at * D + col) =
+              make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
+      }
+    }
 }
 
-// Combines the splits' pieces of a row: D / 4 threads a row.
-__global__ __launch_bounds__(256) void prompt_join_kernel(const PromptParams p, int D) {
+// Combines the pieces of the tiles that were split: a workgroup for kJoinRows rows of a
+// tile and KV head, one thread per four columns.
+constexpr int kJoinRows = 8;
+__global__ __launch_bounds__(256) void prompt_join_kernel(const PromptParams p, int D, int rows) {
+  const int id = blockIdx.x;
+  const int kvh = id % p.Hkv;
+  const PromptPlace tl = prompt_place<true>(p, id / p.Hkv, rows);
+  const long long piece_at = (long long)tl.piece * p.Hkv + kvh;
+  if (tl.b < 0 || tl.splits == 1 || piece_at < 0 ||
+      piece_at + (long long)(tl.splits - 1) * p.Hkv >= p.pieces)
+    return;
+  const int R = tl.n * p.G;
   const int c4 = D >> 2;
-  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-  const size_t rows = (size_t)p.N * p.Hq;
-  const size_t row = (size_t)(t / c4);
-  const int c = (int)(t - (long long)row * c4);
-  if (row >= rows) return;
-  // rows before the first sequence and behind the last are nobody's
-  const int tok = (int)(row / p.Hq);
-  if (tok < p.cu_new[0] || tok >= p.cu_new[p.B]) return;
-  float M = neg_inf();
-  for (int s = 0; s < p.n_splits; ++s) M = max_nan(M, p.part_lse[s * rows + row]);
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  float L = 0.f;
-  if (M != neg_inf())
-    for (int s = 0; s < p.n_splits; ++s) {
-      const float l = p.part_lse[s * rows + row];
-      if (l == neg_inf()) continue;
-      const float w = __expf(l - M);
-      const float4 o = ((const float4*)p.part_out)[(s * rows + row) * c4 + c];
-      L += w;
-      a.x += w * o.x; a.y += w * o.y; a.z += w * o.z; a.w += w * o.w;
-    }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  const float4 o = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-  if (p.out_f32) ((float4*)p.out_f32)[row * c4 + c] = o;
-  if (p.out_bf16)
-    ((uint2*)p.out_bf16)[row * c4 + c] =
-        make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
-  if (p.lse && c == 0) p.lse[row] = L == 0.f ? neg_inf() : M + __logf(L);
+  for (int t = threadIdx.x; t < kJoinRows * c4; t += 256) {
+    const int tr = blockIdx.y * kJoinRows + t / c4;  // row of the tile
+    const int c = t % c4;
+    const int r = tl.tile * rows + tr;
+    if (r >= R) return;
+    const int i = r / p.G;
+    const size_t out_row = (size_t)(tl.c0 + i) * p.Hq + kvh * p.G + (r - i * p.G);
+    const size_t slot = (size_t)piece_at * rows + tr;
+    const size_t step = (size_t)p.Hkv * rows;  // to the row's next piece
+    const PieceAcc x =
+        piece_stream<float4>((const char*)(p.part_out + slot * D + 4 * c), step * D * 4,
+                             p.part_lse + slot, (int)step, 0, 1, tl.splits);
+    const float inv = x.sum == 0.f ? 0.f : 1.f / x.sum;
+    const float4 o = make_float4(x.a.x * inv, x.a.y * inv, x.a.z * inv, x.a.w * inv);
+    if (p.out_f32) ((float4*)p.out_f32)[out_row * c4 + c] = o;
+    if (p.out_bf16)
+      ((uint2*)p.out_bf16)[out_row * c4 + c] =
+          make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
+    if (p.lse && c == 0) p.lse[out_row] = x.sum == 0.f ? neg_inf() : x.m + __logf(x.sum);
+  }
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 static bool prompt_width_ok(int D) { return D >= 32 && D <= kPromptMaxD && D % 32 == 0; }
 
-// How a call runs: rows of a tile and splits of its tokens.
+// How a call runs.
 struct PromptPlan {
-  bool wide;  // four waves a workgroup
-  int rows, tiles, splits;
+  bool wide;         // four waves a workgroup
+  int rows;          // of a tile
+  long long tiles;   // of all sequences and KV heads, at the most
+  int share;         // workgroups the tokens are shared by, where they are split by the lengths
+  long long pieces;  // at the most; 0: no tile is split
+  long long grid;
 };
-// 32-row blocks of a wave: two share a tile's LDS reads (K and V operands) while
-// their sums and queries fit the 512 registers of one wave per SIMD.
-__host__ __device__ constexpr int prompt_row_blocks(int D) { return 1; }
 static PromptPlan prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len, int n_splits) {
   const int G = Hq / Hkv;
   PromptPlan r;
   r.wide = (long long)N * G > 64LL * B;
-  r.rows = r.wide ? 128 * prompt_row_blocks(D) : 32;
-  r.tiles = (int)(((long long)N * G + r.rows - 1) / r.rows) + B;
-  r.splits = n_splits;
-  if (n_splits == 0) {
-    // enough workgroups for the chip, of at least 8 tiles each
-    const int most = std::max(1, max_len / (8 * kPromptTile));
-    const long long wgs = (long long)((N * (long long)G + r.rows - 1) / r.rows) * Hkv;
-    const int want = choose_workgroups(0, r.wide ? 1 : 4, 1LL << 30, 1);
-    r.splits = (int)std::min<long long>(std::max<long long>(want / std::max(wgs, 1LL), 1),
-                                        std::min(most, kPromptMaxSplits));
+  r.rows = r.wide ? 128 : 32;
+  const long long full = ((long long)N * G + r.rows - 1) / r.rows;
+  r.tiles = (full + B) * Hkv;
+  r.share = 0;
+  r.pieces = 0;
+  r.grid = r.tiles;
+  if (n_splits > 1) {
+    r.pieces = r.grid = r.tiles * n_splits;
+  } else if (n_splits == 0) {
+    // two workgroups a CU (what LDS holds) where the tiles are fewer
+    const int fill = choose_workgroups(0, 2, 1LL << 30, 1);
+    if (full * Hkv < fill && max_len > kPromptMinShare * kPromptTile) {
+      r.share = fill;
+      // every split but a tile's last is a whole share (and the shares' total, a sum in
+      // fp32, is off by less than 64 of them)
+      r.pieces = r.grid = r.tiles + fill + 64;
+    }
   }
   return r;
 }
-static size_t prompt_bytes(int N, int Hq, int D, int splits) {
-  if (splits <= 1) return 0;
-  const size_t rows = (size_t)N * Hq * splits;
+static size_t prompt_bytes(const PromptPlan& pl, int D) {
+  if (pl.pieces == 0) return 0;
+  const size_t rows = (size_t)pl.pieces * pl.rows;
   return align256(rows * 4) + rows * D * 4;
 }
 
 template <bool F8>
 static void prompt_launch(const PromptParams& p, const PromptPlan& pl, int D, hipStream_t s) {
-  const dim3 grid((unsigned)pl.tiles * p.Hkv * p.n_splits);
+  const dim3 grid((unsigned)pl.grid);
 #define WS_PROMPT_CASE(DD)                                                              \
   case DD:                                                                              \
     if (pl.wide)                                                                        \
-      hipLaunchKernelGGL((prompt_kernel<DD, F8, prompt_row_blocks(DD), 4>), grid, dim3(256), 0, s, p);      \
+      hipLaunchKernelGGL((prompt_kernel<DD, F8, 4>), grid, dim3(256), 0, s, p);      \
     else                                                                                \
-      hipLaunchKernelGGL((prompt_kernel<DD, F8, 1, 1>), grid, dim3(64), 0, s, p);       \
+      hipLaunchKernelGGL((prompt_kernel<DD, F8, 1>), grid, dim3(64), 0, s, p);       \
     break;
   switch (D) {
     WS_PROMPT_CASE(32) WS_PROMPT_CASE(64) WS_PROMPT_CASE(96) WS_PROMPT_CASE(128)
@@ -879,7 +911,7 @@ static int prompt_sizes(const char* name, int N, int B, int Hq, int Hkv, int D, 
   if ((long long)N * (Hq / Hkv) + 256LL * B >= (1LL << 31) || max_len > (1 << 30))
     return set_error(WS_EINVAL, "%s: %d tokens of %d heads exceed the row index range", name, N, Hq);
   const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, max_len, n_splits);
-  if ((long long)pl.tiles * Hkv * pl.splits * 256 >= (1LL << 32))
+  if (pl.grid * (pl.wide ? 256 : 64) >= (1LL << 32))
     return set_error(WS_EINVAL, "%s: %d tokens of %d heads exceed the launch grid", name, N, Hq);
   return WS_OK;
 }
@@ -889,11 +921,11 @@ static int prompt_sizes(const char* name, int N, int B, int Hq, int Hkv, int D, 
 using namespace ws;
 
 extern "C" int ws_gqa_prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len, int n_splits,
-                                  int* n_splits_out, size_t* workspace_bytes_out) {
+                                  int* pieces_out, size_t* workspace_bytes_out) {
   if (int rc = prompt_sizes("ws_gqa_prompt_plan", N, B, Hq, Hkv, D, max_len, n_splits)) return rc;
   const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, max_len, n_splits);
-  if (n_splits_out) *n_splits_out = pl.splits;
-  if (workspace_bytes_out) *workspace_bytes_out = prompt_bytes(N, Hq, D, pl.splits);
+  if (pieces_out) *pieces_out = (int)pl.pieces;
+  if (workspace_bytes_out) *workspace_bytes_out = prompt_bytes(pl, D);
   return WS_OK;
 }
 
@@ -924,7 +956,7 @@ extern "C" int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void*
   if (!(scale - scale == 0.f)) return set_error(WS_EINVAL, "%s: scale must be finite", name);
   if (N == 0 || B == 0) return WS_OK;
   const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, max_len, n_splits);
-  const size_t need = prompt_bytes(N, Hq, D, pl.splits);
+  const size_t need = prompt_bytes(pl, D);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(WS_EWORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
   if (need > 0 && ((uintptr_t)workspace & 255u) != 0)
@@ -942,7 +974,7 @@ extern "C" int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void*
   p.out_f32 = out_f32;
   p.lse = lse;
   p.part_lse = (float*)workspace;
-  p.part_out = (float*)((char*)workspace + align256((size_t)N * Hq * pl.splits * 4));
+  p.part_out = (float*)((char*)workspace + align256((size_t)pl.pieces * pl.rows * 4));
   p.N = N;
   p.B = B;
   p.Hq = Hq;
@@ -952,8 +984,9 @@ extern "C" int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void*
   p.max_pages = max_pages;
   p.num_pages = num_pages;
   p.cap = (int)std::min<long long>((long long)page_size * max_pages, 1LL << 30);
-  p.n_splits = pl.splits;
-  p.tiles = pl.tiles;
+  p.n_splits = n_splits;
+  p.share = pl.share;
+  p.pieces = pl.pieces;
   p.scale_log2 = (scale < 0.f ? -scale : scale) * kLog2e;
   p.q_sign = scale < 0.f ? 0x80008000u : 0u;
   hipStream_t s = (hipStream_t)stream;
@@ -962,9 +995,8 @@ extern "C" int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void*
   else
     prompt_launch<false>(p, pl, D, s);
   int rc = check_launch(name);
-  if (rc != WS_OK || pl.splits == 1) return rc;
-  const long long threads = (long long)N * Hq * (D / 4);
-  hipLaunchKernelGGL(prompt_join_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s,
-                     p, D);
+  if (rc != WS_OK || pl.pieces == 0) return rc;
+  hipLaunchKernelGGL(prompt_join_kernel, dim3((unsigned)pl.tiles, pl.rows / kJoinRows), dim3(256), 0,
+                     s, p, D, pl.rows);
   return check_launch(name);
 }

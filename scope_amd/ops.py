@@ -1294,7 +1294,8 @@ def gqa8_decode_full(q, k_pages, v_pages, k_scale, v_scale, page_table, gpu_len,
 
 def gqa_prompt_plan(n_tokens: int, batch: int, Hq: int, Hkv: int, D: int, max_len: int,
                     n_splits: int = 0):
-    """(n_splits, workspace_bytes) of a prompt call."""
+    """(pieces, workspace_bytes) of a prompt call: how many pieces its split tiles
+    can leave (0: no tile is split, no workspace)."""
     key = ("prompt", n_tokens, batch, Hq, Hkv, D, max_len, n_splits,
            torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1)
     hit = _plans.get(key)
@@ -1316,7 +1317,9 @@ def gqa_prompt(q, k_pages, v_pages, page_table, kv_len, cu_new, scale, max_len, 
     cu_new[b] .. cu_new[b + 1] and the last of its kv_len[b] tokens in the pages.
     Pools bf16, or 8-bit with k_scale and v_scale.  Returns (out [N, Hq, D] in
     out_dtype (bf16 or fp32), lse [N, Hq] fp32 or None); rows outside
-    [cu_new[0], cu_new[B]) are not written.  max_len must bound every kv_len[b]."""
+    [cu_new[0], cu_new[B]) are not written.  max_len must bound every kv_len[b].
+    n_splits: workgroups that share a tile of rows (0: the library's choice by
+    the lengths)."""
     dev = _gpu(k_pages, "k_pages")
     P, Hkv, PS, D = _pools(k_pages, v_pages, k_scale, v_scale, dev)
     _require(q, "q", torch.bfloat16, dev, 3)
@@ -1346,10 +1349,10 @@ def gqa_prompt(q, k_pages, v_pages, page_table, kv_len, cu_new, scale, max_len, 
             raise ValueError("lse must be [N, Hq]")
     if N == 0 or B == 0:
         return out, lse
-    n, wsb = gqa_prompt_plan(N, B, Hq, Hkv, D, int(max_len), int(n_splits))
+    _, wsb = gqa_prompt_plan(N, B, Hq, Hkv, D, int(max_len), int(n_splits))
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
     o16, o32 = (out, None) if out.dtype == torch.bfloat16 else (None, out)
     _run("ws_gqa_prompt", dev, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
          _ptr(page_table), _ptr(kv_len), _ptr(cu_new), N, B, Hq, Hkv, D, PS, page_table.shape[1], P,
-         int(max_len), n, float(scale), _ptr(o16), _ptr(o32), _ptr(lse), _ptr(ws), wsb)
+         int(max_len), int(n_splits), float(scale), _ptr(o16), _ptr(o32), _ptr(lse), _ptr(ws), wsb)
     return out, lse

@@ -129,13 +129,15 @@ def test_plans():
     assert n == 4
     with pytest.raises(ops.WsError, match="head_dim"):
         ops.gqa8_plan(4, 8, 80, 64)
+    # 40 tokens of 8 sequences, 4 heads a KV head: at most 5 + 8 tiles of 32 rows a KV head
     n, wsb = ops.gqa_prompt_plan(40, 8, 32, 8, 128, 32000, 4)
-    assert n == 4 and wsb == pad(4 * 40 * 32 * 4) + 4 * 40 * 32 * 128 * 4
+    assert n == 13 * 8 * 4 and wsb == pad(n * 32 * 4) + n * 32 * 128 * 4
     # long prompts fill the chip by their rows; one split needs no workspace
-    assert ops.gqa_prompt_plan(8192, 1, 32, 8, 128, 8192) == (1, 0)
+    assert ops.gqa_prompt_plan(8192, 1, 32, 8, 128, 8192) == (0, 0)
+    assert ops.gqa_prompt_plan(40, 8, 32, 8, 128, 32000, 1) == (0, 0)
     # one token over a long cache is split, a short cache is not
-    assert ops.gqa_prompt_plan(1, 1, 32, 8, 128, 100000)[0] > 1
-    assert ops.gqa_prompt_plan(1, 1, 32, 8, 128, 100)[0] == 1
+    assert ops.gqa_prompt_plan(1, 1, 32, 8, 128, 100000)[0] > 8
+    assert ops.gqa_prompt_plan(1, 1, 32, 8, 128, 100) == (0, 0)
     with pytest.raises(ops.WsError, match="bad sizes"):
         ops.gqa_prompt_plan(1, 1, 32, 5, 128, 100)
 
