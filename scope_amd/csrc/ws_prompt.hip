@@ -35,7 +35,6 @@
 namespace ws {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef const int32_t __attribute__((address_space(4))) ConstInt;
 
 constexpr int kPromptMaxD = 256;
 constexpr int kPromptTile = 32;    // tokens of a tile
@@ -247,14 +246,23 @@ struct PromptShape {
   static constexpr int kLoads = (kPieces + kThreads - 1) / kThreads;
 };
 
-// 16 bytes a lane from `base` + off to LDS at `lds` + 16 * lane, with no register between
-// (counted by vmcnt; the caller waits, then passes a barrier).  In assembly because the
-// compiler would wait for every one of them ahead of any LDS read.
+template <int I, int N, class F>
+__device__ __forceinline__ void static_for_prompt(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for_prompt<I + 1, N>(f);
+  }
+}
+
+// 16 bytes a lane from `base` + off to LDS at `lds` + AT + 16 * lane, with no register
+// between (counted by vmcnt; the caller waits, then passes a barrier).  In assembly because
+// the compiler would wait for every one of them ahead of any LDS read.
+template <int AT>
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                :
-               : "v"(off), "s"(base), "s"(lds)
-               : "memory");
+               : "v"(off), "s"(base), "s"(lds), "n"(AT)
+               : "memory", "scc");
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -339,95 +347,86 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     pin_sum<kAcc>(acc[d]);
   }
 
-  // A tile's place: pool token index of its first token, its last row that holds a
-  // token (later rows repeat it), and whether the page id was bad.
-  struct Place {
-    uint32_t tok;
-    int last;
-    bool bad;
+  // Tiles that every row sees whole: [blk0, blkm), in the pipeline; the others up to blk1.
+  const int blkm = max(blk0, min(blk1, max(lim_lo, 0) / kPromptTile));
+  // The pool token index of a tile's first token, for 64 tiles at a time, one a lane (a
+  // load a step would be waited for together with the tiles under way), and the tiles
+  // whose page id is bad.  Tiles past the last are the last one again.
+  int win = 0;
+  uint32_t win_tok = 0;
+  uint64_t win_bad = 0;
+  bool bad_page = false;  // of a tile that every row sees: every row is NaN
+  auto fetch_window = [&](int blk) __attribute__((always_inline)) {
+    win = blk;
+    const int x = min(blk + lane, blk1 - 1);
+    const int t = x * kPromptTile;  // (< len)
+    const int page = t / p.page_size;
+    const int raw = p.page_table[(size_t)tl.b * p.max_pages + page];
+    const int pid = clamp_page(raw, p.num_pages);
+    win_tok = ((uint32_t)pid * (uint32_t)p.Hkv + (uint32_t)kvh) * (uint32_t)p.page_size +
+              (uint32_t)(t - page * p.page_size);
+    win_bad = __builtin_amdgcn_ballot_w64(raw != pid);
+    bad_page |= __builtin_amdgcn_ballot_w64(raw != pid && x < blkm) != 0;
   };
-  // The page id is requested (next_page) a step before it is used (place): tiles are asked
-  // for one after the other, the page and the place in it carried along; past the last
-  // tile it is the last one again.
-  struct PageRef {
-    int raw, off, t;
-  };
-  int at_blk, at_page, at_off;
-  auto seek = [&](int blk) __attribute__((always_inline)) {
-    at_blk = blk;
-    at_page = blk * kPromptTile / p.page_size;
-    at_off = blk * kPromptTile - at_page * p.page_size;
-  };
-  auto next_page = [&]() __attribute__((always_inline)) {
-    PageRef r;
-    // a scalar load (the constant address space): a vector load's result would be
-    // waited for together with the tiles under way
-    r.raw = ((const ConstInt*)p.page_table)[(size_t)tl.b * p.max_pages + at_page];
-    r.off = at_off;
-    r.t = at_blk * kPromptTile;  // (< len)
-    const int more = at_blk + 1 < blk1 ? 1 : 0;
-    at_blk += more;
-    at_off += more * kPromptTile;
-    const int wrap = at_off == p.page_size ? 1 : 0;
-    at_off = wrap ? 0 : at_off;
-    at_page += wrap;
-    return r;
-  };
-  auto place = [&](const PageRef& r) __attribute__((always_inline)) {
-    const int pid = clamp_page(r.raw, p.num_pages);
-    Place x;
-    x.tok = ((uint32_t)pid * (uint32_t)p.Hkv + (uint32_t)kvh) * (uint32_t)p.page_size +
-            (uint32_t)r.off;
-    x.last = min(31, len - 1 - r.t);
-    x.bad = r.raw != pid;
-    return x;
+  // asked for in the tiles' order
+  auto tile_tok = [&](int blk) __attribute__((always_inline)) {
+    if (blk - win >= 64) fetch_window(blk);
+    return (uint32_t)__builtin_amdgcn_readlane((int)win_tok, blk - win);
   };
   const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_k;
   const uint32_t lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_v;
-  // Straight to LDS: chunks of 1 KB, NW of them at a time, one a wave.  A lane's chunk of
-  // the row is the one that belongs at its place; the offsets are the same for every tile.
+  // Straight to LDS: chunks of 1 KB, NW of them at a time, one a wave (a wave past the
+  // tile's end its first one again).  A lane's 16 bytes of the row are those that belong at
+  // its place; the offsets are the same for every tile.
   constexpr int kDma = Sh::kTile / 1024;
-  constexpr int LQ = (kDma + NW - 1) / NW;  // a wave's (the last one twice where NW is too many)
-  uint32_t dma_k[LQ], dma_v[LQ], dma_at[LQ];
+  constexpr int LQ = (kDma + NW - 1) / NW;
+  uint32_t dma_k[LQ], dma_v[LQ];
 #pragma unroll
   for (int u = 0; u < LQ; ++u) {
-    const int q = min(wave + u * NW, kDma - 1);
+    const int q = wave + u * NW < kDma ? wave + u * NW : min(wave, kDma - 1);
     const int at = 64 * q + lane;
     const int row = at / (D / 8);
     const int c = at - row * (D / 8);
-    dma_at[u] = 1024 * q;
     dma_k[u] = row * Sh::kRow + 16 * (c ^ prompt_k_swap(D, row));
     dma_v[u] = row * Sh::kRow + 16 * (c ^ prompt_v_swap(D, row));
   }
-  auto dma_tile = [&](const void* pages, const Place& x, const uint32_t (&off)[LQ], uint32_t slot)
-                      __attribute__((always_inline)) {
-    const char* base = (const char*)pages + (size_t)x.tok * Sh::kRow;
-#pragma unroll
-    for (int u = 0; u < LQ; ++u) load_to_lds(base, off[u], slot + dma_at[u]);
+  const uint32_t lds_kw = lds_k + 1024 * min(wave, kDma - 1);
+  const uint32_t lds_vw = lds_v + 1024 * min(wave, kDma - 1);
+  auto dma_tile = [&](const void* pages, uint32_t tok, const uint32_t (&off)[LQ], uint32_t lds,
+                      auto slot) __attribute__((always_inline)) {
+    constexpr int kSlot = decltype(slot)::value * Sh::kTile;
+    const char* base = (const char*)pages + (size_t)tok * Sh::kRow;
+    static_for_prompt<0, LQ>([&](auto i) __attribute__((always_inline)) {
+      constexpr int u = decltype(i)::value;
+      if constexpr ((u + 1) * NW <= kDma)
+        load_to_lds<kSlot + 1024 * NW * u>(base, off[u], lds);
+      else
+        load_to_lds<kSlot>(base, off[u], wave + u * NW < kDma ? lds + 1024 * NW * u : lds);
+    });
   };
   // Through registers: pieces tid, tid + threads, ... of a tile.
   struct Regs {
     u32x4 w[LD];
     uint32_t s[F8 ? LD : 1];
   };
-  auto load_tile = [&](const void* pages, const uint8_t* scale, const Place& x, Regs& g)
+  auto load_tile = [&](const void* pages, const uint8_t* scale, uint32_t tok, Regs& g)
                        __attribute__((always_inline)) {
-    const char* base = (const char*)pages + (size_t)x.tok * (16 * CH);
+    const char* base = (const char*)pages + (size_t)tok * (16 * CH);
 #pragma unroll
     for (int u = 0; u < LD; ++u) {
       const uint32_t piece = min(tid + u * Sh::kThreads, Sh::kPieces - 1);
       g.w[u] = *(const u32x4*)(base + 16 * piece);
-      if (F8) g.s[u] = *(scale + x.tok + piece / CH);
+      if (F8) g.s[u] = *(scale + tok + piece / CH);
     }
   };
   // The same of a tile that may hold fewer tokens: rows past the last repeat it.
-  auto load_last = [&](const void* pages, const uint8_t* scale, const Place& x, Regs& g)
+  auto load_last = [&](const void* pages, const uint8_t* scale, uint32_t tok, int last, Regs& g)
                        __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < LD; ++u) {
       const int piece = min(tid + u * Sh::kThreads, Sh::kPieces - 1);
       const int t = piece / CH;
-      const size_t row = (size_t)x.tok + min(t, x.last);
+      const size_t row = (size_t)tok + min(t, last);
       g.w[u] = ((const u32x4*)pages)[row * CH + (piece - t * CH)];
       if (F8) g.s[u] = scale[row];
     }
@@ -589,40 +588,33 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     }
   };
 
-  // Tiles that every row sees whole, in the pipeline: [blk0, blkm).
-  const int blkm = max(blk0, min(blk1, max(lim_lo, 0) / kPromptTile));
-  bool bad_page = false;  // one of them lies in a bad page: every row is NaN
   if (blk0 < blkm) {
     const int T = blkm - blk0;
     f32x16 s[2];
     u32x4 pb[2][2];
     Regs kg[2], vg[2];  // (8-bit)
-    // places of tiles t .. t + 4, and the page of t + 5
-    seek(blk0);
-    PageRef ahead[6];
-    Place pl[5];
+    fetch_window(blk0);
+    uint32_t tok[5];  // of tiles t .. t + 4
 #pragma unroll
-    for (int i = 0; i < 6; ++i) ahead[i] = next_page();
-#pragma unroll
-    for (int i = 0; i < 5; ++i) pl[i] = place(ahead[i]);
-    PageRef nx = ahead[5];
+    for (int i = 0; i < 5; ++i) tok[i] = tile_tok(blk0 + i);
     // tile t of K (V) into slot t & 3, in the order of the steps that read them
     if constexpr (F8) {
-      load_tile(p.k_pages, p.k_scale, pl[0], kg[0]);
-      load_tile(p.k_pages, p.k_scale, pl[1], kg[1]);
+      load_tile(p.k_pages, p.k_scale, tok[0], kg[0]);
+      load_tile(p.k_pages, p.k_scale, tok[1], kg[1]);
       store_tile(false, 0, kg[0], nullptr);
       store_tile(false, 1, kg[1], nullptr);
-      load_tile(p.k_pages, p.k_scale, pl[2], kg[0]);
-      load_tile(p.v_pages, p.v_scale, pl[0], vg[0]);
-      load_tile(p.k_pages, p.k_scale, pl[3], kg[1]);
-      load_tile(p.v_pages, p.v_scale, pl[1], vg[1]);
+      load_tile(p.k_pages, p.k_scale, tok[2], kg[0]);
+      load_tile(p.v_pages, p.v_scale, tok[0], vg[0]);
+      load_tile(p.k_pages, p.k_scale, tok[3], kg[1]);
+      load_tile(p.v_pages, p.v_scale, tok[1], vg[1]);
     } else {
-      dma_tile(p.k_pages, pl[0], dma_k, lds_k);
-      dma_tile(p.k_pages, pl[1], dma_k, lds_k + Sh::kTile);
-      dma_tile(p.k_pages, pl[2], dma_k, lds_k + 2 * Sh::kTile);
-      dma_tile(p.v_pages, pl[0], dma_v, lds_v);
-      dma_tile(p.k_pages, pl[3], dma_k, lds_k + 3 * Sh::kTile);
-      dma_tile(p.v_pages, pl[1], dma_v, lds_v + Sh::kTile);
+      using std::integral_constant;
+      dma_tile(p.k_pages, tok[0], dma_k, lds_kw, integral_constant<int, 0>{});
+      dma_tile(p.k_pages, tok[1], dma_k, lds_kw, integral_constant<int, 1>{});
+      dma_tile(p.k_pages, tok[2], dma_k, lds_kw, integral_constant<int, 2>{});
+      dma_tile(p.v_pages, tok[0], dma_v, lds_vw, integral_constant<int, 0>{});
+      dma_tile(p.k_pages, tok[3], dma_k, lds_kw, integral_constant<int, 3>{});
+      dma_tile(p.v_pages, tok[1], dma_v, lds_vw, integral_constant<int, 1>{});
     }
     // the values of "tile -1", which step 0 adds with weights of 0
     for (int i = tid; i < Sh::kTile / 16; i += Sh::kThreads)
@@ -638,20 +630,18 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     auto step = [&](auto slot, int t) __attribute__((always_inline)) {
       constexpr int c = decltype(slot)::value;  // t & 3
       constexpr int u = c & 1;
-      bad_page |= pl[0].bad;
       if constexpr (F8) {  // K of tile t + 2 and V of t; K of t + 4 and V of t + 2 requested
         store_tile(false, c ^ 2, kg[u], nullptr);
         store_tile(true, c, vg[u], nullptr);
-        load_tile(p.k_pages, p.k_scale, pl[4], kg[u]);
-        load_tile(p.v_pages, p.v_scale, pl[2], vg[u]);
+        load_tile(p.k_pages, p.k_scale, tok[4], kg[u]);
+        load_tile(p.v_pages, p.v_scale, tok[2], vg[u]);
       } else {
-        dma_tile(p.k_pages, pl[4], dma_k, lds_k + c * Sh::kTile);
-        dma_tile(p.v_pages, pl[2], dma_v, lds_v + (c ^ 2) * Sh::kTile);
+        dma_tile(p.k_pages, tok[4], dma_k, lds_kw, slot);
+        dma_tile(p.v_pages, tok[2], dma_v, lds_vw, std::integral_constant<int, (c ^ 2)>{});
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pl[i] = pl[i + 1];
-      pl[4] = place(nx);
-      nx = next_page();
+      for (int i = 0; i < 4; ++i) tok[i] = tok[i + 1];
+      tok[4] = tile_tok(blk0 + t + 5);
       // The scores of tile t + 1 under the exponentials of tile t, then the values of
       // tile t - 1 under its sums and the next tile's maximum: one product and its share
       // of the vector work at a time (sched_barrier keeps the order; the compiler's own
@@ -740,23 +730,25 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   if (blkm < blk1) {
     if (tid < 2) s_bad[tid] = 0;
     Regs kg, vg;
-    seek(blkm);
-    Place nx = place(next_page());
-    PageRef far = next_page();
-    load_last(p.k_pages, p.k_scale, nx, kg);
-    load_last(p.v_pages, p.v_scale, nx, vg);
+    fetch_window(blkm);
+    uint32_t tok = tile_tok(blkm);
+    bool next_bad = win_bad & 1;
+    auto last_of = [&](int blk) { return min(kPromptTile, len - blk * kPromptTile) - 1; };
+    load_last(p.k_pages, p.k_scale, tok, last_of(blkm), kg);
+    load_last(p.v_pages, p.v_scale, tok, last_of(blkm), vg);
     __syncthreads();
     int c = 0;
 #pragma unroll 1
     for (int blk = blkm; blk < blk1; ++blk) {
-      const bool bad = nx.bad;
+      const bool bad = next_bad;
       store_tile(false, c, kg, nullptr);
       // (s_bad stays set: the slow sum is right for any tile)
       store_tile(true, c, vg, &s_bad[c]);
-      nx = place(far);
-      far = next_page();
-      load_last(p.k_pages, p.k_scale, nx, kg);
-      load_last(p.v_pages, p.v_scale, nx, vg);
+      const int next = min(blk + 1, blk1 - 1);
+      tok = tile_tok(next);
+      next_bad = (win_bad >> (next - win)) & 1;
+      load_last(p.k_pages, p.k_scale, tok, last_of(next), kg);
+      load_last(p.v_pages, p.v_scale, tok, last_of(next), vg);
       __syncthreads();
       f32x16 s;
       u32x4 pb[2];
