@@ -257,12 +257,20 @@ __device__ __forceinline__ void static_for_prompt(F&& f) {
 // 16 bytes a lane from `base` + off to LDS at `lds` + AT + 16 * lane, with no register
 // between (counted by vmcnt; the caller waits, then passes a barrier).  In assembly because
 // the compiler would wait for every one of them ahead of any LDS read.
-template <int AT>
+// ONCE: the tile is read once (the calls of few rows), so it need not stay in the caches
+// (the non-temporal hint: 140 -> 129 us for 8 x 5 tokens over 4000 to 32000).
+template <int AT, bool ONCE>
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-               :
-               : "v"(off), "s"(base), "s"(lds), "n"(AT)
-               : "memory", "scc");
+  if constexpr (ONCE)
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :
+                 : "v"(off), "s"(base), "s"(lds), "n"(AT)
+                 : "memory", "scc");
+  else
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(off), "s"(base), "s"(lds), "n"(AT)
+                 : "memory", "scc");
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -399,9 +407,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     static_for_prompt<0, LQ>([&](auto i) __attribute__((always_inline)) {
       constexpr int u = decltype(i)::value;
       if constexpr ((u + 1) * NW <= kDma)
-        load_to_lds<kSlot + 1024 * NW * u>(base, off[u], lds);
+        load_to_lds<kSlot + 1024 * NW * u, NW == 1>(base, off[u], lds);
       else
-        load_to_lds<kSlot>(base, off[u], wave + u * NW < kDma ? lds + 1024 * NW * u : lds);
+        load_to_lds<kSlot, NW == 1>(base, off[u], wave + u * NW < kDma ? lds + 1024 * NW * u : lds);
     });
   };
   // Through registers: pieces tid, tid + threads, ... of a tile.
@@ -856,13 +864,17 @@ static PromptPlan prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len,
   if (n_splits > 1) {
     r.pieces = r.grid = r.tiles * n_splits;
   } else if (n_splits == 0) {
-    // two workgroups a CU (what LDS holds) where the tiles are fewer
-    const int fill = choose_workgroups(0, 2, 1LL << 30, 1);
+    // Where the tiles are fewer than the workgroups that fit the chip: shares that make,
+    // with every tile's last one, as many pieces as fit it once.  (8 x 5 tokens of 4 x 8
+    // heads over 4000 to 32000, us with the join: once 97, twice 108, three times 118.)
+    const int lds = 160 * 1024 / (kPromptSlots * 2 * kPromptTile * 2 * D + 256);
+    const int per_cu = r.wide ? (D <= 128 ? 2 : 1) : std::min(lds, 8);
+    const long long fill = choose_workgroups(0, per_cu, 1LL << 30, 1);
     if (full * Hkv < fill && max_len > kPromptMinShare * kPromptTile) {
-      r.share = fill;
+      r.share = (int)std::max(fill - r.tiles, fill / 2);
       // every split but a tile's last is a whole share (and the shares' total, a sum in
       // fp32, is off by less than 64 of them)
-      r.pieces = r.grid = r.tiles + fill + 64;
+      r.pieces = r.grid = r.tiles + r.share + 64;
     }
   }
   return r;
