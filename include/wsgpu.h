@@ -596,12 +596,12 @@ int ws_gqa8_decode_full(const uint16_t* q, const uint8_t* k_pages, const uint8_t
  * n_splits: workgroups that share the tokens of a tile of rows (1 to 64; 0: the
  * library's choice, which splits where the tiles do not fill the device, by the
  * lengths).  max_len bounds kv_len.  Workspace: ws_gqa_prompt_plan's bytes for the same
- * sizes (0: none); pieces_out: how many pieces the split tiles can leave.
+ * sizes (fp8: whether the pools are 8-bit; 0: none); pieces_out: how many pieces the split tiles can leave.
  * The reference runs prompts through its framework's attention (chunks:
  * system/deepseek.py:279-322) on dense buffers.
  */
-int ws_gqa_prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len, int n_splits,
-                       int* pieces_out, size_t* workspace_bytes_out);
+int ws_gqa_prompt_plan(int N, int B, int Hq, int Hkv, int D, int fp8, int max_len,
+                       int n_splits, int* pieces_out, size_t* workspace_bytes_out);
 int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void* v_pages,
                   const uint8_t* k_scale, const uint8_t* v_scale, const int32_t* page_table,
                   const int32_t* kv_len, const int32_t* cu_new, int N, int B, int Hq, int Hkv,

@@ -235,6 +235,7 @@ __device__ __forceinline__ PromptPlace prompt_place(const PromptParams& p, int a
   return r;
 }
 
+constexpr int kPromptWaves = 4;  // of a workgroup (one in calls of few rows, prompt_plan)
 template <int D, bool F8, int NW>
 struct PromptShape {
   static constexpr int kRow = 2 * D;               // bytes of a row in LDS
@@ -290,7 +291,10 @@ __device__ __forceinline__ void wait_loads() {
 // and V of t + 2 in step t, to the slots the step before has left); 8-bit ones through
 // registers, requested two steps before they are converted and written.  One barrier a
 // step.
-template <int D, bool F8, int NW>
+//
+// FEW: calls of few rows.  A tile of tokens is read by one workgroup only, so it need not
+// stay in the caches, and waves without rows only load.
+template <int D, bool F8, int NW, bool FEW>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const PromptParams p) {
   static_assert(D % 32 == 0 && D <= kPromptMaxD, "head width: a multiple of 32 up to 256");
   using Sh = PromptShape<D, F8, NW>;
@@ -332,6 +336,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   // the lane's row, the tokens it sees, and its row of out / lse
   const int tile_row = wave * 32 + n32;
   const bool live = row0 + tile_row < R;
+  const bool idle = FEW && row0 + wave * 32 >= R;  // none of the wave's rows is
   const int r = min(row0 + tile_row, R - 1);
   const int i = r / G;
   const int lim = first_pos + i + 1;
@@ -407,9 +412,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     static_for_prompt<0, LQ>([&](auto i) __attribute__((always_inline)) {
       constexpr int u = decltype(i)::value;
       if constexpr ((u + 1) * NW <= kDma)
-        load_to_lds<kSlot + 1024 * NW * u, NW == 1>(base, off[u], lds);
+        load_to_lds<kSlot + 1024 * NW * u, FEW>(base, off[u], lds);
       else
-        load_to_lds<kSlot, NW == 1>(base, off[u], wave + u * NW < kDma ? lds + 1024 * NW * u : lds);
+        load_to_lds<kSlot, FEW>(base, off[u], wave + u * NW < kDma ? lds + 1024 * NW * u : lds);
     });
   };
   // Through registers: pieces tid, tid + threads, ... of a tile.
@@ -630,10 +635,10 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     pb[1][0] = pb[1][1] = u32x4{0, 0, 0, 0};
     if (!F8) wait_loads<4 * LQ>();
     __syncthreads();
-    scores(0, s[0]);
-    float alpha;   // of the tile whose softmax is next
-    float m_kept;  // the maximum without that tile's
-    alpha = new_max(row_max(s[0]));
+    if (!idle) scores(0, s[0]);
+    float alpha = 1.f;  // of the tile whose softmax is next
+    float m_kept = m_run;  // the maximum without that tile's
+    if (!idle) alpha = new_max(row_max(s[0]));
     __syncthreads();
     auto step = [&](auto slot, int t) __attribute__((always_inline)) {
       constexpr int c = decltype(slot)::value;  // t & 3
@@ -650,68 +655,70 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
 #pragma unroll
       for (int i = 0; i < 4; ++i) tok[i] = tok[i + 1];
       tok[4] = tile_tok(blk0 + t + 5);
-      // The scores of tile t + 1 under the exponentials of tile t, then the values of
-      // tile t - 1 under its sums and the next tile's maximum: one product and its share
-      // of the vector work at a time (sched_barrier keeps the order; the compiler's own
-      // runs the exponentials after the products).
-      constexpr int kExp = 16 / KS > 0 ? (16 + KS - 1) / KS : 1;
-      constexpr int kAhead = DT > 1 ? 3 : 2;  // V operands under way
-      u32x4 a[KS], av[2 * DT];
+      if (!idle) {
+        // The scores of tile t + 1 under the exponentials of tile t, then the values of
+        // tile t - 1 under its sums and the next tile's maximum: one product and its share
+        // of the vector work at a time (sched_barrier keeps the order; the compiler's own
+        // runs the exponentials after the products).
+        constexpr int kExp = 16 / KS > 0 ? (16 + KS - 1) / KS : 1;
+        constexpr int kAhead = DT > 1 ? 3 : 2;  // V operands under way
+        u32x4 a[KS], av[2 * DT];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) a[ks] = lds_read_b128(ka[ks] + ((c + 1) & 3) * Sh::kTile);
-      float mc, ps, bm;
-      mc = ref(m_run);
-      ps = 0.f;
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        s[u ^ 1] = mfma32x32x16(a[ks], qb[ks], ks == 0 ? f32x16{} : s[u ^ 1]);
-        pin_sum<kAcc>(s[u ^ 1]);
-#pragma unroll
-        for (int e = ks * kExp; e < (ks + 1) * kExp && e < 16; ++e) {
-          float x = s[u][e];
-          pin(x);
-          x = __builtin_amdgcn_exp2f(fmaf(x, p.scale_log2, -mc));
-          pin(x);
-          s[u][e] = x;
-        }
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-          if (ks == (KS > kAhead ? KS - kAhead + j : 0))
-            av[j] = values_operand((c + 3) & 3, j / DT, j % DT);
+        for (int ks = 0; ks < KS; ++ks) a[ks] = lds_read_b128(ka[ks] + ((c + 1) & 3) * Sh::kTile);
+        float mc, ps, bm;
+        mc = ref(m_run);
+        ps = 0.f;
         __builtin_amdgcn_sched_barrier(0);
-      }
-      constexpr int kSum = 8 / (2 * DT) > 0 ? (8 + 2 * DT - 1) / (2 * DT) : 1;
-      float next_alpha;
 #pragma unroll
-      for (int j = 0; j < 2 * DT; ++j) {
-        const int f = j + kAhead;
-        if (f < 2 * DT) av[f] = values_operand((c + 3) & 3, f / DT, f % DT);
-        acc[j % DT] = mfma32x32x16(av[j], pb[u ^ 1][j / DT], acc[j % DT]);
-        pin_sum<kAcc>(acc[j % DT]);
+        for (int ks = 0; ks < KS; ++ks) {
+          s[u ^ 1] = mfma32x32x16(a[ks], qb[ks], ks == 0 ? f32x16{} : s[u ^ 1]);
+          pin_sum<kAcc>(s[u ^ 1]);
 #pragma unroll
-        for (int e = j * kSum; e < (j + 1) * kSum && e < 8; ++e) {
-          const int i = 2 * e;
-          const float x = s[u][i], y = s[u][i + 1];
-          pin(ps);
-          ps += x + y;
-          pin(ps);
-          uint32_t w = pack_bf16x2(x, y);
-          pin(w);
-          pb[u][i >> 3][(i >> 1) & 3] = w;
+          for (int e = ks * kExp; e < (ks + 1) * kExp && e < 16; ++e) {
+            float x = s[u][e];
+            pin(x);
+            x = __builtin_amdgcn_exp2f(fmaf(x, p.scale_log2, -mc));
+            pin(x);
+            s[u][e] = x;
+          }
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j)
+            if (ks == (KS > kAhead ? KS - kAhead + j : 0))
+              av[j] = values_operand((c + 3) & 3, j / DT, j % DT);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        if (j == DT) {
-          bm = row_max(s[u ^ 1]);
+        constexpr int kSum = 8 / (2 * DT) > 0 ? (8 + 2 * DT - 1) / (2 * DT) : 1;
+        float next_alpha;
+#pragma unroll
+        for (int j = 0; j < 2 * DT; ++j) {
+          const int f = j + kAhead;
+          if (f < 2 * DT) av[f] = values_operand((c + 3) & 3, f / DT, f % DT);
+          acc[j % DT] = mfma32x32x16(av[j], pb[u ^ 1][j / DT], acc[j % DT]);
+          pin_sum<kAcc>(acc[j % DT]);
+#pragma unroll
+          for (int e = j * kSum; e < (j + 1) * kSum && e < 8; ++e) {
+            const int i = 2 * e;
+            const float x = s[u][i], y = s[u][i + 1];
+            pin(ps);
+            ps += x + y;
+            pin(ps);
+            uint32_t w = pack_bf16x2(x, y);
+            pin(w);
+            pb[u][i >> 3][(i >> 1) & 3] = w;
+          }
+          if (j == DT) {
+            bm = row_max(s[u ^ 1]);
+          }
+          if (j == 2 * DT - 1) {
+            l_run = l_run * alpha + ps;
+            m_kept = m_run;
+            next_alpha = new_max(bm);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        if (j == 2 * DT - 1) {
-          l_run = l_run * alpha + ps;
-          m_kept = m_run;
-          next_alpha = new_max(bm);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        rescale(alpha);
+        alpha = next_alpha;
       }
-      rescale(alpha);
-      alpha = next_alpha;
       if (!F8) wait_loads<4 * LQ>();  // those of this step and the one before may go on
       __syncthreads();
     };
@@ -727,10 +734,12 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     if (t + 1 < T) step(std::integral_constant<int, 1>{}, t + 1);
     if (t + 2 < T) step(std::integral_constant<int, 2>{}, t + 2);
     const int last = (T - 1) & 3;
-    if (last & 1)
-      values(last, pb[1]);
-    else
-      values(last, pb[0]);
+    if (!idle) {
+      if (last & 1)
+        values(last, pb[1]);
+      else
+        values(last, pb[0]);
+    }
     m_run = m_kept;  // (tile T may hold tokens not seen)
     if (!F8) wait_loads<0>();  // the tiles past the last, which nothing reads
   }
@@ -758,16 +767,18 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       load_last(p.k_pages, p.k_scale, tok, last_of(next), kg);
       load_last(p.v_pages, p.v_scale, tok, last_of(next), vg);
       __syncthreads();
-      f32x16 s;
-      u32x4 pb[2];
-      float alpha;
-      scores(c, s);
-      softmax_masked(blk, bad, s, pb, alpha);
-      rescale(alpha);
-      if (uniform(s_bad[c]))
-        values_masked(c, blk, pb);
-      else
-        values(c, pb);
+      if (!idle) {
+        f32x16 s;
+        u32x4 pb[2];
+        float alpha;
+        scores(c, s);
+        softmax_masked(blk, bad, s, pb, alpha);
+        rescale(alpha);
+        if (uniform(s_bad[c]))
+          values_masked(c, blk, pb);
+        else
+          values(c, pb);
+      }
       c ^= 1;
     }
   }
@@ -821,7 +832,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptParams p, 
     const int tr = blockIdx.y * kJoinRows + t / c4;  // row of the tile
     const int c = t % c4;
     const int r = tl.tile * rows + tr;
-    if (r >= R) return;
+    if (r >= R) return;  // (so has every later row)
     const int i = r / p.G;
     const size_t out_row = (size_t)(tl.c0 + i) * p.Hq + kvh * p.G + (r - i * p.G);
     const size_t slot = (size_t)piece_at * rows + tr;
@@ -843,19 +854,30 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 static bool prompt_width_ok(int D) { return D >= 32 && D <= kPromptMaxD && D % 32 == 0; }
 
 // How a call runs.
+//
+// Calls of few rows: a sequence's rows of a KV head fill half a tile on average, at the
+// most, and K and V are read about once, so the reads are the bound.  bf16 up to 128
+// columns: a wave by itself per 32 rows needs no barrier, and several on a CU keep as much
+// under way (8 x 5 tokens of 4 x 8 heads over 4000 to 32000: 97 us against 111 with four
+// waves that share the loads; 16 x 8 over 2000: 34 against 42).  8-bit pages take four
+// waves' conversions (8 x 16 over 8000: 107 us with one wave, 63 with four), and wider heads
+// four waves' registers (256 columns, 8 x 5 over 16000: 262 and 211).
 struct PromptPlan {
-  bool wide;         // four waves a workgroup
-  int rows;          // of a tile
+  bool few;
+  int waves;         // of a workgroup
+  int rows;          // of a tile: 32 a wave
   long long tiles;   // of all sequences and KV heads, at the most
   int share;         // workgroups the tokens are shared by, where they are split by the lengths
   long long pieces;  // at the most; 0: no tile is split
   long long grid;
 };
-static PromptPlan prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len, int n_splits) {
+static PromptPlan prompt_plan(int N, int B, int Hq, int Hkv, int D, bool fp8, int max_len,
+                              int n_splits) {
   const int G = Hq / Hkv;
   PromptPlan r;
-  r.wide = (long long)N * G > 64LL * B;
-  r.rows = r.wide ? 128 : 32;
+  r.few = (long long)N * G <= 64LL * B;
+  r.waves = r.few && !fp8 && D <= 128 ? 1 : kPromptWaves;
+  r.rows = 32 * r.waves;
   const long long full = ((long long)N * G + r.rows - 1) / r.rows;
   r.tiles = (full + B) * Hkv;
   r.share = 0;
@@ -868,7 +890,7 @@ static PromptPlan prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len,
     // with every tile's last one, as many pieces as fit it once.  (8 x 5 tokens of 4 x 8
     // heads over 4000 to 32000, us with the join: once 97, twice 108, three times 118.)
     const int lds = 160 * 1024 / (kPromptSlots * 2 * kPromptTile * 2 * D + 256);
-    const int per_cu = r.wide ? (D <= 128 ? 2 : 1) : std::min(lds, 8);
+    const int per_cu = r.waves == 1 ? std::min(lds, 8) : D <= 128 ? 2 : 1;
     const long long fill = choose_workgroups(0, per_cu, 1LL << 30, 1);
     if (full * Hkv < fill && max_len > kPromptMinShare * kPromptTile) {
       r.share = (int)std::max(fill - r.tiles, fill / 2);
@@ -885,25 +907,32 @@ static size_t prompt_bytes(const PromptPlan& pl, int D) {
   return align256(rows * 4) + rows * D * 4;
 }
 
+template <int D, bool F8>
+static void prompt_launch(const PromptParams& p, const PromptPlan& pl, hipStream_t s) {
+  const dim3 grid((unsigned)pl.grid), block(64 * pl.waves);
+  constexpr int kFewWaves = !F8 && D <= 128 ? 1 : kPromptWaves;  // (prompt_plan)
+  if (pl.few)
+    hipLaunchKernelGGL((prompt_kernel<D, F8, kFewWaves, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((prompt_kernel<D, F8, kPromptWaves, false>), grid, block, 0, s, p);
+}
 template <bool F8>
-static void prompt_launch(const PromptParams& p, const PromptPlan& pl, int D, hipStream_t s) {
-  const dim3 grid((unsigned)pl.grid);
-#define WS_PROMPT_CASE(DD)                                                              \
-  case DD:                                                                              \
-    if (pl.wide)                                                                        \
-      hipLaunchKernelGGL((prompt_kernel<DD, F8, 4>), grid, dim3(256), 0, s, p);      \
-    else                                                                                \
-      hipLaunchKernelGGL((prompt_kernel<DD, F8, 1>), grid, dim3(64), 0, s, p);       \
-    break;
+static void prompt_launch_width(const PromptParams& p, const PromptPlan& pl, int D,
+                                hipStream_t s) {
   switch (D) {
-    WS_PROMPT_CASE(32) WS_PROMPT_CASE(64) WS_PROMPT_CASE(96) WS_PROMPT_CASE(128)
-    WS_PROMPT_CASE(160) WS_PROMPT_CASE(192) WS_PROMPT_CASE(224) WS_PROMPT_CASE(256)
+    case 32: prompt_launch<32, F8>(p, pl, s); break;
+    case 64: prompt_launch<64, F8>(p, pl, s); break;
+    case 96: prompt_launch<96, F8>(p, pl, s); break;
+    case 128: prompt_launch<128, F8>(p, pl, s); break;
+    case 160: prompt_launch<160, F8>(p, pl, s); break;
+    case 192: prompt_launch<192, F8>(p, pl, s); break;
+    case 224: prompt_launch<224, F8>(p, pl, s); break;
+    default: prompt_launch<256, F8>(p, pl, s); break;
   }
-#undef WS_PROMPT_CASE
 }
 
-static int prompt_sizes(const char* name, int N, int B, int Hq, int Hkv, int D, int max_len,
-                        int n_splits) {
+static int prompt_sizes(const char* name, int N, int B, int Hq, int Hkv, int D, bool fp8,
+                        int max_len, int n_splits) {
   if (N < 0 || B < 0 || B > kMaxSeqs || Hkv <= 0 || Hq <= 0 || Hq % Hkv || max_len < 0 ||
       n_splits < 0 || n_splits > kPromptMaxSplits)
     return set_error(WS_EINVAL,
@@ -914,8 +943,8 @@ static int prompt_sizes(const char* name, int N, int B, int Hq, int Hkv, int D, 
     return set_error(WS_EINVAL, "%s: head_dim %d unsupported (multiples of 32 up to 256)", name, D);
   if ((long long)N * (Hq / Hkv) + 256LL * B >= (1LL << 31) || max_len > (1 << 30))
     return set_error(WS_EINVAL, "%s: %d tokens of %d heads exceed the row index range", name, N, Hq);
-  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, max_len, n_splits);
-  if (pl.grid * (pl.wide ? 256 : 64) >= (1LL << 32))
+  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, fp8, max_len, n_splits);
+  if (pl.grid * 64 * pl.waves >= (1LL << 32))
     return set_error(WS_EINVAL, "%s: %d tokens of %d heads exceed the launch grid", name, N, Hq);
   return WS_OK;
 }
@@ -924,10 +953,10 @@ static int prompt_sizes(const char* name, int N, int B, int Hq, int Hkv, int D, 
 
 using namespace ws;
 
-extern "C" int ws_gqa_prompt_plan(int N, int B, int Hq, int Hkv, int D, int max_len, int n_splits,
-                                  int* pieces_out, size_t* workspace_bytes_out) {
-  if (int rc = prompt_sizes("ws_gqa_prompt_plan", N, B, Hq, Hkv, D, max_len, n_splits)) return rc;
-  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, max_len, n_splits);
+extern "C" int ws_gqa_prompt_plan(int N, int B, int Hq, int Hkv, int D, int fp8, int max_len,
+                                  int n_splits, int* pieces_out, size_t* workspace_bytes_out) {
+  if (int rc = prompt_sizes("ws_gqa_prompt_plan", N, B, Hq, Hkv, D, fp8 != 0, max_len, n_splits)) return rc;
+  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, fp8 != 0, max_len, n_splits);
   if (pieces_out) *pieces_out = (int)pl.pieces;
   if (workspace_bytes_out) *workspace_bytes_out = prompt_bytes(pl, D);
   return WS_OK;
@@ -944,7 +973,7 @@ extern "C" int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void*
   if (!q || !k_pages || !v_pages || !page_table || !kv_len || !cu_new || (!out_bf16 && !out_f32) ||
       (k_scale == nullptr) != (v_scale == nullptr))
     return set_error(WS_EINVAL, "%s: null pointer", name);
-  if (int rc = prompt_sizes(name, N, B, Hq, Hkv, D, max_len, n_splits)) return rc;
+  if (int rc = prompt_sizes(name, N, B, Hq, Hkv, D, k_scale != nullptr, max_len, n_splits)) return rc;
   if (page_size <= 0 || page_size % 32 || max_pages <= 0 || num_pages <= 0 ||
       (long long)max_len > (long long)page_size * max_pages)
     return set_error(WS_EINVAL,
@@ -959,7 +988,7 @@ extern "C" int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void*
     return set_error(WS_EINVAL, "%s: buffers must be 16-byte aligned", name);
   if (!(scale - scale == 0.f)) return set_error(WS_EINVAL, "%s: scale must be finite", name);
   if (N == 0 || B == 0) return WS_OK;
-  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, max_len, n_splits);
+  const PromptPlan pl = prompt_plan(N, B, Hq, Hkv, D, k_scale != nullptr, max_len, n_splits);
   const size_t need = prompt_bytes(pl, D);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(WS_EWORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
@@ -995,9 +1024,9 @@ extern "C" int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void*
   p.q_sign = scale < 0.f ? 0x80008000u : 0u;
   hipStream_t s = (hipStream_t)stream;
   if (k_scale)
-    prompt_launch<true>(p, pl, D, s);
+    prompt_launch_width<true>(p, pl, D, s);
   else
-    prompt_launch<false>(p, pl, D, s);
+    prompt_launch_width<false>(p, pl, D, s);
   int rc = check_launch(name);
   if (rc != WS_OK || pl.pieces == 0) return rc;
   hipLaunchKernelGGL(prompt_join_kernel, dim3((unsigned)pl.tiles, pl.rows / kJoinRows), dim3(256), 0,

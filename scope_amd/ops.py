@@ -179,7 +179,7 @@ def lib() -> ctypes.CDLL:
         L.ws_gqa8_decode_full.restype = i32
         L.ws_gqa8_decode_full.argtypes = [vp] * 7 + [i32] * 9 + [f32, vp, vp, vp, vp, sz, vp]
         L.ws_gqa_prompt_plan.restype = i32
-        L.ws_gqa_prompt_plan.argtypes = [i32] * 7 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
+        L.ws_gqa_prompt_plan.argtypes = [i32] * 8 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
         L.ws_gqa_prompt.restype = i32
         L.ws_gqa_prompt.argtypes = [vp] * 8 + [i32] * 10 + [f32, vp, vp, vp, vp, sz, vp]
         _lib = L
@@ -1293,17 +1293,17 @@ def gqa8_decode_full(q, k_pages, v_pages, k_scale, v_scale, page_table, gpu_len,
 
 
 def gqa_prompt_plan(n_tokens: int, batch: int, Hq: int, Hkv: int, D: int, max_len: int,
-                    n_splits: int = 0):
+                    n_splits: int = 0, fp8: bool = False):
     """(pieces, workspace_bytes) of a prompt call: how many pieces its split tiles
     can leave (0: no tile is split, no workspace)."""
-    key = ("prompt", n_tokens, batch, Hq, Hkv, D, max_len, n_splits,
+    key = ("prompt", n_tokens, batch, Hq, Hkv, D, max_len, n_splits, fp8,
            torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1)
     hit = _plans.get(key)
     if hit is not None:
         return hit
     n, wsb = ctypes.c_int(0), ctypes.c_size_t(0)
-    _check(lib().ws_gqa_prompt_plan(n_tokens, batch, Hq, Hkv, D, max_len, n_splits, ctypes.byref(n),
-                                    ctypes.byref(wsb)), "ws_gqa_prompt_plan")
+    _check(lib().ws_gqa_prompt_plan(n_tokens, batch, Hq, Hkv, D, int(fp8), max_len, n_splits,
+                                    ctypes.byref(n), ctypes.byref(wsb)), "ws_gqa_prompt_plan")
     if len(_plans) > 4096:
         _plans.clear()
     _plans[key] = (n.value, wsb.value)
@@ -1349,7 +1349,7 @@ def gqa_prompt(q, k_pages, v_pages, page_table, kv_len, cu_new, scale, max_len, 
             raise ValueError("lse must be [N, Hq]")
     if N == 0 or B == 0:
         return out, lse
-    _, wsb = gqa_prompt_plan(N, B, Hq, Hkv, D, int(max_len), int(n_splits))
+    _, wsb = gqa_prompt_plan(N, B, Hq, Hkv, D, int(max_len), int(n_splits), k_scale is not None)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
     o16, o32 = (out, None) if out.dtype == torch.bfloat16 else (None, out)
     _run("ws_gqa_prompt", dev, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),

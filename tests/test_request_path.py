@@ -129,9 +129,11 @@ def test_plans():
     assert n == 4
     with pytest.raises(ops.WsError, match="head_dim"):
         ops.gqa8_plan(4, 8, 80, 64)
-    # 40 tokens of 8 sequences, 4 heads a KV head: at most 5 + 8 tiles of 32 rows a KV head
-    n, wsb = ops.gqa_prompt_plan(40, 8, 32, 8, 128, 32000, 4)
-    assert n == 13 * 8 * 4 and wsb == pad(n * 32 * 4) + n * 32 * 128 * 4
+    # 40 tokens of 8 sequences, 4 heads a KV head: at most 5 + 8 tiles of 32 rows a KV head,
+    # or 2 + 8 of 128
+    for fp8, tiles, rows in ((False, 13, 32), (True, 10, 128)):
+        n, wsb = ops.gqa_prompt_plan(40, 8, 32, 8, 128, 32000, 4, fp8)
+        assert n == tiles * 8 * 4 and wsb == pad(n * rows * 4) + n * rows * 128 * 4
     # long prompts fill the chip by their rows; one split needs no workspace
     assert ops.gqa_prompt_plan(8192, 1, 32, 8, 128, 8192) == (0, 0)
     assert ops.gqa_prompt_plan(40, 8, 32, 8, 128, 32000, 1) == (0, 0)
