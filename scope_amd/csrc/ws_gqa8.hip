@@ -177,24 +177,27 @@ __global__ __launch_bounds__(64 * kGqa8Waves, gqa8_waves_per_simd(D)) void gqa8_
     // instructions and registers, a cache hit, no HBM traffic
     const size_t tok = valid ? m.tok : 0;
     const int last = valid ? (m.nt & k8NtMask) - 1 : 0;
+    // the block's addresses are uniform, a lane's offsets in it 32-bit
+    const uint8_t* kb = p.k_pages + tok * D;
+    const uint8_t* vb = p.v_pages + tok * D;
+    const uint8_t* ksb = p.k_scale + tok;
+    const uint8_t* vsb = p.v_scale + tok;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      const size_t r = tok + min(16 * tt + n16, last);
-      const uint8_t* kr = p.k_pages + r * D;
+      const uint32_t r = min(16 * tt + n16, last);
 #pragma unroll
-      for (int i = 0; i < P64; ++i) st.k[tt][i] = ld_stream(kr + 64 * i + 16 * j);
-      if (TAIL) st.kt[tt] = *(const uint2*)(kr + 64 * P64 + 8 * j);
-      st.ks[tt] = p.k_scale[r];
+      for (int i = 0; i < P64; ++i) st.k[tt][i] = ld_stream(kb + (r * D + 16 * j) + 64 * i);
+      if (TAIL) st.kt[tt] = *(const uint2*)(kb + (r * D + 8 * j) + 64 * P64);
+      st.ks[tt] = ksb[r];
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const size_t r = tok + min(pv_token(i, j), last);
+      const uint32_t r = min(pv_token(i, j), last);
       st.v[i] = __builtin_nontemporal_load(
-          (const VT*)(p.v_pages + r * D + ((LV == 16 || n16 < LV) ? C * n16 : 0)));
+          (const VT*)(vb + (r * D + ((LV == 16 || n16 < LV) ? C * n16 : 0))));
     }
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
-      st.vs[tt] = *(const uint32_t*)(p.v_scale + tok + 16 * tt + 4 * j);
+    for (int tt = 0; tt < 2; ++tt) st.vs[tt] = *(const uint32_t*)(vsb + (16 * tt + 4 * j));
   };
   // q of a kv row as the QK B operand, in the keys' column order.
   u32x4 qb[KS];
@@ -321,7 +324,7 @@ __global__ __launch_bounds__(64 * kGqa8Waves, gqa8_waves_per_simd(D)) void gqa8_
     run_bad |= (cur.nt & k8BadPage) != 0;
     compute_block(cur, st[s]);
     __builtin_amdgcn_sched_barrier(0);
-    load_q(mq[nx].row);
+    if (mq[nx].row != cur.row) load_q(mq[nx].row);
   };
   int base = 0;
   for (; base + S <= nblk; base += S)
@@ -338,12 +341,16 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 static bool gqa8_width_ok(int D) { return D >= 32 && D <= kGqa8MaxD && D % 32 == 0; }
 
-// Splits (waves) of a call: n_splits when given, else four per CU, at most
-// what the blocks of the longest possible batch feed with 2 each.
+// Splits (waves) of a call: n_splits when given, else per CU what keeps the HBM
+// busy, at most what the blocks of the longest possible batch feed with 2 each.  Steps
+// with their merge, us, at 2 / 4 / 6 / 8 / 12 waves per CU (a workgroup holds two, so odd
+// counts leave CUs with one more than others and lose):
+//   128 columns, 621 MB   123  110  104  105  111     64 columns, 204 MB  70  50  43  42  44
+//   128 columns, 135 MB    32   32   33   35   42    256 columns, 159 MB  33  33  42  38  45
 static int gqa8_splits(int n_splits, int rows_kv, int max_len, int D) {
   if (n_splits > 0) return n_splits;
   const long long max_blocks = (long long)rows_kv * ((max_len + 31) / 32);
-  return choose_workgroups(0, D <= 64 ? 8 : 4, max_blocks, 2);
+  return choose_workgroups(0, D <= 64 ? 8 : D <= 128 ? 6 : 4, max_blocks, 2);
 }
 
 static int gqa8_launch(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pages,

@@ -1033,6 +1033,31 @@ def _gpu(t, name: str) -> torch.device:
     return t.device
 
 
+def _require_all(dev, specs, tensors) -> None:
+    """_require of every (name, dtype, dims) of specs, in one pass while all is well."""
+    idx = dev.index
+    for (_, dtype, ndim), t in zip(specs, tensors):
+        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == idx
+                and t.dim() == ndim and t.is_contiguous()):
+            break
+    else:
+        return
+    for (name, dtype, ndim), t in zip(specs, tensors):
+        _require(t, name, dtype, dev, ndim)
+
+
+_EXTEND_ARGS = (("page_table", torch.int32, 2), ("len_in", torch.int32, 1), ("n_new", torch.int32, 1),
+                ("stack", torch.int32, 1), ("free_in", torch.int32, 1))
+_RELEASE_ARGS = (("page_table", torch.int32, 2), ("len_in", torch.int32, 1), ("done", torch.bool, 1),
+                 ("stack", torch.int32, 1), ("free_in", torch.int32, 1))
+_POOL_ARGS = {bits: (("k_pages", dt, 4), ("v_pages", dt, 4)) for bits, dt in
+              ((16, torch.bfloat16), (8, E4M3))}
+_SCALE_ARGS = (("k_scale", E8M0, 3), ("v_scale", E8M0, 3))
+_DECODE8_ARGS = (("q", torch.bfloat16, 3), ("page_table", torch.int32, 2), ("gpu_len", torch.int32, 1))
+_PROMPT_ARGS = (("q", torch.bfloat16, 3), ("page_table", torch.int32, 2), ("kv_len", torch.int32, 1),
+                ("cu_new", torch.int32, 1))
+
+
 class PageStep(NamedTuple):
     """What pages_extend hands out (all int32 on the GPU)."""
 
@@ -1052,11 +1077,7 @@ def pages_extend(page_table, len_in, n_new, stack, free_in, page_size, num_pages
     batch's tokens, sum(n_new) or more (the rest is padding: slot -1).
     pos_base [B]: what a position counts beside the partition's tokens."""
     dev = _gpu(page_table, "page_table")
-    _require(page_table, "page_table", torch.int32, dev, 2)
-    _require(len_in, "len_in", torch.int32, dev, 1)
-    _require(n_new, "n_new", torch.int32, dev, 1)
-    _require(stack, "stack", torch.int32, dev, 1)
-    _require(free_in, "free_in", torch.int32, dev, 1)
+    _require_all(dev, _EXTEND_ARGS, (page_table, len_in, n_new, stack, free_in))
     B, max_pages = page_table.shape
     N = int(n_tokens)
     if len_in.shape[0] != B or n_new.shape[0] != B or free_in.shape[0] != 1:
@@ -1067,32 +1088,29 @@ def pages_extend(page_table, len_in, n_new, stack, free_in, page_size, num_pages
             raise ValueError("pos_base must be [B]")
     if N < 0:
         raise ValueError(f"n_tokens {N} < 0")
-    step = PageStep(*torch.empty(2 * B + 2 + 2 * N, dtype=torch.int32, device=dev).split_with_sizes(
-        (B, B + 1, N, N, 1)))
-    _run("ws_pages_extend", dev, _ptr(page_table), _ptr(len_in), _ptr(n_new), _ptr(stack),
-         _ptr(free_in), _ptr(pos_base), step.len_out.data_ptr(), step.cu_new.data_ptr(),
-         step.positions.data_ptr(), step.slots.data_ptr(), step.free_out.data_ptr(), B, max_pages,
-         int(num_pages), stack.shape[0], int(page_size), N)
-    return step
+    buf = torch.empty(2 * B + 2 + 2 * N, dtype=torch.int32, device=dev)
+    at = buf.data_ptr()
+    _run("ws_pages_extend", dev, page_table.data_ptr(), len_in.data_ptr(), n_new.data_ptr(),
+         stack.data_ptr(), free_in.data_ptr(), _ptr(pos_base), at, at + 4 * B, at + 8 * B + 4,
+         at + 8 * B + 4 + 4 * N, at + 8 * B + 4 + 8 * N, B, max_pages, int(num_pages),
+         stack.shape[0], int(page_size), N)
+    return PageStep(*buf.split_with_sizes((B, B + 1, N, N, 1)))
 
 
 def pages_release(page_table, len_in, done, stack, free_in, page_size):
     """The pages of the sequences with done[b] (bool [B]) back on the stack, in
     place (ws_pages_release).  Returns (lengths: 0 for those, free pages)."""
     dev = _gpu(page_table, "page_table")
-    _require(page_table, "page_table", torch.int32, dev, 2)
-    _require(len_in, "len_in", torch.int32, dev, 1)
-    _require(done, "done", torch.bool, dev, 1)
-    _require(stack, "stack", torch.int32, dev, 1)
-    _require(free_in, "free_in", torch.int32, dev, 1)
+    _require_all(dev, _RELEASE_ARGS, (page_table, len_in, done, stack, free_in))
     B, max_pages = page_table.shape
     if len_in.shape[0] != B or done.shape[0] != B or free_in.shape[0] != 1:
         raise ValueError("len_in and done must be [B] and free_in [1]")
-    len_out, free_out = torch.empty(B + 1, dtype=torch.int32, device=dev).split_with_sizes((B, 1))
-    _run("ws_pages_release", dev, _ptr(page_table), _ptr(len_in), _ptr(done), _ptr(stack),
-         _ptr(free_in), len_out.data_ptr(), free_out.data_ptr(), B, max_pages, stack.shape[0],
+    buf = torch.empty(B + 1, dtype=torch.int32, device=dev)
+    at = buf.data_ptr()
+    _run("ws_pages_release", dev, page_table.data_ptr(), len_in.data_ptr(), done.data_ptr(),
+         stack.data_ptr(), free_in.data_ptr(), at, at + 4 * B, B, max_pages, stack.shape[0],
          int(page_size))
-    return len_out, free_out
+    return buf.split_with_sizes((B, 1))
 
 
 @functools.lru_cache(maxsize=256)
@@ -1173,19 +1191,19 @@ def rope(q, k, positions, inv_freq, pair_axis=None, adjacent=False, factor=1.0, 
 
 def _pools(k_pages, v_pages, k_scale, v_scale, dev):
     """(num_pages, Hkv, page_size, D) of bf16 pools, or of 8-bit ones with scales."""
-    dt = torch.bfloat16 if k_scale is None else E4M3
-    _require(k_pages, "k_pages", dt, dev, 4)
-    _require(v_pages, "v_pages", dt, dev, 4)
-    if k_pages.shape != v_pages.shape:
-        raise ValueError("k/v page pools differ in shape")
-    if (k_scale is None) != (v_scale is None):
-        raise ValueError("8-bit pools take both k_scale and v_scale")
-    if k_scale is not None:
-        _require(k_scale, "k_scale", E8M0, dev, 3)
-        _require(v_scale, "v_scale", E8M0, dev, 3)
-        if k_scale.shape != k_pages.shape[:3] or v_scale.shape != k_pages.shape[:3]:
+    shape = k_pages.shape
+    if k_scale is None and v_scale is None:
+        _require_all(dev, _POOL_ARGS[16], (k_pages, v_pages))
+    else:
+        if k_scale is None or v_scale is None:
+            raise ValueError("8-bit pools take both k_scale and v_scale")
+        _require_all(dev, _POOL_ARGS[8], (k_pages, v_pages))
+        _require_all(dev, _SCALE_ARGS, (k_scale, v_scale))
+        if k_scale.shape != shape[:3] or v_scale.shape != k_scale.shape:
             raise ValueError("k_scale and v_scale must be [num_pages, Hkv, page_size]")
-    return k_pages.shape
+    if v_pages.shape != shape:
+        raise ValueError("k/v page pools differ in shape")
+    return shape
 
 
 def rope_append(q, k, v, positions, inv_freq, slots, k_pages, v_pages, k_scale=None, v_scale=None,
@@ -1205,9 +1223,10 @@ def rope_append(q, k, v, positions, inv_freq, slots, k_pages, v_pages, k_scale=N
                          f"{tuple(k_pages.shape)} do not match")
     if q_out is None:
         q_out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=dev)
-    _require(q_out, "q_out", torch.bfloat16, dev, 3)
-    if q_out.shape != q.shape:
-        raise ValueError("q_out must have q's shape")
+    else:
+        _require(q_out, "q_out", torch.bfloat16, dev, 3)
+        if q_out.shape != q.shape:
+            raise ValueError("q_out must have q's shape")
     if N == 0:
         return q_out
     _run("ws_rope_append", dev, _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(positions), axes,
@@ -1238,32 +1257,39 @@ def _gqa8_decode(name, q, k_pages, v_pages, k_scale, v_scale, page_table, gpu_le
     if k_scale is None or v_scale is None:
         raise ValueError("8-bit pools take both k_scale and v_scale")
     P, Hkv, PS, D = _pools(k_pages, v_pages, k_scale, v_scale, dev)
-    _require(q, "q", torch.bfloat16, dev, 3)
-    _require(page_table, "page_table", torch.int32, dev, 2)
-    _require(gpu_len, "gpu_len", torch.int32, dev, 1)
+    _require_all(dev, _DECODE8_ARGS, (q, page_table, gpu_len))
     B, Hq, Dq = q.shape
     if Dq != D or Hkv == 0 or Hq % Hkv:
         raise ValueError(f"q {tuple(q.shape)} does not match the pools {tuple(k_pages.shape)}")
     if page_table.shape[0] != B or gpu_len.shape[0] != B:
         raise ValueError("page_table/gpu_len batch mismatch")
-    if out is None:
-        out = torch.empty((B, Hq, D), dtype=torch.float32, device=dev)
     if lse is None:
         lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
-    _require(out, "out", torch.float32, dev, 3)
-    _require(lse, "lse", torch.float32, dev, 2)
-    if out.shape != q.shape or lse.shape != (B, Hq):
-        raise ValueError("out must be [B, Hq, D] and lse [B, Hq]")
+    else:
+        _require(lse, "lse", torch.float32, dev, 2)
+        if lse.shape != (B, Hq):
+            raise ValueError("lse must be [B, Hq]")
+    if out is not None:
+        _require(out, "out", torch.float32, dev, 3)
+        if out.shape != q.shape:
+            raise ValueError("out must be [B, Hq, D]")
+    elif out_bf16 is None:
+        out = torch.empty((B, Hq, D), dtype=torch.float32, device=dev)
     if B == 0:
         return out, lse
     nwg, wsb = gqa8_plan(B * Hkv, Hq // Hkv, D, int(max_len), int(n_workgroups))
     # the call's own: a buffer kept between calls would be shared by graphs that
     # were captured one after the other and replay together
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    outs = (_ptr(out), _ptr(lse)) if out_bf16 is None else (_ptr(out_bf16), _ptr(out), _ptr(lse))
-    _run(name, dev, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
-         _ptr(page_table), _ptr(gpu_len), B, Hq, Hkv, D, PS, page_table.shape[1], P, int(max_len),
-         nwg, float(scale), *outs, _ptr(ws), wsb)
+    wsb = (wsb + 255) & ~255
+    if out_bf16 is None:
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        outs = (out.data_ptr(), lse.data_ptr(), ws.data_ptr())
+    else:  # the fp32 output, which the merge rounds, lies behind the pieces
+        ws = torch.empty(wsb + 4 * B * Hq * D, dtype=torch.uint8, device=dev)
+        outs = (out_bf16.data_ptr(), ws.data_ptr() + wsb, lse.data_ptr(), ws.data_ptr())
+    _run(name, dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(),
+         v_scale.data_ptr(), page_table.data_ptr(), gpu_len.data_ptr(), B, Hq, Hkv, D, PS,
+         page_table.shape[1], P, int(max_len), nwg, float(scale), *outs, wsb)
     return out, lse
 
 
@@ -1322,10 +1348,7 @@ def gqa_prompt(q, k_pages, v_pages, page_table, kv_len, cu_new, scale, max_len, 
     the lengths)."""
     dev = _gpu(k_pages, "k_pages")
     P, Hkv, PS, D = _pools(k_pages, v_pages, k_scale, v_scale, dev)
-    _require(q, "q", torch.bfloat16, dev, 3)
-    _require(page_table, "page_table", torch.int32, dev, 2)
-    _require(kv_len, "kv_len", torch.int32, dev, 1)
-    _require(cu_new, "cu_new", torch.int32, dev, 1)
+    _require_all(dev, _PROMPT_ARGS, (q, page_table, kv_len, cu_new))
     N, Hq, Dq = q.shape
     B = page_table.shape[0]
     if Dq != D or Hkv == 0 or Hq % Hkv or Hq == 0:
@@ -1336,17 +1359,18 @@ def gqa_prompt(q, k_pages, v_pages, page_table, kv_len, cu_new, scale, max_len, 
         if out_dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("out_dtype must be bfloat16 or float32")
         out = torch.empty((N, Hq, D), dtype=out_dtype, device=dev)
-    if want_lse and lse is None:
-        lse = torch.empty((N, Hq), dtype=torch.float32, device=dev)
-    if out.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError("out must be bfloat16 or float32")
-    _require(out, "out", out.dtype, dev, 3)
-    if out.shape != q.shape:
-        raise ValueError("out must have q's shape")
+    else:
+        if out.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError("out must be bfloat16 or float32")
+        _require(out, "out", out.dtype, dev, 3)
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
     if lse is not None:
         _require(lse, "lse", torch.float32, dev, 2)
         if lse.shape != (N, Hq):
             raise ValueError("lse must be [N, Hq]")
+    elif want_lse:
+        lse = torch.empty((N, Hq), dtype=torch.float32, device=dev)
     if N == 0 or B == 0:
         return out, lse
     _, wsb = gqa_prompt_plan(N, B, Hq, Hkv, D, int(max_len), int(n_splits), k_scale is not None)
