@@ -4,7 +4,8 @@ decode attention returning (out, lse), and the LSE merge with the host partial.
 
 Modules
   ops            ctypes operator layer over lib/libwsgpu.so (include/wsgpu.h)
-  cache          paged HBM partitions and host+GPU partitioned caches
+  cache          paged HBM partitions (pages from a host free list, or handed out on
+                 the GPU for requests of any lengths) and host+GPU partitioned caches
   partition      boundary / share / page arithmetic (host integers)
   decode         partitioned decode step (GPU partial || host partial -> merge)
   reference_api  the reference's GPU helper signatures on the new kernels

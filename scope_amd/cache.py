@@ -465,3 +465,121 @@ class PartitionedKVCache:
         n = int(self.host_len[layer, b])
         rows = slice(b * self.num_kv_heads, (b + 1) * self.num_kv_heads)
         return self.host_k[layer][rows, :n], self.host_v[layer][rows, :n]
+
+
+class GqaRequestPartition:
+    """HBM pages of a GQA KV cache for requests of any lengths, handed out on the GPU.
+
+    Where GqaGpuPartition's pages come from a host free list, one copy to the
+    device per sequence that needs some, here one launch gives every sequence of
+    the batch the pages its new tokens need and every token its slot
+    (ops.pages_extend); the host keeps a mirror of the lengths and of the number
+    of free pages, so that nothing waits for the device.  A forward step of the
+    batch is
+      begin(n_new)            pages and slots for n_new[b] tokens of sequence b
+      append(layer, q, k, v)  q rotated; k rotated, and v, into the pages
+      attend(layer, q)        every new token over all the sequence's tokens so far
+    with the tokens of all sequences packed one after the other ([N, heads, D]), for
+    prompts, chunks of them and single tokens alike.  bits 16: bf16 pages; 8: e4m3
+    with one power-of-two scale per token and KV head, half the bytes.
+    """
+
+    def __init__(self, num_layers, batch, num_kv_heads, head_dim, max_tokens, page_size=64,
+                 num_pages=None, bits=16, device="cuda"):
+        if page_size <= 0 or page_size % 32:
+            raise ValueError("page_size must be a positive multiple of 32")
+        if head_dim % 32 or not 32 <= head_dim <= 256:
+            raise ValueError("head_dim must be a multiple of 32 up to 256")
+        if bits not in (8, 16):
+            raise ValueError("bits must be 8 or 16")
+        self.device = torch.device(device)
+        self.num_layers, self.batch, self.bits = num_layers, batch, bits
+        self.num_kv_heads, self.head_dim, self.page_size = num_kv_heads, head_dim, page_size
+        self.max_pages = max(1, pages_for(max_tokens, page_size))
+        self.num_pages = num_pages if num_pages is not None else batch * self.max_pages
+        shape = (num_layers, self.num_pages, num_kv_heads, page_size, head_dim)
+        if bits == 16:
+            self.k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            self.v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            self.k_scale = self.v_scale = None
+        else:
+            self.k, self.v = (torch.empty(shape, dtype=ops.E4M3, device=self.device) for _ in range(2))
+            self.k_scale, self.v_scale = (torch.empty(shape[:4], dtype=ops.E8M0, device=self.device)
+                                          for _ in range(2))
+        int32 = dict(dtype=torch.int32, device=self.device)
+        self.page_table = torch.full((batch, self.max_pages), -1, **int32)
+        self.stack = torch.arange(self.num_pages - 1, -1, -1, **int32)  # page 0 on top
+        self.free_dev = torch.full((1,), self.num_pages, **int32)
+        self.len_dev = torch.zeros(batch, **int32)
+        self.lens = np.zeros(batch, np.int64)  # host mirrors
+        self.free = self.num_pages
+        self.n_new = np.zeros(batch, np.int64)
+        self.step = None  # the ops.PageStep of the latest begin()
+
+    def _pages(self, lens) -> int:
+        return int(((lens + self.page_size - 1) // self.page_size).sum())
+
+    def begin(self, n_new, pos_base=None) -> "ops.PageStep":
+        """Pages and slots for n_new[b] more tokens of every sequence (0: none).
+        pos_base [B] int32 on the device: tokens of each sequence that are held
+        elsewhere, which its positions count too.  What does not fit is refused
+        before anything changes."""
+        n = np.asarray(n_new, np.int64)
+        if n.shape != (self.batch,) or (n < 0).any():
+            raise ValueError(f"n_new must hold {self.batch} counts >= 0")
+        lens = self.lens + n
+        if (lens > self.max_pages * self.page_size).any():
+            raise ValueError(f"a sequence's tokens exceed capacity {self.max_pages * self.page_size}")
+        need = self._pages(lens) - self._pages(self.lens)
+        if need > self.free:
+            raise MemoryError("HBM page pool exhausted")
+        n_dev = torch.from_numpy(n.astype(np.int32)).to(self.device)
+        self.step = ops.pages_extend(self.page_table, self.len_dev, n_dev, self.stack, self.free_dev,
+                                     self.page_size, self.num_pages, int(n.sum()), pos_base)
+        self.len_dev, self.free_dev = self.step.len_out, self.step.free_out
+        self.lens, self.n_new, self.free = lens, n, self.free - need
+        return self.step
+
+    def _step(self) -> "ops.PageStep":
+        if self.step is None:
+            raise RuntimeError("begin() comes first")
+        return self.step
+
+    def append(self, layer: int, q, k, v, inv_freq, positions=None, **rope):
+        """Rotary positions of q [N, Hq, D] and k [N, Hkv, D], and k and v into the
+        step's slots of `layer` (ops.rope_append; positions [N] or [axes, N], the
+        step's own by default).  Returns the rotated q."""
+        step = self._step()
+        return ops.rope_append(
+            q, k, v, step.positions if positions is None else positions, inv_freq, step.slots,
+            self.k[layer], self.v[layer], None if self.bits == 16 else self.k_scale[layer],
+            None if self.bits == 16 else self.v_scale[layer], **rope)
+
+    def attend(self, layer: int, q, scale: float, out_dtype=torch.float32):
+        """The step's tokens, q [N, Hq, D] rotated, over the pages: (out [N, Hq, D] in
+        out_dtype (fp32 or bf16), lse [N, Hq]), which merges with a host partial as
+        the other partitions' (ops.lse_merge).  One token of every sequence runs the
+        decode kernels, anything else the prompt kernel."""
+        self._step()
+        Hq, max_len = q.shape[1], int(self.lens.max()) if self.batch else 0
+        k, v = self.k[layer], self.v[layer]
+        ks, vs = (None, None) if self.bits == 16 else (self.k_scale[layer], self.v_scale[layer])
+        if (self.n_new == 1).all() and Hq <= 16 * self.num_kv_heads and out_dtype == torch.float32:
+            if self.bits == 16:
+                return ops.gqa_decode_partial(q, k, v, self.page_table, self.len_dev, scale, max_len)
+            return ops.gqa8_decode_partial(q, k, v, ks, vs, self.page_table, self.len_dev, scale, max_len)
+        if (self.n_new == 1).all() and Hq <= 16 * self.num_kv_heads and self.bits == 8:
+            return ops.gqa8_decode_full(q, k, v, ks, vs, self.page_table, self.len_dev, scale, max_len)
+        return ops.gqa_prompt(q, k, v, self.page_table, self.len_dev, self.step.cu_new, scale, max_len,
+                              ks, vs, out_dtype=out_dtype)
+
+    def release(self, sequences) -> None:
+        """Drop all tokens of the given sequences; their pages are free again."""
+        done = np.zeros(self.batch, bool)
+        done[list(sequences)] = True
+        self.len_dev, self.free_dev = ops.pages_release(
+            self.page_table, self.len_dev, torch.from_numpy(done).to(self.device), self.stack,
+            self.free_dev, self.page_size)
+        self.free += self._pages(self.lens[done])
+        self.lens = np.where(done, 0, self.lens)
+        self.step = None
