@@ -17,6 +17,10 @@ cache (system/deepseek.py:144-209): the leading `gs` tokens of each sequence
 in pinned host memory, the rest in an MlaGpuPartition.
 PartitionedKVCache is the GQA analogue (system/mixoffload.py:51-144 holds the
 whole cache on the host; here the trailing range lives in HBM).
+
+GqaRequestPartition holds the GQA pages of requests of any lengths, bf16 or
+8-bit: pages and slots handed out on the GPU, rotary positions with the write
+into the pages, prompts and single tokens attended over them.
 """
 from __future__ import annotations
 
@@ -481,7 +485,9 @@ class GqaRequestPartition:
       attend(layer, q)        every new token over all the sequence's tokens so far
     with the tokens of all sequences packed one after the other ([N, heads, D]), for
     prompts, chunks of them and single tokens alike.  bits 16: bf16 pages; 8: e4m3
-    with one power-of-two scale per token and KV head, half the bytes.
+    with one power-of-two scale per token and KV head, half the bytes.  begin() and
+    release() copy counts from the host, so a captured step calls the ops on the
+    partition's tensors instead (with the capacity as max_len).
     """
 
     def __init__(self, num_layers, batch, num_kv_heads, head_dim, max_tokens, page_size=64,
@@ -560,7 +566,11 @@ class GqaRequestPartition:
         out_dtype (fp32 or bf16), lse [N, Hq]), which merges with a host partial as
         the other partitions' (ops.lse_merge).  One token of every sequence runs the
         decode kernels, anything else the prompt kernel."""
-        self._step()
+        step = self._step()
+        if q.dim() != 3 or q.shape[0] != step.slots.shape[0]:
+            raise ValueError(f"q must hold the step's {step.slots.shape[0]} tokens (got {tuple(q.shape)})")
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("out_dtype must be float32 or bfloat16")
         Hq, max_len = q.shape[1], int(self.lens.max()) if self.batch else 0
         k, v = self.k[layer], self.v[layer]
         ks, vs = (None, None) if self.bits == 16 else (self.k_scale[layer], self.v_scale[layer])
@@ -570,7 +580,7 @@ class GqaRequestPartition:
             return ops.gqa8_decode_partial(q, k, v, ks, vs, self.page_table, self.len_dev, scale, max_len)
         if (self.n_new == 1).all() and Hq <= 16 * self.num_kv_heads and self.bits == 8:
             return ops.gqa8_decode_full(q, k, v, ks, vs, self.page_table, self.len_dev, scale, max_len)
-        return ops.gqa_prompt(q, k, v, self.page_table, self.len_dev, self.step.cu_new, scale, max_len,
+        return ops.gqa_prompt(q, k, v, self.page_table, self.len_dev, step.cu_new, scale, max_len,
                               ks, vs, out_dtype=out_dtype)
 
     def release(self, sequences) -> None:

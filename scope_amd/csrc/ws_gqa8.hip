@@ -8,7 +8,7 @@
 //
 //  - A token of a head is D + 1 bytes for K and for V each, half the bf16 pool's,
 //    so a wave's block is half as large: keeping the same bytes in flight takes
-//    twice the waves or stages (kGqa8Stages, gqa8_splits).
+//    twice the waves or stages (gqa8_stages, gqa8_splits).
 //  - The value times its scale is a bf16 number (an e4m3 value has 4 significant
 //    bits, and a power of two moves the exponent only), so converting with the
 //    scale is exact and the matrix products are the bf16 pool's:

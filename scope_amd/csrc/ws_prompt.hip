@@ -6,7 +6,7 @@
 // len - n + i of the len tokens in the pages and sees positions 0 .. its own.
 // The query rows of a KV head are (token, head of the group) pairs, row = i G + g,
 // so the G heads that share K and V share their loads: a workgroup takes a tile of
-// 32 RB NW consecutive rows, a wave 32 RB of them, and walks the tokens in tiles
+// 32 NW consecutive rows, a wave 32 of them, and walks the tokens in tiles
 // of 32 through LDS with a running maximum and sum (one pass over K and V).
 //
 //   S^T[token, row] = K Q^T   A = K from LDS (16 bytes a lane), B = Q in registers
@@ -172,7 +172,7 @@ __device__ __forceinline__ PromptPlace prompt_place(const PromptParams& p, int a
     float total = 0.f;
     for (int k = 0; k < per && b0 + k < p.B; ++k) {
       const PromptSeq s = prompt_seq(p, b0 + k, rows);
-      total += (float)s.tiles * (float)s.blocks;
+      total = fmaf((float)s.tiles, (float)s.blocks, total);  // (the same in both kernels)
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);

@@ -169,7 +169,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p, 
       for (int o = 1; o < (1 << p.lanes_log2); o <<= 1)
         top = max(top, (uint32_t)__shfl_xor((int)top, o));
       const int byte = e8m0_of(top);
-      // 2^(127 - byte), a denormal for byte 254 (e = 127)
+      // 2^(127 - byte) (bytes 1 to 247)
       const float s = byte == 255 ? qnan() : ldexpf(1.f, 127 - byte);
       uint8_t* dst = (uint8_t*)(is_v ? p.v_pages : p.k_pages) + row * p.D;
       if (on && put) {

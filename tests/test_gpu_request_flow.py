@@ -130,6 +130,21 @@ def test_partition_refuses_before_anything_changes():
                                           max_tokens=10), **bad})
 
 
+@pytest.mark.parametrize("bits", (16, 8))
+def test_attend_refuses_what_is_not_the_step(bits):
+    part = GqaRequestPartition(1, 2, 1, 64, 128, 32, bits=bits)
+    part.begin([3, 2])
+    q = torch.zeros((5, 1, 64), dtype=torch.bfloat16, device=DEV)
+    for bad in (q[:4], torch.cat((q, q[:1])), q[:, 0]):
+        with pytest.raises(ValueError, match="5 tokens"):
+            part.attend(0, bad, 1.0)
+    with pytest.raises(TypeError, match="out_dtype"):
+        part.attend(0, q, 1.0, torch.float16)
+    part.begin([1, 1])
+    with pytest.raises(TypeError, match="out_dtype"):
+        part.attend(0, q[:2], 1.0, torch.float16)
+
+
 def test_merge_with_a_host_share():
     """The leading tokens of a prompt on the host, the rest in the pages: positions
     count both, queries that stand before the partition see nothing of it, and the
