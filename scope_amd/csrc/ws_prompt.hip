@@ -348,6 +348,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     qb[s] = qp[2 * s + h];
 #pragma unroll
     for (int e = 0; e < 4; ++e) qb[s][e] ^= p.q_sign;
+    if constexpr (D > 192) asm volatile("" : "+a"(qb[s]));  // (there is room beside the sums)
   }
 
   f32x16 acc[DT];
@@ -474,15 +475,21 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     return m == neg_inf() ? 0.f : m * p.scale_log2;
   };
   // S^T of a K slot
-  uint32_t ka[KS];
+  // (the order within a group of chunks is every group's, so are the addresses)
+  constexpr int kGroup = prompt_pow2(D);
+  uint32_t ka[kGroup / 2];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
+  for (int ks = 0; ks < kGroup / 2; ++ks)
     ka[ks] = lds_k + n32 * Sh::kRow + 16 * ((2 * ks + h) ^ prompt_k_swap(D, n32));
+  auto keys_operand = [&](int slot, int ks) __attribute__((always_inline)) {
+    return lds_read_b128(ka[ks % (kGroup / 2)] + slot * Sh::kTile +
+                         16 * kGroup * (ks / (kGroup / 2)));
+  };
   auto scores = [&](int slot, f32x16& s) __attribute__((always_inline)) {
     s = f32x16{};
     u32x4 a[KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) a[ks] = lds_read_b128(ka[ks] + slot * Sh::kTile);
+    for (int ks = 0; ks < KS; ++ks) a[ks] = keys_operand(slot, ks);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
       s = mfma32x32x16(a[ks], qb[ks], s);
@@ -532,15 +539,17 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   // transposed
   const int g4 = lane >> 4;
   const int l16 = lane & 15;
-  uint32_t va[DT];
+  constexpr int kVa = kGroup / 4;
+  uint32_t va[kVa];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) {
+  for (int d = 0; d < kVa; ++d) {
     const int row = 4 * (g4 >> 1) + (l16 >> 2);  // (its swap is that of rows 8 k away)
     va[d] = lds_v + row * Sh::kRow + 8 * (l16 & 1) +
             16 * ((4 * d + 2 * (g4 & 1) + ((l16 & 3) >> 1)) ^ prompt_v_swap(D, row));
   }
   auto values_operand = [&](int slot, int ks, int d) __attribute__((always_inline)) {
-    const uint32_t at = va[d] + slot * Sh::kTile + 16 * ks * Sh::kRow;
+    const uint32_t at =
+        va[d % kVa] + slot * Sh::kTile + 16 * ks * Sh::kRow + 16 * kGroup * (d / kVa);
     const uint2 x = lds_read_tr_b64(at);
     const uint2 y = lds_read_tr_b64(at + 8 * Sh::kRow);
     return u32x4{x.x, x.y, y.x, y.y};
@@ -552,6 +561,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
       for (int d = 0; d < DT; ++d) {
         const u32x4 a = values_operand(slot, ks, d);
         acc[d] = mfma32x32x16(a, pb[ks], acc[d]);
+        if (kAcc) pin_sum<kAcc>(acc[d]);
       }
   };
   // The same where the slot holds an infinity or a NaN that some rows do not see: the
@@ -586,11 +596,11 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
         if (pos[i] > 0.f) acc[d][i] -= neg_inf();
         if (neg[i] > 0.f) acc[d][i] += neg_inf();
       }
+      if (kAcc) pin_sum<kAcc>(acc[d]);
     }
   };
   // acc times alpha, where some row's maximum moved
   auto rescale = [&](const float& alpha) __attribute__((always_inline)) {
-    
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(alpha != 1.f) == 0, 1)) return;
     float f = alpha;
     asm("" : "+v"(f));  // (else the products are taken every step, ahead of the test)
@@ -662,9 +672,10 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
         // runs the exponentials after the products).
         constexpr int kExp = 16 / KS > 0 ? (16 + KS - 1) / KS : 1;
         constexpr int kAhead = DT > 1 ? 3 : 2;  // V operands under way
+        constexpr int kKeys = 8;                // and K operands
         u32x4 a[KS], av[2 * DT];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) a[ks] = lds_read_b128(ka[ks] + ((c + 1) & 3) * Sh::kTile);
+        for (int ks = 0; ks < KS && ks < kKeys; ++ks) a[ks] = keys_operand((c + 1) & 3, ks);
         float mc, ps, bm;
         mc = ref(m_run);
         ps = 0.f;
@@ -673,6 +684,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
         for (int ks = 0; ks < KS; ++ks) {
           s[u ^ 1] = mfma32x32x16(a[ks], qb[ks], ks == 0 ? f32x16{} : s[u ^ 1]);
           pin_sum<kAcc>(s[u ^ 1]);
+          if (ks + kKeys < KS) a[ks + kKeys] = keys_operand((c + 1) & 3, ks + kKeys);
 #pragma unroll
           for (int e = ks * kExp; e < (ks + 1) * kExp && e < 16; ++e) {
             float x = s[u][e];
