@@ -25,6 +25,11 @@
 // With few rows the tokens are split over several workgroups of a tile, so that all
 // take about as many, whatever the sequences' lengths; prompt_join_kernel combines
 // their pieces (fp32, with their lse).
+//
+// Long prompts are bound by the power of the products and by the vector work beside them:
+// 8192 tokens of 8 x 4 heads of 128 take 525 to 542 us (1.01 to 1.05 PFLOP/s; 392 on
+// zeros, at a higher clock).  Few rows are bound by HBM: 567 MB in 93.7 us (6.1 TB/s) and
+// the join 5.0.
 #include <algorithm>
 #include <type_traits>
 
