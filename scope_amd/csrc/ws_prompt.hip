@@ -240,7 +240,7 @@ __device__ __forceinline__ PromptPlace prompt_place(const PromptParams& p, int a
   return r;
 }
 
-constexpr int kPromptWaves = 4;  // of a workgroup (one in calls of few rows, prompt_plan)
+constexpr int kPromptWaves = 4;  // of a workgroup (one in some calls, prompt_plan)
 template <int D, bool F8, int NW>
 struct PromptShape {
   static constexpr int kRow = 2 * D;               // bytes of a row in LDS
@@ -874,11 +874,14 @@ static bool prompt_width_ok(int D) { return D >= 32 && D <= kPromptMaxD && D % 3
 //
 // Calls of few rows: a sequence's rows of a KV head fill half a tile on average, at the
 // most, and K and V are read about once, so the reads are the bound.  bf16 up to 128
-// columns: a wave by itself per 32 rows needs no barrier, and several on a CU keep as much
-// under way (8 x 5 tokens of 4 x 8 heads over 4000 to 32000: 97 us against 111 with four
-// waves that share the loads; 16 x 8 over 2000: 34 against 42).  8-bit pages take four
-// waves' conversions (8 x 16 over 8000: 107 us with one wave, 63 with four), and wider heads
-// four waves' registers (256 columns, 8 x 5 over 16000: 262 and 211).
+// columns, rows that one wave holds: a wave by itself needs no barrier, and several on a CU
+// keep as much under way (8 x 5 tokens of 8 x 4 heads over 4000 to 32000: 97 us against 111
+// with four waves that share the loads; 16 x 8 over 2000: 34 against 42).  Twice the rows
+// would read K and V twice (12 tokens over 16000: 130 us with one wave, 110 with four; 16
+// over 8000 81 and 68, the other way in a small batch, 4 x 8 of 4 x 8 heads, 29 and 31).
+// 8-bit pages take four waves' conversions (8 x 16 over 8000: 107 us with one wave, 63 with
+// four), and wider heads four waves' registers (256 columns, 8 x 5 over 16000, at the time
+// 262 and 211).
 struct PromptPlan {
   bool few;
   int waves;         // of a workgroup
@@ -893,7 +896,7 @@ static PromptPlan prompt_plan(int N, int B, int Hq, int Hkv, int D, bool fp8, in
   const int G = Hq / Hkv;
   PromptPlan r;
   r.few = (long long)N * G <= 64LL * B;
-  r.waves = r.few && !fp8 && D <= 128 ? 1 : kPromptWaves;
+  r.waves = (long long)N * G <= 32LL * B && !fp8 && D <= 128 ? 1 : kPromptWaves;
   r.rows = 32 * r.waves;
   const long long full = ((long long)N * G + r.rows - 1) / r.rows;
   r.tiles = (full + B) * Hkv;
@@ -927,9 +930,14 @@ static size_t prompt_bytes(const PromptPlan& pl, int D) {
 template <int D, bool F8>
 static void prompt_launch(const PromptParams& p, const PromptPlan& pl, hipStream_t s) {
   const dim3 grid((unsigned)pl.grid), block(64 * pl.waves);
-  constexpr int kFewWaves = !F8 && D <= 128 ? 1 : kPromptWaves;  // (prompt_plan)
+  if constexpr (!F8 && D <= 128) {
+    if (pl.waves == 1) {
+      hipLaunchKernelGGL((prompt_kernel<D, F8, 1, true>), grid, block, 0, s, p);
+      return;
+    }
+  }
   if (pl.few)
-    hipLaunchKernelGGL((prompt_kernel<D, F8, kFewWaves, true>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((prompt_kernel<D, F8, kPromptWaves, true>), grid, block, 0, s, p);
   else
     hipLaunchKernelGGL((prompt_kernel<D, F8, kPromptWaves, false>), grid, block, 0, s, p);
 }
