@@ -421,6 +421,26 @@ def test_prompt(bits, D, Hkv, G, page, lens, new, splits):
     R.check(o16, want_o, tol_o + want_o.abs() * 2.0 ** -8, "bf16 out")
 
 
+@pytest.mark.parametrize("bits", (16, 8))
+@pytest.mark.parametrize("splits", (0, 1, 4))
+@pytest.mark.parametrize("D, G, lens, new", [
+    # rows of more than one wave and up to two, on average
+    (32, 3, [700, 90], [14, 9]), (64, 7, [64, 900, 31], [9, 6, 4]), (96, 2, [520, 33], [32, 20]),
+    (128, 4, [1000, 40, 65], [16, 9, 11]), (160, 3, [300, 310], [20, 12]), (256, 8, [290, 64], [7, 5]),
+    # few on average, but many of one sequence
+    (128, 1, [400, 9, 5, 70, 33, 32, 64], [300, 1, 0, 3, 2, 1, 1]), (64, 2, [200] + [40] * 12, [150] + [1] * 12)])
+def test_prompt_few_rows(bits, splits, D, G, lens, new):
+    page = 64
+    table, P, cpu, (k, v, ks, vs) = pools_of(lens, 2, D, page, bits, 31 + D)
+    q, scale = bf16_randn((sum(new), 2 * G, D), 8), D ** -0.5
+    want_o, want_l, tol_o, tol_l = prompt_want(q, cpu, table, lens, new, page, 2, scale)
+    out, lse = ops.gqa_prompt(q.to(DEV), k, v, ints(table), ints(lens),
+                              ints(np.concatenate([[0], np.cumsum(new)])), scale, max(lens), ks, vs,
+                              n_splits=splits, out_dtype=torch.float32)
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
+
+
 def test_prompt_packed_elsewhere():
     """Rows before the first and behind the last sequence keep what they held, at any
     split count."""
