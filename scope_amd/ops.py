@@ -1137,6 +1137,12 @@ def rope_sections(sections, interleaved=False) -> list:
 def _rope_rows(t, name, dev, N=None, D=None):
     """(heads, token stride) of a [N, heads, D] bf16 operand whose tokens may be
     strided (a slice of a fused projection's rows)."""
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.get_device() == dev.index
+            and t.dim() == 3):  # (as below, in one pass while all is well)
+        n, heads, d = t.shape
+        st, sh, sd = t.stride()
+        if n and heads and sd == 1 and sh == d and (N is None or n == N) and (D is None or d == D):
+            return heads, (st if n > 1 else heads * d)
     _require(t, name, torch.bfloat16, dev, 3, contiguous=False)
     n, heads, d = t.shape
     if (N is not None and n != N) or (D is not None and d != D):
@@ -1152,9 +1158,10 @@ def _rope_args(q, k, positions, inv_freq, pair_axis, dev):
     Hkv, k_stride = _rope_rows(k, "k", dev, N, D)
     _require(positions, "positions", torch.int32, dev)
     _require(inv_freq, "inv_freq", torch.float32, dev, 1)
-    if positions.dim() not in (1, 2) or positions.shape[-1] != N:
-        raise ValueError(f"positions must be [N] or [axes, N], N = {N} (got {tuple(positions.shape)})")
-    axes = positions.shape[0] if positions.dim() == 2 else 1
+    shape = positions.shape
+    if len(shape) not in (1, 2) or shape[-1] != N:
+        raise ValueError(f"positions must be [N] or [axes, N], N = {N} (got {tuple(shape)})")
+    axes = shape[0] if len(shape) == 2 else 1
     half = inv_freq.shape[0]
     axis = None
     if pair_axis is not None:
@@ -1175,11 +1182,13 @@ def rope(q, k, positions, inv_freq, pair_axis=None, adjacent=False, factor=1.0, 
     dev = _gpu(q, "q")
     N, Hq, Hkv, D, qs, ks, axes, axis, rot = _rope_args(q, k, positions, inv_freq, pair_axis, dev)
     if q_out is None:
-        q_out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=dev)
+        q_out = q.new_empty((N, Hq, D))
+    else:
+        _require(q_out, "q_out", torch.bfloat16, dev, 3)
     if k_out is None:
-        k_out = torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=dev)
-    _require(q_out, "q_out", torch.bfloat16, dev, 3)
-    _require(k_out, "k_out", torch.bfloat16, dev, 3)
+        k_out = k.new_empty((N, Hkv, D))
+    else:
+        _require(k_out, "k_out", torch.bfloat16, dev, 3)
     if q_out.shape != q.shape or k_out.shape != k.shape:
         raise ValueError("q_out and k_out must have q's and k's shapes")
     if N == 0:
@@ -1222,7 +1231,7 @@ def rope_append(q, k, v, positions, inv_freq, slots, k_pages, v_pages, k_scale=N
         raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)}, slots {tuple(slots.shape)} and pools "
                          f"{tuple(k_pages.shape)} do not match")
     if q_out is None:
-        q_out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=dev)
+        q_out = q.new_empty((N, Hq, D))
     else:
         _require(q_out, "q_out", torch.bfloat16, dev, 3)
         if q_out.shape != q.shape:
@@ -1309,10 +1318,12 @@ def gqa8_decode_full(q, k_pages, v_pages, k_scale, v_scale, page_table, gpu_len,
     (out [B, Hq, D] bf16, lse [B, Hq] fp32)."""
     dev = _gpu(q, "q")
     if out_bf16 is None:
-        out_bf16 = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
-    _require(out_bf16, "out_bf16", torch.bfloat16, dev, 3)
-    if out_bf16.shape != q.shape:
-        raise ValueError("out_bf16 must have q's shape")
+        _require(q, "q", torch.bfloat16, dev, 3)
+        out_bf16 = torch.empty_like(q)
+    else:
+        _require(out_bf16, "out_bf16", torch.bfloat16, dev, 3)
+        if out_bf16.shape != q.shape:
+            raise ValueError("out_bf16 must have q's shape")
     _, lse = _gqa8_decode("ws_gqa8_decode_full", q, k_pages, v_pages, k_scale, v_scale, page_table,
                           gpu_len, scale, max_len, n_workgroups, out_bf16, None, lse)
     return out_bf16, lse
@@ -1358,7 +1369,7 @@ def gqa_prompt(q, k_pages, v_pages, page_table, kv_len, cu_new, scale, max_len, 
     if out is None:
         if out_dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("out_dtype must be bfloat16 or float32")
-        out = torch.empty((N, Hq, D), dtype=out_dtype, device=dev)
+        out = torch.empty_like(q, dtype=out_dtype)
     else:
         if out.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("out must be bfloat16 or float32")
