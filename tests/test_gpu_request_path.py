@@ -579,3 +579,43 @@ def test_refused_tensors():
         ops.gqa_prompt(x, pool, pool, t, l, l, 1.0, 3)
     with pytest.raises(TypeError, match="bfloat16 or float32"):
         ops.gqa_prompt(x, pool, pool, t, l, pos[:3], 1.0, 3, out_dtype=torch.float16)
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+def test_pools_past_4_gib(bits):
+    """The same pages at the far end of pools of more than 2^32 bytes: the same bits."""
+    D, Hkv, page, lens, new = 256, 2, 64, [200, 90], [40, 3]
+    table, P, _, small = pools_of(lens, Hkv, D, page, bits, 77)
+    Pb = 70000 * 16 // bits
+    shift = Pb - P
+    far = np.where(table >= 0, table + shift, table).astype(np.int32)
+    big = [None if t is None else torch.zeros((Pb,) + t.shape[1:], dtype=torch.uint8, device=DEV).view(t.dtype)
+           if t.element_size() == 1 else torch.zeros((Pb,) + t.shape[1:], dtype=t.dtype, device=DEV)
+           for t in small]
+    assert big[0].numel() * big[0].element_size() > 1 << 32
+
+    def raw(t):
+        return t.view(torch.uint8)
+
+    N = 50
+    q, k, v = (bf16_randn((N, h, D), 5 + i).to(DEV) for i, h in enumerate((4, Hkv, Hkv)))
+    pos, inv = ints(np.arange(N)), (1e4 ** (-torch.arange(D // 2) / (D // 2))).float().to(DEV)
+    slots = np.array([int(table[0, t // page]) * page + t % page for t in range(100, 100 + N)])
+    for pools, t, s in ((small, table, slots), (big, far, slots + shift * page)):
+        if pools is big:
+            for a, b in zip(pools, start):
+                if a is not None:
+                    raw(a)[shift:] = raw(b)
+        else:
+            start = [None if x is None else x.clone() for x in small]
+        ops.rope_append(q, k, v, pos, inv, ints(s), *pools)
+    for a, b in zip(big, small):
+        if a is not None:
+            assert torch.equal(raw(a)[shift:], raw(b)) and not bool(a.view(torch.int32)[:shift].any())
+    q = q[:sum(new)]
+    calls = [lambda p, t: ops.gqa_prompt(q, p[0], p[1], ints(t), ints(lens), ints([0, 40, 43]), 0.1, 200, p[2], p[3])]
+    if bits == 8:
+        calls.append(lambda p, t: ops.gqa8_decode_partial(q[:2], *p, ints(t), ints(lens), 0.1, 200))
+    for call in calls:
+        for x, y in zip(call(small, table), call(big, far)):
+            assert bool(x.isfinite().all()) and torch.equal(x, y)
