@@ -308,9 +308,14 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   constexpr int CH = Sh::kRowPieces;
   constexpr int LD = Sh::kLoads;
   constexpr int kRows = 32 * NW;
+  // k-steps whose q lies in LDS, for the registers that 8-bit tiles take on their way: what
+  // the compiler spilled instead came back behind the loads under way, which memory answers
+  // in order (8 x 12 tokens over 16000: 114 -> 88 us, 8-bit chunks 381 -> 362)
+  constexpr int kQl = F8 && D == 128 ? 2 : 0;
   constexpr bool kAcc = D > 128 || NW == 1;  // more than 256 registers
   __shared__ __attribute__((aligned(256))) char s_k[kPromptSlots * Sh::kTile];
   __shared__ __attribute__((aligned(256))) char s_v[kPromptSlots * Sh::kTile];
+  __shared__ u32x4 s_q[kQl > 0 ? kQl * Sh::kThreads : 1];
   __shared__ int s_bad[2];  // a slot's values held an infinity or a NaN (masked tiles only)
 
   const int tid = threadIdx.x;
@@ -355,6 +360,12 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     for (int e = 0; e < 4; ++e) qb[s][e] ^= p.q_sign;
     if constexpr (D > 192) asm volatile("" : "+a"(qb[s]));  // (there is room beside the sums)
   }
+
+#pragma unroll
+  for (int j = 0; j < kQl; ++j) s_q[j * Sh::kThreads + tid] = qb[KS - kQl + j];  // (the lane's own)
+  auto q_operand = [&](int ks) __attribute__((always_inline)) {
+    return ks < KS - kQl ? qb[ks] : s_q[(ks - (KS - kQl)) * Sh::kThreads + tid];
+  };
 
   f32x16 acc[DT];
   float m_run, l_run;
@@ -497,7 +508,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
     for (int ks = 0; ks < KS; ++ks) a[ks] = keys_operand(slot, ks);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-      s = mfma32x32x16(a[ks], qb[ks], s);
+      s = mfma32x32x16(a[ks], q_operand(ks), s);
   };
   // a lane's largest score of a tile
   auto row_max = [&](const f32x16& s) __attribute__((always_inline)) {
@@ -678,7 +689,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
         constexpr int kExp = 16 / KS > 0 ? (16 + KS - 1) / KS : 1;
         constexpr int kAhead = DT > 1 ? 3 : 2;  // V operands under way
         constexpr int kKeys = 8;                // and K operands
-        u32x4 a[KS], av[2 * DT];
+        u32x4 a[KS], av[2 * DT], ql[kQl > 0 ? kQl : 1];
 #pragma unroll
         for (int ks = 0; ks < KS && ks < kKeys; ++ks) a[ks] = keys_operand((c + 1) & 3, ks);
         float mc, ps, bm;
@@ -687,8 +698,12 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          s[u ^ 1] = mfma32x32x16(a[ks], qb[ks], ks == 0 ? f32x16{} : s[u ^ 1]);
+          s[u ^ 1] = mfma32x32x16(a[ks], ks < KS - kQl ? qb[ks] : ql[ks - (KS - kQl)],
+                                  ks == 0 ? f32x16{} : s[u ^ 1]);
           pin_sum<kAcc>(s[u ^ 1]);
+#pragma unroll
+          for (int j = 0; j < kQl; ++j)
+            if (ks == KS - kQl + j - 3) ql[j] = q_operand(KS - kQl + j);
           if (ks + kKeys < KS) a[ks + kKeys] = keys_operand((c + 1) & 3, ks + kKeys);
 #pragma unroll
           for (int e = ks * kExp; e < (ks + 1) * kExp && e < 16; ++e) {
@@ -879,7 +894,7 @@ static bool prompt_width_ok(int D) { return D >= 32 && D <= kPromptMaxD && D % 3
 // with four waves that share the loads; 16 x 8 over 2000: 34 against 42).  Twice the rows
 // would read K and V twice (12 tokens over 16000: 130 us with one wave, 110 with four; 16
 // over 8000 81 and 68, the other way in a small batch, 4 x 8 of 4 x 8 heads, 29 and 31).
-// 8-bit pages take four waves' conversions (8 x 16 over 8000: 107 us with one wave, 63 with
+// 8-bit pages take four waves' conversions (8 x 16 over 8000: 107 us with one wave, 57 with
 // four), and wider heads four waves' registers (256 columns, 8 x 5 over 16000, at the time
 // 262 and 211).
 struct PromptPlan {
