@@ -387,10 +387,10 @@ static int gqa8_launch(const uint16_t* q, const uint8_t* k_pages, const uint8_t*
       !aligned16(out_bf16) || ((uintptr_t)v_scale & 3u))
     return set_error(WS_EINVAL, "%s: buffers must be 16-byte aligned (scales: 4)", name);
   if (B == 0) return WS_OK;
+  if (!plan_fits(B, Hkv, max_len))
+    return set_error(WS_EINVAL, "%s: %lld kv rows of %d tokens exceed the block index range", name,
+                     (long long)B * Hkv, max_len);
   const int rows_kv = B * Hkv;
-  if ((long long)rows_kv * ((max_len + 32) / 32) * 4096 >= (1LL << 31))
-    return set_error(WS_EINVAL, "%s: %d kv rows of %d tokens exceed the block index range", name,
-                     rows_kv, max_len);
   const int n = gqa8_splits(n_splits, rows_kv, max_len, D);
   if (n > kMaxSplits)
     return set_error(WS_EINVAL, "%s: %d splits exceed the merge's %d", name, n, kMaxSplits);

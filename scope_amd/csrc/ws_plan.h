@@ -24,7 +24,7 @@ constexpr int kMaxSeqs = 2048;
 constexpr int kMaxSplits = 4096;
 
 struct Plan {
-  int T;  // total blocks (the host keeps it below 2^31 / grid)
+  int T;  // total blocks (the host keeps it below 2^31: plan_fits)
   int n;  // workgroups with work (min(grid, T)), at most kMaxSplits
   int q, r;  // T = q n + r
   // The calling split's range [begin, end) and the sequence of block `begin`.
@@ -45,6 +45,18 @@ constexpr int kSeqPlanMax = 256;
 // KB of outputs out) about ten.
 constexpr int kAlignStep = 1;
 constexpr int kAlignStepWide = 3;
+
+// Whether 32-bit numbers hold for a batch of B sequences of up to max_len tokens (one
+// appended token among them) with R rows each, whatever the lengths: the rows (a merge's
+// grid), the blocks, with room for a metadata window past a range's end, and in the
+// sequence-aligned plan the product of a split's number (up to kMaxSplits) and a
+// sequence's blocks.
+inline bool plan_fits(int B, int R, int max_len) {
+  const long long rows = (long long)B * R;
+  const long long nb = ((long long)max_len + 32) / 32;
+  if (rows > (1LL << 24) || rows * nb >= (1LL << 31) - (1LL << 16)) return false;
+  return R != 1 || B < 2 || B > kSeqPlanMax || nb * kMaxSplits < (1LL << 31);
+}
 
 // Workgroup-uniform value moved to a scalar register.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }

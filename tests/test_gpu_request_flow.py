@@ -284,3 +284,37 @@ def test_two_graphs_and_streams_at_once():
     torch.cuda.synchronize()
     for o, w in zip(got, want):
         assert all(torch.equal(a, b) for a, b in zip(o, w)), "eager on two streams"
+
+
+@pytest.mark.parametrize("bits", (8, 16))
+def test_single_tokens_beside_one_long_request(bits):
+    """A token of each of 256 sequences, one of them long: the worst case of the batch (256
+    times the longest) is past half a million blocks, and the step runs."""
+    B, Hkv, G, D, ps, L = 256, 8, 1, 32, 64, 8200
+    part = GqaRequestPartition(1, B, Hkv, D, L + ps, ps, num_pages=B + L // ps + 2, bits=bits)
+    n_new = np.ones(B, np.int64)
+    n_new[7] = L
+    for n in (n_new, np.ones(B, np.int64)):
+        step = part.begin(n)
+        N = int(n.sum())
+        w = bf16_randn((N, (G + 2) * Hkv * D), 60 + N).to(DEV)
+        q, k, v = (x.view(N, -1, D) for x in w.split((G * Hkv * D, Hkv * D, Hkv * D), 1))
+        inv = torch.zeros(D // 2, device=DEV)  # no turn: the keys are as they came, to a rounding
+        qr = part.append(0, q, k, v, inv)
+    assert int(step.slots.min()) >= 0
+    out, lse = part.attend(0, qr, 0.2)
+    want = [torch.zeros(t, dtype=torch.float64) for t in ((B, Hkv * G, D), (B, Hkv * G)) * 2]
+    table, qc = part.page_table.cpu(), qr.cpu().double()
+    pools = [(p[0].cpu(), None if s is None else s[0].cpu())
+             for p, s in ((part.k, part.k_scale), (part.v, part.v_scale))]
+    for b in range(B):
+        for h in range(Hkv * G):
+            n = int(part.lens[b])
+            kb, vb = (R.tokens_of(p, s, table[b], h // G, n, ps) for p, s in pools)
+            for r, x in zip(want, R.attend(qc[b:b + 1, h], kb, vb, [n], 0.2)):
+                r[b, h] = x[0]
+    want_o, want_l, tol_o, tol_l = want
+    if bits == 16:
+        tol_o = 2 * tol_o  # bf16 pieces: each off by another 2^-8 of its own weighted sum of |v|
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")

@@ -619,3 +619,24 @@ def test_pools_past_4_gib(bits):
     for call in calls:
         for x, y in zip(call(small, table), call(big, far)):
             assert bool(x.isfinite().all()) and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("bits", (8, 16))
+@pytest.mark.parametrize("B, Hkv", [(256, 2), (256, 1), (300, 1)])
+def test_decode_at_a_long_capacity(bits, B, Hkv):
+    """Many sequences, one of them long, with the row's capacity as max_len (a captured
+    step's): the worst case is millions of blocks, the lengths are a few hundred."""
+    D, G, page, cap = 64, 2, 64, 1 << 17
+    lens = [int(x) for x in np.random.default_rng(B).integers(0, 70, B)]
+    lens[B // 3] = 4100
+    table, P, cpu, (k, v, ks, vs) = pools_of(lens, Hkv, D, page, bits, B + Hkv)
+    table = np.concatenate([table, np.full((B, cap // page - table.shape[1]), -1, np.int32)], 1)
+    q = bf16_randn((B, G * Hkv, D), 4)
+    want_o, want_l, tol_o, tol_l = decode_want(q, cpu, table, lens, page, Hkv, 0.125)
+    if bits == 8:
+        out, lse = ops.gqa8_decode_partial(q.to(DEV), k, v, ks, vs, ints(table), ints(lens), 0.125, cap)
+    else:
+        out, lse = ops.gqa_decode_partial(q.to(DEV), k, v, ints(table), ints(lens), 0.125, cap)
+        tol_o = 2 * tol_o  # bf16 pieces: each off by another 2^-8 of its own weighted sum of |v|
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")

@@ -178,3 +178,46 @@ def test_quantise_rule():
     q, s = R.quantise(x)
     assert s.view(torch.uint8).tolist() == [127, 128, 127, 1, 247]
     assert q.float()[0].tolist() == [448.0, 1.0] and q.float()[1].tolist() == [224.0, -0.5]
+
+
+def decode16(**kw):
+    a = dict(q=FAKE, kp=FAKE, vp=FAKE, table=FAKE, lens=FAKE, B=1, Hq=32, Hkv=8, D=128, page=64, max_pages=4,
+             P=4, max_len=100, n=0, scale=1.0, out=FAKE, lse=FAKE, ws=None, wsb=0)
+    a.update(kw)
+    return ops.lib().ws_gqa_decode_partial(*a.values(), None)
+
+
+LONG = dict(page=64, max_pages=1 << 19, P=600, n=16)
+
+
+@pytest.mark.parametrize("call", (decode8, decode16))
+@pytest.mark.parametrize("kw, fits", [
+    # a batch of worst cases far above what any cache holds: the lengths decide, not max_len
+    (dict(B=256, max_len=8192), True), (dict(B=2048, max_len=1 << 17), True),
+    (dict(B=256, Hkv=1, Hq=4, max_len=1 << 23), True), (dict(B=1, Hkv=1, Hq=4, max_len=1 << 25), True),
+    (dict(B=2048, max_len=1 << 22), False), (dict(B=2, Hkv=1, Hq=4, max_len=1 << 24), False),
+    (dict(B=257, Hkv=1, Hq=4, max_len=1 << 24), True), (dict(B=2048, Hkv=16384, Hq=16384, max_len=64, P=1), False)])
+def test_decode_block_range(call, kw, fits):
+    """Refused only where 32-bit block numbers do not hold (what fits goes on to the
+    workspace, which is missing)."""
+    rc = call(**{**LONG, **kw})
+    assert (rc == -3 and "workspace" in err()) if fits else (rc == -1 and "block index range" in err())
+
+
+def test_plan_numbers_hold_to_the_limit():
+    """The split plan's arithmetic (start of split g: floor(g T / n) from 32-bit products;
+    split of a block: a quotient in 64-bit floating point) up to the largest total."""
+    rng = np.random.default_rng(1)
+    totals = [1, 31, 4096, 4097, (1 << 19) + 1, (1 << 31) - (1 << 16) - 1] + \
+        [int(x) for x in np.exp2(rng.uniform(12, 31, 40)) if x < (1 << 31) - (1 << 16)]
+    for T in totals:
+        for grid in (1, 7, 512, 2048, 4095, 4096):
+            n = min(grid, T)
+            q, r = T // n, T - T // n * n
+            g = np.arange(n + 1, dtype=np.int64)
+            assert (g * r < 1 << 32).all()
+            start = g * q + (g * r) // n
+            assert (start == np.array([int(i) * T // n for i in g])).all() and start[-1] == T < 1 << 31
+            for blk in (start[:-1], start[1:] - 1):  # a range's first and last block
+                owner = np.ceil((blk + 1).astype(np.float64) * float(n) / float(T)).astype(np.int64) - 1
+                assert (owner == g[:-1]).all()
