@@ -525,6 +525,14 @@ class GqaRequestPartition:
     def _pages(self, lens) -> int:
         return int(((lens + self.page_size - 1) // self.page_size).sum())
 
+    def _to_device(self, values, dtype) -> torch.Tensor:
+        """values [batch] on the device, without waiting for the work queued there (a
+        copy from pageable memory would): through pinned memory, which torch's
+        allocator gives out again only when the copy has run."""
+        host = torch.empty(self.batch, dtype=dtype, pin_memory=True)
+        host.numpy()[:] = values
+        return host.to(self.device, non_blocking=True)
+
     def begin(self, n_new, pos_base=None) -> "ops.PageStep":
         """Pages and slots for n_new[b] more tokens of every sequence (0: none).
         pos_base [B] int32 on the device: tokens of each sequence that are held
@@ -539,7 +547,7 @@ class GqaRequestPartition:
         need = self._pages(lens) - self._pages(self.lens)
         if need > self.free:
             raise MemoryError("HBM page pool exhausted")
-        n_dev = torch.from_numpy(n.astype(np.int32)).to(self.device)
+        n_dev = self._to_device(n, torch.int32)
         self.step = ops.pages_extend(self.page_table, self.len_dev, n_dev, self.stack, self.free_dev,
                                      self.page_size, self.num_pages, int(n.sum()), pos_base)
         self.len_dev, self.free_dev = self.step.len_out, self.step.free_out
@@ -588,8 +596,8 @@ class GqaRequestPartition:
         done = np.zeros(self.batch, bool)
         done[list(sequences)] = True
         self.len_dev, self.free_dev = ops.pages_release(
-            self.page_table, self.len_dev, torch.from_numpy(done).to(self.device), self.stack,
-            self.free_dev, self.page_size)
+            self.page_table, self.len_dev, self._to_device(done, torch.bool), self.stack, self.free_dev,
+            self.page_size)
         self.free += self._pages(self.lens[done])
         self.lens = np.where(done, 0, self.lens)
         self.step = None

@@ -318,3 +318,48 @@ def test_single_tokens_beside_one_long_request(bits):
         tol_o = 2 * tol_o  # bf16 pieces: each off by another 2^-8 of its own weighted sum of |v|
     R.check(out, want_o, tol_o, "out")
     R.check(lse, want_l, tol_l, "lse")
+
+
+def test_begin_and_release_do_not_wait_for_the_device():
+    """Steps queued behind work that is still running: the calls return before it has
+    ended, and every step gets its own counts."""
+    B, ps, P = 4, 32, 60
+    counts = [[5, 0, 40, 1], [1, 1, 1, 1], [33, 2, 0, 7], "release 2", [1, 64, 3, 1], [0, 1, 1, 90]]
+
+    def run(part):
+        steps = []
+        for n in counts:
+            if n == "release 2":
+                part.release([2])
+            else:
+                steps.append((*part.begin(n), part.page_table.clone()))
+        return steps
+
+    make = lambda: GqaRequestPartition(1, B, 1, 32, 256, ps, num_pages=P)
+    run(make())  # (loads the library's kernels)
+    part = make()
+    x = torch.randn((8192, 8192), device=DEV, dtype=torch.bfloat16)
+    y = x @ x
+    end = torch.cuda.Event()
+    torch.cuda.synchronize()
+    for _ in range(100):  # some 80 ms
+        torch.mm(x, x, out=y)
+    end.record()
+    steps = run(part)
+    running = not end.query()
+    torch.cuda.synchronize()
+    assert running, "begin() or release() waited for the work ahead of it"
+    table, lens = np.full((B, 8), -1, np.int32), np.zeros(B, np.int32)
+    stack, free, at = np.arange(P - 1, -1, -1).astype(np.int32), P, iter(steps)
+    for n in counts:
+        if n == "release 2":
+            held = -(-int(lens[2]) // ps)
+            stack[free:free + held] = table[2, :held]
+            free, lens[2] = free + held, 0
+            continue
+        want = R.extend(table, lens, n, stack, free, ps, P, sum(n))
+        len_out, cu, positions, slots, free_out, got_table = next(at)
+        for got, w in zip((got_table, len_out, cu, positions, slots), want):
+            assert got.cpu().tolist() == w.tolist(), n
+        table, lens, free = want[0], want[1], want[5]
+        assert int(free_out) == free
