@@ -640,3 +640,75 @@ def test_decode_at_a_long_capacity(bits, B, Hkv):
         tol_o = 2 * tol_o  # bf16 pieces: each off by another 2^-8 of its own weighted sum of |v|
     R.check(out, want_o, tol_o, "out")
     R.check(lse, want_l, tol_l, "lse")
+
+
+def prompt_on(q, dev, table, lens, new, scale, **kw):
+    return ops.gqa_prompt(q.to(DEV), dev[0], dev[1], ints(table), ints(lens),
+                          ints(np.concatenate([[0], np.cumsum(new)])), scale, max(lens), dev[2], dev[3],
+                          out_dtype=torch.float32, **kw)
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+@pytest.mark.parametrize("L, n, D", [(2090, 3, 64), (2130, 70, 64), (2165, 5, 96), (4230, 2, 64), (4200, 130, 64),
+                                     (2300, 9, 256)])
+def test_prompt_windows_of_page_ids(bits, L, n, D):
+    """One workgroup walks more than 64 tiles: its window of page ids is fetched again, with
+    0 to 3 steps behind the last whole turn; a bad page in a later window is seen."""
+    page, G = 32, 2
+    table, P, cpu, dev = pools_of([L, 50], 1, D, page, bits, L + n)
+    new = [n, 1]
+    q, scale = bf16_randn((n + 1, G, D), 2), D ** -0.5
+    want_o, want_l, tol_o, tol_l = prompt_want(q, cpu, table, [L, 50], new, page, 1, scale)
+    out, lse = prompt_on(q, dev, table, [L, 50], new, scale, n_splits=1)
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
+    table[0, 65] = P + 3  # (a page a tile; seen by every row)
+    out, lse = prompt_on(q, dev, table, [L, 50], new, scale, n_splits=1)
+    if L - n >= 66 * 32:
+        assert bool(out[:n].isnan().all()) and bool(lse[:n].isnan().all())
+    else:  # the rows that see its first token
+        seen = 65 * 32 - (L - n)
+        R.check(out[:max(seen, 0)], want_o[:max(seen, 0)], tol_o[:max(seen, 0)], "rows before the bad page")
+        assert bool(out[max(seen, 0):n].isnan().all()) and bool(lse[max(seen, 0):n].isnan().all())
+    R.check(out[n:], want_o[n:], tol_o[n:], "the other sequence")
+
+
+@pytest.mark.parametrize("D, Hkv, lens, splits", [
+    (64, 1, [4500], 1), (128, 2, [2016, 2100, 40], 1), (96, 1, [2048, 1, 2080, 4129], 2), (256, 1, [2044, 33, 4500], 1),
+    (64, 3, [2080, 31, 0, 4100], 3)])
+def test_decode8_windows_of_page_ids(D, Hkv, lens, splits):
+    """A split of more than 64 blocks fetches its blocks' metadata again, with rows that end
+    before, at and behind a window's edge; a bad page in a later window is seen."""
+    page, G = 32, 2
+    table, P, cpu, dev = pools_of(lens, Hkv, D, page, 8, sum(lens))
+    q, scale = bf16_randn((len(lens), G * Hkv, D), 6), D ** -0.5
+    want_o, want_l, tol_o, tol_l = decode_want(q, cpu, table, lens, page, Hkv, scale)
+    args = lambda: (q.to(DEV), *dev, ints(table), ints(lens), scale, max(lens), splits)
+    out, lse = ops.gqa8_decode_partial(*args())
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
+    b = int(np.argmax(lens))
+    table[b, -(-lens[b] // page) - 1] = P  # its last page
+    out, lse = ops.gqa8_decode_partial(*args())
+    assert bool(out[b].isnan().all()) and bool(lse[b].isnan().all())
+    for i in range(len(lens)):
+        if i != b:
+            R.check(out[i], want_o[i], tol_o[i], "the other sequences")
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+@pytest.mark.parametrize("B, splits", [(70, 3), (70, 0), (300, 3), (300, 0), (129, 0)])
+def test_prompt_many_split_sequences(bits, B, splits):
+    """More sequences than a wave's lanes, split: both kernels number the pieces of a lane's
+    sequences alike.  A few are long, so that they are split where the lengths decide."""
+    D, page, G, rng = 32, 64, 2, np.random.default_rng(B)
+    lens = rng.integers(1, 60, B)
+    lens[rng.permutation(B)[:4]] = (700, 1500, 333, 900)
+    new = np.minimum(lens, rng.integers(0, 5, B))
+    new[int(np.argmax(lens))] = 40  # (bf16: three tiles of rows)
+    table, P, cpu, dev = pools_of(lens, 1, D, page, bits, B)
+    q = bf16_randn((int(new.sum()), G, D), 3)
+    want_o, want_l, tol_o, tol_l = prompt_want(q, cpu, table, lens, new, page, 1, 0.2)
+    out, lse = prompt_on(q, dev, table, lens, new, 0.2, n_splits=splits)
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
