@@ -75,7 +75,7 @@ struct PromptParams {
   uint16_t* out_bf16;
   float* out_f32;
   float* lse;
-  float* part_out;  // [pieces][rows of a tile][D], with part_lse [pieces][rows]
+  float* part_out;  // [pieces][rows of a tile][D], with part_lse [pieces][rows] (split tiles')
   float* part_lse;
   int N, B, Hq, Hkv, G, page_size, max_pages, num_pages, cap;
   int n_splits;  // of every tile; 0: by the lengths, `share` workgroups in all (0: one a tile)
@@ -143,7 +143,7 @@ struct PromptPlace {
   int b;              // the sequence (< 0: past the list's end)
   int tile;           // tile of its rows
   int split, splits;  // and which of the tile's splits
-  int piece;          // the split's piece, less the KV head: (piece * Hkv + kvh)
+  int piece;          // a split tile's piece, less the KV head: (piece * Hkv + kvh)
   int c0, n;          // the sequence's first row of q and its tokens
   int len;
 };
@@ -191,8 +191,9 @@ __device__ __forceinline__ PromptPlace prompt_place(const PromptParams& p, int a
   int items = 0, units = 0, key = -1;
   for (int k = 0; k < per && b0 + k < p.B; ++k) {
     const PromptSeq s = prompt_seq(p, b0 + k, rows);
-    units += s.tiles * splits_of(s);
-    items += TILES ? s.tiles : s.tiles * splits_of(s);
+    const int splits = splits_of(s);
+    units += splits > 1 ? s.tiles * splits : 0;
+    items += TILES ? s.tiles : s.tiles * splits;
     key = s.blocks;
   }
   const int before = __ockl_wfscan_add_i32(units, true) - units;
@@ -235,7 +236,7 @@ __device__ __forceinline__ PromptPlace prompt_place(const PromptParams& p, int a
       break;
     }
     left -= here;
-    piece += uniform(s.tiles) * splits;
+    piece += splits > 1 ? uniform(s.tiles) * splits : 0;
   }
   return r;
 }
@@ -930,8 +931,10 @@ static PromptPlan prompt_plan(int N, int B, int Hq, int Hkv, int D, bool fp8, in
     if (full * Hkv < fill && max_len > kPromptMinShare * kPromptTile) {
       r.share = (int)std::max(fill - r.tiles, fill / 2);
       // every split but a tile's last is a whole share (and the shares' total, a sum in
-      // fp32, is off by less than 64 of them)
-      r.pieces = r.grid = r.tiles + r.share + 64;
+      // fp32, is off by less than 64 of them); only tiles longer than a share are split,
+      // and only split ones leave pieces
+      r.grid = r.tiles + r.share + 64;
+      r.pieces = std::min<long long>(r.tiles, r.share) + r.share + 64;
     }
   }
   return r;

@@ -221,3 +221,15 @@ def test_plan_numbers_hold_to_the_limit():
             for blk in (start[:-1], start[1:] - 1):  # a range's first and last block
                 owner = np.ceil((blk + 1).astype(np.float64) * float(n) / float(T)).astype(np.int64) - 1
                 assert (owner == g[:-1]).all()
+
+
+@pytest.mark.parametrize("B, Hkv, D, fp8", [(1000, 8, 128, True), (2048, 8, 128, True), (256, 8, 64, False),
+                                            (2000, 1, 128, True)])
+def test_prompt_workspace_of_many_sequences(B, Hkv, D, fp8):
+    """A batch of single tokens: pieces for the tiles that can be split (at most as many as
+    shares), not for one of every sequence and KV head."""
+    n, wsb = ops.gqa_prompt_plan(B, B, 4 * Hkv, Hkv, D, 8192, fp8=fp8)
+    fill = 256 * 8  # the most workgroups at once, on 256 CUs
+    assert n <= 2 * fill + 64 and n < B * Hkv + fill
+    rows = 128 if fp8 else 32
+    assert wsb <= n * rows * (D + 1) * 4 + 256 and wsb < 64 << 20
