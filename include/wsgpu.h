@@ -216,6 +216,22 @@ int ws_gqa_decode_partial(const uint16_t* q,
                           void* stream);
 
 /*
+ * ws_gqa_decode_partial for a partition that holds every token: out_bf16 [B][Hq][D]
+ * also takes the output rounded to bf16, in the same two launches.
+ * Replaces _resident_layer followed by the final o / sum and bf16 cast
+ * (roofline/bench_resident_kv.py:261-271, 350) where the token was appended before.
+ */
+int ws_gqa_decode_full(const uint16_t* q,
+                       const uint16_t* k_pages, const uint16_t* v_pages,
+                       const int32_t* page_table, const int32_t* gpu_len,
+                       int B, int Hq, int Hkv, int D,
+                       int page_size, int max_pages, int num_pages,
+                       int max_len, int n_splits, float scale,
+                       uint16_t* out_bf16, float* out, float* lse,
+                       void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
  * One decode step of the GPU partition in one launch: append the new token of
  * every sequence and attend over the partition including it.
  * k_new, v_new: [B][Hkv][1][D] bf16.  Token len_in[b] of sequence b is the new

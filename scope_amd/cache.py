@@ -572,8 +572,9 @@ class GqaRequestPartition:
     def attend(self, layer: int, q, scale: float, out_dtype=torch.float32):
         """The step's tokens, q [N, Hq, D] rotated, over the pages: (out [N, Hq, D] in
         out_dtype (fp32 or bf16), lse [N, Hq]), which merges with a host partial as
-        the other partitions' (ops.lse_merge).  One token of every sequence runs the
-        decode kernels, anything else the prompt kernel."""
+        the other partitions' (ops.lse_merge).  One token of every sequence (at most
+        16 query heads a KV head) runs the decode kernels, anything else the prompt
+        kernel."""
         step = self._step()
         if q.dim() != 3 or q.shape[0] != step.slots.shape[0]:
             raise ValueError(f"q must hold the step's {step.slots.shape[0]} tokens (got {tuple(q.shape)})")
@@ -582,12 +583,11 @@ class GqaRequestPartition:
         Hq, max_len = q.shape[1], int(self.lens.max()) if self.batch else 0
         k, v = self.k[layer], self.v[layer]
         ks, vs = (None, None) if self.bits == 16 else (self.k_scale[layer], self.v_scale[layer])
-        if (self.n_new == 1).all() and Hq <= 16 * self.num_kv_heads and out_dtype == torch.float32:
-            if self.bits == 16:
-                return ops.gqa_decode_partial(q, k, v, self.page_table, self.len_dev, scale, max_len)
-            return ops.gqa8_decode_partial(q, k, v, ks, vs, self.page_table, self.len_dev, scale, max_len)
-        if (self.n_new == 1).all() and Hq <= 16 * self.num_kv_heads and self.bits == 8:
-            return ops.gqa8_decode_full(q, k, v, ks, vs, self.page_table, self.len_dev, scale, max_len)
+        if (self.n_new == 1).all() and Hq <= 16 * self.num_kv_heads:
+            pools = (k, v) if self.bits == 16 else (k, v, ks, vs)
+            decode = {(16, torch.float32): ops.gqa_decode_partial, (16, torch.bfloat16): ops.gqa_decode_full,
+                      (8, torch.float32): ops.gqa8_decode_partial, (8, torch.bfloat16): ops.gqa8_decode_full}
+            return decode[self.bits, out_dtype](q, *pools, self.page_table, self.len_dev, scale, max_len)
         return ops.gqa_prompt(q, k, v, self.page_table, self.len_dev, step.cu_new, scale, max_len,
                               ks, vs, out_dtype=out_dtype)
 

@@ -772,3 +772,19 @@ extern "C" int ws_gqa_append_decode_full(
                     Hkv, D, D, page_size, max_pages, num_pages, max_len, n_splits, scale, out,
                     lse, workspace, workspace_bytes, stream, true, name, out_bf16);
 }
+
+extern "C" int ws_gqa_decode_full(
+    const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
+    const int32_t* page_table, const int32_t* gpu_len, int B, int Hq, int Hkv, int D,
+    int page_size, int max_pages, int num_pages, int max_len, int n_splits, float scale,
+    uint16_t* out_bf16, float* out, float* lse, void* workspace, size_t workspace_bytes,
+    void* stream) {
+  static const char* name = "ws_gqa_decode_full";
+  if (!out_bf16) return set_error(WS_EINVAL, "%s: out_bf16 is null", name);
+  if (((uintptr_t)out_bf16 & 15u) != 0)
+    return set_error(WS_EINVAL, "%s: buffers must be 16-byte aligned", name);
+  return gqa_launch(q, nullptr, nullptr, (uint16_t*)k_pages, (uint16_t*)v_pages, page_table,
+                    gpu_len, nullptr, B, Hq, Hkv, D, D, page_size, max_pages, num_pages, max_len,
+                    n_splits, scale, out, lse, workspace, workspace_bytes, stream, true, name,
+                    out_bf16);
+}

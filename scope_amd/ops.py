@@ -41,6 +41,7 @@ EXPORTS = (
     "ws_mla_decode_partial",
     "ws_mla_append_decode_partial",
     "ws_gqa_append_decode_split",
+    "ws_gqa_decode_full",
     "ws_gqa_append_decode_full",
     "ws_mla_append_decode_split",
     "ws_merge_split",
@@ -121,6 +122,8 @@ def lib() -> ctypes.CDLL:
         L.ws_gqa_append_decode_partial.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp,
                                                    i32, i32, i32, i32, i32, i32, i32,
                                                    i32, i32, f32, vp, vp, vp, sz, vp]
+        L.ws_gqa_decode_full.restype = i32
+        L.ws_gqa_decode_full.argtypes = [vp] * 5 + [i32] * 9 + [f32, vp, vp, vp, vp, sz, vp]
         L.ws_gqa_append_decode_full.restype = i32
         L.ws_gqa_append_decode_full.argtypes = [vp] * 8 + [i32] * 9 + [f32, vp, vp, vp, vp, sz,
                                                                         vp]
@@ -460,6 +463,41 @@ def gqa_decode_partial(q, k_pages, v_pages, page_table, gpu_len, scale, max_len,
         B, Hq, Hkv, D, PS, page_table.shape[1], P, int(max_len), nwg, float(scale),
         _ptr(out), _ptr(lse), _ptr(ws), wsb, _stream(dev)), "ws_gqa_decode_partial")
     return out, lse
+
+
+def gqa_decode_full(q, k_pages, v_pages, page_table, gpu_len, scale, max_len,
+                    n_workgroups=0, out_bf16=None, lse=None):
+    """gqa_decode_partial for a partition that holds every token: returns
+    (out [B, Hq, D] bf16, the rounded fp32 output; lse [B, Hq] fp32)."""
+    dev = _gpu(k_pages, "k_pages")
+    _require_all(dev, _DECODE16_ARGS, (q, k_pages, v_pages, page_table, gpu_len))
+    B, Hq, D = q.shape
+    P, Hkv, PS, D2 = k_pages.shape
+    if v_pages.shape != k_pages.shape or D2 != D or Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"q {tuple(q.shape)} does not match the pools {tuple(k_pages.shape)}")
+    if page_table.shape[0] != B or gpu_len.shape[0] != B:
+        raise ValueError("page_table/gpu_len batch mismatch")
+    if out_bf16 is None:
+        out_bf16 = torch.empty_like(q)
+    else:
+        _require(out_bf16, "out_bf16", torch.bfloat16, dev, 3)
+    if lse is None:
+        lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
+    else:
+        _require(lse, "lse", torch.float32, dev, 2)
+    if out_bf16.shape != q.shape or lse.shape != (B, Hq):
+        raise ValueError("out_bf16 must be [B, Hq, D] and lse [B, Hq]")
+    if B == 0:
+        return out_bf16, lse
+    nwg, wsb = gqa_plan(B * Hkv, Hq // Hkv, D, D, int(max_len), int(n_workgroups))
+    wsb = (wsb + 255) & ~255
+    # the call's own, with the fp32 output behind the pieces
+    ws = torch.empty(wsb + 4 * B * Hq * D, dtype=torch.uint8, device=dev)
+    _run("ws_gqa_decode_full", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+         page_table.data_ptr(), gpu_len.data_ptr(), B, Hq, Hkv, D, PS, page_table.shape[1], P,
+         int(max_len), nwg, float(scale), out_bf16.data_ptr(), ws.data_ptr() + wsb, lse.data_ptr(),
+         ws.data_ptr(), wsb)
+    return out_bf16, lse
 
 
 def attn_decode_partial(q, k_pages, v_pages, page_table, gpu_len, scale, max_len,
@@ -1053,6 +1091,8 @@ _RELEASE_ARGS = (("page_table", torch.int32, 2), ("len_in", torch.int32, 1), ("d
 _POOL_ARGS = {bits: (("k_pages", dt, 4), ("v_pages", dt, 4)) for bits, dt in
               ((16, torch.bfloat16), (8, E4M3))}
 _SCALE_ARGS = (("k_scale", E8M0, 3), ("v_scale", E8M0, 3))
+_DECODE16_ARGS = (("q", torch.bfloat16, 3), ("k_pages", torch.bfloat16, 4), ("v_pages", torch.bfloat16, 4),
+                  ("page_table", torch.int32, 2), ("gpu_len", torch.int32, 1))
 _DECODE8_ARGS = (("q", torch.bfloat16, 3), ("page_table", torch.int32, 2), ("gpu_len", torch.int32, 1))
 _PROMPT_ARGS = (("q", torch.bfloat16, 3), ("page_table", torch.int32, 2), ("kv_len", torch.int32, 1),
                 ("cu_new", torch.int32, 1))

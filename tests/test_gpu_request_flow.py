@@ -363,3 +363,19 @@ def test_begin_and_release_do_not_wait_for_the_device():
             assert got.cpu().tolist() == w.tolist(), n
         table, lens, free = want[0], want[1], want[5]
         assert int(free_out) == free
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+def test_attend_single_tokens_round_the_decode_output(bits):
+    """A step of one token of every sequence runs the same kernels for either output
+    type: the bf16 output is the fp32 one, rounded, and the lse is the same."""
+    B, Hq, Hkv, D = 3, 8, 2, 64
+    part = GqaRequestPartition(1, B, Hkv, D, 2048, 64, bits=bits)
+    for n in ([1500, 3, 70], [1, 1, 1]):
+        part.begin(n)
+        w = bf16_randn((sum(n), (Hq + 2 * Hkv) * D), 5 + n[0]).to(DEV)
+        q, k, v = (x.view(sum(n), -1, D) for x in w.split((Hq * D, Hkv * D, Hkv * D), 1))
+        qr = part.append(0, q, k, v, torch.ones(D // 2, device=DEV))
+    want, want_l = part.attend(0, qr, 0.125)
+    out, lse = part.attend(0, qr, 0.125, torch.bfloat16)
+    assert out.dtype == torch.bfloat16 and torch.equal(out, want.bfloat16()) and torch.equal(lse, want_l)

@@ -712,3 +712,26 @@ def test_prompt_many_split_sequences(bits, B, splits):
     out, lse = prompt_on(q, dev, table, lens, new, 0.2, n_splits=splits)
     R.check(out, want_o, tol_o, "out")
     R.check(lse, want_l, tol_l, "lse")
+
+
+@pytest.mark.parametrize("D, Hkv, G, lens, splits", [
+    (128, 2, 4, [1], 0), (128, 2, 4, [31, 0, 33, 700], 0), (80, 1, 3, [200, 65], 3), (256, 2, 16, [257, 5], 6),
+    (64, 2, 1, [40] * 70, 0), (16, 1, 2, [129], 1)])
+def test_decode_full(D, Hkv, G, lens, splits):
+    table, P, cpu, (k, v, _, _) = pools_of(lens, Hkv, D, 64, 16, D + len(lens))
+    q, scale = bf16_randn((len(lens), Hkv * G, D), 9), D ** -0.5
+    want_o, want_l, tol_o, tol_l = decode_want(q, cpu, table, lens, 64, Hkv, scale)
+    args = (q.to(DEV), k, v, ints(table), ints(lens), scale, max(lens), splits)
+    out, lse = ops.gqa_decode_full(*args)
+    # bf16 pieces: each off by another 2^-8 of its own weighted sum of |v|; then the output's rounding
+    R.check(out, want_o, 2 * tol_o + want_o.abs() * 2.0 ** -8, "out")
+    R.check(lse, want_l, tol_l, "lse")
+    part, part_l = ops.gqa_decode_partial(*args)
+    assert torch.equal(out, part.bfloat16()) and torch.equal(lse, part_l)
+    mine = torch.empty_like(out), torch.empty_like(lse)
+    assert ops.gqa_decode_full(*args, *mine)[0] is mine[0] and torch.equal(mine[0], out)
+    for bad, err, says in ((dict(out_bf16=part), TypeError, "out_bf16"), (dict(lse=lse[:, :1]), ValueError, "lse")):
+        with pytest.raises(err, match=says):
+            ops.gqa_decode_full(*args, **{**bad, **({"lse": bad["lse"].contiguous()} if "lse" in bad else {})})
+    with pytest.raises(ValueError, match="match the pools"):
+        ops.gqa_decode_full(q[..., :8].contiguous().to(DEV), *args[1:])

@@ -233,3 +233,13 @@ def test_prompt_workspace_of_many_sequences(B, Hkv, D, fp8):
     assert n <= 2 * fill + 64 and n < B * Hkv + fill
     rows = 128 if fp8 else 32
     assert wsb <= n * rows * (D + 1) * 4 + 256 and wsb < 64 << 20
+
+
+@pytest.mark.parametrize("kw, rc, says", [
+    (dict(o16=None), -1, "out_bf16 is null"), (dict(o16=ODD), -1, "aligned"), (dict(q=None), -1, "null"),
+    (dict(out=None), -1, "null"), (dict(Hq=33), -1, "heads"), (dict(D=40), -1, "head_dim"), (dict(n=16), -3, "workspace")])
+def test_decode_full_refusals(kw, rc, says):
+    a = dict(q=FAKE, kp=FAKE, vp=FAKE, table=FAKE, lens=FAKE, B=1, Hq=32, Hkv=8, D=128, page=64, max_pages=4,
+             P=4, max_len=100, n=0, scale=1.0, o16=FAKE, out=FAKE, lse=FAKE, ws=None, wsb=0)
+    a.update(kw)
+    assert ops.lib().ws_gqa_decode_full(*a.values(), None) == rc and says in err()
