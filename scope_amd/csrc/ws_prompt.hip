@@ -266,19 +266,24 @@ __device__ __forceinline__ void static_for_prompt(F&& f) {
 // the compiler would wait for every one of them ahead of any LDS read.
 // ONCE: the tile is read once (the calls of few rows), so it need not stay in the caches
 // (the non-temporal hint: 140 -> 129 us for 8 x 5 tokens over 4000 to 32000).
+// m0 is named as written, though the compiler says that it need not keep a reserved
+// register across the block: what counts is that it expects no old value there.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int AT, bool ONCE>
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {
   if constexpr (ONCE)
     asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
                  :
                  : "v"(off), "s"(base), "s"(lds), "n"(AT)
-                 : "memory", "scc");
+                 : "memory", "scc", "m0");
   else
     asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :
                  : "v"(off), "s"(base), "s"(lds), "n"(AT)
-                 : "memory", "scc");
+                 : "memory", "scc", "m0");
 }
+#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N < 63 ? N : 63) : "memory");
