@@ -514,6 +514,7 @@ class GqaRequestPartition:
                                           for _ in range(2))
         int32 = dict(dtype=torch.int32, device=self.device)
         self.page_table = torch.full((batch, self.max_pages), -1, **int32)
+        self.device = self.page_table.device  # (with its number, whatever device is current later)
         self.stack = torch.arange(self.num_pages - 1, -1, -1, **int32)  # page 0 on top
         self.free_dev = torch.full((1,), self.num_pages, **int32)
         self.len_dev = torch.zeros(batch, **int32)

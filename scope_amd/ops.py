@@ -458,10 +458,9 @@ def gqa_decode_partial(q, k_pages, v_pages, page_table, gpu_len, scale, max_len,
     _require(lse, "lse", torch.float32, dev, 2)
     nwg, wsb = gqa_plan(B * Hkv, Hq // Hkv, D, D, int(max_len), int(n_workgroups))
     ws = _workspace(dev, wsb)
-    _check(lib().ws_gqa_decode_partial(
-        _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(gpu_len),
-        B, Hq, Hkv, D, PS, page_table.shape[1], P, int(max_len), nwg, float(scale),
-        _ptr(out), _ptr(lse), _ptr(ws), wsb, _stream(dev)), "ws_gqa_decode_partial")
+    _run("ws_gqa_decode_partial", dev, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(page_table),
+         _ptr(gpu_len), B, Hq, Hkv, D, PS, page_table.shape[1], P, int(max_len), nwg, float(scale),
+         _ptr(out), _ptr(lse), _ptr(ws), wsb)
     return out, lse
 
 

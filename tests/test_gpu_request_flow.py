@@ -379,3 +379,11 @@ def test_attend_single_tokens_round_the_decode_output(bits):
     want, want_l = part.attend(0, qr, 0.125)
     out, lse = part.attend(0, qr, 0.125, torch.bfloat16)
     assert out.dtype == torch.bfloat16 and torch.equal(out, want.bfloat16()) and torch.equal(lse, want_l)
+
+
+def test_partition_knows_its_device():
+    """A partition on "cuda" stays on the device that was current when it was made: its
+    counts go there by number."""
+    part = GqaRequestPartition(1, 2, 1, 64, 128, 32, device="cuda")
+    assert part.device == part.page_table.device and part.device.index is not None
+    assert part._to_device([1, 2], torch.int32).device == part.page_table.device
