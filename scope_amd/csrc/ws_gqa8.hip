@@ -17,11 +17,12 @@
 //    feeds two k-steps: lane group j's eight columns of k-step 2 i and 2 i + 1
 //    are columns 64 i + 16 j .. + 7 and + 8 .. + 15.
 //  - Pieces are fp32: a bf16 piece would round the outputs once more, which shows
-//    beside the rounding of the probabilities (error against 64 bits 1.4 of the
-//    plain form's with fp32 pieces, 1.6 with bf16 ones).
+//    beside the rounding of the probabilities to bf16 for the values' product
+//    (softmax_block; their sums are fp32): error against 64 bits 1.4 of the plain
+//    form's with fp32 pieces, 1.6 with bf16 ones.
 //
 // Bound by HBM: 621 MB (16 sequences of 1000 to 32000 tokens, 8 x 4 heads of 128) take
-// 102.7 us, 6.0 TB/s, and their merge 4.7; 8192 tokens of 4 x 8 heads 5.6 and 5.8 (the
+// 102.6 to 103.9 us, 6.0 TB/s, and their merge 4.9; 8192 tokens of 4 x 8 heads 5.6 and 5.9 (the
 // start chain: lengths, page ids, blocks).
 #include <algorithm>
 #include <type_traits>

@@ -14,7 +14,7 @@
 // of the tokens, one thread a token, which finds its sequence by bisection.  A
 // token that opens a page also writes the page's table entry: no other thread
 // reads it, the others take the id from the stack as well.  16 sequences of one token
-// take 3.0 us, 512 with 113981 tokens 9.6, the release of 37 sequences 3.5.
+// take 3.0 to 3.2 us, 512 with 113981 tokens 9.6, the release of 37 sequences 3.5 to 3.7.
 #include "ws_common.h"
 #include "ws_plan.h"
 

@@ -17,6 +17,11 @@
 // A row is one lane column: its maximum takes one exchange between the lane halves,
 // its rescaling no exchange at all.
 //
+// P is rounded to bf16 for the values' product, the matrix cores' operand type (as the
+// decode kernels round theirs); its row sum takes the values before, in fp32 as the maximum,
+// the output's sums and the pieces.  Error against 64 bits: 2.0e-3 to 2.3e-3 of the
+// output, where fp32 work rounded to bf16 at the end has 1.5e-3 to 1.7e-3.
+//
 // A row sees nothing of the tokens past its position: their scores are masked, and
 // so are their values, which P = 0 alone would not do for an infinity or a NaN
 // (0 * inf): where a tile that some row masks holds one, values_masked adds it to the rows
@@ -27,7 +32,7 @@
 // their pieces (fp32, with their lse).
 //
 // Long prompts are bound by the power of the products and by the vector work beside them:
-// 8192 tokens of 8 x 4 heads of 128 take 525 to 542 us (1.01 to 1.05 PFLOP/s; 392 on
+// 8192 tokens of 8 x 4 heads of 128 take 525 to 550 us (1.00 to 1.05 PFLOP/s; 392 on
 // zeros, at a higher clock).  Few rows are bound by HBM: 567 MB in 93.7 us (6.1 TB/s) and
 // the join 5.0.
 #include <algorithm>
@@ -316,7 +321,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(const
   constexpr int kRows = 32 * NW;
   // k-steps whose q lies in LDS, for the registers that 8-bit tiles take on their way: what
   // the compiler spilled instead came back behind the loads under way, which memory answers
-  // in order (8 x 12 tokens over 16000: 114 -> 88 us, 8-bit chunks 381 -> 362)
+  // in order (8 x 12 tokens over 16000: 114 -> 88 us, 8-bit chunks 381 -> 362).  The loop of
+  // the calls of few rows spills nothing since; the other one still reloads six registers
+  // in four steps.  Narrower heads need fewer registers, wider ones have twice as many.
   constexpr int kQl = F8 && D == 128 ? 2 : 0;
   constexpr bool kAcc = D > 128 || NW == 1;  // more than 256 registers
   __shared__ __attribute__((aligned(256))) char s_k[kPromptSlots * Sh::kTile];

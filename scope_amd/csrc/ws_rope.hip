@@ -17,9 +17,9 @@
 // holds 16 columns of a head row, the pairs' both halves among them, as two
 // 16-byte loads; a row takes D / 16 lanes (rounded up to a power of two, so that
 // the 8-bit write finds the row's maximum with lane exchanges).  16637 tokens of
-// 32 + 4 + 4 heads of 128 columns (341 MB) take 66.6 us, 5.1 TB/s, as a large copy does;
-// 3765 tokens of 24 + 8 + 8 heads of 96 into 8-bit pages 12.2 us (4.3 TB/s); a step of 32
-// tokens 4.3 us.
+// 32 + 4 + 4 heads of 128 columns (341 MB) take 66.6 to 67.1 us, 5.1 TB/s, as a large
+// copy does; 3765 tokens of 24 + 8 + 8 heads of 96 into 8-bit pages 12.2 to 12.5 us (4.3
+// TB/s); a step of 32 tokens 4.4 us.
 //
 // 8-bit pages hold e4m3 values with one power-of-two scale (e8m0 byte) per
 // token and KV head: 2^e, e the least with max|x| <= 448 * 2^e.  A power of

@@ -387,3 +387,34 @@ def test_partition_knows_its_device():
     part = GqaRequestPartition(1, 2, 1, 64, 128, 32, device="cuda")
     assert part.device == part.page_table.device and part.device.index is not None
     assert part._to_device([1, 2], torch.int32).device == part.page_table.device
+
+
+def test_decode_full_in_two_graphs_at_once():
+    """Each captured call has a workspace of its own: two graphs replayed on two streams at
+    once, with eager calls between the replays, give the eager results bit for bit."""
+    B, Hkv, G, D, L = 2, 2, 4, 128, 3000  # (split rows: pieces in the workspace)
+    made = []
+    for i in range(2):
+        k, v = (bf16_randn((B * 47, Hkv, 64, D), 70 + 2 * i + j).to(DEV) for j in range(2))
+        table = torch.arange(B * 47, dtype=torch.int32, device=DEV).view(B, 47).flip(0).contiguous()
+        lens = torch.tensor([L, L - 100 * i], dtype=torch.int32, device=DEV)
+        made.append((bf16_randn((B, Hkv * G, D), 80 + i).to(DEV), k, v, table, lens, D ** -0.5, L))
+    want = [ops.gqa_decode_full(*a) for a in made]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for a in made:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.gqa_decode_full(*a))
+        graphs.append(g)
+    for i in range(6):
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w, a in zip(outs, want, made):
+            assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1]), f"replay {i}"
+            assert torch.equal(ops.gqa_decode_full(*a)[0], w[0]), f"eager after replay {i}"
