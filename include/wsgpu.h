@@ -20,6 +20,9 @@
  *                                     into the pages (bf16 or 8-bit)
  *   ws_gqa8_decode_partial            decode attention over 8-bit pages
  *   ws_gqa_prompt                     prompt attention over the pages
+ *   ws_latent_rope_append / ws_latent_gather  latents into bf16 or 8-bit pages, and back
+ *   ws_mla8_decode_partial            MLA decode over 8-bit latent pages
+ *   ws_mla_prompt                     MLA attention of many new tokens over latent pages
  *
  * Conventions
  *   - bf16 tensors are passed as uint16_t bit patterns; fp32 as float.
@@ -624,6 +627,100 @@ int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void* v_pages,
                   int D, int page_size, int max_pages, int num_pages, int max_len,
                   int n_splits, float scale, uint16_t* out_bf16, float* out_f32, float* lse,
                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The latents of absorbed MLA into their pages, with the rotary positions of the heads'
+ * q_pe.  Token t's latent is
+ *   [ c rsqrt(mean(c^2) + eps) norm_weight , R(positions[t]) pe ]   (512 + 64 columns)
+ * (norm_weight NULL: c as it is; weight_f32: 512 fp32 values, else bf16), computed in fp32
+ * and rounded once, at slot slots[t] = page * page_size + offset of latent_pages
+ * [num_pages][page_size][576]; a slot outside [0, num_pages * page_size) writes nothing.
+ * Slots must differ.  R turns pair i of 32 by positions[t] * inv_freq[i], columns (i, i + 32)
+ * or (2 i, 2 i + 1) with adjacent != 0, times factor, as ws_rope; q_out [N][H][64] is R of
+ * q_pe (token stride q_stride, head stride q_head_stride, in elements as c's and pe's
+ * strides: multiples of 8), and may be q_pe itself where that is contiguous.
+ * latent_scale == NULL: bf16 pages.  Otherwise 8-bit pages: e4m3 values, and an e8m0 byte
+ * for every scale_block slots (latent_scale [num_pages][page_size / scale_block]; scale_block
+ * a power of two that divides page_size) for 2^(byte - 127), the least power of two >= 2^-126
+ * with max|x| <= 448 times it over the block's tokens.  With scale_block > 1 the tokens of a
+ * block follow one another in a call, and slots of the block below the call's lowest hold
+ * tokens from before: the scale is no less than theirs, and where it rises their values
+ * are rounded again.  An infinity or a NaN becomes NaN in its place and has no part in the
+ * scale.
+ * The reference computes the norm and the rotation in the model library and copies the
+ * result into dense host and GPU buffers (system/deepseek.py:251, 171-192).
+ */
+int ws_latent_rope_append(const uint16_t* c, int64_t c_stride, const uint16_t* pe,
+                          int64_t pe_stride, const uint16_t* q_pe, int64_t q_stride,
+                          int64_t q_head_stride, const int32_t* positions,
+                          const float* inv_freq, int adjacent, float factor,
+                          const void* norm_weight, int weight_f32, float eps,
+                          const int32_t* slots, uint16_t* q_out, void* latent_pages,
+                          uint8_t* latent_scale, int scale_block, int N, int H, int page_size,
+                          int num_pages, void* stream);
+
+/*
+ * Tokens of the latent pages (ws_latent_rope_append's pools) as bf16 rows: row r, cu_rows[b]
+ * <= r < cu_rows[b + 1] (cu_rows [B + 1] non-decreasing), is token start[b] + r - cu_rows[b]
+ * of sequence b (start NULL: 0), its 512 columns to c_out + r * c_stride and its 64 rotary ones
+ * to pe_out + r * pe_stride (strides in elements, multiples of 8); exact from 8-bit pages.
+ * Rows outside [cu_rows[0], cu_rows[B]) and past N are not written.  A token outside the
+ * capacity or in a page with an id outside the pool gives a row of NaN.
+ * The reference reads its dense buffers in place (system/deepseek.py:194-202).
+ */
+int ws_latent_gather(const void* latent_pages, const uint8_t* latent_scale, int scale_block,
+                     const int32_t* page_table, const int32_t* start, const int32_t* cu_rows,
+                     uint16_t* c_out, int64_t c_stride, uint16_t* pe_out, int64_t pe_stride,
+                     int N, int B, int page_size, int max_pages, int num_pages, void* stream);
+
+/*
+ * Absorbed-MLA decode attention over 8-bit latent pages (ws_latent_rope_append's):
+ * ws_mla_decode_partial's result, for any number of heads up to 1024.  q_nope [B][H][512],
+ * q_pe [B][H][64] bf16; page_size a multiple of 32.  ws_mla8_decode_full writes the output in
+ * bf16 instead.  A sequence of length 0 gives (0, -inf), one with a length outside
+ * [0, capacity] NaN, and so does a page id outside the pool that a length reaches.
+ * n_splits: workgroups that share a sequence's tokens (1 to 256; 0: the library's choice by
+ * the lengths).  max_len bounds gpu_len.  Workspace: ws_mla8_decode_plan's bytes for the same
+ * sizes (0: none); pieces_out: the pieces that split sequences can leave in it.
+ */
+int ws_mla8_decode_plan(int B, int H, int max_len, int n_splits, int* pieces_out,
+                        size_t* workspace_bytes_out);
+int ws_mla8_decode_partial(const uint16_t* q_nope, const uint16_t* q_pe,
+                           const uint8_t* latent_pages, const uint8_t* latent_scale,
+                           const int32_t* page_table, const int32_t* gpu_len, int B, int H,
+                           int page_size, int max_pages, int num_pages, int scale_block,
+                           int max_len, int n_splits, float scale, float* out, float* lse,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int ws_mla8_decode_full(const uint16_t* q_nope, const uint16_t* q_pe,
+                        const uint8_t* latent_pages, const uint8_t* latent_scale,
+                        const int32_t* page_table, const int32_t* gpu_len, int B, int H,
+                        int page_size, int max_pages, int num_pages, int scale_block,
+                        int max_len, int n_splits, float scale, uint16_t* out_bf16, float* lse,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * ws_gqa_prompt over latent pages, in the absorbed form: q_nope [N][H][512] and q_pe
+ * [N][H][64] bf16, packed; sequence b's n = cu_new[b + 1] - cu_new[b] queries are rows
+ * cu_new[b] .. and stand at the last n of its kv_len[b] tokens, each seeing the tokens up to
+ * its own (one at a negative position: out 0, lse -inf).  latent_scale == NULL: bf16 pages
+ * (scale_block is not looked at).  H up to 1024, page_size a multiple of 32.
+ * Outputs: any of out_bf16 / out_f32 [N][H][512] (not both NULL) and lse [N][H] (may be NULL),
+ * mergeable with a host partial (ws_lse_merge).  Rows outside [cu_new[0], cu_new[B]) are
+ * not written.  A row that sees a token in a page with an id outside the pool is NaN, and
+ * so is every row of a sequence whose length is outside [0, capacity]; an infinity or a NaN
+ * in a token changes only the rows that see it.
+ * n_splits, max_len and the workspace (ws_mla_prompt_plan) as ws_mla8_decode_partial's.
+ * The reference runs prompts through its framework's attention on expanded keys and values
+ * (system/deepseek.py:279-322).
+ */
+int ws_mla_prompt_plan(int N, int B, int H, int max_len, int n_splits, int* pieces_out,
+                       size_t* workspace_bytes_out);
+int ws_mla_prompt(const uint16_t* q_nope, const uint16_t* q_pe, const void* latent_pages,
+                  const uint8_t* latent_scale, const int32_t* page_table, const int32_t* kv_len,
+                  const int32_t* cu_new, int N, int B, int H, int page_size, int max_pages,
+                  int num_pages, int scale_block, int max_len, int n_splits, float scale,
+                  uint16_t* out_bf16, float* out_f32, float* lse, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

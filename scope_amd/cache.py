@@ -471,47 +471,18 @@ class PartitionedKVCache:
         return self.host_k[layer][rows, :n], self.host_v[layer][rows, :n]
 
 
-class GqaRequestPartition:
-    """HBM pages of a GQA KV cache for requests of any lengths, handed out on the GPU.
+class _RequestPages:
+    """Pages of a batch of requests, handed out on the GPU (ops.pages_extend), with a host
+    mirror of the lengths and of the number of free pages, so that nothing waits for the
+    device.  The request partitions keep their pools on it."""
 
-    Where GqaGpuPartition's pages come from a host free list, one copy to the
-    device per sequence that needs some, here one launch gives every sequence of
-    the batch the pages its new tokens need and every token its slot
-    (ops.pages_extend); the host keeps a mirror of the lengths and of the number
-    of free pages, so that nothing waits for the device.  A forward step of the
-    batch is
-      begin(n_new)            pages and slots for n_new[b] tokens of sequence b
-      append(layer, q, k, v)  q rotated; k rotated, and v, into the pages
-      attend(layer, q)        every new token over all the sequence's tokens so far
-    with the tokens of all sequences packed one after the other ([N, heads, D]), for
-    prompts, chunks of them and single tokens alike.  bits 16: bf16 pages; 8: e4m3
-    with one power-of-two scale per token and KV head, half the bytes.  begin() and
-    release() copy counts from the host, so a captured step calls the ops on the
-    partition's tensors instead (with the capacity as max_len).
-    """
-
-    def __init__(self, num_layers, batch, num_kv_heads, head_dim, max_tokens, page_size=64,
-                 num_pages=None, bits=16, device="cuda"):
+    def __init__(self, num_layers, batch, max_tokens, page_size, num_pages, device):
         if page_size <= 0 or page_size % 32:
             raise ValueError("page_size must be a positive multiple of 32")
-        if head_dim % 32 or not 32 <= head_dim <= 256:
-            raise ValueError("head_dim must be a multiple of 32 up to 256")
-        if bits not in (8, 16):
-            raise ValueError("bits must be 8 or 16")
         self.device = torch.device(device)
-        self.num_layers, self.batch, self.bits = num_layers, batch, bits
-        self.num_kv_heads, self.head_dim, self.page_size = num_kv_heads, head_dim, page_size
+        self.num_layers, self.batch, self.page_size = num_layers, batch, page_size
         self.max_pages = max(1, pages_for(max_tokens, page_size))
         self.num_pages = num_pages if num_pages is not None else batch * self.max_pages
-        shape = (num_layers, self.num_pages, num_kv_heads, page_size, head_dim)
-        if bits == 16:
-            self.k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-            self.v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-            self.k_scale = self.v_scale = None
-        else:
-            self.k, self.v = (torch.empty(shape, dtype=ops.E4M3, device=self.device) for _ in range(2))
-            self.k_scale, self.v_scale = (torch.empty(shape[:4], dtype=ops.E8M0, device=self.device)
-                                          for _ in range(2))
         int32 = dict(dtype=torch.int32, device=self.device)
         self.page_table = torch.full((batch, self.max_pages), -1, **int32)
         self.device = self.page_table.device  # (with its number, whatever device is current later)
@@ -560,6 +531,55 @@ class GqaRequestPartition:
             raise RuntimeError("begin() comes first")
         return self.step
 
+    def release(self, sequences) -> None:
+        """Drop all tokens of the given sequences; their pages are free again."""
+        done = np.zeros(self.batch, bool)
+        done[list(sequences)] = True
+        self.len_dev, self.free_dev = ops.pages_release(
+            self.page_table, self.len_dev, self._to_device(done, torch.bool), self.stack, self.free_dev,
+            self.page_size)
+        self.free += self._pages(self.lens[done])
+        self.lens = np.where(done, 0, self.lens)
+        self.step = None
+
+
+class GqaRequestPartition(_RequestPages):
+    """HBM pages of a GQA KV cache for requests of any lengths, handed out on the GPU.
+
+    Where GqaGpuPartition's pages come from a host free list, one copy to the
+    device per sequence that needs some, here one launch gives every sequence of
+    the batch the pages its new tokens need and every token its slot
+    (ops.pages_extend); the host keeps a mirror of the lengths and of the number
+    of free pages, so that nothing waits for the device.  A forward step of the
+    batch is
+      begin(n_new)            pages and slots for n_new[b] tokens of sequence b
+      append(layer, q, k, v)  q rotated; k rotated, and v, into the pages
+      attend(layer, q)        every new token over all the sequence's tokens so far
+    with the tokens of all sequences packed one after the other ([N, heads, D]), for
+    prompts, chunks of them and single tokens alike.  bits 16: bf16 pages; 8: e4m3
+    with one power-of-two scale per token and KV head, half the bytes.  begin() and
+    release() copy counts from the host, so a captured step calls the ops on the
+    partition's tensors instead (with the capacity as max_len).
+    """
+
+    def __init__(self, num_layers, batch, num_kv_heads, head_dim, max_tokens, page_size=64,
+                 num_pages=None, bits=16, device="cuda"):
+        if head_dim % 32 or not 32 <= head_dim <= 256:
+            raise ValueError("head_dim must be a multiple of 32 up to 256")
+        if bits not in (8, 16):
+            raise ValueError("bits must be 8 or 16")
+        super().__init__(num_layers, batch, max_tokens, page_size, num_pages, device)
+        self.bits, self.num_kv_heads, self.head_dim = bits, num_kv_heads, head_dim
+        shape = (num_layers, self.num_pages, num_kv_heads, page_size, head_dim)
+        if bits == 16:
+            self.k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            self.v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            self.k_scale = self.v_scale = None
+        else:
+            self.k, self.v = (torch.empty(shape, dtype=ops.E4M3, device=self.device) for _ in range(2))
+            self.k_scale, self.v_scale = (torch.empty(shape[:4], dtype=ops.E8M0, device=self.device)
+                                          for _ in range(2))
+
     def append(self, layer: int, q, k, v, inv_freq, positions=None, **rope):
         """Rotary positions of q [N, Hq, D] and k [N, Hkv, D], and k and v into the
         step's slots of `layer` (ops.rope_append; positions [N] or [axes, N], the
@@ -592,13 +612,89 @@ class GqaRequestPartition:
         return ops.gqa_prompt(q, k, v, self.page_table, self.len_dev, step.cu_new, scale, max_len,
                               ks, vs, out_dtype=out_dtype)
 
-    def release(self, sequences) -> None:
-        """Drop all tokens of the given sequences; their pages are free again."""
-        done = np.zeros(self.batch, bool)
-        done[list(sequences)] = True
-        self.len_dev, self.free_dev = ops.pages_release(
-            self.page_table, self.len_dev, self._to_device(done, torch.bool), self.stack, self.free_dev,
-            self.page_size)
-        self.free += self._pages(self.lens[done])
-        self.lens = np.where(done, 0, self.lens)
-        self.step = None
+
+class MlaRequestPartition(_RequestPages):
+    """HBM pages of an absorbed-MLA latent cache for requests of any lengths: what
+    GqaRequestPartition is for GQA, with the same forward step,
+      begin(n_new)                   pages and slots for n_new[b] tokens of sequence b
+      append(layer, c, pe, q_pe, ..) the latents normalised, turned and into the pages;
+                                     q_pe turned
+      attend(layer, q_nope, q_pe, ..)  every new token over all the sequence's tokens so far
+    and read_back(layer, start, count), the tokens' latents as rows again, for what takes
+    them outside the pages (the expanded keys and values of a cached prefix, a host
+    segment).  bits 16: bf16 pages; 8: e4m3 with one power of two per scale_block tokens,
+    half the bytes (1: the least error; more: a scale that every token of the block
+    shares, raised where a later token needs it).
+    """
+
+    def __init__(self, num_layers, batch, max_tokens, page_size=64, num_pages=None, bits=16,
+                 scale_block=1, device="cuda"):
+        if bits not in (8, 16):
+            raise ValueError("bits must be 8 or 16")
+        if scale_block < 1 or scale_block & (scale_block - 1) or page_size % scale_block:
+            raise ValueError("scale_block must be a power of two that divides page_size")
+        super().__init__(num_layers, batch, max_tokens, page_size, num_pages, device)
+        self.bits, self.scale_block = bits, scale_block
+        shape = (num_layers, self.num_pages, page_size, ops.MLA_LATENT)
+        if bits == 16:
+            self.latent = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            self.scale = None
+        else:
+            self.latent = torch.empty(shape, dtype=ops.E4M3, device=self.device)
+            self.scale = torch.empty((num_layers, self.num_pages, page_size // scale_block), dtype=ops.E8M0,
+                                     device=self.device)
+
+    def _scale(self, layer: int):
+        return None if self.scale is None else self.scale[layer]
+
+    def append(self, layer: int, c, pe, q_pe, inv_freq, positions=None, **write):
+        """The step's latents, c [N, 512] and pe [N, 64], into their slots of `layer`, and q_pe
+        [N, H, 64] turned (ops.latent_rope_append, which names the keywords: norm_weight,
+        eps, adjacent, ...; positions [N], the step's own by default).  Returns the
+        turned q_pe."""
+        step = self._step()
+        return ops.latent_rope_append(c, pe, q_pe, step.positions if positions is None else positions,
+                                      inv_freq, step.slots, self.latent[layer], self._scale(layer), **write)
+
+    def attend(self, layer: int, q_nope, q_pe, scale: float, out_dtype=torch.float32):
+        """The step's tokens, q_nope [N, H, 512] and q_pe [N, H, 64] turned, over the pages:
+        (out [N, H, 512] in out_dtype (fp32 or bf16), lse [N, H]), which merges with a host
+        partial as the other partitions' (ops.lse_merge).  One token of every sequence
+        runs the decode kernels where there is one for the pages and the output,
+        anything else the prompt kernel."""
+        step = self._step()
+        if q_nope.dim() != 3 or q_nope.shape[0] != step.slots.shape[0]:
+            raise ValueError(f"q_nope must hold the step's {step.slots.shape[0]} tokens "
+                             f"(got {tuple(q_nope.shape)})")
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("out_dtype must be float32 or bfloat16")
+        H, max_len = q_nope.shape[1], int(self.lens.max()) if self.batch else 0
+        single = bool((self.n_new == 1).all())
+        if single and self.bits == 8:
+            decode = ops.mla8_decode_partial if out_dtype == torch.float32 else ops.mla8_decode_full
+            return decode(q_nope, q_pe, self.latent[layer], self.scale[layer], self.page_table, self.len_dev,
+                          scale, max_len)
+        if single and self.batch and out_dtype == torch.float32 and H % 16 == 0 and self.batch * H // 16 <= 2048:
+            if q_pe.shape != (self.batch, H, ops.MLA_PE) or not (q_nope.is_contiguous() and q_pe.is_contiguous()):
+                raise ValueError(f"q_pe must be [{self.batch}, {H}, {ops.MLA_PE}], and both queries contiguous")
+            out, lse = ops.mla_decode_partial(q_nope.view(-1, q_nope.shape[2]), q_pe.view(-1, ops.MLA_PE),
+                                              self.latent[layer], self.page_table, self.len_dev, scale, max_len)
+            return out.view(self.batch, H, ops.MLA_C), lse.view(self.batch, H)
+        return ops.mla_prompt(q_nope, q_pe, self.latent[layer], self.page_table, self.len_dev, step.cu_new,
+                              scale, max_len, self._scale(layer), out_dtype=out_dtype)
+
+    def read_back(self, layer: int, start, count):
+        """Tokens start[b] .. start[b] + count[b] of every sequence, one after the other:
+        (c [sum(count), 512], pe [sum(count), 64]) in bf16 (ops.latent_gather)."""
+        start, count = np.asarray(start, np.int64), np.asarray(count, np.int64)
+        if start.shape != (self.batch,) or count.shape != (self.batch,):
+            raise ValueError(f"start and count must hold {self.batch} values")
+        if (start < 0).any() or (count < 0).any() or (start + count > self.lens).any():
+            raise ValueError("start and count reach outside a sequence's tokens")
+        cu = np.concatenate([[0], np.cumsum(count)])
+        # one copy through pinned memory, as _to_device's
+        host = torch.empty(2 * self.batch + 1, dtype=torch.int32, pin_memory=True)
+        host.numpy()[:] = np.concatenate([start, cu])
+        start_dev, cu_dev = host.to(self.device, non_blocking=True).split((self.batch, self.batch + 1))
+        return ops.latent_gather(self.latent[layer], self.page_table, cu_dev, int(cu[-1]), start=start_dev,
+                                 latent_scale=self._scale(layer))

@@ -13,6 +13,9 @@ Tensor conventions (all CUDA/HIP tensors, contiguous):
   8-bit pools k_pages, v_pages  [num_pages, Hkv, page_size, D] float8_e4m3fn with
               k_scale, v_scale  [num_pages, Hkv, page_size]    float8_e8m0fnu
               (one power of two per token and KV head)
+  8-bit MLA   latent_pages [num_pages, page_size, 576] float8_e4m3fn with
+              latent_scale [num_pages, page_size / block] float8_e8m0fnu (one
+              power of two per `block` tokens, a power of two itself)
 """
 from __future__ import annotations
 
@@ -63,6 +66,13 @@ EXPORTS = (
     "ws_gqa8_decode_full",
     "ws_gqa_prompt_plan",
     "ws_gqa_prompt",
+    "ws_latent_rope_append",
+    "ws_latent_gather",
+    "ws_mla8_decode_plan",
+    "ws_mla8_decode_partial",
+    "ws_mla8_decode_full",
+    "ws_mla_prompt_plan",
+    "ws_mla_prompt",
 )
 
 # Formats of the second operand of lse_merge (include/wsgpu.h).
@@ -185,6 +195,20 @@ def lib() -> ctypes.CDLL:
         L.ws_gqa_prompt_plan.argtypes = [i32] * 8 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
         L.ws_gqa_prompt.restype = i32
         L.ws_gqa_prompt.argtypes = [vp] * 8 + [i32] * 10 + [f32, vp, vp, vp, vp, sz, vp]
+        L.ws_latent_rope_append.restype = i32
+        L.ws_latent_rope_append.argtypes = [vp, i64, vp, i64, vp, i64, i64, vp, vp, i32, f32, vp, i32,
+                                            f32, vp, vp, vp, vp] + [i32] * 5 + [vp]
+        L.ws_latent_gather.restype = i32
+        L.ws_latent_gather.argtypes = [vp, vp, i32, vp, vp, vp, vp, i64, vp, i64] + [i32] * 5 + [vp]
+        L.ws_mla8_decode_plan.restype = i32
+        L.ws_mla8_decode_plan.argtypes = [i32] * 4 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
+        for fn in (L.ws_mla8_decode_partial, L.ws_mla8_decode_full):
+            fn.restype = i32
+            fn.argtypes = [vp] * 6 + [i32] * 8 + [f32, vp, vp, vp, sz, vp]
+        L.ws_mla_prompt_plan.restype = i32
+        L.ws_mla_prompt_plan.argtypes = [i32] * 5 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
+        L.ws_mla_prompt.restype = i32
+        L.ws_mla_prompt.argtypes = [vp] * 7 + [i32] * 9 + [f32, vp, vp, vp, vp, sz, vp]
         _lib = L
     return _lib
 
@@ -583,10 +607,9 @@ def mla_decode_partial(q_nope, q_pe, latent_pages, page_table, gpu_len, scale, m
     _require(lse, "lse", torch.float32, dev, 1)
     nwg, wsb = decode_plan(1, B, H, int(max_len), int(n_workgroups))
     ws = _workspace(dev, wsb)
-    _check(lib().ws_mla_decode_partial(
-        _ptr(q_nope), _ptr(q_pe), _ptr(latent_pages), _ptr(page_table), _ptr(gpu_len),
-        B, H, PS, page_table.shape[1], P, int(max_len), nwg, float(scale),
-        _ptr(out), _ptr(lse), _ptr(ws), wsb, _stream(dev)), "ws_mla_decode_partial")
+    _run("ws_mla_decode_partial", dev, _ptr(q_nope), _ptr(q_pe), _ptr(latent_pages), _ptr(page_table),
+         _ptr(gpu_len), B, H, PS, page_table.shape[1], P, int(max_len), nwg, float(scale), _ptr(out),
+         _ptr(lse), _ptr(ws), wsb)
     return out, lse
 
 
@@ -1093,6 +1116,7 @@ _SCALE_ARGS = (("k_scale", E8M0, 3), ("v_scale", E8M0, 3))
 _DECODE16_ARGS = (("q", torch.bfloat16, 3), ("k_pages", torch.bfloat16, 4), ("v_pages", torch.bfloat16, 4),
                   ("page_table", torch.int32, 2), ("gpu_len", torch.int32, 1))
 _DECODE8_ARGS = (("q", torch.bfloat16, 3), ("page_table", torch.int32, 2), ("gpu_len", torch.int32, 1))
+_LATENT_ARGS = (("q_nope", torch.bfloat16, 3), ("q_pe", torch.bfloat16, 3), ("page_table", torch.int32, 2))
 _PROMPT_ARGS = (("q", torch.bfloat16, 3), ("page_table", torch.int32, 2), ("kv_len", torch.int32, 1),
                 ("cu_new", torch.int32, 1))
 
@@ -1428,5 +1452,236 @@ def gqa_prompt(q, k_pages, v_pages, page_table, kv_len, cu_new, scale, max_len, 
     o16, o32 = (out, None) if out.dtype == torch.bfloat16 else (None, out)
     _run("ws_gqa_prompt", dev, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
          _ptr(page_table), _ptr(kv_len), _ptr(cu_new), N, B, Hq, Hkv, D, PS, page_table.shape[1], P,
+         int(max_len), int(n_splits), float(scale), _ptr(o16), _ptr(o32), _ptr(lse), _ptr(ws), wsb)
+    return out, lse
+
+
+# ---------------------------------------------------------------------------
+# the same path over latent pages (absorbed MLA)
+
+
+def _latent_pool(latent_pages, latent_scale, dev):
+    """(num_pages, page_size, block) of a bf16 latent pool (block 0), or of an 8-bit
+    one with its scales."""
+    _require(latent_pages, "latent_pages", torch.bfloat16 if latent_scale is None else E4M3, dev, 3)
+    P, PS, L = latent_pages.shape
+    if L != MLA_LATENT:
+        raise ValueError(f"latent_pages must be [num_pages, page_size, {MLA_LATENT}]")
+    if latent_scale is None:
+        return P, PS, 0
+    _require(latent_scale, "latent_scale", E8M0, dev, 2)
+    n = latent_scale.shape[1]
+    block = PS // n if n else 0
+    if latent_scale.shape[0] != P or block < 1 or block * n != PS or block & (block - 1):
+        raise ValueError(f"latent_scale {tuple(latent_scale.shape)} must be [num_pages, page_size / block] "
+                         f"for latent_pages {tuple(latent_pages.shape)}, block a power of two")
+    return P, PS, block
+
+
+def _latent_rows(t, name, dev, N, width):
+    """The row stride of a [N, width] bf16 operand whose rows may be strided."""
+    _require(t, name, torch.bfloat16, dev, 2, contiguous=False)
+    if t.shape != (N, width) or (N > 0 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be [{N}, {width}] with unit last stride "
+                         f"(got {tuple(t.shape)}, strides {t.stride()})")
+    return t.stride(0) if N > 1 else width
+
+
+def latent_rope_append(c, pe, q_pe, positions, inv_freq, slots, latent_pages, latent_scale=None,
+                       norm_weight=None, eps=1e-6, adjacent=False, factor=1.0, q_out=None):
+    """A forward step's latents into their pages, and the heads' q_pe turned with them
+    (ws_latent_rope_append).  c [N, 512] and pe [N, 64] (rows may be strided: parts of
+    the down projection's output), q_pe [N, H, 64] (tokens and heads may be strided:
+    a part of every head's query); positions [N] int32, inv_freq [32] fp32.  Token t's
+    latent, c through an RMS norm with norm_weight [512] (bf16 or fp32; None: as it is)
+    and pe turned by its position, goes to slot slots[t] (pages_extend), in bf16 or, with
+    latent_scale, in 8 bits: e4m3 with one power of two per block of tokens.  A block
+    that holds tokens keeps at least its scale; the tokens of a block follow one
+    another in a call.  A slot outside the pool (-1) writes nothing; slots must
+    differ.  adjacent and factor as rope()'s.  Returns q_out [N, H, 64]."""
+    dev = _gpu(c, "c")
+    _require(q_pe, "q_pe", torch.bfloat16, dev, 3, contiguous=False)
+    N, H, W = q_pe.shape
+    c_stride, pe_stride = _latent_rows(c, "c", dev, N, MLA_C), _latent_rows(pe, "pe", dev, N, MLA_PE)
+    if W != MLA_PE or H == 0 or (N > 0 and q_pe.stride(2) != 1):
+        raise ValueError(f"q_pe must be [{N}, H, {MLA_PE}] with unit last stride (got {tuple(q_pe.shape)}, "
+                         f"strides {q_pe.stride()})")
+    q_head = q_pe.stride(1) if H > 1 else MLA_PE
+    q_stride = q_pe.stride(0) if N > 1 else H * q_head
+    _require(positions, "positions", torch.int32, dev, 1)
+    _require(slots, "slots", torch.int32, dev, 1)
+    _require(inv_freq, "inv_freq", torch.float32, dev, 1)
+    if positions.shape[0] != N or slots.shape[0] != N or inv_freq.shape[0] != MLA_PE // 2:
+        raise ValueError(f"positions and slots must be [{N}] and inv_freq [{MLA_PE // 2}]")
+    P, PS, block = _latent_pool(latent_pages, latent_scale, dev)
+    f32 = 0
+    if norm_weight is not None:
+        f32 = int(isinstance(norm_weight, torch.Tensor) and norm_weight.dtype == torch.float32)
+        _require(norm_weight, "norm_weight", torch.float32 if f32 else torch.bfloat16, dev, 1)
+        if norm_weight.shape[0] != MLA_C:
+            raise ValueError(f"norm_weight must be [{MLA_C}]")
+    if q_out is None:
+        q_out = torch.empty((N, H, W), dtype=torch.bfloat16, device=dev)
+    else:
+        _require(q_out, "q_out", torch.bfloat16, dev, 3)
+        if q_out.shape != q_pe.shape:
+            raise ValueError("q_out must have q_pe's shape")
+    if N == 0:
+        return q_out
+    _run("ws_latent_rope_append", dev, _ptr(c), c_stride, _ptr(pe), pe_stride, _ptr(q_pe), q_stride,
+         q_head, _ptr(positions), _ptr(inv_freq), int(bool(adjacent)), float(factor), _ptr(norm_weight),
+         f32, float(eps), _ptr(slots), _ptr(q_out), _ptr(latent_pages), _ptr(latent_scale), block, N, H,
+         PS, P)
+    return q_out
+
+
+def latent_gather(latent_pages, page_table, cu_rows, n_rows, start=None, latent_scale=None, c_out=None,
+                  pe_out=None):
+    """Ranges of tokens read back from latent pages, bf16 or 8-bit (ws_latent_gather):
+    rows cu_rows[b] .. cu_rows[b + 1] of (c [n_rows, 512], pe [n_rows, 64]), both bf16, are
+    sequence b's tokens from start[b] on (None: 0); exact.  c_out and pe_out may be
+    strided (parts of one [n_rows, 576] tensor); rows outside [cu_rows[0], cu_rows[B])
+    are left as they are (uninitialised in new tensors).  A token outside the
+    capacity, or in a page outside the pool, gives NaN."""
+    dev = _gpu(latent_pages, "latent_pages")
+    P, PS, block = _latent_pool(latent_pages, latent_scale, dev)
+    _require(page_table, "page_table", torch.int32, dev, 2)
+    _require(cu_rows, "cu_rows", torch.int32, dev, 1)
+    B, N = page_table.shape[0], int(n_rows)
+    if cu_rows.shape[0] != B + 1 or N < 0:
+        raise ValueError("cu_rows must be [B + 1] for page_table's B rows, and n_rows >= 0")
+    if start is not None:
+        _require(start, "start", torch.int32, dev, 1)
+        if start.shape[0] != B:
+            raise ValueError("start must be [B]")
+    if c_out is None:
+        c_out = torch.empty((N, MLA_C), dtype=torch.bfloat16, device=dev)
+    if pe_out is None:
+        pe_out = torch.empty((N, MLA_PE), dtype=torch.bfloat16, device=dev)
+    c_stride = _latent_rows(c_out, "c_out", dev, N, MLA_C)
+    pe_stride = _latent_rows(pe_out, "pe_out", dev, N, MLA_PE)
+    if N == 0 or B == 0:
+        return c_out, pe_out
+    _run("ws_latent_gather", dev, _ptr(latent_pages), _ptr(latent_scale), block, _ptr(page_table),
+         _ptr(start), _ptr(cu_rows), _ptr(c_out), c_stride, _ptr(pe_out), pe_stride, N, B, PS,
+         page_table.shape[1], P)
+    return c_out, pe_out
+
+
+def _mla_rows_plan(name, *sizes):
+    key = (name, *sizes, torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1)
+    hit = _plans.get(key)
+    if hit is not None:
+        return hit
+    n, wsb = ctypes.c_int(0), ctypes.c_size_t(0)
+    _check(getattr(lib(), name)(*sizes, ctypes.byref(n), ctypes.byref(wsb)), name)
+    if len(_plans) > 4096:
+        _plans.clear()
+    _plans[key] = (n.value, wsb.value)
+    return n.value, wsb.value
+
+
+def mla8_plan(batch: int, H: int, max_len: int, n_splits: int = 0):
+    """(pieces, workspace_bytes) of a decode call over 8-bit latent pages."""
+    return _mla_rows_plan("ws_mla8_decode_plan", batch, H, max_len, n_splits)
+
+
+def mla_prompt_plan(n_tokens: int, batch: int, H: int, max_len: int, n_splits: int = 0):
+    """(pieces, workspace_bytes) of an MLA prompt call."""
+    return _mla_rows_plan("ws_mla_prompt_plan", n_tokens, batch, H, max_len, n_splits)
+
+
+def _latent_queries(q_nope, q_pe, page_table, dev):
+    _require_all(dev, _LATENT_ARGS, (q_nope, q_pe, page_table))
+    N, H, C = q_nope.shape
+    if C != MLA_C or q_pe.shape != (N, H, MLA_PE) or H == 0:
+        raise ValueError(f"q_nope {tuple(q_nope.shape)} and q_pe {tuple(q_pe.shape)} must be [N, H, {MLA_C}] "
+                         f"and [N, H, {MLA_PE}]")
+    return N, H
+
+
+def _latent_out(out, lse, N, H, dtype, dev, want_lse=True, name="out"):
+    if out is None:
+        out = torch.empty((N, H, MLA_C), dtype=dtype, device=dev)
+    else:
+        _require(out, name, dtype, dev, 3)
+        if out.shape != (N, H, MLA_C):
+            raise ValueError(f"{name} must be [{N}, {H}, {MLA_C}]")
+    if lse is not None:
+        _require(lse, "lse", torch.float32, dev, 2)
+        if lse.shape != (N, H):
+            raise ValueError(f"lse must be [{N}, {H}]")
+    elif want_lse:
+        lse = torch.empty((N, H), dtype=torch.float32, device=dev)
+    return out, lse
+
+
+def _mla8_decode(name, dtype, q_nope, q_pe, latent_pages, latent_scale, page_table, gpu_len, scale,
+                 max_len, n_splits, out, lse):
+    dev = _gpu(q_nope, "q_nope")
+    if latent_scale is None:
+        raise TypeError("latent_scale must be a tensor")
+    P, PS, block = _latent_pool(latent_pages, latent_scale, dev)
+    B, H = _latent_queries(q_nope, q_pe, page_table, dev)
+    _require(gpu_len, "gpu_len", torch.int32, dev, 1)
+    if page_table.shape[0] != B or gpu_len.shape[0] != B:
+        raise ValueError("page_table/gpu_len batch mismatch")
+    out, lse = _latent_out(out, lse, B, H, dtype, dev, name="out" if dtype == torch.float32 else "out_bf16")
+    if B == 0:
+        return out, lse
+    _, wsb = mla8_plan(B, H, int(max_len), int(n_splits))
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    _run(name, dev, _ptr(q_nope), _ptr(q_pe), _ptr(latent_pages), _ptr(latent_scale), _ptr(page_table),
+         _ptr(gpu_len), B, H, PS, page_table.shape[1], P, block, int(max_len), int(n_splits), float(scale),
+         _ptr(out), _ptr(lse), _ptr(ws), wsb)
+    return out, lse
+
+
+def mla8_decode_partial(q_nope, q_pe, latent_pages, latent_scale, page_table, gpu_len, scale, max_len,
+                        n_splits=0, out=None, lse=None):
+    """mla_decode_partial over 8-bit latent pages (ws_mla8_decode_partial): q_nope
+    [B, H, 512], q_pe [B, H, 64] bf16, H up to 1024 -> (out [B, H, 512] fp32 normalised,
+    lse [B, H] fp32).  max_len must bound every gpu_len[b].  n_splits: workgroups that
+    share a sequence's tokens (0: the library's choice by the lengths)."""
+    return _mla8_decode("ws_mla8_decode_partial", torch.float32, q_nope, q_pe, latent_pages, latent_scale,
+                        page_table, gpu_len, scale, max_len, n_splits, out, lse)
+
+
+def mla8_decode_full(q_nope, q_pe, latent_pages, latent_scale, page_table, gpu_len, scale, max_len,
+                     n_splits=0, out_bf16=None, lse=None):
+    """mla8_decode_partial for a partition that holds every token: returns
+    (out [B, H, 512] bf16, lse [B, H] fp32)."""
+    return _mla8_decode("ws_mla8_decode_full", torch.bfloat16, q_nope, q_pe, latent_pages, latent_scale,
+                        page_table, gpu_len, scale, max_len, n_splits, out_bf16, lse)
+
+
+def mla_prompt(q_nope, q_pe, latent_pages, page_table, kv_len, cu_new, scale, max_len, latent_scale=None,
+               n_splits=0, out_dtype=torch.bfloat16, want_lse=True, out=None, lse=None):
+    """gqa_prompt over latent pages, absorbed (ws_mla_prompt): q_nope [N, H, 512] and
+    q_pe [N, H, 64] bf16, packed; sequence b's queries are rows cu_new[b] ..
+    cu_new[b + 1] and the last of its kv_len[b] tokens in the pages, bf16 or (with
+    latent_scale) 8-bit.  Returns (out [N, H, 512] in out_dtype (bf16 or fp32), lse
+    [N, H] fp32 or None); rows outside [cu_new[0], cu_new[B]) are not written.
+    max_len must bound every kv_len[b].  n_splits: workgroups that share a tile of
+    rows (0: the library's choice by the lengths)."""
+    dev = _gpu(q_nope, "q_nope")
+    P, PS, block = _latent_pool(latent_pages, latent_scale, dev)
+    N, H = _latent_queries(q_nope, q_pe, page_table, dev)
+    _require(kv_len, "kv_len", torch.int32, dev, 1)
+    _require(cu_new, "cu_new", torch.int32, dev, 1)
+    B = page_table.shape[0]
+    if kv_len.shape[0] != B or cu_new.shape[0] != B + 1:
+        raise ValueError("kv_len must be [B] and cu_new [B + 1] for page_table's B rows")
+    dtype = out_dtype if out is None else getattr(out, "dtype", None)
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("out_dtype must be bfloat16 or float32")
+    out, lse = _latent_out(out, lse, N, H, dtype, dev, want_lse)
+    if N == 0 or B == 0:
+        return out, lse
+    _, wsb = mla_prompt_plan(N, B, H, int(max_len), int(n_splits))
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    o16, o32 = (out, None) if dtype == torch.bfloat16 else (None, out)
+    _run("ws_mla_prompt", dev, _ptr(q_nope), _ptr(q_pe), _ptr(latent_pages), _ptr(latent_scale),
+         _ptr(page_table), _ptr(kv_len), _ptr(cu_new), N, B, H, PS, page_table.shape[1], P, block,
          int(max_len), int(n_splits), float(scale), _ptr(o16), _ptr(o32), _ptr(lse), _ptr(ws), wsb)
     return out, lse
