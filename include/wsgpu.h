@@ -709,11 +709,12 @@ int ws_mla8_decode_full(const uint16_t* q_nope, const uint16_t* q_pe,
  * not written.  A row that sees a token in a page with an id outside the pool is NaN, and
  * so is every row of a sequence whose length is outside [0, capacity]; an infinity or a NaN
  * in a token changes only the rows that see it.
- * n_splits, max_len and the workspace (ws_mla_prompt_plan) as ws_mla8_decode_partial's.
+ * n_splits, max_len and the workspace (ws_mla_prompt_plan; fp8: whether the pages are
+ * 8-bit) as ws_mla8_decode_partial's.
  * The reference runs prompts through its framework's attention on expanded keys and values
  * (system/deepseek.py:279-322).
  */
-int ws_mla_prompt_plan(int N, int B, int H, int max_len, int n_splits, int* pieces_out,
+int ws_mla_prompt_plan(int N, int B, int H, int fp8, int max_len, int n_splits, int* pieces_out,
                        size_t* workspace_bytes_out);
 int ws_mla_prompt(const uint16_t* q_nope, const uint16_t* q_pe, const void* latent_pages,
                   const uint8_t* latent_scale, const int32_t* page_table, const int32_t* kv_len,

@@ -16,18 +16,14 @@
 // k + 1's scores and block k's values' product interleaved, the output in 256
 // accumulator registers that nothing rescales.
 //
-// 8-bit pages (e4m3, a power of two per `block` tokens) lie in LDS as they are, half the
-// bytes, and are never widened for the scores: v_mfma_scale_f32_32x32x64_f8f6f4 takes
-// e4m3 operands with a power of two per 32 columns, so the latents enter with their
-// tokens' scales as they are stored.  The query is split into two e4m3 values,
-//   q = 2^e (hi + lo / 16),  hi = e4m3(q / 2^e), lo = e4m3(16 (q / 2^e - hi)),
-// e the least that keeps the row's largest at 448: bf16 has 8 significant bits, e4m3 has 4,
-// and the rest of a rounding to 4 of 8 bits has 4, so the split is exact for every column
-// within 2^-14 of the row's largest (2^-22 of it for the smaller ones).  Two products at
-// twice the bf16 rate take the time of one in bf16, without the 144 conversions that
-// widening would cost a wave and block.  The values' product has P in bf16: its operand is
-// read transposed in 8 bits and widened (four instructions an MFMA), and a token's scale
-// goes to its probability instead of its 512 columns.
+// 8-bit pages (e4m3, a power of two per `block` tokens) are widened once for the four waves:
+// a wave's part of a block comes to LDS as it is, is read back, multiplied by its tokens'
+// scales (exact in bf16) and written into the block's bf16 tile, two steps ahead.
+//
+// The scores stay with bf16 products.  gfx950's scaled 8-bit products take e4m3 latents and
+// a query split into two e4m3 halves without any widening, at the same rate, but add up
+// their 64 terms in some 17 bits below the largest one, not in fp32: an lse off by 4e-5, a
+// hundred times this kernel's (2700 against 2900 cycles a step).
 #include <math.h>
 
 #include <algorithm>
@@ -40,11 +36,9 @@
 
 namespace ws {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
 constexpr int kRowsC = 512;
 constexpr int kRowsPe = 64;
-constexpr int kRowsTile = 128;       // rows of a tile, 32 a wave
+constexpr int kRowsTile = 128;       // rows of a tile, 32 a wave (mla_few_kernel: 32)
 constexpr int kRowsMaxSplits = 256;  // of a tile
 constexpr int kRowsMinShare = 4;     // blocks of a split, at the least
 
@@ -59,7 +53,7 @@ struct RowsParams {
   uint16_t* out_bf16;
   float* out_f32;
   float* lse;
-  float* part_out;  // [pieces][piece_rows][512], with part_lse [pieces][piece_rows]
+  uint16_t* part_out;  // [pieces][piece_rows][512], with part_lse [pieces][piece_rows]
   float* part_lse;
   int N, B, H, page_size, max_pages, num_pages, cap, block_log2;
   int n_splits;  // of every tile; 0: by the lengths, about `fill` workgroups in all
@@ -67,6 +61,7 @@ struct RowsParams {
   bool fit;       // the tiles are fewer than `fill`: all items are to fit
   int pieces;     // room for them
   int piece_rows;
+  int tile;       // rows of a tile
   float scale_log2;  // > 0
   uint32_t q_sign;   // 0x80008000 where the caller's scale is negative
 };
@@ -86,7 +81,7 @@ __device__ __forceinline__ RowsSeq rows_seq(const RowsParams& p, int b) {
     s.n = min(max(p.cu_new[b + 1], s.c0), p.N) - s.c0;
   }
   s.len = p.kv_len[b];
-  s.tiles = (s.n * p.H + kRowsTile - 1) / kRowsTile;
+  s.tiles = (s.n * p.H + p.tile - 1) / p.tile;
   s.blocks = len_ok(s.len, 0, p.cap) ? (s.len + 31) / 32 : 0;
   return s;
 }
@@ -99,7 +94,7 @@ struct RowsPlace {
   int c0, n, len;
 };
 
-// Item `at` of the list of all tiles' splits (TILES: of all tiles): longest sequences
+// Item `at` of the list of all tiles' splits (TILES: of the split tiles): longest sequences
 // first (up to 64 of them), their last tile first.  A tile has one split for every M of
 // its sequence's blocks, M the batch's blocks over `fill` workgroups, and where the tiles
 // alone are fewer than those the least M (within 2^-6) at which all items fit.  Every
@@ -172,7 +167,7 @@ __device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
     const RowsSeq s = rows_seq(p, b0 + k);
     const int splits = splits_of(s);
     units += splits > 1 ? s.tiles * splits : 0;
-    items += TILES ? s.tiles : s.tiles * splits;
+    items += !TILES ? s.tiles * splits : splits > 1 ? s.tiles : 0;
     key = s.blocks;
   }
   const int before = __ockl_wfscan_add_i32(units, true) - units;
@@ -201,7 +196,7 @@ __device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
     const RowsSeq s = rows_seq(p, b);
     const int splits = uniform(splits_of(s));
     const int tiles = uniform(s.tiles);
-    const int here = TILES ? tiles : tiles * splits;
+    const int here = !TILES ? tiles * splits : splits > 1 ? tiles : 0;
     if (left < here) {
       const int t = TILES ? left : left / splits;
       r.b = b;
@@ -223,38 +218,25 @@ __device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
 // ---------------------------------------------------------------------------
 // the LDS ring
 
+// Both kinds of pages have ws_mla_ring.h's bf16 tiles.  bf16: four, loaded three blocks ahead.
+// 8 bits: three, and per wave two slots for its eight rows of a block as they are in the
+// pages, 288 chunks of 16 bytes and the block's scales, loaded four blocks ahead.
+constexpr int kRowsTileBytes = 16 * kWideTileAlloc;
+constexpr int kRawRows = 8;             // of a wave
+constexpr int kRawChunks = 36 * kRawRows;
+constexpr int kRawDma = 5;              // load instructions, and one for the scales
+constexpr int kRawBytes = 1024 * kRawDma;
 template <bool F8>
-struct RowsRing;
-// bf16: ws_mla_wide.h's tiles, three blocks ahead.
-template <>
-struct RowsRing<false> {
-  static constexpr int kTiles = kWideTiles;
-  static constexpr int kDma = kWideTileDma;  // 1 KB load instructions of a block
-  static constexpr int kPer = kWideDmaPerWave;
-  static constexpr int kRowBytes = 1152;
-  static constexpr int kRowsS = kWideRowsS;
-  __host__ __device__ static constexpr int row_off(int r) { return wide_row_off(r); }
-  __device__ static int row_of(int c) { return wide_row_of(c); }
+struct RowsRing {
+  static constexpr int kTiles = F8 ? 3 : kWideTiles;
+  static constexpr int kRowBytes = F8 ? 576 : 1152;
+  // LDS: tiles, then the bf16 sink or the waves' raw slots, then the raw slots' scales
+  static constexpr int kRaw = kTiles * kRowsTileBytes;
+  static constexpr int kScales = kRaw + (F8 ? 4 * 2 * kRawBytes : 1024);
+  static constexpr int kLds = kScales + (F8 ? 4 * 2 * 256 : 0);
 };
-// 8 bits: rows of 36 chunks of 16 bytes and one chunk of padding every four rows, so that
-// the score reads (16 rows, one chunk each) meet 16 chunk slots mod 16 and the transposed
-// reads (rows 4 j .. 4 j + 3 and 8 more, 32 bytes of each) 8 different pairs of them.  19
-// instructions fill a tile: five a wave but the last, whose fifth loads the block's scales.
-template <>
-struct RowsRing<true> {
-  static constexpr int kTiles = 8;
-  static constexpr int kDma = 19;
-  static constexpr int kPer = 5;
-  static constexpr int kRowBytes = 576;
-  static constexpr int kRowsS = 580;  // chunks from row r to r + 16
-  __host__ __device__ static constexpr int row_off(int r) { return 36 * r + (r >> 2); }
-  __device__ static int row_of(int c) {
-    const int g = min(c / 145, 7);
-    return 4 * g + min((c - 145 * g) / 36, 3);
-  }
-};
-static_assert(RowsRing<true>::row_off(31) + 36 <= 64 * RowsRing<true>::kDma, "a tile's chunks");
-static_assert(RowsRing<true>::row_off(16 + 8 + 4 + 3) == 580 + 290 + 145 + 108, "row offsets add up");
+static_assert(RowsRing<true>::kLds <= 160 * 1024 - 64 && RowsRing<false>::kLds <= 160 * 1024 - 64, "LDS");
+static_assert(RowsRing<true>::kScales >= kRowsTile * 65 * 16, "the queries are staged in the tiles");
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -275,23 +257,6 @@ __device__ __forceinline__ void rows_dma1(uint32_t off, const void* sbase, uint3
 }
 #pragma clang diagnostic pop
 
-// Score products with their accumulator in VGPRs (ws_mla_ring.h qk_*).  The s_nop: the
-// latents' registers may just have been moved, which the compiler does not see an MFMA
-// read here.
-__device__ __forceinline__ void qk8_first(f32x16& c, const i32x8& a, const i32x8& b, int sa,
-                                          int sb) {
-  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel_hi:[0,0,0]"
-               : "=&v"(c)
-               : "v"(a), "v"(b), "v"(sa), "v"(sb)
-               : "memory");
-}
-__device__ __forceinline__ void qk8_next(f32x16& c, const i32x8& a, const i32x8& b, int sa,
-                                         int sb) {
-  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
-               : "+v"(c)
-               : "v"(a), "v"(b), "v"(sa), "v"(sb)
-               : "memory");
-}
 // The wait states that a VALU read of the last product's result asks for (16 passes and
 // four).
 __device__ __forceinline__ void qk_settle(f32x16& c) {
@@ -302,51 +267,27 @@ __device__ __forceinline__ void qk_settle_short(f32x16& c) {
   asm volatile("s_nop 3" : "+v"(c) : : "memory");
 }
 
-// Has a value in registers at this point.  (A function: as a statement of the kernel itself,
-// the host's compiler refuses the wider registers and leaves the kernel out.)
-template <class T>
-__device__ __forceinline__ void hold(T& x) {
-  asm volatile("" : "+v"(x) : : "memory");
-}
-
-// Four columns of a query (bf16 pairs w0, w1) over `unit` as e4m3, and what that leaves
-// over `sub`.
-__device__ __forceinline__ void split_query4(uint32_t w0, uint32_t w1, float unit, float sub,
-                                             int& hi, int& lo) {
-  typedef short s16x2_t __attribute__((ext_vector_type(2)));
-  typedef float f32x2_t __attribute__((ext_vector_type(2)));
-  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-  s16x2_t h8 = {0, 0}, l8 = {0, 0};
-  h8 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h8, __builtin_bit_cast(bf16x2_t, w0), unit, false);
-  h8 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h8, __builtin_bit_cast(bf16x2_t, w1), unit, true);
-  const uint32_t hw = __builtin_bit_cast(uint32_t, h8);
-  const f32x2_t b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, unit, false);
-  const f32x2_t b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, unit, true);
-  const float r0 = __builtin_bit_cast(float, w0 << 16) - b0[0];
-  const float r1 = __builtin_bit_cast(float, w0 & 0xffff0000u) - b0[1];
-  const float r2 = __builtin_bit_cast(float, w1 << 16) - b1[0];
-  const float r3 = __builtin_bit_cast(float, w1 & 0xffff0000u) - b1[1];
-  l8 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l8, r0, r1, sub, false);
-  l8 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l8, r2, r3, sub, true);
-  hi = (int)hw;
-  lo = __builtin_bit_cast(int, l8);
-}
-
 template <bool HI>
-__device__ __forceinline__ uint32_t widen2(uint32_t w) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
+__device__ __forceinline__ uint32_t widen2(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
 }
-// Eight e4m3 values as bf16 (exact).
-__device__ __forceinline__ u32x4 widen8(const uint2& w) {
-  return u32x4{widen2<false>(w.x), widen2<true>(w.x), widen2<false>(w.y), widen2<true>(w.y)};
+// Eight e4m3 values times a power of two as bf16 (exact).
+__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float scale) {
+  return u32x4{widen2<false>(lo, scale), widen2<true>(lo, scale), widen2<false>(hi, scale),
+               widen2<true>(hi, scale)};
 }
-// ds_read_b64_tr_b8: in each 16-lane group lanes 2 e and 2 e + 1 address the halves of
-// row e's 16 bytes; result lane i holds byte i of rows 0 .. 7 (measured in bounds).
-__device__ __forceinline__ uint2 lds_read_tr8_b64(uint32_t addr) {
-  typedef int i32x2_t __attribute__((ext_vector_type(2)));
-  typedef __attribute__((address_space(3))) i32x2_t lds_i32x2_t;
-  const i32x2_t v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t*)(uintptr_t)addr);
-  return make_uint2((uint32_t)v[0], (uint32_t)v[1]);
+__device__ __forceinline__ u32x4 rows_lds_b128(uint32_t addr) {
+  return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)addr;
+}
+__device__ __forceinline__ uint32_t rows_lds_b32(uint32_t addr) {
+  return *(const __attribute__((address_space(3))) uint32_t*)(uintptr_t)addr;
+}
+__device__ __forceinline__ void rows_lds_put(uint32_t addr, const u32x4& v) {
+  *(__attribute__((address_space(3))) u32x4*)(uintptr_t)addr = v;
+}
+template <int N>
+__device__ __forceinline__ void rows_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
 // Stores `rows` staged 1 KB rows (row h at src + 260 h dwords, lane part at src) to dst + h *
@@ -370,109 +311,118 @@ __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
   const uint32_t hit = (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15;
   return hit * 0xffffu;
 }
-// The bytes of four e4m3 values that are NaN, all set.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
-  const uint32_t hit = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-  return hit * 0xffu;
+// A workgroup's rows and tokens, and where its outputs go.
+struct RowsWork {
+  RowsPlace pl;
+  bool piece, len_good;
+  int R_all, row0, here, first_pos, lim_lo, nblk, t_begin, t_end;
+  size_t g_row0, o_row0;  // the tile's first row of q, and of the outputs (or its piece)
+};
+// False: the workgroup has nothing to do (it is past the list, or its rows see nothing and
+// are written here: (0, -inf), NaN for an invalid length).
+__device__ __forceinline__ bool rows_work(const RowsParams& p, RowsWork& w) {
+  const int tid = threadIdx.x;
+  w.pl = rows_place<false>(p, blockIdx.x);
+  const RowsPlace& pl = w.pl;
+  w.piece = pl.splits > 1;
+  if (pl.b < 0 || (w.piece && (pl.piece < 0 || pl.piece >= p.pieces))) return false;
+  w.R_all = pl.n * p.H;
+  w.row0 = pl.tile * p.tile;
+  w.here = min(p.tile, w.R_all - w.row0);
+  w.len_good = len_ok(pl.len, 0, p.cap);
+  w.first_pos = pl.len - pl.n;  // position of the sequence's first query
+  // tokens that the tile's first row and its last one see
+  w.lim_lo = w.first_pos + w.row0 / p.H + 1;
+  const int lim_hi = w.len_good ? max(w.first_pos + (w.row0 + w.here - 1) / p.H + 1, 0) : 0;
+  const int nb = (lim_hi + 31) / 32;
+  const int blk0 = (int)((long long)pl.split * nb / pl.splits);
+  const int blk1 = (int)((long long)(pl.split + 1) * nb / pl.splits);
+  w.nblk = blk1 - blk0;
+  w.t_begin = 32 * blk0;
+  w.t_end = min(lim_hi, 32 * blk1);
+  w.g_row0 = (size_t)pl.c0 * p.H + w.row0;
+  w.o_row0 = w.piece ? (size_t)pl.piece * p.piece_rows : w.g_row0;
+  if (w.nblk > 0) return true;
+  const float fill = w.len_good ? 0.f : qnan();
+  const uint32_t fill2 = pack_bf16x2(fill, fill);
+  for (int x = tid; x < w.here * (kRowsC / 4); x += 256) {
+    const size_t at = w.o_row0 * (kRowsC / 4) + x;
+    if (w.piece) {
+      ((uint2*)p.part_out)[at] = make_uint2(fill2, fill2);
+    } else {
+      if (p.out_f32) ((float4*)p.out_f32)[at] = make_float4(fill, fill, fill, fill);
+      if (p.out_bf16) ((uint2*)p.out_bf16)[at] = make_uint2(fill2, fill2);
+    }
+  }
+  if (tid < w.here) {
+    const float l = w.len_good ? neg_inf() : qnan();
+    if (w.piece) p.part_lse[w.o_row0 + tid] = l;
+    else if (p.lse) p.lse[w.o_row0 + tid] = l;
+  }
+  return false;
 }
 
 template <bool F8>
 __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   using R = RowsRing<F8>;
-  constexpr int kAlloc = 64 * R::kDma;
-  constexpr int kAhead = R::kTiles - 1;  // blocks requested ahead of the one whose values are taken
   constexpr int kRow = R::kRowBytes;
-  constexpr int kChunks = kRow / 16;
-  __shared__ u32x4 s_tile[R::kTiles][kAlloc];
-  __shared__ u32x4 s_sink[F8 ? 1 : 64];
-  __shared__ uint32_t s_scale[F8 ? R::kTiles : 1][64];
+  constexpr int kTileChunks = kWideTileAlloc;
+  constexpr int kPer = F8 ? kRawDma + 1 : kWideDmaPerWave;  // a wave's load instructions of a block
+  __shared__ __attribute__((aligned(1024))) char s_mem[R::kLds];
   __shared__ int s_redo;
-  static_assert(R::kTiles * kAlloc >= kRowsTile * 65, "the queries are staged in the tiles");
   const int tid = threadIdx.x;
   const int wave = uniform(tid >> 6);
   const int lane = tid & 63;
   const int n32 = lane & 31;  // row of the wave (QK B, PV B, output) or token (A operands)
   const int j2 = lane >> 5;
   const int H = p.H;
-
-  const RowsPlace pl = rows_place<false>(p, blockIdx.x);
-  const bool piece = pl.splits > 1;
-  if (pl.b < 0 || (piece && (pl.piece < 0 || pl.piece >= p.pieces))) return;
+  RowsWork w;
+  if (!rows_work(p, w)) return;
   if (tid == 0) s_redo = 0;  // read after the ring's barriers
-  const int R_all = pl.n * H;
-  const int row0 = pl.tile * kRowsTile;
-  const int here = min(kRowsTile, R_all - row0);
+  const int nblk = w.nblk, t_begin = w.t_begin, t_end = w.t_end, here = w.here;
   const int rows = min(max(here - 32 * wave, 0), 32);  // this wave's
-  const bool len_good = len_ok(pl.len, 0, p.cap);
-  const int first_pos = pl.len - pl.n;  // position of the sequence's first query
-  // tokens that the tile's first row and its last one see
-  const int lim_lo = first_pos + row0 / H + 1;
-  const int lim_hi = len_good ? max(first_pos + (row0 + here - 1) / H + 1, 0) : 0;
-  const int nb = (lim_hi + 31) / 32;
-  const int blk0 = (int)((long long)pl.split * nb / pl.splits);
-  const int blk1 = (int)((long long)(pl.split + 1) * nb / pl.splits);
-  const int nblk = blk1 - blk0;
-  const int t_begin = 32 * blk0;
-  const int t_end = min(lim_hi, 32 * blk1);
-  const size_t g_row0 = (size_t)pl.c0 * H + row0;  // of q, out and lse
-  const size_t o_row0 = piece ? (size_t)pl.piece * p.piece_rows : g_row0;
-  if (nblk <= 0) {  // nothing to see: (0, -inf), or NaN for an invalid length
-    const float fill = len_good ? 0.f : qnan();
-    for (int x = tid; x < here * (kRowsC / 4); x += 256) {
-      const size_t at = o_row0 * (kRowsC / 4) + x;
-      if (piece) {
-        ((float4*)p.part_out)[at] = make_float4(fill, fill, fill, fill);
-      } else {
-        if (p.out_f32) ((float4*)p.out_f32)[at] = make_float4(fill, fill, fill, fill);
-        if (p.out_bf16) ((uint2*)p.out_bf16)[at] = make_uint2(pack_bf16x2(fill, fill), pack_bf16x2(fill, fill));
-      }
-    }
-    if (tid < here) {
-      const float l = len_good ? neg_inf() : qnan();
-      if (piece) p.part_lse[o_row0 + tid] = l;
-      else if (p.lse) p.lse[o_row0 + tid] = l;
-    }
-    return;
-  }
   // the tokens that the lane's row sees (past the rows: the last one again)
-  const int lim_lane = first_pos + min(row0 + 32 * wave + n32, R_all - 1) / H + 1;
+  const int lim_lane = w.first_pos + min(w.row0 + 32 * wave + n32, w.R_all - 1) / H + 1;
 
-  const uint32_t tile_base0 = (uint32_t)uniform((int)(uint32_t)(uintptr_t)&s_tile[0][0]);
-  const uint32_t sink_base = (uint32_t)uniform((int)(uint32_t)(uintptr_t)&s_sink[0]);
-  const uint32_t scale_base = (uint32_t)uniform((int)(uint32_t)(uintptr_t)&s_scale[0][0]);
-  // Byte offsets, within a block's rows in HBM, of the chunks this lane loads, two to a
-  // register (the largest is 31 * 1152 + 1136).
-  constexpr int kOff = (R::kPer + 1) / 2;
+  const uint32_t lds0 =
+      (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem);
+  u32x4* const s_tile = (u32x4*)s_mem;
+  const uint32_t raw0 = lds0 + R::kRaw + 2 * kRawBytes * wave;       // this wave's (8 bits)
+  const uint32_t scale0 = lds0 + R::kScales + 2 * 256 * wave;
+  // bf16: byte offsets, within a block's rows in HBM, of the chunks this lane loads, two to a
+  // register (the largest is 31 * 1152 + 1136).  8 bits: for each of the lane's chunks of
+  // the wave's raw slot, where it goes in a tile, in 16-byte units from the wave's first row
+  // (10 bits), and its row less that one.
+  constexpr int kOff = F8 ? (kRawDma + 1) / 2 : kPer / 2;
   uint32_t offp[kOff];
 #pragma unroll
   for (int j = 0; j < kOff; ++j) {
     uint32_t v = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int c = 64 * min(wave + 4 * (2 * j + h), R::kDma - 1) + lane;
-      const int r = R::row_of(c);
-      const int x = min(c - R::row_off(r), kChunks - 1);
-      v |= (uint32_t)(r * kRow + 16 * x) << (16 * h);
+      if constexpr (F8) {
+        const int c = min(64 * (2 * j + h) + lane, kRawChunks - 1);
+        const int r = c / 36;  // (rows 8 apart are kWideRowsT chunks apart)
+        v |= (uint32_t)(wide_row_off(r) + 2 * (c - 36 * r) + 1024 * r) << (16 * h);
+      } else {
+        const int c = 64 * min(wave + 4 * (2 * j + h), kWideTileDma - 1) + lane;
+        const int r = wide_row_of(c);
+        const int x = min(c - wide_row_off(r), kWideRowData - 1);
+        v |= (uint32_t)(r * kRow + 16 * x) << (16 * h);
+      }
     }
     offp[j] = v;
   }
-  // Per-lane part of the transposed reads.  bf16: lane 4 e + r of a 16-lane group
-  // addresses token row 4 j2 + e, columns 4 r .. 4 r + 3 of the group's 16.  8 bits: lanes 2
-  // e and 2 e + 1 token row 8 (e / 4) + 4 j2 + e % 4, 8 columns each.
+  // Per-lane part of the transposed reads: lane 4 e + r of a 16-lane group addresses token
+  // row 4 j2 + e, columns 4 r .. 4 r + 3 of the group's 16.
   const uint32_t v_lane = [&] {
-    const int ch = (lane >> 4) & 1;
-    if constexpr (F8) {
-      const int e = (lane & 15) >> 1;
-      return (uint32_t)(16 * R::row_off(8 * (e >> 2) + 4 * j2 + (e & 3)) + 16 * ch + 8 * (lane & 1));
-    } else {
-      const int e = (lane >> 2) & 3, r = lane & 3;
-      return (uint32_t)(16 * R::row_off(4 * j2 + e) + 2 * (16 * ch + 4 * r));
-    }
+    const int ch = (lane >> 4) & 1, e = (lane >> 2) & 3, r = lane & 3;
+    return (uint32_t)(16 * wide_row_off(4 * j2 + e) + 2 * (16 * ch + 4 * r));
   }();
 
   // Pool token index of the first row of each block, 64 at a time (lane l: block pid_base +
   // l); a page id outside the pool is clamped and marks the index with bit 31.
-  const int32_t* pt = p.page_table + (size_t)pl.b * p.max_pages;
+  const int32_t* pt = p.page_table + (size_t)w.pl.b * p.max_pages;
   int pid_base = 0;
   int m_tok = 0;
   uint32_t bad_bits = 0;  // of the blocks requested last: whether their page id was bad
@@ -488,74 +438,37 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   auto fetch_pids = [&]() __attribute__((always_inline)) { set_pids(pt[first_tok() / p.page_size]); };
   int raw_pid = pt[first_tok() / p.page_size];
 
-  // Q^T of this wave's rows, through LDS a 1 KB row an instruction (row slots of 65 chunks).
-  // bf16: k-step u holds columns 16 u + 8 j2 .. + 8; 8 bits: 64 u + 32 j2 .. + 32, hi and lo.
-  constexpr int kSteps = F8 ? 9 : 36;
-  using QReg = typename std::conditional<F8, i32x8, u32x4>::type;
-  QReg qb[F8 ? 18 : 36];
-  float sx = p.scale_log2;  // of the raw scores
+  // Q^T of this wave's rows, through LDS a 1 KB row an instruction (row slots of 65 chunks):
+  // k-step u holds columns 16 u + 8 j2 .. + 8.
+  u32x4 qb[36];
   {
-    const uint16_t* qrow0 = p.q_nope + (g_row0 + 32 * wave) * kRowsC;
-    const uint32_t qst = tile_base0 + (uint32_t)(32 * wave * 65 * 16);
+    const uint16_t* qrow0 = p.q_nope + (w.g_row0 + 32 * wave) * kRowsC;
+    const uint32_t qst = lds0 + (uint32_t)(32 * wave * 65 * 16);
     if (rows > 0)
       for (int h = 0; h < 32; ++h)
         rows_dma16(16 * lane, qrow0 + (size_t)min(h, rows - 1) * kRowsC, qst + (uint32_t)(h * 65 * 16), 0);
     const u32x4* pe =
-        (const u32x4*)(p.q_pe + (g_row0 + min(32 * wave + n32, here - 1)) * kRowsPe);
-    u32x4 pe_q[4];
+        (const u32x4*)(p.q_pe + (w.g_row0 + min(32 * wave + n32, here - 1)) * kRowsPe);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) pe_q[c] = pe[F8 ? 4 * j2 + c : 2 * c + j2];
+    for (int u = 32; u < 36; ++u) qb[u] = pe[2 * (u - 32) + j2];
     asm volatile("s_waitcnt vmcnt(0)" : "+v"(raw_pid) : : "memory");
     set_pids(raw_pid);
-    const u32x4* qs = &s_tile[0][0] + (32 * wave + n32) * 65;
-    if constexpr (F8) {
-      auto chunk = [&](int u, int c) __attribute__((always_inline)) {
-        return u < 8 ? qs[8 * u + 4 * j2 + c] : pe_q[c];
-      };
-      uint32_t top = 0;  // the row's largest magnitude (bf16 bits)
+    const u32x4* qs = s_tile + (32 * wave + n32) * 65 + j2;
 #pragma unroll
-      for (int u = 0; u < 9; ++u)
+    for (int u = 0; u < 32; ++u) qb[u] = qs[2 * u];
+    if (p.q_sign) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const u32x4 w = chunk(u, c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
-        }
-      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-      // 2^e with top <= 448 2^e (and 2^(e - 4) normal); a row with an infinity or a NaN is
-      // NaN whole
-      const int byte = max((int)(((top << 16) + 0x1fffffu) >> 23) - 8, 5);
-      const float unit = __builtin_bit_cast(float, (uint32_t)byte << 23);
-      const float sub = __builtin_bit_cast(float, (uint32_t)(byte - 4) << 23);
-      sx = top >= 0x7f80u ? qnan() : fmaxf(sx * unit, 1.17549435e-38f);
-#pragma unroll
-      for (int u = 0; u < 9; ++u) {
-        int hi[8], lo[8];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const u32x4 w = chunk(u, c) ^ p.q_sign;
-          split_query4(w[0], w[1], unit, sub, hi[2 * c], lo[2 * c]);
-          split_query4(w[2], w[3], unit, sub, hi[2 * c + 1], lo[2 * c + 1]);
-        }
-        qb[2 * u] = i32x8{hi[0], hi[1], hi[2], hi[3], hi[4], hi[5], hi[6], hi[7]};
-        qb[2 * u + 1] = i32x8{lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]};
-        // one k-step's registers at a time
-        hold(qb[2 * u]);
-        hold(qb[2 * u + 1]);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 36; ++u) qb[u] = (u < 32 ? qs[2 * u + j2] : pe_q[u - 32]) ^ p.q_sign;
+      for (int u = 0; u < 36; ++u) qb[u] ^= p.q_sign;
     }
   }
   // the queries in registers, and every wave done with its staged rows, before the loads
 #pragma unroll
-  for (int u = 0; u < (F8 ? 18 : 36); ++u) hold(qb[u]);
+  for (int u = 0; u < 36; ++u) asm volatile("" : : "v"(qb[u]));
   wide_lds_barrier();
 
-  // Block k into tile k % kTiles: this wave's kPer instructions.  Rows past t_end read the
-  // last row's last chunk; a block past the last is the last one again, in a tile that
-  // nothing reads.
+  // Block k's loads, this wave's kPer instructions: bf16 into tile k % 4, 8 bits into raw slot
+  // k % 2.  Rows past t_end read the last row's last chunk; a block past the last is the last
+  // one again, for a tile that nothing reads.
   const char* g0 = (const char*)p.latent;
   struct Dma {
     const char* sb;
@@ -575,92 +488,101 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     const int nt = min(t_end - (t_begin + 32 * kc), 32);
     Dma d;
     d.sb = g0 + (size_t)tok * kRow;
-    d.lim = nt >= 32 ? 0xffffu : (uint32_t)((nt - 1) * kRow + 16 * (kChunks - 1));
-    const int slot = k & (R::kTiles - 1);
-    const uint32_t tb = tile_base0 + (uint32_t)slot * (kAlloc * 16);
-    d.wbase = tb + 1024 * wave;
+    d.lim = nt >= 32 ? 0xffffu : (uint32_t)((nt - 1) * kRow + kRow - 16);
     if constexpr (F8) {
+      d.wbase = raw0 + kRawBytes * (k & 1);
+      d.last = scale0 + 256 * (k & 1);
       d.ss = p.scale + (tok >> p.block_log2);
       d.lim_s = (uint32_t)(nt - 1) >> p.block_log2;
-      d.last = scale_base + 256 * slot;
     } else {
-      d.last = wave == 0 ? tb + 1024 * (R::kDma - 1) : sink_base;
+      const uint32_t tb = lds0 + (uint32_t)(k & 3) * kRowsTileBytes;
+      d.wbase = tb + 1024 * wave;
+      d.last = wave == 0 ? tb + 1024 * (kWideTileDma - 1) : lds0 + R::kRaw;
     }
     // recomputed per block (not hoisted)
     asm volatile("" : "+s"(d.wbase), "+s"(d.last));
     return d;
   };
   auto dma_one = [&](const Dma& d, int i) __attribute__((always_inline)) {
-    asm volatile("" : "+v"(offp[i >> 1]));  // unpacked at each use
-    const uint32_t pr = offp[i >> 1];
-    const uint32_t off = min((i & 1) ? pr >> 16 : pr & 0xffffu, d.lim);
-    if (i < R::kPer - 1) {
-      rows_dma16(off, d.sb, d.wbase, 4 * 1024 * i);
-    } else if constexpr (F8) {
-      if (wave == 3)
-        rows_dma1(min((uint32_t)n32 >> p.block_log2, d.lim_s), d.ss, d.last);
+    if constexpr (F8) {
+      int l = lane;
+      asm volatile("" : "+v"(l));  // (recomputed at each use)
+      if (i < kRawDma)
+        rows_dma16(min((uint32_t)(16 * (kRawChunks * wave + min(64 * i + l, kRawChunks - 1))), d.lim), d.sb,
+                   d.wbase, 1024 * i);
       else
-        rows_dma16(off, d.sb, d.wbase, 4 * 1024 * i);
+        rows_dma1(min((uint32_t)(l & 31) >> p.block_log2, d.lim_s), d.ss, d.last);
     } else {
-      rows_dma16(off, d.sb, d.last, 0);
+      asm volatile("" : "+v"(offp[i >> 1]));  // unpacked at each use
+      const uint32_t pr = offp[i >> 1];
+      const uint32_t off = min((i & 1) ? pr >> 16 : pr & 0xffffu, d.lim);
+      if (i < kPer - 1) rows_dma16(off, d.sb, d.wbase, 4 * 1024 * i);
+      else rows_dma16(off, d.sb, d.last, 0);
     }
   };
   auto issue = [&](int k) __attribute__((always_inline)) {
     const Dma d = issue_begin(k);
 #pragma unroll
-    for (int i = 0; i < R::kPer; ++i) dma_one(d, i);
+    for (int i = 0; i < kPer; ++i) dma_one(d, i);
   };
-
+  // 8 bits: chunk i of this wave's part of block k, as it is in its raw slot (its loads done),
+  // and into the tile
+  struct Raw {
+    u32x4 w;
+    uint32_t s;
+  };
+  auto raw_read = [&](int k, int i) __attribute__((always_inline)) {
+    uint32_t at = raw0 + kRawBytes * (k & 1) + 1024 * i;
+    const uint32_t sc = scale0 + 256 * (k & 1) + 4 * kRawRows * wave;
+    if (i < kRawDma - 1) {
+      at += 16 * lane;
+    } else {
+      at += 16 * min(lane, kRawChunks - 1 - 64 * (kRawDma - 1));
+    }
+    asm volatile("" : "+v"(offp[i >> 1]));  // unpacked at each use
+    const uint32_t r = offp[i >> 1] >> (16 * (i & 1) + 10) & 7u;
+    return Raw{rows_lds_b128(at), rows_lds_b32(sc + 4 * r)};
+  };
+  auto raw_put = [&](const Raw& r, uint32_t tile, int i) __attribute__((always_inline)) {
+    const float sc = __builtin_bit_cast(float, r.s << 23);
+    asm volatile("" : "+v"(offp[i >> 1]));
+    const uint32_t to = tile + 16 * (offp[i >> 1] >> (16 * (i & 1)) & 1023u);
+    rows_lds_put(to, widen8(r.w[0], r.w[1], sc));
+    rows_lds_put(to + 16, widen8(r.w[2], r.w[3], sc));
+  };
+  auto tile_of = [&](int k) __attribute__((always_inline)) {
+    return F8 ? (int)((unsigned)k % 3u) : k & 3;
+  };
+  auto widen_block = [&](int k) __attribute__((always_inline)) {
+    const uint32_t tile = lds0 + (uint32_t)tile_of(k) * kRowsTileBytes + 16 * kWideRowsT * wave;
+#pragma unroll
+    for (int i = 0; i < kRawDma; ++i) raw_put(raw_read(k, i), tile, i);
+  };
   f32x16 acc[16];
   float m_run = neg_inf();  // reference of the lane's row: its largest score in the first block
   float m_max = neg_inf();  // the lane's largest raw score so far
-  float l_run = 0.f;  // bf16: the lane's sum of probabilities as rounded
+  float l_run = 0.f;  // the lane's sum of probabilities as rounded
   float s_run = 0.f;  // and in fp32
 
-  // QK operand u of a tile, and its product
-  using KReg = QReg;
-  const u32x4* arow0 = &s_tile[0][0] + R::row_off(n32) + (F8 ? 2 * j2 : j2);
+  const u32x4* arow0 = s_tile + wide_row_off(n32) + j2;
   auto qk_read = [&](int tile, int u) __attribute__((always_inline)) {
-    if constexpr (F8) {
-      const u32x4 a = arow0[tile * kAlloc + 4 * u], b = arow0[tile * kAlloc + 4 * u + 1];
-      return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
-    } else {
-      return arow0[tile * kAlloc + 2 * u];
-    }
+    return arow0[tile * kTileChunks + 2 * u];
   };
-  // link v of the chain: bf16 k-step v; 8 bits k-step v / 2, hi then lo (2^-4)
-  constexpr int kLinks = F8 ? 18 : 36;
-  int one = 127, sixteenth = 123;
-  auto qk_link = [&](f32x16& sc, const KReg& kr, int tok_scale, int v) __attribute__((always_inline)) {
-    if constexpr (F8) {
-      if (v == 0) qk8_first(sc, kr, qb[0], tok_scale, one);
-      else qk8_next(sc, kr, qb[v], tok_scale, (v & 1) ? sixteenth : one);
-    } else {
-      if (v == 0) qk_first(sc, kr, qb[0]);
-      else qk_next(sc, kr, qb[v]);
-    }
+  auto qk_link = [&](f32x16& sc, const u32x4& kr, int u) __attribute__((always_inline)) {
+    if (u == 0) qk_first(sc, kr, qb[0]);
+    else qk_next(sc, kr, qb[u]);
   };
   auto vbase = [&](int tile) __attribute__((always_inline)) {
     uint32_t vl = v_lane;
     asm volatile("" : "+v"(vl));  // (one register, the rest in the instruction's offset)
-    return tile_base0 + (uint32_t)tile * (kAlloc * 16) + vl;
+    return lds0 + (uint32_t)tile * kRowsTileBytes + vl;
   };
-  // V^T operand of MFMA m (tokens 16 (m / 16) .., columns 32 (m % 16) ..), as read
-  using VReg = typename std::conditional<F8, uint2, u32x4>::type;
+  // V^T operand of MFMA m: tokens 16 (m / 16) .., columns 32 (m % 16) ..
   auto vread = [&](uint32_t vt, int m) __attribute__((always_inline)) {
-    const int sv = m >> 4, ct = m & 15;
-    const uint32_t a = vt + 16 * R::kRowsS * sv + (F8 ? 32 : 64) * ct;
-    if constexpr (F8) {
-      return lds_read_tr8_b64(a);
-    } else {
-      const uint2 lo = lds_read_tr_b64(a);
-      const uint2 hi = lds_read_tr_b64(a + 16 * kWideRowsT);
-      return u32x4{lo.x, lo.y, hi.x, hi.y};
-    }
-  };
-  auto widened = [&](const VReg& v) __attribute__((always_inline)) {
-    if constexpr (F8) return widen8(v);
-    else return v;
+    const uint32_t a = vt + 16 * kWideRowsS * (m >> 4) + 64 * (m & 15);
+    const uint2 lo = lds_read_tr_b64(a);
+    const uint2 hi = lds_read_tr_b64(a + 16 * kWideRowsT);
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
   };
   // the memory clobber keeps the operand reads where the source puts them
   auto pv_mfma = [&](const u32x4& va, const u32x4& pbs, int m) __attribute__((always_inline)) {
@@ -669,6 +591,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     asm volatile("" : "+a"(a));
     asm volatile("" : : : "memory");
   };
+  const float sx = p.scale_log2;
   // The scores of block kb in the log2 domain less the reference (xa: the first 16 tokens',
   // xh: the others').  In the blocks that the tile's first row does not see whole, a score
   // that a row does not see is -inf, and an infinity or a NaN in a token shows in its
@@ -680,7 +603,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     f32x16 v = sc;
     bool odd = false;
     const bool bad_page = (bad_bits >> (kb & 31)) & 1;
-    if (t0 + 32 > lim_lo || bad_page) {
+    if (t0 + 32 > w.lim_lo || bad_page) {
       int l = lane;  // recomputed here rather than kept live
       asm volatile("" : "+v"(l));
       const int lim = lim_lane - t0 - 4 * (l >> 5);
@@ -714,66 +637,33 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     }
     return odd;
   };
-  // The scales of the tokens of dwords 2 g and 2 g + 1 of k-step s of P
-  auto p_scales = [&](int tile, int s, int g) __attribute__((always_inline)) {
-    if constexpr (F8) return *(const u32x4*)&s_scale[tile][16 * s + 8 * g + 4 * j2];
-    else return u32x4{};
-  };
-  // One dword of a k-step's P^T (two exp2)
-  auto soft_p = [&](float (&xs)[8], const u32x4& ts, u32x4& pbs, int dd) __attribute__((always_inline)) {
+  // One dword of a k-step's P^T (two exp2), its probabilities added to the row sum as rounded
+  auto soft_p = [&](float (&xs)[8], u32x4& pbs, int dd) __attribute__((always_inline)) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
     xs[2 * dd] = __builtin_amdgcn_exp2f(xs[2 * dd]);
     xs[2 * dd + 1] = __builtin_amdgcn_exp2f(xs[2 * dd + 1]);
-    if constexpr (F8) {
-      const float s0 = __builtin_bit_cast(float, ts[2 * (dd & 1)] << 23);
-      const float s1 = __builtin_bit_cast(float, ts[2 * (dd & 1) + 1] << 23);
-      pbs[dd] = pack_bf16x2(xs[2 * dd] * s0, xs[2 * dd + 1] * s1);
-    } else {
-      typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-      const uint32_t pk = pack_bf16x2(xs[2 * dd], xs[2 * dd + 1]);
-      pbs[dd] = pk;
-      l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pk),
-                                              __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l_run, false);
-    }
+    const uint32_t pk = pack_bf16x2(xs[2 * dd], xs[2 * dd + 1]);
+    pbs[dd] = pk;
+    l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pk),
+                                            __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l_run, false);
   };
   auto soft_s = [&](const float (&xa)[8], const float (&xh)[8]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) s_run += xa[i] + xh[i];
   };
-  auto token_scale = [&](int tile) __attribute__((always_inline)) {
-    return F8 ? (int)s_scale[F8 ? tile : 0][n32] : 0;
-  };
-  auto scores = [&](int tile, f32x16& sc) __attribute__((always_inline)) {
-    const int ts = token_scale(tile);
-    KReg kr[2];
-    kr[0] = qk_read(tile, 0);
-#pragma unroll
-    for (int v = 0; v < kLinks; ++v) {
-      const int u = F8 ? v >> 1 : v;
-      if ((!F8 || !(v & 1)) && u + 1 < kSteps) kr[(u + 1) & 1] = qk_read(tile, u + 1);
-      qk_link(sc, kr[u & 1], ts, v);
-    }
-    qk_settle(sc);
-  };
-  auto probabilities = [&](int tile, float (&xa)[8], float (&xh)[8], u32x4 (&pb)[2])
-      __attribute__((always_inline)) {
-#pragma unroll
-    for (int dd = 0; dd < 4; ++dd) soft_p(xa, p_scales(tile, 0, dd >> 1), pb[0], dd);
-#pragma unroll
-    for (int dd = 0; dd < 4; ++dd) soft_p(xh, p_scales(tile, 1, dd >> 1), pb[1], dd);
-  };
-  // A block's values' product by itself (its tile is in and synchronised)
+  // The last block's values' product by itself (its tile is in and synchronised)
   auto values = [&](int kk, float (&xa)[8], float (&xh)[8]) __attribute__((always_inline)) {
-    const int tp = kk & (R::kTiles - 1);
-    const uint32_t vt = vbase(tp);
-    VReg va[4];
-    u32x4 pb[2];
+    const uint32_t vt = vbase(tile_of(kk));
+    u32x4 va[4], pb[2];
+#pragma unroll
+    for (int dd = 0; dd < 4; ++dd) soft_p(xa, pb[0], dd);
 #pragma unroll
     for (int m = 0; m < 3; ++m) va[m] = vread(vt, m);
-    probabilities(tp, xa, xh, pb);
 #pragma unroll
     for (int m = 0; m < 32; ++m) {
       if (m + 3 < 32) va[(m + 3) & 3] = vread(vt, m + 3);
-      pv_mfma(widened(va[m & 3]), pb[m >> 4], m);
+      pv_mfma(va[m & 3], pb[m >> 4], m);
+      if (m < 16 && (m & 3) == 1) soft_p(xh, pb[1], m >> 2);
     }
     soft_s(xa, xh);
   };
@@ -782,81 +672,54 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   // at which every wave has its scores of the tile; a row that sees one is NaN by its score
   // (soft_x), whatever it finds in the tile.
   auto clean = [&](int kk) __attribute__((always_inline)) {
-    const int tp = kk & (R::kTiles - 1);
+    u32x4* tile = s_tile + tile_of(kk) * kTileChunks;
 #pragma clang loop unroll(disable)
-    for (int c = lane; c < kAlloc; c += 64) {
-      u32x4 w = s_tile[tp][c];
+    for (int c = lane; c < kTileChunks; c += 64) {
+      u32x4 x = tile[c];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] &= ~(F8 ? nan_bytes(w[e]) : nonfinite_halves(w[e]));
-      s_tile[tp][c] = w;
+      for (int e = 0; e < 4; ++e) x[e] &= ~nonfinite_halves(x[e]);
+      tile[c] = x;
     }
-    if constexpr (F8)
-      if (s_scale[tp][n32] == 255) s_scale[tp][n32] = 0;
     wide_lds_wait();
   };
 
   // Step kk of the ring (ws_mla_wide.h): block kk + 1's scores with block kk's values'
-  // product between their links, block kk + kAhead's loads over them, and the softmax of
+  // product between their links, the loads over them (bf16: block kk + 3's; 8 bits: block kk
+  // + 4's, behind the widening of this wave's part of block kk + 2), and the softmax of
   // block kk + 1 beside the last products.
   auto step = [&](int kk, float (&xa)[8], float (&xh)[8], bool& odd) __attribute__((always_inline)) {
-    const int tp = kk & (R::kTiles - 1), tq = (kk + 1) & (R::kTiles - 1);
-    wide_wait_barrier<(kAhead - 2) * R::kPer>();
+    const int tp = tile_of(kk), tq = tile_of(kk + 1);
+    if constexpr (F8) wide_lds_barrier();
+    else wide_wait_barrier<kPer>();
     if (__builtin_expect(odd, 0)) clean(kk);
-    const Dma d = issue_begin(kk + kAhead);
+    if constexpr (F8) rows_wait<kPer>();  // block kk + 2's loads
+    const Dma d = issue_begin(kk + (F8 ? 4 : 3));
+    const uint32_t to = lds0 + (uint32_t)tile_of(kk + 2) * kRowsTileBytes + 16 * kWideRowsT * wave;
     f32x16 sc;
-    VReg va[4];
-    u32x4 pb[2];
+    u32x4 kr[5], va[4], pb[2];
+    Raw raw[2];
     const uint32_t vt = vbase(tp);
-    const int ts = token_scale(tq);
-    if constexpr (F8) {
-      KReg kr[2];
-      u32x4 sa = p_scales(tp, 0, 0), sb = p_scales(tp, 0, 1);
-      kr[0] = qk_read(tq, 0);
 #pragma unroll
-      for (int m = 0; m < 3; ++m) va[m] = vread(vt, m);
-      int m = 0;
-      auto pv = [&]() __attribute__((always_inline)) {
+    for (int u = 0; u < 4; ++u) kr[u] = qk_read(tq, u);
+#pragma unroll
+    for (int m = 0; m < 3; ++m) va[m] = vread(vt, m);
+#pragma unroll
+    for (int u = 0; u < 36; ++u) {
+      if (u + 4 < 36) kr[(u + 4) % 5] = qk_read(tq, u + 4);
+      qk_link(sc, kr[u % 5], u);
+      if (u < 4) {
+        soft_p(xa, pb[0], u);
+      } else if ((u - 4) % 4 != 3) {
+        const int m = 3 * ((u - 4) / 4) + (u - 4) % 4;
         va[(m + 3) & 3] = vread(vt, m + 3);
-        pv_mfma(widened(va[m & 3]), pb[m >> 4], m);
-        if (m == 0) sa = p_scales(tp, 1, 0);
-        if (m == 6) sb = p_scales(tp, 1, 1);
-        if (m < 16 && (m & 3) == 1) soft_p(xh, m < 8 ? sa : sb, pb[1], m >> 2);
-        ++m;
-      };
-#pragma unroll
-      for (int v = 0; v < 18; ++v) {
-        if (!(v & 1) && v + 2 < 18) kr[((v >> 1) + 1) & 1] = qk_read(tq, (v >> 1) + 1);
-        qk_link(sc, kr[(v >> 1) & 1], ts, v);
-        if (v == 0) {
-          soft_p(xa, sa, pb[0], 0);
-          soft_p(xa, sa, pb[0], 1);
-        } else if (v == 1) {
-          soft_p(xa, sb, pb[0], 2);
-          soft_p(xa, sb, pb[0], 3);
-        } else {
-          pv();
-          if (!(v & 1)) pv();
-        }
-        if (v % 3 == 2 && v < 15) dma_one(d, v / 3);
+        pv_mfma(va[m & 3], pb[m >> 4], m);
+        if (m < 16 && (m & 3) == 1) soft_p(xh, pb[1], m >> 2);
       }
-    } else {
-      KReg kr[5];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) kr[u] = qk_read(tq, u);
-#pragma unroll
-      for (int m = 0; m < 3; ++m) va[m] = vread(vt, m);
-#pragma unroll
-      for (int u = 0; u < 36; ++u) {
-        if (u + 4 < 36) kr[(u + 4) % 5] = qk_read(tq, u + 4);
-        qk_link(sc, kr[u % 5], ts, u);
-        if (u < 4) {
-          soft_p(xa, u32x4{}, pb[0], u);
-        } else if ((u - 4) % 4 != 3) {
-          const int m = 3 * ((u - 4) / 4) + (u - 4) % 4;
-          va[(m + 3) & 3] = vread(vt, m + 3);
-          pv_mfma(va[m & 3], pb[m >> 4], m);
-          if (m < 16 && (m & 3) == 1) soft_p(xh, u32x4{}, pb[1], m >> 2);
-        }
+      if constexpr (F8) {
+        if (u % 5 == 0 && u / 5 < kRawDma) raw[(u / 5) & 1] = raw_read(kk + 2, u / 5);
+        if (u % 5 == 3 && u / 5 < kRawDma) raw_put(raw[(u / 5) & 1], to, u / 5);
+        if (u >= 5 * kRawDma && u < 5 * kRawDma + kPer) dma_one(d, u - 5 * kRawDma);
+      } else {
         if (u % 4 == 2) dma_one(d, u / 4);
       }
     }
@@ -869,7 +732,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
         odd = soft_x(kk + 1, sc, xa, xh, false);
       }
       if (m + 3 < 32) va[(m + 3) & 3] = vread(vt, m + 3);
-      pv_mfma(widened(va[m & 3]), pb[1], m);
+      pv_mfma(va[m & 3], pb[1], m);
       if (m == 24) {
         asm volatile("" : "+v"(s_run));  // not ahead of the MFMA
         soft_s(xa, xh);
@@ -877,6 +740,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
       if (!F8 && m == 27) dma_one(d, 9);
     }
   };
+
   for (int pass = 0;; ++pass) {
 #pragma unroll
     for (int e = 0; e < 16; ++e)
@@ -888,29 +752,58 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
       pid_base = 0;
       fetch_pids();
     }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) issue(k);
-    wide_wait_barrier<(kAhead - 1) * R::kPer>();
+    if constexpr (F8) {
+      issue(0);
+      issue(1);
+      rows_wait<kPer>();
+      widen_block(0);
+      wide_lds_wait();  // the raw slot is read
+      issue(2);
+      rows_wait<kPer>();
+      widen_block(1);
+      wide_lds_wait();
+      issue(3);
+      wide_lds_barrier();
+    } else {
+      issue(0);
+      issue(1);
+      issue(2);
+      wide_wait_barrier<2 * kPer>();
+    }
     if (rows > 0) {
       float xa[8], xh[8];
       bool odd;
       {
         f32x16 sc;
-        scores(0, sc);
+        u32x4 kr[5];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) kr[u] = qk_read(0, u);
+#pragma unroll
+        for (int u = 0; u < 36; ++u) {
+          if (u + 4 < 36) kr[(u + 4) % 5] = qk_read(0, u + 4);
+          qk_link(sc, kr[u % 5], u);
+        }
+        qk_settle(sc);
         odd = soft_x(0, sc, xa, xh, true);
       }
 #pragma clang loop unroll(disable)
-      for (int k = 0; k + 1 < nblk; ++k) {
-        step(k, xa, xh, odd);
-      }
-      wide_lds_barrier();
+      for (int k = 0; k + 1 < nblk; ++k) step(k, xa, xh, odd);
+      wide_lds_barrier();  // every wave has its scores of the last tile
       if (__builtin_expect(odd, 0)) clean(nblk - 1);
       values(nblk - 1, xa, xh);
     } else {  // the ring's waits, barriers and loads alone
 #pragma clang loop unroll(disable)
       for (int k = 0; k + 1 < nblk; ++k) {
-        wide_wait_barrier<(kAhead - 2) * R::kPer>();
-        issue(k + kAhead);
+        if constexpr (F8) {
+          wide_lds_barrier();
+          rows_wait<kPer>();
+          widen_block(k + 2);
+          wide_lds_wait();
+          issue(k + 4);
+        } else {
+          wide_wait_barrier<kPer>();
+          issue(k + 3);
+        }
       }
       wide_lds_barrier();
     }
@@ -935,20 +828,21 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   float lo, hi;
   pair_xor32(s_run, lo, hi);
   const float s_tot = lo + hi;
-  pair_xor32(F8 ? s_run : l_run, lo, hi);
+  pair_xor32(l_run, lo, hi);
   const float l_tot = lo + hi;
   const float inv_l = s_tot == 0.f ? 0.f : 1.f / l_tot;
   const float lse_v = s_tot == 0.f ? neg_inf() : (m_run + __log2f(s_tot)) * kLn2;
   if (j2 == 0 && n32 < rows) {
-    const size_t at = o_row0 + 32 * wave + n32;
-    if (piece) p.part_lse[at] = lse_v;
+    const size_t at = w.o_row0 + 32 * wave + n32;
+    if (w.piece) p.part_lse[at] = lse_v;
     else if (p.lse) p.lse[at] = lse_v;
   }
   // The outputs leave through LDS, 1 KB a store instruction: accumulator ct value i is
   // column 32 ct + 8 (i / 4) + 4 j2 + i % 4.
-  uint32_t* stage = (uint32_t*)&s_tile[0][0] + (size_t)(32 * wave) * 260;
+  uint32_t* stage = (uint32_t*)s_mem + (size_t)(32 * wave) * 260;
   if (rows == 0) return;
-  if (!piece && p.out_bf16) {
+  uint16_t* to16 = w.piece ? p.part_out : p.out_bf16;
+  if (to16) {
 #pragma unroll
     for (int ct = 0; ct < 16; ++ct)
 #pragma unroll
@@ -957,13 +851,12 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
             make_uint2(pack_bf16x2(acc[ct][4 * q] * inv_l, acc[ct][4 * q + 1] * inv_l),
                        pack_bf16x2(acc[ct][4 * q + 2] * inv_l, acc[ct][4 * q + 3] * inv_l));
     wide_lds_wait();
-    rows_store((char*)(p.out_bf16 + (o_row0 + 32 * wave) * kRowsC), kRowsC * 2, stage + 4 * lane,
+    rows_store((char*)(to16 + (w.o_row0 + 32 * wave) * kRowsC), kRowsC * 2, stage + 4 * lane,
                16 * lane, rows);
     wide_lds_wait();
   }
-  float* to = piece ? p.part_out : p.out_f32;
-  if (to) {
-    char* dst = (char*)(to + (o_row0 + 32 * wave) * kRowsC);
+  if (!w.piece && p.out_f32) {
+    char* dst = (char*)(p.out_f32 + (w.o_row0 + 32 * wave) * kRowsC);
 #pragma unroll
     for (int hc = 0; hc < 2; ++hc) {
 #pragma unroll
@@ -982,65 +875,470 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   }
 }
 
-// Combines the pieces of the tiles that were split: two rows a workgroup, one thread per
-// four columns.
-constexpr int kRowsJoin = 2;
+// 8-bit pages under few rows (at most 32 of a sequence, on average): a tile is one wave's 32
+// rows, the four waves take every fourth block of its tokens each, and their sums meet in LDS
+// at the end.  With 16 rows the products are small beside the loads, so what counts is that
+// each wave keeps a block on its way while it works on another, without a barrier: a block
+// takes a wave about 5000 cycles, the HBM 4 x 1900.  The latents are widened where they are
+// read: the scores' operand by its token's scale, the values' operand as it is, with the
+// scale on the token's probability.
+constexpr int kFewTile = 32;
+constexpr int kFewDma = 19;  // 1 KB load instructions of a block, and one for the scales
+constexpr int kFewSlot = 1024 * kFewDma;
+constexpr int kFewWave = 2 * (kFewSlot + 256);
+// Rows of 36 chunks of 16 bytes and one chunk of padding every four rows: the score reads (16
+// rows, one chunk each) meet 16 chunk slots mod 16, and the transposed reads (rows 4 j .. 4 j
+// + 3 and those 8 further on, 32 bytes of each) 8 different pairs of them.
+__host__ __device__ constexpr int few_row_off(int r) { return 36 * r + (r >> 2); }
+static_assert(few_row_off(31) + 36 <= 64 * kFewDma, "a block fills its load instructions");
+static_assert(few_row_off(16 + 8 + 4 + 3) == 580 + 290 + 145 + 108, "row offsets add up");
+static_assert(32 * 260 * 4 <= kFewWave && 32 * 65 * 16 <= 2 * kFewSlot, "outputs and queries are staged there");
+
+// ds_read_b64_tr_b8: in each 16-lane group lanes 2 e and 2 e + 1 address the halves of
+// row e's 16 bytes; result lane i holds byte i of rows 0 .. 7 (measured in bounds).
+__device__ __forceinline__ uint2 lds_read_tr8_b64(uint32_t addr) {
+  typedef int i32x2_t __attribute__((ext_vector_type(2)));
+  typedef __attribute__((address_space(3))) i32x2_t lds_i32x2_t;
+  const i32x2_t v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t*)(uintptr_t)addr);
+  return make_uint2((uint32_t)v[0], (uint32_t)v[1]);
+}
+// qk_first and qk_next with an operand that has just been computed (two wait states).
+__device__ __forceinline__ void qk_first_new(f32x16& c, const u32x4& a, const u32x4& b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b) : "memory");
+}
+__device__ __forceinline__ void qk_next_new(f32x16& c, const u32x4& a, const u32x4& b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b) : "memory");
+}
+// The bytes of four e4m3 values that are NaN, all set.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  const uint32_t hit = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+  return hit * 0xffu;
+}
+
+__global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
+  constexpr int kRow = 576;
+  __shared__ __attribute__((aligned(1024))) char s_mem[4 * kFewWave];
+  __shared__ float2 s_ml[4][32];
+  const int tid = threadIdx.x;
+  const int wave = uniform(tid >> 6);
+  const int lane = tid & 63;
+  const int n32 = lane & 31;
+  const int j2 = lane >> 5;
+  RowsWork w;
+  if (!rows_work(p, w)) return;
+  const int t_begin = w.t_begin, t_end = w.t_end, here = w.here;
+  const int nblk = max((w.nblk - wave + 3) >> 2, 0);  // this wave's
+  const int lim_lane = w.first_pos + min(w.row0 + n32, w.R_all - 1) / p.H + 1;
+  const uint32_t lds0 = (uint32_t)uniform(
+      (int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem + kFewWave * wave));
+  char* const mem = s_mem + kFewWave * wave;
+  // offsets, within a block's rows in HBM, of the chunks this lane loads, two to a register
+  constexpr int kOff = (kFewDma + 1) / 2;
+  uint32_t offp[kOff];
+#pragma unroll
+  for (int j = 0; j < kOff; ++j) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = 64 * min(2 * j + h, kFewDma - 1) + lane;
+      const int g = min(c / 145, 7);
+      const int r = 4 * g + min((c - 145 * g) / 36, 3);
+      v |= (uint32_t)(r * kRow + 16 * min(c - few_row_off(r), 35)) << (16 * h);
+    }
+    offp[j] = v;
+  }
+  const uint32_t v_lane = [&] {
+    const int ch = (lane >> 4) & 1, e = (lane & 15) >> 1;
+    return (uint32_t)(16 * few_row_off(8 * (e >> 2) + 4 * j2 + (e & 3)) + 16 * ch + 8 * (lane & 1));
+  }();
+
+  // Pool token index of the wave's blocks, 64 at a time (ws_mla_wide.h), bit 31: a bad page.
+  const int32_t* pt = p.page_table + (size_t)w.pl.b * p.max_pages;
+  int pid_base = 0, m_tok = 0;
+  auto first_tok = [&]() __attribute__((always_inline)) {
+    return t_begin + 32 * (wave + 4 * min(pid_base + lane, nblk - 1));
+  };
+  auto set_pids = [&](int raw) __attribute__((always_inline)) {
+    const int t0 = first_tok();
+    const int page = t0 / p.page_size;
+    const int pid = clamp_page(raw, p.num_pages);
+    m_tok = (pid * p.page_size + (t0 - page * p.page_size)) | (raw == pid ? 0 : (int)0x80000000u);
+  };
+  uint32_t bad_bits = 0;
+  // Block i's loads into slot i % 2
+  auto issue = [&](int i) __attribute__((always_inline)) {
+    if (i - pid_base >= 64) {
+      pid_base += 64;
+      set_pids(pt[first_tok() / p.page_size]);
+    }
+    const int tok_raw = __builtin_amdgcn_readlane(m_tok, i - pid_base);
+    const uint32_t bit = 1u << (i & 1);
+    bad_bits = tok_raw < 0 ? bad_bits | bit : bad_bits & ~bit;
+    const uint32_t tok = (uint32_t)tok_raw & 0x7fffffffu;
+    const int nt = min(t_end - (t_begin + 32 * (wave + 4 * i)), 32);
+    const char* sb = (const char*)p.latent + (size_t)tok * kRow;
+    const uint32_t lim = nt >= 32 ? 0xffffu : (uint32_t)((nt - 1) * kRow + kRow - 16);
+    const uint32_t base = lds0 + kFewSlot * (i & 1);
+#pragma unroll
+    for (int j = 0; j < kFewDma; ++j) {
+      asm volatile("" : "+v"(offp[j >> 1]));
+      const uint32_t pr = offp[j >> 1];
+      rows_dma16(min((j & 1) ? pr >> 16 : pr & 0xffffu, lim), sb, base, 1024 * j);
+    }
+    rows_dma1(min((uint32_t)n32 >> p.block_log2, (uint32_t)(nt - 1) >> p.block_log2),
+              p.scale + (tok >> p.block_log2), lds0 + 2 * kFewSlot + 256 * (i & 1));
+  };
+
+  // Q^T of the tile's rows: k-steps 2 u and 2 u + 1 hold columns 32 u + 16 j2 .. + 8 and the
+  // eight behind them, as a 16-byte read of the latents delivers them.
+  u32x4 qb[36];
+  if (nblk > 0) {
+    int raw_pid = pt[first_tok() / p.page_size];
+    const uint16_t* qrow0 = p.q_nope + w.g_row0 * kRowsC;
+    for (int h = 0; h < 32; ++h)
+      rows_dma16(16 * lane, qrow0 + (size_t)min(h, here - 1) * kRowsC, lds0 + (uint32_t)(h * 65 * 16), 0);
+    const u32x4* pe = (const u32x4*)(p.q_pe + (w.g_row0 + min(n32, here - 1)) * kRowsPe);
+#pragma unroll
+    for (int u = 32; u < 36; ++u) qb[u] = pe[4 * ((u - 32) >> 1) + 2 * j2 + (u & 1)];
+    asm volatile("s_waitcnt vmcnt(0)" : "+v"(raw_pid) : : "memory");
+    set_pids(raw_pid);
+    const u32x4* qs = (const u32x4*)mem + n32 * 65;
+#pragma unroll
+    for (int u = 0; u < 32; ++u) qb[u] = qs[4 * (u >> 1) + 2 * j2 + (u & 1)];
+    if (p.q_sign) {
+#pragma unroll
+      for (int u = 0; u < 36; ++u) qb[u] ^= p.q_sign;
+    }
+#pragma unroll
+    for (int u = 0; u < 36; ++u) asm volatile("" : : "v"(qb[u]));
+    wide_lds_wait();  // the staged rows are read
+  }
+
+  f32x16 acc[16];
+  float m_run = neg_inf(), m_max = neg_inf(), s_run = 0.f;
+  const float sx = p.scale_log2;
+  auto pv_mfma = [&](const u32x4& va, const u32x4& pbs, int m) __attribute__((always_inline)) {
+    f32x16& a = acc[m & 15];
+    a = mfma32x32x16(va, pbs, a);
+    asm volatile("" : "+a"(a));
+    asm volatile("" : : : "memory");
+  };
+  auto block = [&](int i) __attribute__((always_inline)) {
+    const uint32_t tile = lds0 + kFewSlot * (i & 1);
+    const uint32_t scales = lds0 + 2 * kFewSlot + 256 * (i & 1);
+    const int t0 = t_begin + 32 * (wave + 4 * i);
+    f32x16 v;
+    {
+      const float ts = __builtin_bit_cast(float, rows_lds_b32(scales + 4 * n32) << 23);
+      uint32_t row = 16 * (uint32_t)few_row_off(n32) + 16 * j2;
+      asm volatile("" : "+v"(row));
+      u32x4 kr[4];
+#pragma unroll
+      for (int u = 0; u < 3; ++u) kr[u] = rows_lds_b128(tile + row + 32 * u);
+#pragma unroll
+      for (int u = 0; u < 18; ++u) {
+        if (u + 3 < 18) kr[(u + 3) & 3] = rows_lds_b128(tile + row + 32 * (u + 3));
+        const u32x4& k = kr[u & 3];
+        if (u == 0) qk_first_new(v, widen8(k[0], k[1], ts), qb[0]);
+        else qk_next_new(v, widen8(k[0], k[1], ts), qb[2 * u]);
+        qk_next_new(v, widen8(k[2], k[3], ts), qb[2 * u + 1]);
+      }
+      qk_settle(v);
+    }
+    // (mla_rows_kernel's soft_x)
+    bool odd = false;
+    const bool bad_page = (bad_bits >> (i & 1)) & 1;
+    const int lim = lim_lane - t0 - 4 * j2;
+    if (t0 + 32 > w.lim_lo || bad_page) {
+      bool hidden = false;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const bool seen = 8 * (e >> 2) + (e & 3) < lim;
+        const bool finite = __builtin_fabsf(v[e]) < __builtin_inff();
+        hidden |= !seen && !finite;
+        const float x = bad_page || !finite ? qnan() : v[e];
+        v[e] = seen ? x : neg_inf();
+      }
+      odd = __builtin_amdgcn_ballot_w64(hidden) != 0;
+    }
+    float r = max3(v[0], v[1], v[2]);
+#pragma unroll
+    for (int e = 3; e < 15; e += 2) r = max3(r, v[e], v[e + 1]);
+    m_max = max3(r, v[15], m_max);
+    if (i == 0) {
+      float lo, hi;
+      pair_xor32(m_max * sx, lo, hi);
+      m_run = m_run == neg_inf() ? fmaxf(lo, hi) : m_run;
+      m_run = m_run == neg_inf() ? 0.f : m_run;
+    }
+    if (__builtin_expect(odd, 0)) {  // (mla_rows_kernel's clean: the slot is the wave's own)
+#pragma clang loop unroll(disable)
+      for (int c = lane; c < kFewSlot / 16; c += 64) {
+        u32x4 x = rows_lds_b128(tile + 16 * c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] &= ~nan_bytes(x[e]);
+        rows_lds_put(tile + 16 * c, x);
+      }
+      uint32_t* sp = (uint32_t*)(mem + 2 * kFewSlot + 256 * (i & 1)) + lane;
+      if (*sp == 255) *sp = 0;
+      wide_lds_wait();
+    }
+    u32x4 pb[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const u32x4 ts = rows_lds_b128(scales + 4 * (16 * s + 8 * g + 4 * j2));
+        float e[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          e[c] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[8 * s + 4 * g + c], sx, -m_run));
+          s_run += e[c];
+          e[c] *= __builtin_bit_cast(float, ts[c] << 23);
+        }
+        pb[s][2 * g] = pack_bf16x2(e[0], e[1]);
+        pb[s][2 * g + 1] = pack_bf16x2(e[2], e[3]);
+      }
+    uint32_t vt = v_lane;
+    asm volatile("" : "+v"(vt));
+    vt += tile;
+    auto vread = [&](int m) __attribute__((always_inline)) {
+      return lds_read_tr8_b64(vt + 16 * 580 * (m >> 4) + 32 * (m & 15));
+    };
+    uint2 va[4];
+#pragma unroll
+    for (int m = 0; m < 3; ++m) va[m] = vread(m);
+    u32x4 cur = widen8(va[0].x, va[0].y, 1.f);
+#pragma unroll
+    for (int m = 0; m < 32; ++m) {
+      if (m + 3 < 32) va[(m + 3) & 3] = vread(m + 3);
+      const u32x4 now = cur;
+      if (m + 1 < 32) cur = widen8(va[(m + 1) & 3].x, va[(m + 1) & 3].y, 1.f);
+      pv_mfma(now, pb[m >> 4], m);
+    }
+  };
+
+  for (int pass = 0;; ++pass) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[e][i] = 0.f;
+    s_run = 0.f;
+    if (nblk == 0) break;
+    if (pid_base != 0) {
+      pid_base = 0;
+      set_pids(pt[first_tok() / p.page_size]);
+    }
+    issue(0);
+    if (nblk > 1) issue(1);
+#pragma clang loop unroll(disable)
+    for (int i = 0; i < nblk; ++i) {
+      if (i + 1 < nblk) rows_wait<kFewDma + 1>();
+      else rows_wait<0>();
+      block(i);
+      wide_lds_wait();  // the slot is read
+      if (i + 2 < nblk) issue(i + 2);
+    }
+    float lo, hi;
+    pair_xor32(m_max, lo, hi);
+    m_max = fmaxf(lo, hi);
+    const float top = m_max * sx;
+    if (pass > 0 || __builtin_amdgcn_ballot_w64(top > m_run + kWideHeadroomLog2) == 0) break;
+    m_run = top == neg_inf() ? 0.f : top;
+  }
+
+  // The waves' sums at the largest of their references
+  float lo, hi;
+  pair_xor32(s_run, lo, hi);
+  const float l_w = lo + hi;
+  if (j2 == 0) s_ml[wave][n32] = make_float2(l_w == 0.f ? neg_inf() : m_run, l_w);
+  __syncthreads();
+  float M = neg_inf(), total = 0.f;
+#pragma unroll
+  for (int o = 0; o < 4; ++o) M = fmaxf(M, s_ml[o][n32].x);
+#pragma unroll
+  for (int o = 0; o < 4; ++o) {
+    const float2 ml = s_ml[o][n32];
+    total += ml.x == neg_inf() ? 0.f : __builtin_amdgcn_exp2f(ml.x - M) * ml.y;
+  }
+  const float f = l_w == 0.f ? 0.f : __builtin_amdgcn_exp2f(m_run - M) / total;
+  if (wave == 0 && j2 == 0 && n32 < here) {
+    const float lse_v = total == 0.f ? neg_inf() : (M + __log2f(total)) * kLn2;
+    const size_t at = w.o_row0 + n32;
+    if (w.piece) p.part_lse[at] = lse_v;
+    else if (p.lse) p.lse[at] = lse_v;
+  }
+  uint16_t* to16 = w.piece ? p.part_out : p.out_bf16;
+  float* to32 = w.piece ? nullptr : p.out_f32;
+  float* stage = (float*)mem;
+#pragma unroll
+  for (int hc = 0; hc < 2; ++hc) {  // 256 columns at a time
+    if (hc > 0) __syncthreads();
+#pragma unroll
+    for (int c8 = 0; c8 < 8; ++c8)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int ct = 8 * hc + c8;
+        *(float4*)(stage + n32 * 260 + 32 * c8 + 8 * q + 4 * j2) =
+            make_float4(acc[ct][4 * q] * f, acc[ct][4 * q + 1] * f, acc[ct][4 * q + 2] * f,
+                        acc[ct][4 * q + 3] * f);
+      }
+    __syncthreads();
+    for (int row = wave; row < here; row += 4) {
+      float4 x = *(const float4*)((const float*)s_mem + row * 260 + 4 * lane);
+#pragma unroll
+      for (int o = 1; o < 4; ++o) {
+        const float4 y = *(const float4*)((const float*)(s_mem + kFewWave * o) + row * 260 + 4 * lane);
+        x.x += y.x;
+        x.y += y.y;
+        x.z += y.z;
+        x.w += y.w;
+      }
+      const size_t at = (w.o_row0 + row) * (kRowsC / 4) + 64 * hc + lane;
+      if (to16) ((uint2*)to16)[at] = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+      if (to32) ((float4*)to32)[at] = x;
+    }
+  }
+}
+
+// Combines the pieces of the tiles that were split, four rows a workgroup: a wave a row, or,
+// from kJoinShared pieces on, the four waves a row after the other, each a quarter of the
+// pieces.  A lane has eight columns.
+constexpr int kJoinRows = 4;
+constexpr int kJoinShared = 16;
+struct JoinAcc {
+  float m, sum;
+  float a[8];
+};
+__device__ __forceinline__ void join_pieces(JoinAcc& x, const uint16_t* out, const float* lse,
+                                            int rows, int first, int step, int n) {
+  const int lane = threadIdx.x & 63;
+  constexpr int U = 8;  // pieces under way
+  for (int s = first; s < n; s += U * step) {
+    float l[U];
+    u32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) l[u] = lse[(size_t)min(s + u * step, n - 1) * rows];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      v[u] = ((const u32x4*)(out + (size_t)min(s + u * step, n - 1) * rows * kRowsC))[lane];
+    float m = x.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s + u * step >= n) l[u] = neg_inf();
+      m = fmaxf(m, l[u]);
+    }
+    const float f = acc_factor(x.m, m);
+    x.m = m;
+    x.sum *= f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.a[i] *= f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s + u * step >= n) continue;
+      const float wt = piece_weight(l[u], m);
+      x.sum += wt;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x.a[2 * i] += wt * __builtin_bit_cast(float, v[u][i] << 16);
+        x.a[2 * i + 1] += wt * __builtin_bit_cast(float, v[u][i] & 0xffff0000u);
+      }
+    }
+  }
+}
 __global__ __launch_bounds__(256) void mla_rows_join_kernel(const RowsParams p) {
+  __shared__ JoinAcc s_acc[3][64];
   const RowsPlace tl = rows_place<true>(p, blockIdx.x);
   if (tl.b < 0 || tl.splits == 1 || tl.piece < 0 || tl.piece + tl.splits > p.pieces) return;
-  const int c = threadIdx.x & 127;
-  const int tr = blockIdx.y * kRowsJoin + (threadIdx.x >> 7);  // row of the tile
-  const int r = tl.tile * kRowsTile + tr;
-  if (r >= tl.n * p.H || tr >= p.piece_rows) return;
-  const size_t slot = (size_t)tl.piece * p.piece_rows + tr;
-  const PieceAcc x = piece_stream<float4>((const char*)(p.part_out + slot * kRowsC + 4 * c),
-                                          (size_t)p.piece_rows * kRowsC * 4, p.part_lse + slot,
-                                          p.piece_rows, 0, 1, tl.splits);
-  const float inv = x.sum == 0.f ? 0.f : 1.f / x.sum;
-  const float4 o = make_float4(x.a.x * inv, x.a.y * inv, x.a.z * inv, x.a.w * inv);
-  const size_t at = (size_t)tl.c0 * p.H + r;
-  if (p.out_f32) ((float4*)p.out_f32)[at * (kRowsC / 4) + c] = o;
-  if (p.out_bf16)
-    ((uint2*)p.out_bf16)[at * (kRowsC / 4) + c] =
-        make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
-  if (p.lse && c == 0) p.lse[at] = x.sum == 0.f ? neg_inf() : x.m + __logf(x.sum);
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int here = min(p.tile, tl.n * p.H - tl.tile * p.tile);
+  const bool shared = tl.splits >= kJoinShared;
+  for (int i = 0; i < (shared ? kJoinRows : 1); ++i) {
+    const int tr = blockIdx.y * kJoinRows + (shared ? i : wave);  // row of the tile
+    JoinAcc x;
+    x.m = neg_inf();
+    x.sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) x.a[c] = 0.f;
+    const size_t slot = (size_t)tl.piece * p.piece_rows + tr;
+    if (tr < here)
+      join_pieces(x, p.part_out + slot * kRowsC, p.part_lse + slot, p.piece_rows, shared ? wave : 0,
+                  shared ? 4 : 1, tl.splits);
+    if (shared) {
+      if (i > 0) __syncthreads();
+      if (wave > 0) s_acc[wave - 1][lane] = x;
+      __syncthreads();
+      if (wave > 0) continue;
+#pragma unroll
+      for (int o = 0; o < 3; ++o) {
+        const JoinAcc y = s_acc[o][lane];
+        const float m = fmaxf(x.m, y.m);
+        const float fx = acc_factor(x.m, m), fy = acc_factor(y.m, m);
+        x.m = m;
+        x.sum = x.sum * fx + y.sum * fy;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) x.a[c] = x.a[c] * fx + y.a[c] * fy;
+      }
+    }
+    if (tr >= here) continue;
+    const float inv = x.sum == 0.f ? 0.f : 1.f / x.sum;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) x.a[c] *= inv;
+    const size_t at = (size_t)tl.c0 * p.H + tl.tile * p.tile + tr;
+    if (p.out_f32) {
+      float4* dst = (float4*)(p.out_f32 + at * kRowsC) + 2 * lane;
+      dst[0] = make_float4(x.a[0], x.a[1], x.a[2], x.a[3]);
+      dst[1] = make_float4(x.a[4], x.a[5], x.a[6], x.a[7]);
+    }
+    if (p.out_bf16) {
+      u32x4 o;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = pack_bf16x2(x.a[2 * c], x.a[2 * c + 1]);
+      ((u32x4*)(p.out_bf16 + at * kRowsC))[lane] = o;
+    }
+    if (p.lse && lane == 0) p.lse[at] = x.sum == 0.f ? neg_inf() : x.m + __logf(x.sum);
+  }
 }
 
 // ---------------------------------------------------------------------------
 
 struct RowsPlan {
-  long long tiles, grid, pieces;
-  int fill, piece_rows;
-  bool fit;
+  long long tiles, grid, pieces, joins;
+  int fill, piece_rows, tile;
+  bool fit, few;
 };
 // decode: one token a sequence
-static RowsPlan rows_plan(int N, int B, int H, bool decode, int max_len, int n_splits) {
+static RowsPlan rows_plan(int N, int B, int H, bool decode, bool fp8, int max_len, int n_splits) {
   RowsPlan r;
-  const long long each = (H + kRowsTile - 1) / kRowsTile;
-  r.tiles = decode ? B * each : std::min((long long)N * H / kRowsTile + B, (long long)N * each);
+  r.few = fp8 && (long long)N * H <= (long long)kFewTile * B;
+  r.tile = r.few ? kFewTile : kRowsTile;
+  const long long each = (H + r.tile - 1) / r.tile;
+  r.tiles = decode ? B * each : std::min((long long)N * H / r.tile + B, (long long)N * each);
   r.fill = choose_workgroups(0, 1, 1LL << 30, 1);
   r.fit = r.tiles < r.fill && B <= 256;
-  r.piece_rows = (int)std::min<long long>(kRowsTile, decode ? H : (long long)N * H);
+  r.piece_rows = (int)std::min<long long>(r.tile, decode ? H : (long long)N * H);
   r.grid = r.tiles;
-  r.pieces = 0;
+  r.pieces = r.joins = 0;
   if (n_splits > 1) {
     r.pieces = r.grid = r.tiles * n_splits;
+    r.joins = r.tiles;
   } else if (n_splits == 0 && max_len > 32 * kRowsMinShare) {
     // Only a tile of more than M blocks is split.  All items fit `fill`, or M is the blocks
     // over `fill`, and then split tiles are fewer than `fill` and leave twice as many pieces
     // at the most.
     r.pieces = r.fit ? r.fill : 2LL * r.fill + 64;
     r.grid = r.fit ? r.fill : r.tiles + r.pieces;
+    r.joins = std::min<long long>(r.tiles, r.fill);
   }
   return r;
 }
 static size_t rows_bytes(const RowsPlan& pl) {
   if (pl.pieces == 0) return 0;
   const size_t rows = (size_t)pl.pieces * pl.piece_rows;
-  return align256(rows * 4) + rows * kRowsC * 4;
+  return align256(rows * 4) + rows * kRowsC * 2;
 }
 
-static int rows_sizes(const char* name, int N, int B, int H, bool decode, int max_len,
+static int rows_sizes(const char* name, int N, int B, int H, bool decode, bool fp8, int max_len,
                       int n_splits) {
   if (N < 0 || B < 0 || B > kMaxSeqs || H <= 0 || H > 1024 || max_len < 0 || n_splits < 0 ||
       n_splits > kRowsMaxSplits)
@@ -1050,7 +1348,7 @@ static int rows_sizes(const char* name, int N, int B, int H, bool decode, int ma
                      name, N, B, H, max_len, n_splits, kMaxSeqs, kRowsMaxSplits);
   if ((long long)N * H + 256LL * B >= (1LL << 31) || max_len > (1 << 30))
     return set_error(WS_EINVAL, "%s: %d tokens of %d heads exceed the row index range", name, N, H);
-  if (rows_plan(N, B, H, decode, max_len, n_splits).grid * 256 >= (1LL << 32))
+  if (rows_plan(N, B, H, decode, fp8, max_len, n_splits).grid * 256 >= (1LL << 32))
     return set_error(WS_EINVAL, "%s: %d tokens of %d heads exceed the launch grid", name, N, H);
   return WS_OK;
 }
@@ -1066,7 +1364,7 @@ static int rows_run(const char* name, const uint16_t* q_nope, const uint16_t* q_
   if (!q_nope || !q_pe || !latent_pages || !page_table || !kv_len || (!out_bf16 && !out_f32))
     return set_error(WS_EINVAL, "%s: null pointer", name);
   const bool decode = !cu_new;
-  if (int rc = rows_sizes(name, N, B, H, decode, max_len, n_splits)) return rc;
+  if (int rc = rows_sizes(name, N, B, H, decode, latent_scale != nullptr, max_len, n_splits)) return rc;
   if (page_size <= 0 || page_size % 32 || max_pages <= 0 || num_pages <= 0 ||
       (long long)max_len > (long long)page_size * max_pages)
     return set_error(WS_EINVAL,
@@ -1084,7 +1382,7 @@ static int rows_run(const char* name, const uint16_t* q_nope, const uint16_t* q_
     return set_error(WS_EINVAL, "%s: buffers must be 16-byte aligned", name);
   if (!(scale - scale == 0.f)) return set_error(WS_EINVAL, "%s: scale must be finite", name);
   if (N == 0 || B == 0) return WS_OK;
-  const RowsPlan pl = rows_plan(N, B, H, decode, max_len, n_splits);
+  const RowsPlan pl = rows_plan(N, B, H, decode, latent_scale != nullptr, max_len, n_splits);
   const size_t need = rows_bytes(pl);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(WS_EWORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
@@ -1102,7 +1400,7 @@ static int rows_run(const char* name, const uint16_t* q_nope, const uint16_t* q_
   p.out_f32 = out_f32;
   p.lse = lse;
   p.part_lse = (float*)workspace;
-  p.part_out = (float*)((char*)workspace + align256((size_t)pl.pieces * pl.piece_rows * 4));
+  p.part_out = (uint16_t*)((char*)workspace + align256((size_t)pl.pieces * pl.piece_rows * 4));
   p.N = N;
   p.B = B;
   p.H = H;
@@ -1117,28 +1415,31 @@ static int rows_run(const char* name, const uint16_t* q_nope, const uint16_t* q_
   p.fit = pl.fit;
   p.pieces = (int)pl.pieces;
   p.piece_rows = pl.piece_rows;
+  p.tile = pl.tile;
   // the smallest normal float for 0: every finite score then rounds to the same
   // probability, and masked tokens stay -inf
   p.scale_log2 = std::max((scale < 0.f ? -scale : scale) * kLog2e, 1.17549435e-38f);
   p.q_sign = scale < 0.f ? 0x80008000u : 0u;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)pl.grid), block(256);
-  if (latent_scale)
+  if (pl.few)
+    hipLaunchKernelGGL(mla_few_kernel, grid, block, 0, s, p);
+  else if (latent_scale)
     hipLaunchKernelGGL(mla_rows_kernel<true>, grid, block, 0, s, p);
   else
     hipLaunchKernelGGL(mla_rows_kernel<false>, grid, block, 0, s, p);
   int rc = check_launch(name);
   if (rc != WS_OK || pl.pieces == 0) return rc;
   hipLaunchKernelGGL(mla_rows_join_kernel,
-                     dim3((unsigned)pl.tiles, (pl.piece_rows + kRowsJoin - 1) / kRowsJoin), block, 0,
+                     dim3((unsigned)pl.joins, (pl.piece_rows + kJoinRows - 1) / kJoinRows), block, 0,
                      s, p);
   return check_launch(name);
 }
 
-static int rows_plan_out(const char* name, int N, int B, int H, bool decode, int max_len,
+static int rows_plan_out(const char* name, int N, int B, int H, bool decode, bool fp8, int max_len,
                          int n_splits, int* pieces_out, size_t* bytes_out) {
-  if (int rc = rows_sizes(name, N, B, H, decode, max_len, n_splits)) return rc;
-  const RowsPlan pl = rows_plan(N, B, H, decode, max_len, n_splits);
+  if (int rc = rows_sizes(name, N, B, H, decode, fp8, max_len, n_splits)) return rc;
+  const RowsPlan pl = rows_plan(N, B, H, decode, fp8, max_len, n_splits);
   if (pieces_out) *pieces_out = (int)pl.pieces;
   if (bytes_out) *bytes_out = rows_bytes(pl);
   return WS_OK;
@@ -1148,9 +1449,9 @@ static int rows_plan_out(const char* name, int N, int B, int H, bool decode, int
 
 using namespace ws;
 
-extern "C" int ws_mla_prompt_plan(int N, int B, int H, int max_len, int n_splits, int* pieces_out,
-                                  size_t* workspace_bytes_out) {
-  return rows_plan_out("ws_mla_prompt_plan", N, B, H, false, max_len, n_splits, pieces_out,
+extern "C" int ws_mla_prompt_plan(int N, int B, int H, int fp8, int max_len, int n_splits,
+                                  int* pieces_out, size_t* workspace_bytes_out) {
+  return rows_plan_out("ws_mla_prompt_plan", N, B, H, false, fp8 != 0, max_len, n_splits, pieces_out,
                        workspace_bytes_out);
 }
 
@@ -1169,7 +1470,7 @@ extern "C" int ws_mla_prompt(const uint16_t* q_nope, const uint16_t* q_pe, const
 
 extern "C" int ws_mla8_decode_plan(int B, int H, int max_len, int n_splits, int* pieces_out,
                                    size_t* workspace_bytes_out) {
-  return rows_plan_out("ws_mla8_decode_plan", B, B, H, true, max_len, n_splits, pieces_out,
+  return rows_plan_out("ws_mla8_decode_plan", B, B, H, true, true, max_len, n_splits, pieces_out,
                        workspace_bytes_out);
 }
 

@@ -206,7 +206,7 @@ def lib() -> ctypes.CDLL:
             fn.restype = i32
             fn.argtypes = [vp] * 6 + [i32] * 8 + [f32, vp, vp, vp, sz, vp]
         L.ws_mla_prompt_plan.restype = i32
-        L.ws_mla_prompt_plan.argtypes = [i32] * 5 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
+        L.ws_mla_prompt_plan.argtypes = [i32] * 6 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
         L.ws_mla_prompt.restype = i32
         L.ws_mla_prompt.argtypes = [vp] * 7 + [i32] * 9 + [f32, vp, vp, vp, vp, sz, vp]
         _lib = L
@@ -1586,9 +1586,9 @@ def mla8_plan(batch: int, H: int, max_len: int, n_splits: int = 0):
     return _mla_rows_plan("ws_mla8_decode_plan", batch, H, max_len, n_splits)
 
 
-def mla_prompt_plan(n_tokens: int, batch: int, H: int, max_len: int, n_splits: int = 0):
+def mla_prompt_plan(n_tokens: int, batch: int, H: int, max_len: int, n_splits: int = 0, fp8: bool = False):
     """(pieces, workspace_bytes) of an MLA prompt call."""
-    return _mla_rows_plan("ws_mla_prompt_plan", n_tokens, batch, H, max_len, n_splits)
+    return _mla_rows_plan("ws_mla_prompt_plan", n_tokens, batch, H, int(fp8), max_len, n_splits)
 
 
 def _latent_queries(q_nope, q_pe, page_table, dev):
@@ -1678,7 +1678,7 @@ def mla_prompt(q_nope, q_pe, latent_pages, page_table, kv_len, cu_new, scale, ma
     out, lse = _latent_out(out, lse, N, H, dtype, dev, want_lse)
     if N == 0 or B == 0:
         return out, lse
-    _, wsb = mla_prompt_plan(N, B, H, int(max_len), int(n_splits))
+    _, wsb = mla_prompt_plan(N, B, H, int(max_len), int(n_splits), latent_scale is not None)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
     o16, o32 = (out, None) if dtype == torch.bfloat16 else (None, out)
     _run("ws_mla_prompt", dev, _ptr(q_nope), _ptr(q_pe), _ptr(latent_pages), _ptr(latent_scale),

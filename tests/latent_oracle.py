@@ -2,11 +2,9 @@
 attention over latent pages) on the CPU, one sequence or token at a time.
 
 Bounds, beside request_oracle's.  The RMS norm is fp32 work: a sum of 512 squares (9 adds
-a lane, 6 across), a root, a division and two products, under 2^-18 of the value.  8-bit
-pages take the query as two e4m3 values: exact for a column within 2^-14 of the row's
-largest, else off by at most half the smallest step of the second one, 2^-10 of its unit,
-which is 2^-4 of the first one's, itself at most 2 / 448 of the row's largest: under 2^-21 of
-the row's largest, times the token's column.
+a lane, 6 across), a root, a division and two products, under 2^-18 of the value.  Where
+several workgroups share a row's tokens, each leaves its share's output rounded to bf16, off
+by 2^-8 of it, so by 2^-8 of the share's part of sum_t w_t |v_t|: `pieces`.
 """
 from __future__ import annotations
 
@@ -80,7 +78,7 @@ def pools(lens, page, bits, block, seed, sigma=1.0):
     return table, P, (pool.view(R.E4M3), scale.view(R.E8M0))
 
 
-def attend(q, rows, visible, scale, eight):
+def attend(q, rows, visible, scale, pieces):
     """q [n, H, 576] fp64, rows [T, 576] fp64, visible [n] tokens each query sees (a prefix)
     -> (out [n, H, 512], lse [n, H], bound of out, bound of lse), without reading what a query
     does not see."""
@@ -96,16 +94,14 @@ def attend(q, rows, visible, scale, eight):
         z = torch.logsumexp(s, -1)
         w = torch.exp(s - z[:, None])
         size = (q[i].abs() @ k.abs().T).amax(-1) * (W + 8) * 2.0 ** -24
-        if eight:
-            size = size + q[i].abs().amax(-1) * float(k.abs().sum(-1).max()) * 2.0 ** -21
         delta = size * abs(scale)
         out[i], lse[i] = w @ k[:, :C], z
-        tol_o[i] = (2.0 ** -8 + 2.0 ** -12 + 2 * delta)[:, None] * (w @ k[:, :C].abs())
+        tol_o[i] = ((1 + pieces) * 2.0 ** -8 + 2.0 ** -12 + 2 * delta)[:, None] * (w @ k[:, :C].abs())
         tol_l[i] = delta + 2.0 ** -18 * (1 + z.abs())
     return out, lse, tol_o, tol_l
 
 
-def attention(qn, qp, cpu, table, lens, new, page, block, scale, c0=0):
+def attention(qn, qp, cpu, table, lens, new, page, block, scale, c0=0, pieces=True):
     """attend() for every sequence's new tokens (new None: one row a sequence, which sees
     lens[b] tokens)."""
     pool, sc = cpu
@@ -118,7 +114,7 @@ def attention(qn, qp, cpu, table, lens, new, page, block, scale, c0=0):
         n = 1 if new is None else new[b]
         rows = rows_of(pool, sc, table[b], L, page, block)
         vis = [L] if new is None else [max(0, L - n + i + 1) for i in range(n)]
-        for r, x in zip(res, attend(q[at:at + n], rows, vis, scale, sc is not None)):
+        for r, x in zip(res, attend(q[at:at + n], rows, vis, scale, pieces)):
             r[at:at + n] = x
         at += n
     return res

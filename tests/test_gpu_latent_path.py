@@ -282,7 +282,7 @@ SCALE = 192 ** -0.5
 def test_decode8(H, page, block, lens, splits):
     table, P, cpu = L.pools(lens, page, 8, block, H + len(lens))
     qn, qp = queries(len(lens), H, 9)
-    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, None, page, block, SCALE)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, None, page, block, SCALE, pieces=splits != 1)
     args = (qn.to(DEV), qp.to(DEV), *dev(cpu), ints(table), ints(lens), SCALE, max(lens), splits)
     out, lse = ops.mla8_decode_partial(*args)
     R.check(out, want_o, tol_o, "out")
@@ -367,7 +367,7 @@ def test_prompt(bits, block, H, page, lens, new, splits):
     """(30 queries of a 10-token partition: the first 20 see nothing.)"""
     table, P, cpu = L.pools(lens, page, bits, block, H + len(lens))
     qn, qp = queries(sum(new), H, 9)
-    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, new, page, block, SCALE)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, new, page, block, SCALE, pieces=splits != 1)
     out, lse = prompt_on(qn, qp, cpu, table, lens, new, SCALE, n_splits=splits)
     R.check(out, want_o, tol_o, "out")
     R.check(lse, want_l, tol_l, "lse")
@@ -413,7 +413,7 @@ def test_prompt_nonfinite_tokens(bits, n, H, splits, column):
         pool.view(torch.uint8)[pid, off, column] = 0x7f
     qn, qp = queries(n, H, 3)
     out, lse = prompt_on(qn, qp, (pool, sc), table, [T], [n], 0.125, n_splits=splits)
-    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, (pool, sc), table, [T], [n], page, 1, 0.125)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, (pool, sc), table, [T], [n], page, 1, 0.125, pieces=splits != 1)
     clean = at - (T - n)  # rows before it
     assert clean > 0
     R.check(out[:clean], want_o[:clean], tol_o[:clean], "rows that do not see it")
@@ -462,7 +462,7 @@ def test_prompt_large_scores(bits, H, T, n):
     page = 32
     table, P, cpu = L.pools([T], page, bits, 1, 12, sigma=2.0)
     qn, qp = queries(n, H, 1, 4.0)
-    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, [T], [n], page, 1, 1.0)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, [T], [n], page, 1, 1.0, pieces=False)
     out, lse = prompt_on(qn, qp, cpu, table, [T], [n], 1.0, n_splits=1)
     R.check(out, want_o, tol_o, "out")
     R.check(lse, want_l, tol_l, "lse")
@@ -498,7 +498,7 @@ def test_windows_of_page_ids(bits, T, n, H):
     page, lens, new = 32, [T, 50], [n, 1]
     table, P, cpu = L.pools(lens, page, bits, 1, T + n)
     qn, qp = queries(n + 1, H, 2)
-    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, new, page, 1, SCALE)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, new, page, 1, SCALE, pieces=False)
     out, lse = prompt_on(qn, qp, cpu, table, lens, new, SCALE, n_splits=1)
     R.check(out, want_o, tol_o, "out")
     R.check(lse, want_l, tol_l, "lse")
