@@ -32,6 +32,19 @@ constexpr int kLatPe = 64;
 constexpr int kLatW = kLatC + kLatPe;
 constexpr int kLatPairs = kLatPe / 2;
 constexpr int kLatTokens = 4;  // most tokens of a workgroup, one a wave
+// With a scale for several tokens: waves of a workgroup, tokens a wave takes at a time (in
+// registers between the two looks at them), the most tokens whose runs a workgroup looks for,
+// and the workgroups of a call where it takes more than one (two a CU fit at a time).
+constexpr int kRunWaves = 8;
+constexpr int kRunTokens = 4;
+constexpr int kRunChunk = kRunWaves * kRunTokens;
+constexpr int kRunWindow = 16;
+constexpr int kRunGroups = 768;
+
+// Wave sums and maxima of the ROCm device library (DPP sequences; every lane active).
+extern "C" __device__ float __ockl_wfred_add_f32(float);
+extern "C" __device__ uint32_t __ockl_wfred_max_u32(uint32_t);
+extern "C" __device__ int __ockl_wfred_min_i32(int);
 
 struct LatentParams {
   const uint16_t* c;
@@ -45,7 +58,7 @@ struct LatentParams {
   uint16_t* q_out;
   void* pages;
   uint8_t* scale;
-  int N, H, num_slots, block_log2, tokens;
+  int N, H, num_slots, block_log2, tokens, window;
   int turn_groups;  // workgroups that turn q_pe (and write, with a scale a token)
   bool weight_f32;
   float eps, factor;
@@ -140,9 +153,7 @@ __device__ __forceinline__ void lat_load(const LatentParams& p, int tok, const f
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum = fmaf(x.c[i], x.c[i], sum);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
-    const float r = 1.f / sqrtf(sum * (1.f / kLatC) + p.eps);
+    const float r = 1.f / sqrtf(__ockl_wfred_add_f32(sum) * (1.f / kLatC) + p.eps);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x.c[i] = x.c[i] * r * weight[i];
   }
@@ -163,10 +174,7 @@ __device__ __forceinline__ void lat_put8(const LatentParams& p, int slot, const 
   }
 }
 __device__ __forceinline__ uint32_t lat_wave_top(const Latent& x) {
-  uint32_t top = lat_top<16>(x.pe, lat_top<8>(x.c, 0u));  // (lanes past 3 hold zeros of pe)
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-  return top;
+  return __ockl_wfred_max_u32(lat_top<16>(x.pe, lat_top<8>(x.c, 0u)));  // (lanes past 3 hold zeros of pe)
 }
 __device__ __forceinline__ void lat_weight(const LatentParams& p, float* w) {
   const int lane = threadIdx.x & 63;
@@ -184,65 +192,142 @@ __device__ __forceinline__ bool lat_slot_ok(const LatentParams& p, int slot) {
   return slot >= 0 && slot < p.num_slots;
 }
 
-// With a scale for several tokens, a workgroup takes the run of tokens from tok on whose
-// slots lie in one block, if it is the run's first: the block's tokens follow one another in
-// a call, so nobody else writes the block.  Two passes over the tokens, a wave each: their
-// largest magnitude, then (again from the cache) their values.
+// kRunTokens tokens across a wave: lane l holds columns 8 l .. 8 l + 7 of each one's c, and
+// lane 4 t + q (t < kRunTokens) quarter q of token t's pe, turned.
+struct Latents {
+  float c[kRunTokens][8];
+  float pe[16];
+};
+// Tokens tok .. tok + n - 1 (the last one again past those).  s_cs: the wave's part of LDS.
 template <bool ADJACENT>
-__device__ void lat_block(const LatentParams& p, int tok, float2* s_cs, int* s_int) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int slot = p.slots[tok];
-  if (!lat_slot_ok(p, slot)) return;
-  const int block = slot >> p.block_log2;
-  if (tok > 0) {
-    const int prev = p.slots[tok - 1];
-    if (lat_slot_ok(p, prev) && prev >> p.block_log2 == block) return;
-  }
-  // the run's tokens and its lowest slot, alike in every wave
-  int count = 0, low = slot;
-  for (;;) {
-    const int t = tok + count + lane;
-    const int s = t < p.N ? p.slots[t] : -1;
-    const bool in = lat_slot_ok(p, s) && s >> p.block_log2 == block;
-    const uint64_t out = __builtin_amdgcn_ballot_w64(!in);
-    const int n = out ? __builtin_ctzll(out) : 64;
-    int m = lane < n ? s : low;
+__device__ __forceinline__ void lat_load_run(const LatentParams& p, int tok, int n, const float* weight,
+                                             float2* s_cs, Latents& x) {
+  const int lane = threadIdx.x & 63;
+  u32x4 wc[kRunTokens];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = min(m, __shfl_xor(m, o));
-    low = min(low, m);
-    count += n;
-    if (n < 64) break;
+  for (int t = 0; t < kRunTokens; ++t)
+    wc[t] = *(const u32x4*)(p.c + (size_t)(tok + min(t, n - 1)) * p.c_stride + 8 * lane);
+  u32x4 wa = {0, 0, 0, 0}, wb = {0, 0, 0, 0};
+  const int q = lane & 3;
+  if (lane < 4 * kRunTokens) {
+    const uint16_t* pe = p.pe + (size_t)(tok + min(lane >> 2, n - 1)) * p.pe_stride;
+    wa = *(const u32x4*)(pe + PeCols<ADJACENT>::first(q));
+    wb = *(const u32x4*)(pe + PeCols<ADJACENT>::second(q));
   }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the angles before are read)
+#pragma unroll
+  for (int i = 0; i < kRunTokens * kLatPairs; i += 64) {
+    const int t = (i + lane) / kLatPairs;
+    s_cs[i + lane] = lat_angle(p, tok + min(t, n - 1), (i + lane) % kLatPairs);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+  for (int t = 0; t < kRunTokens; ++t) lat_unpack8(wc[t], x.c[t]);
+  if (p.weight) {
+    float sum[kRunTokens];
+#pragma unroll
+    for (int t = 0; t < kRunTokens; ++t) {
+      sum[t] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[t] = fmaf(x.c[t][i], x.c[t][i], sum[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < kRunTokens; ++t) sum[t] = __ockl_wfred_add_f32(sum[t]);
+#pragma unroll
+    for (int t = 0; t < kRunTokens; ++t) {
+      const float r = 1.f / sqrtf(sum[t] * (1.f / kLatC) + p.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.c[t][i] = x.c[t][i] * r * weight[i];
+    }
+  }
+  lat_unpack8(wa, x.pe);
+  lat_unpack8(wb, x.pe + 8);
+  if (lane < 4 * kRunTokens) lat_turn<ADJACENT>(x.pe, s_cs + (lane >> 2) * kLatPairs + 8 * q);
+}
+template <bool ADJACENT>
+__device__ __forceinline__ void lat_put_run(const LatentParams& p, int tok, int n, const Latents& x,
+                                            float s) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int t = 0; t < kRunTokens; ++t) {
+    if (t >= n) break;
+    uint8_t* row = (uint8_t*)p.pages + (size_t)p.slots[tok + t] * kLatW;
+    *(uint2*)(row + 8 * lane) = make_uint2(lat_pack4(x.c[t], s), lat_pack4(x.c[t] + 4, s));
+  }
+  if (lane < 4 * n) {
+    const int q = lane & 3;
+    uint8_t* row = (uint8_t*)p.pages + (size_t)p.slots[tok + (lane >> 2)] * kLatW + kLatC;
+    *(uint2*)(row + PeCols<ADJACENT>::first(q)) = make_uint2(lat_pack4(x.pe, s), lat_pack4(x.pe + 4, s));
+    *(uint2*)(row + PeCols<ADJACENT>::second(q)) =
+        make_uint2(lat_pack4(x.pe + 8, s), lat_pack4(x.pe + 12, s));
+  }
+}
+
+// With a scale for several tokens, a workgroup takes the run of tokens from tok on whose
+// slots lie in one block, if tok is the run's first: the block's tokens follow one another in
+// a call, so nobody else writes the block.  Two looks at the tokens: their largest magnitude,
+// then their values (the first kRunChunk tokens from the registers, others from the cache
+// again).  (A wave for every fourth token, one at a time, and read again: 4651 tokens to
+// blocks of 32 53.7 us.)
+//
+// at: the lane of the run's first token in `slots`, which holds the slots of tokens base +
+// lane (-1 outside the call).
+template <bool ADJACENT>
+__device__ void lat_block(const LatentParams& p, int base, int at, int slots, float2* s_all, int* s_top) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tok = base + at;
+  const int block = __builtin_amdgcn_readlane(slots, at) >> p.block_log2;
+  // the run's tokens and its lowest slot, alike in every wave
+  int low = 0x7fffffff, end = at;
+  for (;;) {
+    const bool in = lat_slot_ok(p, slots) && slots >> p.block_log2 == block;
+    const uint64_t out = __builtin_amdgcn_ballot_w64(!in) & (~0ull << end);
+    const int stop = out ? __builtin_ctzll(out) : 64;
+    low = min(low, __ockl_wfred_min_i32(lane >= end && lane < stop ? slots : 0x7fffffff));
+    end = stop;
+    if (stop < 64) break;
+    base += 64;
+    slots = base + lane < p.N ? p.slots[base + lane] : -1;
+    end = 0;
+  }
+  const int count = uniform(base + end - tok);
+  low = uniform(low);
   const int first = low - (block << p.block_log2);  // tokens that the block held before
+  const int had = first > 0 ? p.scale[block] : 0;
   float w[8];
   lat_weight(p, w);
-  if (tid == 0) s_int[0] = 0;
+  float2* s_cs = s_all + wave * (kRunTokens * kLatPairs);
+  __syncthreads();  // (the run before is done with s_top and the scale)
+  if (tid == 0) *s_top = 0;
   __syncthreads();
-  Latent x;
+  Latents keep;
+  const int own = kRunTokens * wave;  // the wave's first token of a chunk
   uint32_t top = 0;
-  for (int i = wave; i < count; i += kLatTokens) {
-    if (lane < kLatPairs) s_cs[wave * kLatPairs + lane] = lat_angle(p, tok + i, lane);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    lat_load<ADJACENT>(p, tok + i, w, s_cs + wave * kLatPairs, x);
-    top = max(top, lat_wave_top(x));
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (int i = own; i < count; i += kRunChunk) {
+    Latents x;
+    lat_load_run<ADJACENT>(p, tok + i, min(count - i, kRunTokens), w, s_cs, x);
+    uint32_t m = lat_top<16>(x.pe, 0u);  // (lanes past the tokens hold zeros of pe)
+#pragma unroll
+    for (int t = 0; t < kRunTokens; ++t) m = lat_top<8>(x.c[t], m);
+    top = max(top, m);
+    if (i == own) keep = x;
   }
-  if (lane == 0) atomicMax(&s_int[0], (int)top);
+  top = __ockl_wfred_max_u32(top);
+  if (lane == 0) atomicMax(s_top, (int)top);
   __syncthreads();
-  const int had = first > 0 ? p.scale[block] : 0;
-  const int byte = max(lat_byte((uint32_t)s_int[0]), had);
+  const int byte = max(lat_byte((uint32_t)*s_top), had);
   const float s = lat_inverse(byte);
-  for (int i = wave; i < count; i += kLatTokens) {
-    if (lane < kLatPairs) s_cs[wave * kLatPairs + lane] = lat_angle(p, tok + i, lane);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    lat_load<ADJACENT>(p, tok + i, w, s_cs + wave * kLatPairs, x);
-    lat_put8<ADJACENT>(p, p.slots[tok + i], x, s);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (own < count) lat_put_run<ADJACENT>(p, tok + own, min(count - own, kRunTokens), keep, s);
+  for (int i = own + kRunChunk; i < count; i += kRunChunk) {
+    Latents x;
+    const int n = min(count - i, kRunTokens);
+    lat_load_run<ADJACENT>(p, tok + i, n, w, s_cs, x);
+    lat_put_run<ADJACENT>(p, tok + i, n, x, s);
   }
   if (byte > had && first > 0) {  // the older tokens at the new scale
     const float f = ldexpf(1.f, had - byte);
     uint32_t* old = (uint32_t*)((uint8_t*)p.pages + ((size_t)block << p.block_log2) * kLatW);
-    for (int i = tid; i < first * (kLatW / 4); i += 256) {
+    for (int i = tid; i < first * (kLatW / 4); i += 64 * kRunWaves) {
       typedef float f32x2_t __attribute__((ext_vector_type(2)));
       const uint32_t v = old[i];
       const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(v, false);
@@ -251,17 +336,27 @@ __device__ void lat_block(const LatentParams& p, int tok, float2* s_cs, int* s_i
       old[i] = lat_pack4(y, f);
     }
   }
-  __syncthreads();  // (every thread has read the old scale)
   if (tid == 0) p.scale[block] = (uint8_t)byte;
 }
 
-template <bool ADJACENT>
-__global__ __launch_bounds__(256) void latent_append_kernel(const LatentParams p) {
-  __shared__ float2 s_cs[kLatTokens * kLatPairs];
-  __shared__ int s_int[1];
+// RUNS: 8-bit pages with a scale for several tokens.
+template <bool ADJACENT, bool RUNS>
+__global__ __launch_bounds__(RUNS ? 64 * kRunWaves : 256) void latent_append_kernel(const LatentParams p) {
+  constexpr int kThreads = RUNS ? 64 * kRunWaves : 256;
+  __shared__ float2 s_cs[(RUNS ? kRunChunk : kLatTokens) * kLatPairs];
+  __shared__ int s_top;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if ((int)blockIdx.x >= p.turn_groups) {  // a block's run
-    lat_block<ADJACENT>(p, (int)blockIdx.x - p.turn_groups, s_cs, s_int);
+  if (RUNS && (int)blockIdx.x >= p.turn_groups) {
+    const int base = ((int)blockIdx.x - p.turn_groups) * p.window - 1;
+    const int t = base + lane;
+    const int slots = t >= 0 && t < p.N ? p.slots[t] : -1;
+    const int prev = __shfl_up(slots, 1);
+    // tokens of the window that begin a run
+    uint64_t begins = __builtin_amdgcn_ballot_w64(
+        lane >= 1 && lane <= p.window && lat_slot_ok(p, slots) &&
+        !(lat_slot_ok(p, prev) && prev >> p.block_log2 == slots >> p.block_log2));
+    for (; begins; begins &= begins - 1)
+      lat_block<ADJACENT>(p, base, __builtin_ctzll(begins), slots, s_cs, &s_top);
     return;
   }
   const int t0 = (int)blockIdx.x * p.tokens;
@@ -269,8 +364,7 @@ __global__ __launch_bounds__(256) void latent_append_kernel(const LatentParams p
   if (tid < nt * kLatPairs)
     s_cs[tid] = lat_angle(p, t0 + tid / kLatPairs, tid % kLatPairs);
   __syncthreads();
-  const bool runs = p.scale && p.block_log2 > 0;
-  if (!runs && wave < nt) {
+  if (!RUNS && wave < nt) {
     const int tok = t0 + wave;
     const int slot = p.slots[tok];
     float w[8];
@@ -294,7 +388,7 @@ __global__ __launch_bounds__(256) void latent_append_kernel(const LatentParams p
   }
   // q_pe: four lanes a head
   const int l = tid & 3;
-  for (int r = tid >> 2; r < nt * p.H; r += 64) {
+  for (int r = tid >> 2; r < nt * p.H; r += kThreads / 4) {
     const int t = r / p.H;
     const int h = r - t * p.H;
     const size_t tok = (size_t)(t0 + t);
@@ -481,15 +575,14 @@ extern "C" int ws_latent_rope_append(const uint16_t* c, int64_t c_stride, const 
   p.tokens = N >= 2048 ? kLatTokens : 1;
   p.turn_groups = (N + p.tokens - 1) / p.tokens;
   const bool runs = latent_scale && p.block_log2 > 0;
-  const long long grid = (long long)p.turn_groups + (runs ? N : 0);
-  if (grid * 256 >= (1LL << 32))
+  p.window = std::min(std::max(N / kRunGroups, 1), kRunWindow);
+  const long long grid = (long long)p.turn_groups + (runs ? (N + p.window - 1) / p.window : 0);
+  const int threads = runs ? 64 * kRunWaves : 256;
+  if (grid * threads >= (1LL << 32))
     return set_error(WS_EINVAL, "%s: %d tokens exceed the launch grid", name, N);
-  const dim3 g((unsigned)grid), b(256);
-  hipStream_t s = (hipStream_t)stream;
-  if (adjacent)
-    hipLaunchKernelGGL(latent_append_kernel<true>, g, b, 0, s, p);
-  else
-    hipLaunchKernelGGL(latent_append_kernel<false>, g, b, 0, s, p);
+  const auto kernel = runs ? (adjacent ? latent_append_kernel<true, true> : latent_append_kernel<false, true>)
+                           : (adjacent ? latent_append_kernel<true, false> : latent_append_kernel<false, false>);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3((unsigned)threads), 0, (hipStream_t)stream, p);
   return check_launch(name);
 }
 

@@ -20,6 +20,9 @@
 // a wave's part of a block comes to LDS as it is, is read back, multiplied by its tokens'
 // scales (exact in bf16) and written into the block's bf16 tile, two steps ahead.
 //
+// Prompts of many tiles a sequence have the latents widened once for all tiles, in a pass of
+// its own, and run over that copy (kWidenTiles).
+//
 // The scores stay with bf16 products.  gfx950's scaled 8-bit products take e4m3 latents and
 // a query split into two e4m3 halves without any widening, at the same rate, but add up
 // their 64 terms in some 17 bits below the largest one, not in fp32: an lse off by 4e-5, a
@@ -59,6 +62,7 @@ struct RowsParams {
   int n_splits;  // of every tile; 0: by the lengths, about `fill` workgroups in all
   int fill;
   bool fit;       // the tiles are fewer than `fill`: all items are to fit
+  bool join_shared;
   int pieces;     // room for them
   int piece_rows;
   int tile;       // rows of a tile
@@ -94,66 +98,72 @@ struct RowsPlace {
   int c0, n, len;
 };
 
+// Wave sums and maxima of the ROCm device library (DPP sequences; every lane active).
+extern "C" __device__ unsigned long long __ockl_wfred_add_u64(unsigned long long);
+extern "C" __device__ int __ockl_wfred_max_i32(int);
+
 // Item `at` of the list of all tiles' splits (TILES: of the split tiles): longest sequences
 // first (up to 64 of them), their last tile first.  A tile has one split for every M of
-// its sequence's blocks, M the batch's blocks over `fill` workgroups, and where the tiles
-// alone are fewer than those the least M (within 2^-6) at which all items fit.  Every
-// kernel of a call finds the same.  Every lane must call it; the result is uniform.
-template <bool TILES>
-__device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
-  constexpr int kRegs = 4;  // sequences a lane holds while M is searched
+// its sequence's blocks, M the batch's blocks over `fill` workgroups; where the tiles alone
+// are fewer than those, M is the least of four between that and the blocks over `fill` less
+// the tiles at which all items fit (the last one fits for sure: a split more than M's
+// quotient for every tile).  Every kernel of a call finds the same.  Every lane must call
+// it; the result is uniform.  PER: sequences of a lane (0: any number, in a loop that reads
+// them again; they are not split to fit).
+template <bool TILES, int PER>
+__device__ __forceinline__ RowsPlace rows_place_n(const RowsParams& p, int at) {
   const int lane = threadIdx.x & 63;
-  const int per = (p.B + 63) >> 6;
+  const int per = PER > 0 ? PER : (p.B + 63) >> 6;
   const int b0 = lane * per;
+  RowsSeq held[PER > 0 ? PER : 1];
+  auto seq = [&](int k) __attribute__((always_inline)) {
+    if constexpr (PER > 0) return held[k];
+    else return rows_seq(p, b0 + k);
+  };
+  if constexpr (PER > 0) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      held[k] = rows_seq(p, min(b0 + k, p.B - 1));
+      if (b0 + k >= p.B) held[k].tiles = held[k].blocks = 0;
+    }
+  }
+  const int mine = PER > 0 ? PER : max(min(per, p.B - b0), 0);
   float rM = 0.f;
   if (p.n_splits == 0) {
-    int til[kRegs] = {}, blk[kRegs] = {};
-    unsigned long long total = 0;
-    int tiles = 0, longest = 0;
-    for (int k = 0; k < per && b0 + k < p.B; ++k) {
-      const RowsSeq s = rows_seq(p, b0 + k);
-#pragma unroll
-      for (int j = 0; j < kRegs; ++j)
-        if (k == j) {
-          til[j] = s.tiles;
-          blk[j] = s.blocks;
-        }
-      total += (unsigned long long)s.tiles * (unsigned)s.blocks;
+    unsigned long long sum = 0;
+    int tiles = 0;
+#pragma unroll 4
+    for (int k = 0; k < mine; ++k) {
+      const RowsSeq s = seq(k);
+      sum += (unsigned long long)s.tiles * (unsigned)s.blocks;
       tiles += s.tiles;
-      longest = max(longest, s.blocks);
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      total += __shfl_xor(total, o);
-      tiles += __shfl_xor(tiles, o);
-      longest = max(longest, __shfl_xor(longest, o));
-    }
+    const float total = (float)__ockl_wfred_add_u64(sum);
     auto blocks_at = [&](int places) {
-      const double m = (double)total / (double)max(places, 1);
-      return (int)ceil(min(max(m, (double)kRowsMinShare), 1e9));
+      return (int)fminf(ceilf(fmaxf(total * __builtin_amdgcn_rcpf((float)max(places, 1)), (float)kRowsMinShare)),
+                        1e9f);
     };
-    int M = blocks_at(p.fill);
-    if (p.fit) {
-      auto fits = [&](int m) {
-        const float r = __builtin_amdgcn_rcpf((float)m);
-        int items = 0;
-        for (int j = 0; j < kRegs; ++j) {
-          if (j >= per) break;
-          items += til[j] * max(plan_nsplits(blk[j], r), 1);
-        }
-        return uniform((int)__ockl_wfred_add_u32((unsigned)items)) <= p.fill;
-      };
-      int lo = M;
-      int hi = uniform(max(min(blocks_at(p.fill - tiles), longest), lo));
-      if (!fits(lo)) {
-        if (!fits(hi)) hi = max(longest, 1);  // (a split a sequence and tile)
-        for (int i = 0; i < 6 && hi - lo > 1; ++i) {
-          const int mid = (lo + hi) >> 1;
-          if (fits(mid)) hi = mid;
-          else lo = mid;
-        }
-        M = hi;
+    int M = uniform(blocks_at(p.fill));
+    if (PER > 0 && p.fit) {
+      const int room = p.fill - uniform((int)__ockl_wfred_add_u32((unsigned)tiles));
+      const int gap = uniform(blocks_at(room)) + 1 - M;
+      uint32_t cnt[2] = {0, 0};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float r = __builtin_amdgcn_rcpf((float)(M + (gap * c + 2) / 3));
+        uint32_t n = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+          n += held[k].tiles * min(max(plan_nsplits(held[k].blocks, r), 1), kRowsMaxSplits);
+        cnt[c >> 1] += min(n, 1023u) << (16 * (c & 1));  // (sums of 64 lanes stay below 2^16)
       }
+      cnt[0] = uniform((int)__ockl_wfred_add_u32(cnt[0]));
+      cnt[1] = uniform((int)__ockl_wfred_add_u32(cnt[1]));
+      int best = M + gap;
+#pragma unroll
+      for (int c = 2; c >= 0; --c)
+        if ((int)((cnt[c >> 1] >> (16 * (c & 1))) & 0xffffu) <= p.fill) best = M + (gap * c + 2) / 3;
+      M = best;
     }
     rM = __builtin_amdgcn_rcpf((float)M);
   }
@@ -163,8 +173,9 @@ __device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
   };
   // a lane's items, and the pieces before its first sequence in the batch's order
   int items = 0, units = 0, key = -1;
-  for (int k = 0; k < per && b0 + k < p.B; ++k) {
-    const RowsSeq s = rows_seq(p, b0 + k);
+#pragma unroll 4
+  for (int k = 0; k < mine; ++k) {
+    const RowsSeq s = seq(k);
     const int splits = splits_of(s);
     units += splits > 1 ? s.tiles * splits : 0;
     items += !TILES ? s.tiles * splits : splits > 1 ? s.tiles : 0;
@@ -172,7 +183,7 @@ __device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
   }
   const int before = __ockl_wfscan_add_i32(units, true) - units;
   int from = lane;  // the lane whose sequences stand at this lane's place in the list
-  if (!TILES && per == 1 && p.B > 1) {
+  if (!TILES && PER == 1 && p.B > 1) {
     int rank = 0;
     for (int j = 0; j < p.B; ++j) {
       const int other = __builtin_amdgcn_readlane(key, j);
@@ -190,10 +201,19 @@ __device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
   int left = at - __builtin_amdgcn_readlane(incl - items, slot);
   const int owner = __builtin_amdgcn_readlane(from, slot);
   int piece = __builtin_amdgcn_readlane(before, owner);
-  for (int k = 0; k < per; ++k) {
+  auto take = [&](int k) __attribute__((always_inline)) {  // whether the item is sequence k's
     const int b = uniform(owner * per + k);
-    if (b >= p.B || left < 0) break;  // (left < 0: sums past 2^31, cu_new not non-decreasing)
-    const RowsSeq s = rows_seq(p, b);
+    if (b >= p.B || left < 0) return true;  // (left < 0: sums past 2^31, cu_new not non-decreasing)
+    RowsSeq s;
+    if constexpr (PER > 0) {
+      s.c0 = __builtin_amdgcn_readlane(held[k].c0, owner);
+      s.n = __builtin_amdgcn_readlane(held[k].n, owner);
+      s.len = __builtin_amdgcn_readlane(held[k].len, owner);
+      s.tiles = __builtin_amdgcn_readlane(held[k].tiles, owner);
+      s.blocks = __builtin_amdgcn_readlane(held[k].blocks, owner);
+    } else {
+      s = rows_seq(p, b);
+    }
     const int splits = uniform(splits_of(s));
     const int tiles = uniform(s.tiles);
     const int here = !TILES ? tiles * splits : splits > 1 ? tiles : 0;
@@ -207,12 +227,27 @@ __device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
       r.c0 = uniform(s.c0);
       r.n = uniform(s.n);
       r.len = uniform(s.len);
-      break;
+      return true;
     }
     left -= here;
     piece += splits > 1 ? tiles * splits : 0;
+    return false;
+  };
+  if constexpr (PER > 0) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (r.b < 0 && left >= 0 && take(k)) break;
+  } else {
+    for (int k = 0; k < per; ++k)
+      if (take(k)) break;
   }
   return r;
+}
+template <bool TILES>
+__device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
+  if (p.B <= 64) return rows_place_n<TILES, 1>(p, at);
+  if (p.B <= 256) return rows_place_n<TILES, 4>(p, at);
+  return rows_place_n<TILES, 0>(p, at);
 }
 
 // ---------------------------------------------------------------------------
@@ -1201,11 +1236,11 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
   }
 }
 
-// Combines the pieces of the tiles that were split, four rows a workgroup: a wave a row, or,
-// from kJoinShared pieces on, the four waves a row after the other, each a quarter of the
-// pieces.  A lane has eight columns.
-constexpr int kJoinRows = 4;
-constexpr int kJoinShared = 16;
+// Combines the pieces of the tiles that were split: a wave a row, or (p.join_shared: many
+// pieces a tile, on average) a workgroup a row, each wave a quarter of the pieces.  A lane has
+// eight columns.  (Without shared rows a workgroup takes kJoinRows: in a call whose tiles
+// fill the chip hardly any is split, and every workgroup looks for its tile first.)
+constexpr int kJoinRows = 16;
 struct JoinAcc {
   float m, sum;
   float a[8];
@@ -1213,7 +1248,7 @@ struct JoinAcc {
 __device__ __forceinline__ void join_pieces(JoinAcc& x, const uint16_t* out, const float* lse,
                                             int rows, int first, int step, int n) {
   const int lane = threadIdx.x & 63;
-  constexpr int U = 8;  // pieces under way
+  constexpr int U = 16;  // pieces under way
   for (int s = first; s < n; s += U * step) {
     float l[U];
     u32x4 v[U];
@@ -1246,64 +1281,102 @@ __device__ __forceinline__ void join_pieces(JoinAcc& x, const uint16_t* out, con
     }
   }
 }
+__device__ __forceinline__ void join_row(const RowsParams& p, const RowsPlace& tl, int tr, bool shared,
+                                         JoinAcc (*s_acc)[64]) {
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  JoinAcc x;
+  x.m = neg_inf();
+  x.sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) x.a[c] = 0.f;
+  const size_t slot = (size_t)tl.piece * p.piece_rows + tr;
+  join_pieces(x, p.part_out + slot * kRowsC, p.part_lse + slot, p.piece_rows, shared ? wave : 0,
+              shared ? 4 : 1, tl.splits);
+  if (shared) {
+    if (wave > 0) s_acc[wave - 1][lane] = x;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int o = 0; o < 3; ++o) {
+      const JoinAcc y = s_acc[o][lane];
+      const float m = fmaxf(x.m, y.m);
+      const float fx = acc_factor(x.m, m), fy = acc_factor(y.m, m);
+      x.m = m;
+      x.sum = x.sum * fx + y.sum * fy;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) x.a[c] = x.a[c] * fx + y.a[c] * fy;
+    }
+  }
+  const float inv = x.sum == 0.f ? 0.f : 1.f / x.sum;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) x.a[c] *= inv;
+  const size_t at = (size_t)tl.c0 * p.H + tl.tile * p.tile + tr;
+  if (p.out_f32) {
+    float4* dst = (float4*)(p.out_f32 + at * kRowsC) + 2 * lane;
+    dst[0] = make_float4(x.a[0], x.a[1], x.a[2], x.a[3]);
+    dst[1] = make_float4(x.a[4], x.a[5], x.a[6], x.a[7]);
+  }
+  if (p.out_bf16) {
+    u32x4 o;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = pack_bf16x2(x.a[2 * c], x.a[2 * c + 1]);
+    ((u32x4*)(p.out_bf16 + at * kRowsC))[lane] = o;
+  }
+  if (p.lse && lane == 0) p.lse[at] = x.sum == 0.f ? neg_inf() : x.m + __logf(x.sum);
+}
 __global__ __launch_bounds__(256) void mla_rows_join_kernel(const RowsParams p) {
   __shared__ JoinAcc s_acc[3][64];
   const RowsPlace tl = rows_place<true>(p, blockIdx.x);
   if (tl.b < 0 || tl.splits == 1 || tl.piece < 0 || tl.piece + tl.splits > p.pieces) return;
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = uniform(threadIdx.x >> 6);
   const int here = min(p.tile, tl.n * p.H - tl.tile * p.tile);
-  const bool shared = tl.splits >= kJoinShared;
-  for (int i = 0; i < (shared ? kJoinRows : 1); ++i) {
-    const int tr = blockIdx.y * kJoinRows + (shared ? i : wave);  // row of the tile
-    JoinAcc x;
-    x.m = neg_inf();
-    x.sum = 0.f;
+  const bool shared = p.join_shared;
+  // row of the tile (with `shared` the whole workgroup's)
+  int tr = shared ? blockIdx.y : blockIdx.y * kJoinRows + wave;
+  for (int more = shared ? 1 : kJoinRows / 4; more > 0 && tr < here; --more, tr += 4)
+    join_row(p, tl, tr, shared, s_acc);
+}
+
+// Every sequence's tokens from 8-bit pages as bf16 rows [b][pad], one page a sequence (table:
+// its id), for prompts whose tiles read them many times.  Tokens in a bad page are NaN.
+constexpr int kWidenTokens = 32;  // of a workgroup
+__global__ __launch_bounds__(256) void latent_widen_kernel(const RowsParams p, uint16_t* copy,
+                                                           int32_t* table, int pad) {
+  const int b = blockIdx.y, t0 = blockIdx.x * kWidenTokens;
+  if (blockIdx.x == 0 && threadIdx.x == 0) table[b] = b;
+  const int len = p.kv_len[b];
+  if (!len_ok(len, 0, min(p.cap, pad)) || t0 >= len) return;
+  const int page = t0 / p.page_size;  // (32 tokens lie in one page)
+  const int raw = p.page_table[(size_t)b * p.max_pages + page];
+  const int pid = clamp_page(raw, p.num_pages);
+  const size_t tok = (size_t)pid * p.page_size + (t0 - page * p.page_size);
+  const u32x4* src = (const u32x4*)((const uint8_t*)p.latent + tok * 576);
+  u32x4* dst = (u32x4*)(copy + ((size_t)b * pad + t0) * 576);
+  const int n = min(kWidenTokens, len - t0) * 36;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) x.a[c] = 0.f;
-    const size_t slot = (size_t)tl.piece * p.piece_rows + tr;
-    if (tr < here)
-      join_pieces(x, p.part_out + slot * kRowsC, p.part_lse + slot, p.piece_rows, shared ? wave : 0,
-                  shared ? 4 : 1, tl.splits);
-    if (shared) {
-      if (i > 0) __syncthreads();
-      if (wave > 0) s_acc[wave - 1][lane] = x;
-      __syncthreads();
-      if (wave > 0) continue;
-#pragma unroll
-      for (int o = 0; o < 3; ++o) {
-        const JoinAcc y = s_acc[o][lane];
-        const float m = fmaxf(x.m, y.m);
-        const float fx = acc_factor(x.m, m), fy = acc_factor(y.m, m);
-        x.m = m;
-        x.sum = x.sum * fx + y.sum * fy;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) x.a[c] = x.a[c] * fx + y.a[c] * fy;
-      }
-    }
-    if (tr >= here) continue;
-    const float inv = x.sum == 0.f ? 0.f : 1.f / x.sum;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) x.a[c] *= inv;
-    const size_t at = (size_t)tl.c0 * p.H + tl.tile * p.tile + tr;
-    if (p.out_f32) {
-      float4* dst = (float4*)(p.out_f32 + at * kRowsC) + 2 * lane;
-      dst[0] = make_float4(x.a[0], x.a[1], x.a[2], x.a[3]);
-      dst[1] = make_float4(x.a[4], x.a[5], x.a[6], x.a[7]);
-    }
-    if (p.out_bf16) {
-      u32x4 o;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] = pack_bf16x2(x.a[2 * c], x.a[2 * c + 1]);
-      ((u32x4*)(p.out_bf16 + at * kRowsC))[lane] = o;
-    }
-    if (p.lse && lane == 0) p.lse[at] = x.sum == 0.f ? neg_inf() : x.m + __logf(x.sum);
+  for (int j = 0; j < (kWidenTokens * 36 + 255) / 256; ++j) {
+    const int i = threadIdx.x + 256 * j;
+    if (i >= n) break;
+    const u32x4 w = src[i];
+    const float s =
+        raw == pid ? __builtin_bit_cast(float, (uint32_t)p.scale[(tok + i / 36) >> p.block_log2] << 23) : qnan();
+    dst[2 * i] = widen8(w[0], w[1], s);
+    dst[2 * i + 1] = widen8(w[2], w[3], s);
   }
 }
 
 // ---------------------------------------------------------------------------
 
+// Tiles of a sequence, on average, from which its latents are widened in a pass of their own,
+// and the largest copy.  A block of the copy costs its bytes once (11 ns of the chip), widening
+// it in the steps some 0.4 us of a CU, 1.5 ns of the chip, a tile.
+constexpr int kWidenTiles = 12;
+constexpr size_t kWidenBytes = 256u << 20;
+
 struct RowsPlan {
   long long tiles, grid, pieces, joins;
+  size_t copy;  // bytes of the widened latents (0: none)
+  int pad;      // tokens of a sequence there
   int fill, piece_rows, tile;
   bool fit, few;
 };
@@ -1314,6 +1387,11 @@ static RowsPlan rows_plan(int N, int B, int H, bool decode, bool fp8, int max_le
   r.tile = r.few ? kFewTile : kRowsTile;
   const long long each = (H + r.tile - 1) / r.tile;
   r.tiles = decode ? B * each : std::min((long long)N * H / r.tile + B, (long long)N * each);
+  r.pad = std::max((max_len + 31) & ~31, 32);
+  r.copy = fp8 && !decode && (long long)N * H >= (long long)kWidenTiles * r.tile * B
+               ? (size_t)B * r.pad * 1152
+               : 0;
+  if (r.copy > kWidenBytes) r.copy = 0;
   r.fill = choose_workgroups(0, 1, 1LL << 30, 1);
   r.fit = r.tiles < r.fill && B <= 256;
   r.piece_rows = (int)std::min<long long>(r.tile, decode ? H : (long long)N * H);
@@ -1332,10 +1410,13 @@ static RowsPlan rows_plan(int N, int B, int H, bool decode, bool fp8, int max_le
   }
   return r;
 }
-static size_t rows_bytes(const RowsPlan& pl) {
-  if (pl.pieces == 0) return 0;
+// The workspace: the pieces' lse and outputs, the copy's table and rows.
+static size_t rows_piece_bytes(const RowsPlan& pl) {
   const size_t rows = (size_t)pl.pieces * pl.piece_rows;
-  return align256(rows * 4) + rows * kRowsC * 2;
+  return align256(rows * 4) + align256(rows * kRowsC * 2);
+}
+static size_t rows_bytes(const RowsPlan& pl, int B) {
+  return rows_piece_bytes(pl) + (pl.copy ? align256((size_t)B * 4) + pl.copy : 0);
 }
 
 static int rows_sizes(const char* name, int N, int B, int H, bool decode, bool fp8, int max_len,
@@ -1383,7 +1464,7 @@ static int rows_run(const char* name, const uint16_t* q_nope, const uint16_t* q_
   if (!(scale - scale == 0.f)) return set_error(WS_EINVAL, "%s: scale must be finite", name);
   if (N == 0 || B == 0) return WS_OK;
   const RowsPlan pl = rows_plan(N, B, H, decode, latent_scale != nullptr, max_len, n_splits);
-  const size_t need = rows_bytes(pl);
+  const size_t need = rows_bytes(pl, B);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(WS_EWORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
   if (need > 0 && ((uintptr_t)workspace & 255u) != 0)
@@ -1416,23 +1497,36 @@ static int rows_run(const char* name, const uint16_t* q_nope, const uint16_t* q_
   p.pieces = (int)pl.pieces;
   p.piece_rows = pl.piece_rows;
   p.tile = pl.tile;
+  p.join_shared = pl.pieces >= 12 * pl.tiles;
   // the smallest normal float for 0: every finite score then rounds to the same
   // probability, and masked tokens stay -inf
   p.scale_log2 = std::max((scale < 0.f ? -scale : scale) * kLog2e, 1.17549435e-38f);
   p.q_sign = scale < 0.f ? 0x80008000u : 0u;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)pl.grid), block(256);
+  if (pl.copy) {
+    int32_t* table = (int32_t*)((char*)workspace + rows_piece_bytes(pl));
+    uint16_t* copy = (uint16_t*)((char*)table + align256((size_t)B * 4));
+    hipLaunchKernelGGL(latent_widen_kernel, dim3((unsigned)(pl.pad / kWidenTokens), (unsigned)B), block, 0, s,
+                       p, copy, table, pl.pad);
+    if (int rc = check_launch(name)) return rc;
+    p.latent = copy;
+    p.page_table = table;
+    p.page_size = p.cap = pl.pad;  // (a length past max_len, which the call rules out, is NaN)
+    p.max_pages = 1;
+    p.num_pages = B;
+  }
   if (pl.few)
     hipLaunchKernelGGL(mla_few_kernel, grid, block, 0, s, p);
-  else if (latent_scale)
+  else if (latent_scale && !pl.copy)
     hipLaunchKernelGGL(mla_rows_kernel<true>, grid, block, 0, s, p);
   else
     hipLaunchKernelGGL(mla_rows_kernel<false>, grid, block, 0, s, p);
   int rc = check_launch(name);
   if (rc != WS_OK || pl.pieces == 0) return rc;
   hipLaunchKernelGGL(mla_rows_join_kernel,
-                     dim3((unsigned)pl.joins, (pl.piece_rows + kJoinRows - 1) / kJoinRows), block, 0,
-                     s, p);
+                     dim3((unsigned)pl.joins, p.join_shared ? pl.piece_rows : (pl.piece_rows + kJoinRows - 1) / kJoinRows),
+                     block, 0, s, p);
   return check_launch(name);
 }
 
@@ -1441,7 +1535,7 @@ static int rows_plan_out(const char* name, int N, int B, int H, bool decode, boo
   if (int rc = rows_sizes(name, N, B, H, decode, fp8, max_len, n_splits)) return rc;
   const RowsPlan pl = rows_plan(N, B, H, decode, fp8, max_len, n_splits);
   if (pieces_out) *pieces_out = (int)pl.pieces;
-  if (bytes_out) *bytes_out = rows_bytes(pl);
+  if (bytes_out) *bytes_out = rows_bytes(pl, B);
   return WS_OK;
 }
 

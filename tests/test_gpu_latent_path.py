@@ -440,6 +440,33 @@ def test_prompt_nan_scale(H, n):
     assert bool(out[clean:].isnan().all()) and bool(lse[clean:].isnan().all())
 
 
+@pytest.mark.parametrize("block, splits", [(1, 0), (32, 1), (8, 3)])
+def test_prompt_many_tiles_over_8_bits(block, splits):
+    """Prompts of many tiles a sequence, whose latents are widened in a pass of their own: NaN
+    codes, NaN scales and bad pages reach the rows that see them, and lengths out of range
+    their own sequence."""
+    lens, new, page, H = [330, 200, 64, 40, 100], [180, 130, 0, 30, 100], 32, 20
+    assert sum(new) * H >= 12 * 128 * len(new)
+    table, P, (pool, sc) = L.pools(lens, page, 8, block, 41)
+    place = lambda b, t: (int(table[b, t // page]), t % page)
+    p, o = place(0, 250)
+    pool.view(torch.uint8)[p, o, 77] = 0x7f
+    p, o = place(1, 150)
+    sc.view(torch.uint8)[p, o // block] = 255
+    qn, qp = queries(sum(new), H, 3)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, (pool, sc), table, lens, new, page, block, 0.1, pieces=splits != 1)
+    table[4, 2] = P + 1  # tokens 64 .. 95
+    lens[3] = -1
+    out, lse = prompt_on(qn, qp, (pool, sc), table, lens, new, 0.1, n_splits=splits)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    seen = {0: 250 - 150, 1: 150 // block * block - 70, 3: 0, 4: 64}  # rows that see nothing odd
+    for b, n in seen.items():
+        fine, gone = slice(cu[b], cu[b] + n), slice(cu[b] + n, cu[b + 1])
+        R.check(out[fine], want_o[fine], tol_o[fine], f"fine rows of {b}")
+        R.check(lse[fine], want_l[fine], tol_l[fine], f"fine rows of {b}")
+        assert bool(out[gone].isnan().all()) and bool(lse[gone].isnan().all()), b
+
+
 @pytest.mark.parametrize("bits", (16, 8))
 def test_prompt_scale_signs(bits):
     """A negative scale, and zero (the mean of what a row sees)."""
