@@ -102,8 +102,8 @@ struct RowsPlace {
 extern "C" __device__ unsigned long long __ockl_wfred_add_u64(unsigned long long);
 extern "C" __device__ int __ockl_wfred_max_i32(int);
 
-// Item `at` of the list of all tiles' splits (TILES: of the split tiles): longest sequences
-// first (up to 64 of them), their last tile first.  A tile has one split for every M of
+// Item `at` of the list of all tiles' splits (TILES: of the split tiles): where the items do
+// not fit the chip at once, longest sequences first (up to 64 of them), their last tile first.  A tile has one split for every M of
 // its sequence's blocks, M the batch's blocks over `fill` workgroups; where the tiles alone
 // are fewer than those, M is the least of four between that and the blocks over `fill` less
 // the tiles at which all items fit (the last one fits for sure: a split more than M's
@@ -183,7 +183,7 @@ __device__ __forceinline__ RowsPlace rows_place_n(const RowsParams& p, int at) {
   }
   const int before = __ockl_wfscan_add_i32(units, true) - units;
   int from = lane;  // the lane whose sequences stand at this lane's place in the list
-  if (!TILES && PER == 1 && p.B > 1) {
+  if (!TILES && PER == 1 && !p.fit && p.B > 1) {  // (splits that fit once are alike)
     int rank = 0;
     for (int j = 0; j < p.B; ++j) {
       const int other = __builtin_amdgcn_readlane(key, j);
@@ -255,10 +255,12 @@ __device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
 
 // Both kinds of pages have ws_mla_ring.h's bf16 tiles.  bf16: four, loaded three blocks ahead.
 // 8 bits: three, and per wave two slots for its eight rows of a block as they are in the
-// pages, 288 chunks of 16 bytes and the block's scales, loaded four blocks ahead.
+// pages, 36 chunks of 16 bytes each, and the rows' scales, loaded four blocks ahead.  Lane l has
+// chunks l / 8 + 8 i (i < 5; past the 36th the last one) of row l % 8: one scale a lane, one
+// address and constant steps on either side, and 16 lanes' writes into the tile meet 16
+// chunk slots mod 16.
 constexpr int kRowsTileBytes = 16 * kWideTileAlloc;
 constexpr int kRawRows = 8;             // of a wave
-constexpr int kRawChunks = 36 * kRawRows;
 constexpr int kRawDma = 5;              // load instructions, and one for the scales
 constexpr int kRawBytes = 1024 * kRawDma;
 template <bool F8>
@@ -268,7 +270,11 @@ struct RowsRing {
   // LDS: tiles, then the bf16 sink or the waves' raw slots, then the raw slots' scales
   static constexpr int kRaw = kTiles * kRowsTileBytes;
   static constexpr int kScales = kRaw + (F8 ? 4 * 2 * kRawBytes : 1024);
-  static constexpr int kLds = kScales + (F8 ? 4 * 2 * 256 : 0);
+  // and, for 8 bits, the last k-step of the queries (a lane's own 16 bytes), whose registers
+  // the widening takes: what the compiler spilled instead came back behind the loads under
+  // way, which memory answers in order
+  static constexpr int kQuery = kScales + (F8 ? 4 * 2 * 256 : 0);
+  static constexpr int kLds = kQuery + (F8 ? 256 * 16 : 0);
 };
 static_assert(RowsRing<true>::kLds <= 160 * 1024 - 64 && RowsRing<false>::kLds <= 160 * 1024 - 64, "LDS");
 static_assert(RowsRing<true>::kScales >= kRowsTile * 65 * 16, "the queries are staged in the tiles");
@@ -329,16 +335,12 @@ __device__ __forceinline__ void rows_wait() {
 // row_bytes + col_byte.
 __device__ __forceinline__ void rows_store(char* dst, int row_bytes, const uint32_t* src,
                                            int col_byte, int rows) {
-#pragma unroll
-  for (int h0 = 0; h0 < 32; h0 += 8) {
-    if (h0 >= rows) break;
-    u32x4 v[8];
-#pragma unroll
-    for (int h = 0; h < 8; ++h) v[h] = *(const u32x4*)(src + (h0 + h) * 260);
-#pragma unroll
-    for (int h = 0; h < 8; ++h)
-      if (h0 + h < rows) *(u32x4*)(dst + (size_t)(h0 + h) * row_bytes + col_byte) = v[h];
+  if (rows == 32) {
+    wide_store_rows(dst, row_bytes, src, col_byte, 32);
+    return;
   }
+  for (int h = 0; h < rows; ++h)
+    *(u32x4*)(dst + (size_t)h * row_bytes + col_byte) = *(const u32x4*)(src + h * 260);
 }
 
 // What a bf16 pair holds of infinities and NaN: their halves' bits, all set.
@@ -370,8 +372,10 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, RowsWork& w) {
   w.lim_lo = w.first_pos + w.row0 / p.H + 1;
   const int lim_hi = w.len_good ? max(w.first_pos + (w.row0 + w.here - 1) / p.H + 1, 0) : 0;
   const int nb = (lim_hi + 31) / 32;
-  const int blk0 = (int)((long long)pl.split * nb / pl.splits);
-  const int blk1 = (int)((long long)(pl.split + 1) * nb / pl.splits);
+  // (nb split / splits without 64 bits: splits is at most kRowsMaxSplits)
+  const unsigned each = (unsigned)nb / (unsigned)pl.splits, rest = (unsigned)nb - each * (unsigned)pl.splits;
+  const int blk0 = (int)(pl.split * each + pl.split * rest / (unsigned)pl.splits);
+  const int blk1 = (int)((pl.split + 1) * each + (pl.split + 1) * rest / (unsigned)pl.splits);
   w.nblk = blk1 - blk0;
   w.t_begin = 32 * blk0;
   w.t_end = min(lim_hi, 32 * blk1);
@@ -425,28 +429,24 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   const uint32_t raw0 = lds0 + R::kRaw + 2 * kRawBytes * wave;       // this wave's (8 bits)
   const uint32_t scale0 = lds0 + R::kScales + 2 * 256 * wave;
   // bf16: byte offsets, within a block's rows in HBM, of the chunks this lane loads, two to a
-  // register (the largest is 31 * 1152 + 1136).  8 bits: for each of the lane's chunks of
-  // the wave's raw slot, where it goes in a tile, in 16-byte units from the wave's first row
-  // (10 bits), and its row less that one.
-  constexpr int kOff = F8 ? (kRawDma + 1) / 2 : kPer / 2;
+  // register (the largest is 31 * 1152 + 1136).  8 bits: the lane's first chunk in a tile.
+  constexpr int kOff = F8 ? 1 : kPer / 2;
   uint32_t offp[kOff];
+  if constexpr (F8) {
+    offp[0] = 16 * (uint32_t)(wide_row_off(lane & 7) + kWideRowsT * wave + 2 * (lane >> 3));
+  } else {
 #pragma unroll
-  for (int j = 0; j < kOff; ++j) {
-    uint32_t v = 0;
+    for (int j = 0; j < kOff; ++j) {
+      uint32_t v = 0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if constexpr (F8) {
-        const int c = min(64 * (2 * j + h) + lane, kRawChunks - 1);
-        const int r = c / 36;  // (rows 8 apart are kWideRowsT chunks apart)
-        v |= (uint32_t)(wide_row_off(r) + 2 * (c - 36 * r) + 1024 * r) << (16 * h);
-      } else {
+      for (int h = 0; h < 2; ++h) {
         const int c = 64 * min(wave + 4 * (2 * j + h), kWideTileDma - 1) + lane;
         const int r = wide_row_of(c);
         const int x = min(c - wide_row_off(r), kWideRowData - 1);
         v |= (uint32_t)(r * kRow + 16 * x) << (16 * h);
       }
+      offp[j] = v;
     }
-    offp[j] = v;
   }
   // Per-lane part of the transposed reads: lane 4 e + r of a 16-lane group addresses token
   // row 4 j2 + e, columns 4 r .. 4 r + 3 of the group's 16.
@@ -479,16 +479,16 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   {
     const uint16_t* qrow0 = p.q_nope + (w.g_row0 + 32 * wave) * kRowsC;
     const uint32_t qst = lds0 + (uint32_t)(32 * wave * 65 * 16);
-    if (rows > 0)
-      for (int h = 0; h < 32; ++h)
-        rows_dma16(16 * lane, qrow0 + (size_t)min(h, rows - 1) * kRowsC, qst + (uint32_t)(h * 65 * 16), 0);
+#pragma clang loop unroll(disable)
+    for (int h = 0; h < rows; ++h)
+      rows_dma16(16 * lane, qrow0 + h * kRowsC, qst + (uint32_t)(h * 65 * 16), 0);
     const u32x4* pe =
         (const u32x4*)(p.q_pe + (w.g_row0 + min(32 * wave + n32, here - 1)) * kRowsPe);
 #pragma unroll
     for (int u = 32; u < 36; ++u) qb[u] = pe[2 * (u - 32) + j2];
     asm volatile("s_waitcnt vmcnt(0)" : "+v"(raw_pid) : : "memory");
     set_pids(raw_pid);
-    const u32x4* qs = s_tile + (32 * wave + n32) * 65 + j2;
+    const u32x4* qs = s_tile + (32 * wave + min(n32, max(rows - 1, 0))) * 65 + j2;
 #pragma unroll
     for (int u = 0; u < 32; ++u) qb[u] = qs[2 * u];
     if (p.q_sign) {
@@ -496,6 +496,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
       for (int u = 0; u < 36; ++u) qb[u] ^= p.q_sign;
     }
   }
+  if constexpr (F8) rows_lds_put(lds0 + R::kQuery + 16 * tid, qb[35]);
   // the queries in registers, and every wave done with its staged rows, before the loads
 #pragma unroll
   for (int u = 0; u < 36; ++u) asm volatile("" : : "v"(qb[u]));
@@ -508,7 +509,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   struct Dma {
     const char* sb;
     const uint8_t* ss;
-    uint32_t wbase, last, lim, lim_s;
+    uint32_t wbase, last, lim;  // (8 bits, lim: the block's last row)
   };
   auto issue_begin = [&](int k) __attribute__((always_inline)) {
     const int kc = min(k, nblk - 1);
@@ -523,13 +524,13 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     const int nt = min(t_end - (t_begin + 32 * kc), 32);
     Dma d;
     d.sb = g0 + (size_t)tok * kRow;
-    d.lim = nt >= 32 ? 0xffffu : (uint32_t)((nt - 1) * kRow + kRow - 16);
     if constexpr (F8) {
+      d.lim = (uint32_t)(nt - 1);
       d.wbase = raw0 + kRawBytes * (k & 1);
       d.last = scale0 + 256 * (k & 1);
       d.ss = p.scale + (tok >> p.block_log2);
-      d.lim_s = (uint32_t)(nt - 1) >> p.block_log2;
     } else {
+      d.lim = nt >= 32 ? 0xffffu : (uint32_t)((nt - 1) * kRow + kRow - 16);
       const uint32_t tb = lds0 + (uint32_t)(k & 3) * kRowsTileBytes;
       d.wbase = tb + 1024 * wave;
       d.last = wave == 0 ? tb + 1024 * (kWideTileDma - 1) : lds0 + R::kRaw;
@@ -542,11 +543,11 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     if constexpr (F8) {
       int l = lane;
       asm volatile("" : "+v"(l));  // (recomputed at each use)
+      const uint32_t row = min((uint32_t)(kRawRows * wave + (l & 7)), d.lim);
       if (i < kRawDma)
-        rows_dma16(min((uint32_t)(16 * (kRawChunks * wave + min(64 * i + l, kRawChunks - 1))), d.lim), d.sb,
-                   d.wbase, 1024 * i);
+        rows_dma16(row * kRow + 16 * min(8 * i + (l >> 3), 35), d.sb, d.wbase, 1024 * i);
       else
-        rows_dma1(min((uint32_t)(l & 31) >> p.block_log2, d.lim_s), d.ss, d.last);
+        rows_dma1(row >> p.block_log2, d.ss, d.last);
     } else {
       asm volatile("" : "+v"(offp[i >> 1]));  // unpacked at each use
       const uint32_t pr = offp[i >> 1];
@@ -560,38 +561,31 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) dma_one(d, i);
   };
-  // 8 bits: chunk i of this wave's part of block k, as it is in its raw slot (its loads done),
-  // and into the tile
-  struct Raw {
-    u32x4 w;
-    uint32_t s;
+  // 8 bits: the lane's scale and chunk i of its row of block k, as they are in the raw slot (its
+  // loads done), and the chunk into the tile (`to`: the lane's first place there)
+  auto raw_scale = [&](int k) __attribute__((always_inline)) {
+    return __builtin_bit_cast(float, rows_lds_b32(scale0 + 256 * (k & 1) + 4 * lane) << 23);
   };
   auto raw_read = [&](int k, int i) __attribute__((always_inline)) {
-    uint32_t at = raw0 + kRawBytes * (k & 1) + 1024 * i;
-    const uint32_t sc = scale0 + 256 * (k & 1) + 4 * kRawRows * wave;
-    if (i < kRawDma - 1) {
-      at += 16 * lane;
-    } else {
-      at += 16 * min(lane, kRawChunks - 1 - 64 * (kRawDma - 1));
-    }
-    asm volatile("" : "+v"(offp[i >> 1]));  // unpacked at each use
-    const uint32_t r = offp[i >> 1] >> (16 * (i & 1) + 10) & 7u;
-    return Raw{rows_lds_b128(at), rows_lds_b32(sc + 4 * r)};
+    return rows_lds_b128(raw0 + kRawBytes * (k & 1) + 16 * lane + 1024 * i);
   };
-  auto raw_put = [&](const Raw& r, uint32_t tile, int i) __attribute__((always_inline)) {
-    const float sc = __builtin_bit_cast(float, r.s << 23);
-    asm volatile("" : "+v"(offp[i >> 1]));
-    const uint32_t to = tile + 16 * (offp[i >> 1] >> (16 * (i & 1)) & 1023u);
-    rows_lds_put(to, widen8(r.w[0], r.w[1], sc));
-    rows_lds_put(to + 16, widen8(r.w[2], r.w[3], sc));
+  auto raw_put = [&](const u32x4& x, float sc, uint32_t to, int i) __attribute__((always_inline)) {
+    if (i == kRawDma - 1) {  // (lanes from 32 on: chunk 35 once more)
+      int l = lane;
+      asm volatile("" : "+v"(l));
+      to -= 32 * max((l >> 3) - 3, 0);
+    }
+    rows_lds_put(to + 256 * i, widen8(x[0], x[1], sc));
+    rows_lds_put(to + 256 * i + 16, widen8(x[2], x[3], sc));
   };
   auto tile_of = [&](int k) __attribute__((always_inline)) {
     return F8 ? (int)((unsigned)k % 3u) : k & 3;
   };
   auto widen_block = [&](int k) __attribute__((always_inline)) {
-    const uint32_t tile = lds0 + (uint32_t)tile_of(k) * kRowsTileBytes + 16 * kWideRowsT * wave;
+    const uint32_t to = lds0 + (uint32_t)tile_of(k) * kRowsTileBytes + offp[0];
+    const float sc = raw_scale(k);
 #pragma unroll
-    for (int i = 0; i < kRawDma; ++i) raw_put(raw_read(k, i), tile, i);
+    for (int i = 0; i < kRawDma; ++i) raw_put(raw_read(k, i), sc, to, i);
   };
   f32x16 acc[16];
   float m_run = neg_inf();  // reference of the lane's row: its largest score in the first block
@@ -603,9 +597,13 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   auto qk_read = [&](int tile, int u) __attribute__((always_inline)) {
     return arow0[tile * kTileChunks + 2 * u];
   };
-  auto qk_link = [&](f32x16& sc, const u32x4& kr, int u) __attribute__((always_inline)) {
+  auto last_query = [&]() __attribute__((always_inline)) {
+    if constexpr (F8) return rows_lds_b128(lds0 + R::kQuery + 16 * tid);
+    else return qb[35];
+  };
+  auto qk_link = [&](f32x16& sc, const u32x4& kr, int u, const u32x4& last) __attribute__((always_inline)) {
     if (u == 0) qk_first(sc, kr, qb[0]);
-    else qk_next(sc, kr, qb[u]);
+    else qk_next(sc, kr, u == 35 ? last : qb[u]);
   };
   auto vbase = [&](int tile) __attribute__((always_inline)) {
     uint32_t vl = v_lane;
@@ -729,19 +727,22 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     if (__builtin_expect(odd, 0)) clean(kk);
     if constexpr (F8) rows_wait<kPer>();  // block kk + 2's loads
     const Dma d = issue_begin(kk + (F8 ? 4 : 3));
-    const uint32_t to = lds0 + (uint32_t)tile_of(kk + 2) * kRowsTileBytes + 16 * kWideRowsT * wave;
+    const uint32_t to = lds0 + (uint32_t)tile_of(kk + 2) * kRowsTileBytes + offp[0];
     f32x16 sc;
-    u32x4 kr[5], va[4], pb[2];
-    Raw raw[2];
+    constexpr int kLead = F8 ? 3 : 4;  // links that an operand is read ahead
+    u32x4 kr[kLead + 1], va[4], pb[2], raw, last;
+    float rs = 1.f;
+    if constexpr (F8) rs = raw_scale(kk + 2);
     const uint32_t vt = vbase(tp);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) kr[u] = qk_read(tq, u);
+    for (int u = 0; u < kLead; ++u) kr[u] = qk_read(tq, u);
 #pragma unroll
     for (int m = 0; m < 3; ++m) va[m] = vread(vt, m);
 #pragma unroll
     for (int u = 0; u < 36; ++u) {
-      if (u + 4 < 36) kr[(u + 4) % 5] = qk_read(tq, u + 4);
-      qk_link(sc, kr[u % 5], u);
+      if (u + kLead < 36) kr[(u + kLead) % (kLead + 1)] = qk_read(tq, u + kLead);
+      if (u == 32) last = last_query();
+      qk_link(sc, kr[u % (kLead + 1)], u, last);
       if (u < 4) {
         soft_p(xa, pb[0], u);
       } else if ((u - 4) % 4 != 3) {
@@ -751,8 +752,8 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
         if (m < 16 && (m & 3) == 1) soft_p(xh, pb[1], m >> 2);
       }
       if constexpr (F8) {
-        if (u % 5 == 0 && u / 5 < kRawDma) raw[(u / 5) & 1] = raw_read(kk + 2, u / 5);
-        if (u % 5 == 3 && u / 5 < kRawDma) raw_put(raw[(u / 5) & 1], to, u / 5);
+        if (u % 5 == 0 && u / 5 < kRawDma) raw = raw_read(kk + 2, u / 5);
+        if (u % 5 == 3 && u / 5 < kRawDma) raw_put(raw, rs, to, u / 5);
         if (u >= 5 * kRawDma && u < 5 * kRawDma + kPer) dma_one(d, u - 5 * kRawDma);
       } else {
         if (u % 4 == 2) dma_one(d, u / 4);
@@ -811,12 +812,13 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
       {
         f32x16 sc;
         u32x4 kr[5];
+        const u32x4 last = last_query();
 #pragma unroll
         for (int u = 0; u < 4; ++u) kr[u] = qk_read(0, u);
 #pragma unroll
         for (int u = 0; u < 36; ++u) {
           if (u + 4 < 36) kr[(u + 4) % 5] = qk_read(0, u + 4);
-          qk_link(sc, kr[u % 5], u);
+          qk_link(sc, kr[u % 5], u, last);
         }
         qk_settle(sc);
         odd = soft_x(0, sc, xa, xh, true);
@@ -1030,14 +1032,15 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
   if (nblk > 0) {
     int raw_pid = pt[first_tok() / p.page_size];
     const uint16_t* qrow0 = p.q_nope + w.g_row0 * kRowsC;
-    for (int h = 0; h < 32; ++h)
-      rows_dma16(16 * lane, qrow0 + (size_t)min(h, here - 1) * kRowsC, lds0 + (uint32_t)(h * 65 * 16), 0);
+#pragma clang loop unroll(disable)
+    for (int h = 0; h < here; ++h)
+      rows_dma16(16 * lane, qrow0 + h * kRowsC, lds0 + (uint32_t)(h * 65 * 16), 0);
     const u32x4* pe = (const u32x4*)(p.q_pe + (w.g_row0 + min(n32, here - 1)) * kRowsPe);
 #pragma unroll
     for (int u = 32; u < 36; ++u) qb[u] = pe[4 * ((u - 32) >> 1) + 2 * j2 + (u & 1)];
     asm volatile("s_waitcnt vmcnt(0)" : "+v"(raw_pid) : : "memory");
     set_pids(raw_pid);
-    const u32x4* qs = (const u32x4*)mem + n32 * 65;
+    const u32x4* qs = (const u32x4*)mem + min(n32, here - 1) * 65;
 #pragma unroll
     for (int u = 0; u < 32; ++u) qb[u] = qs[4 * (u >> 1) + 2 * j2 + (u & 1)];
     if (p.q_sign) {
@@ -1209,6 +1212,7 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
 #pragma unroll
   for (int hc = 0; hc < 2; ++hc) {  // 256 columns at a time
     if (hc > 0) __syncthreads();
+    if (n32 < here)
 #pragma unroll
     for (int c8 = 0; c8 < 8; ++c8)
 #pragma unroll
