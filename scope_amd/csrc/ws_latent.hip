@@ -40,6 +40,7 @@ constexpr int kRunTokens = 4;
 constexpr int kRunChunk = kRunWaves * kRunTokens;
 constexpr int kRunWindow = 16;
 constexpr int kRunGroups = 768;
+constexpr int kRunTurns = 8;  // tokens whose q_pe a workgroup turns there
 
 // Wave sums and maxima of the ROCm device library (DPP sequences; every lane active).
 extern "C" __device__ float __ockl_wfred_add_f32(float);
@@ -59,7 +60,7 @@ struct LatentParams {
   void* pages;
   uint8_t* scale;
   int N, H, num_slots, block_log2, tokens, window;
-  int turn_groups;  // workgroups that turn q_pe (and write, with a scale a token)
+  int run_groups;  // workgroups that write runs, ahead of those that turn q_pe (and write the rest)
   bool weight_f32;
   float eps, factor;
 };
@@ -192,82 +193,98 @@ __device__ __forceinline__ bool lat_slot_ok(const LatentParams& p, int slot) {
   return slot >= 0 && slot < p.num_slots;
 }
 
-// kRunTokens tokens across a wave: lane l holds columns 8 l .. 8 l + 7 of each one's c, and
-// lane 4 t + q (t < kRunTokens) quarter q of token t's pe, turned.
-struct Latents {
-  float c[kRunTokens][8];
-  float pe[16];
+// kRunTokens tokens across a wave, as they are: lane l holds columns 8 l .. 8 l + 7 of each
+// one's c and its norm's factor, and lane 4 t + q (t < kRunTokens) quarter q of token t's pe.
+struct Run {
+  u32x4 c[kRunTokens];
+  u32x4 pe[2];
+  float r[kRunTokens];
 };
-// Tokens tok .. tok + n - 1 (the last one again past those).  s_cs: the wave's part of LDS.
+// Tokens tok .. tok + n - 1 (the last one again past those), and their angles to s_cs, the
+// wave's part of LDS.
 template <bool ADJACENT>
-__device__ __forceinline__ void lat_load_run(const LatentParams& p, int tok, int n, const float* weight,
-                                             float2* s_cs, Latents& x) {
-  const int lane = threadIdx.x & 63;
-  u32x4 wc[kRunTokens];
+__device__ __forceinline__ void run_load(const LatentParams& p, int tok, int n, float2* s_cs, Run& x) {
+  const int lane = threadIdx.x & 63, q = lane & 3;
 #pragma unroll
   for (int t = 0; t < kRunTokens; ++t)
-    wc[t] = *(const u32x4*)(p.c + (size_t)(tok + min(t, n - 1)) * p.c_stride + 8 * lane);
-  u32x4 wa = {0, 0, 0, 0}, wb = {0, 0, 0, 0};
-  const int q = lane & 3;
+    x.c[t] = *(const u32x4*)(p.c + (size_t)(tok + min(t, n - 1)) * p.c_stride + 8 * lane);
+  x.pe[0] = x.pe[1] = u32x4{0, 0, 0, 0};
   if (lane < 4 * kRunTokens) {
     const uint16_t* pe = p.pe + (size_t)(tok + min(lane >> 2, n - 1)) * p.pe_stride;
-    wa = *(const u32x4*)(pe + PeCols<ADJACENT>::first(q));
-    wb = *(const u32x4*)(pe + PeCols<ADJACENT>::second(q));
+    x.pe[0] = *(const u32x4*)(pe + PeCols<ADJACENT>::first(q));
+    x.pe[1] = *(const u32x4*)(pe + PeCols<ADJACENT>::second(q));
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the angles before are read)
-#pragma unroll
-  for (int i = 0; i < kRunTokens * kLatPairs; i += 64) {
-    const int t = (i + lane) / kLatPairs;
-    s_cs[i + lane] = lat_angle(p, tok + min(t, n - 1), (i + lane) % kLatPairs);
-  }
+#pragma unroll 1
+  for (int i = lane; i < kRunTokens * kLatPairs; i += 64)
+    s_cs[i] = lat_angle(p, tok + min(i / kLatPairs, n - 1), i % kLatPairs);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-  for (int t = 0; t < kRunTokens; ++t) lat_unpack8(wc[t], x.c[t]);
-  if (p.weight) {
-    float sum[kRunTokens];
+  for (int t = 0; t < kRunTokens; ++t) x.r[t] = 1.f;
+  if (!p.weight) return;
 #pragma unroll
-    for (int t = 0; t < kRunTokens; ++t) {
-      sum[t] = 0.f;
+  for (int t = 0; t < kRunTokens; ++t) {
+    float v[8];
+    lat_unpack8(x.c[t], v);
+    float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[t] = fmaf(x.c[t][i], x.c[t][i], sum[t]);
-    }
-#pragma unroll
-    for (int t = 0; t < kRunTokens; ++t) sum[t] = __ockl_wfred_add_f32(sum[t]);
-#pragma unroll
-    for (int t = 0; t < kRunTokens; ++t) {
-      const float r = 1.f / sqrtf(sum[t] * (1.f / kLatC) + p.eps);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x.c[t][i] = x.c[t][i] * r * weight[i];
-    }
+    for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
+    x.r[t] = sum;
   }
-  lat_unpack8(wa, x.pe);
-  lat_unpack8(wb, x.pe + 8);
-  if (lane < 4 * kRunTokens) lat_turn<ADJACENT>(x.pe, s_cs + (lane >> 2) * kLatPairs + 8 * q);
+#pragma unroll
+  for (int t = 0; t < kRunTokens; ++t)
+    x.r[t] = 1.f / sqrtf(__ockl_wfred_add_f32(x.r[t]) * (1.f / kLatC) + p.eps);
+}
+// Eight columns of token t's c, normalised; the lane's sixteen columns of pe, turned.
+__device__ __forceinline__ void run_c(const Run& x, int t, const float* weight, float* v) {
+  lat_unpack8(x.c[t], v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = v[i] * x.r[t] * weight[i];
 }
 template <bool ADJACENT>
-__device__ __forceinline__ void lat_put_run(const LatentParams& p, int tok, int n, const Latents& x,
-                                            float s) {
+__device__ __forceinline__ void run_pe(const Run& x, const float2* s_cs, float* v) {
   const int lane = threadIdx.x & 63;
+  lat_unpack8(x.pe[0], v);
+  lat_unpack8(x.pe[1], v + 8);
+  if (lane < 4 * kRunTokens) lat_turn<ADJACENT>(v, s_cs + (lane >> 2) * kLatPairs + 8 * (lane & 3));
+}
+template <bool ADJACENT>
+__device__ __forceinline__ uint32_t run_top(const Run& x, const float* weight, const float2* s_cs) {
+  float v[16];
+  run_pe<ADJACENT>(x, s_cs, v);
+  uint32_t top = lat_top<16>(v, 0u);  // (lanes past the tokens hold zeros)
+#pragma unroll
+  for (int t = 0; t < kRunTokens; ++t) {
+    run_c(x, t, weight, v);
+    top = lat_top<8>(v, top);
+  }
+  return top;
+}
+template <bool ADJACENT>
+__device__ __forceinline__ void run_put(const LatentParams& p, int tok, int n, const Run& x, const float* weight,
+                                        const float2* s_cs, float s) {
+  const int lane = threadIdx.x & 63;
+  float v[16];
 #pragma unroll
   for (int t = 0; t < kRunTokens; ++t) {
     if (t >= n) break;
+    run_c(x, t, weight, v);
     uint8_t* row = (uint8_t*)p.pages + (size_t)p.slots[tok + t] * kLatW;
-    *(uint2*)(row + 8 * lane) = make_uint2(lat_pack4(x.c[t], s), lat_pack4(x.c[t] + 4, s));
+    *(uint2*)(row + 8 * lane) = make_uint2(lat_pack4(v, s), lat_pack4(v + 4, s));
   }
+  run_pe<ADJACENT>(x, s_cs, v);
   if (lane < 4 * n) {
     const int q = lane & 3;
     uint8_t* row = (uint8_t*)p.pages + (size_t)p.slots[tok + (lane >> 2)] * kLatW + kLatC;
-    *(uint2*)(row + PeCols<ADJACENT>::first(q)) = make_uint2(lat_pack4(x.pe, s), lat_pack4(x.pe + 4, s));
-    *(uint2*)(row + PeCols<ADJACENT>::second(q)) =
-        make_uint2(lat_pack4(x.pe + 8, s), lat_pack4(x.pe + 12, s));
+    *(uint2*)(row + PeCols<ADJACENT>::first(q)) = make_uint2(lat_pack4(v, s), lat_pack4(v + 4, s));
+    *(uint2*)(row + PeCols<ADJACENT>::second(q)) = make_uint2(lat_pack4(v + 8, s), lat_pack4(v + 12, s));
   }
 }
 
 // With a scale for several tokens, a workgroup takes the run of tokens from tok on whose
 // slots lie in one block, if tok is the run's first: the block's tokens follow one another in
 // a call, so nobody else writes the block.  Two looks at the tokens: their largest magnitude,
-// then their values (the first kRunChunk tokens from the registers, others from the cache
-// again).  (A wave for every fourth token, one at a time, and read again: 4651 tokens to
+// then their values (up to kRunChunk tokens from the registers, more from the cache again).  (A wave for every fourth token, one at a time, and read again: 4651 tokens to
 // blocks of 32 53.7 us.)
 //
 // at: the lane of the run's first token in `slots`, which holds the slots of tokens base +
@@ -300,29 +317,23 @@ __device__ void lat_block(const LatentParams& p, int base, int at, int slots, fl
   __syncthreads();  // (the run before is done with s_top and the scale)
   if (tid == 0) *s_top = 0;
   __syncthreads();
-  Latents keep;
+  Run x;
   const int own = kRunTokens * wave;  // the wave's first token of a chunk
+  const bool once = count <= kRunChunk;
   uint32_t top = 0;
   for (int i = own; i < count; i += kRunChunk) {
-    Latents x;
-    lat_load_run<ADJACENT>(p, tok + i, min(count - i, kRunTokens), w, s_cs, x);
-    uint32_t m = lat_top<16>(x.pe, 0u);  // (lanes past the tokens hold zeros of pe)
-#pragma unroll
-    for (int t = 0; t < kRunTokens; ++t) m = lat_top<8>(x.c[t], m);
-    top = max(top, m);
-    if (i == own) keep = x;
+    run_load<ADJACENT>(p, tok + i, min(count - i, kRunTokens), s_cs, x);
+    top = max(top, run_top<ADJACENT>(x, w, s_cs));
   }
   top = __ockl_wfred_max_u32(top);
   if (lane == 0) atomicMax(s_top, (int)top);
   __syncthreads();
   const int byte = max(lat_byte((uint32_t)*s_top), had);
   const float s = lat_inverse(byte);
-  if (own < count) lat_put_run<ADJACENT>(p, tok + own, min(count - own, kRunTokens), keep, s);
-  for (int i = own + kRunChunk; i < count; i += kRunChunk) {
-    Latents x;
+  for (int i = own; i < count; i += kRunChunk) {
     const int n = min(count - i, kRunTokens);
-    lat_load_run<ADJACENT>(p, tok + i, n, w, s_cs, x);
-    lat_put_run<ADJACENT>(p, tok + i, n, x, s);
+    if (!once) run_load<ADJACENT>(p, tok + i, n, s_cs, x);
+    run_put<ADJACENT>(p, tok + i, n, x, w, s_cs, s);
   }
   if (byte > had && first > 0) {  // the older tokens at the new scale
     const float f = ldexpf(1.f, had - byte);
@@ -341,13 +352,13 @@ __device__ void lat_block(const LatentParams& p, int base, int at, int slots, fl
 
 // RUNS: 8-bit pages with a scale for several tokens.
 template <bool ADJACENT, bool RUNS>
-__global__ __launch_bounds__(RUNS ? 64 * kRunWaves : 256) void latent_append_kernel(const LatentParams p) {
+__global__ __launch_bounds__(RUNS ? 64 * kRunWaves : 256, RUNS ? 4 : 1) void latent_append_kernel(const LatentParams p) {
   constexpr int kThreads = RUNS ? 64 * kRunWaves : 256;
   __shared__ float2 s_cs[(RUNS ? kRunChunk : kLatTokens) * kLatPairs];
   __shared__ int s_top;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (RUNS && (int)blockIdx.x >= p.turn_groups) {
-    const int base = ((int)blockIdx.x - p.turn_groups) * p.window - 1;
+  if (RUNS && (int)blockIdx.x < p.run_groups) {
+    const int base = (int)blockIdx.x * p.window - 1;
     const int t = base + lane;
     const int slots = t >= 0 && t < p.N ? p.slots[t] : -1;
     const int prev = __shfl_up(slots, 1);
@@ -359,7 +370,7 @@ __global__ __launch_bounds__(RUNS ? 64 * kRunWaves : 256) void latent_append_ker
       lat_block<ADJACENT>(p, base, __builtin_ctzll(begins), slots, s_cs, &s_top);
     return;
   }
-  const int t0 = (int)blockIdx.x * p.tokens;
+  const int t0 = ((int)blockIdx.x - (RUNS ? p.run_groups : 0)) * p.tokens;
   const int nt = min(p.tokens, p.N - t0);
   if (tid < nt * kLatPairs)
     s_cs[tid] = lat_angle(p, t0 + tid / kLatPairs, tid % kLatPairs);
@@ -572,11 +583,12 @@ extern "C" int ws_latent_rope_append(const uint16_t* c, int64_t c_stride, const 
   p.H = H;
   p.num_slots = num_pages * page_size;
   // a token a workgroup while there are few, four once those fill the chip
-  p.tokens = N >= 2048 ? kLatTokens : 1;
-  p.turn_groups = (N + p.tokens - 1) / p.tokens;
   const bool runs = latent_scale && p.block_log2 > 0;
+  p.tokens = N < 2048 ? 1 : runs ? kRunTurns : kLatTokens;
+  const int turn_groups = (N + p.tokens - 1) / p.tokens;
   p.window = std::min(std::max(N / kRunGroups, 1), kRunWindow);
-  const long long grid = (long long)p.turn_groups + (runs ? (N + p.window - 1) / p.window : 0);
+  p.run_groups = runs ? (N + p.window - 1) / p.window : 0;
+  const long long grid = (long long)turn_groups + p.run_groups;
   const int threads = runs ? 64 * kRunWaves : 256;
   if (grid * threads >= (1LL << 32))
     return set_error(WS_EINVAL, "%s: %d tokens exceed the launch grid", name, N);

@@ -1460,9 +1460,24 @@ def gqa_prompt(q, k_pages, v_pages, page_table, kv_len, cu_new, scale, max_len, 
 # the same path over latent pages (absorbed MLA)
 
 
+def _fine(t, dtype, idx, shape) -> bool:
+    """Whether t is a contiguous tensor of that type, GPU and shape (a check's quick way)."""
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == idx and t.shape == shape
+            and t.is_contiguous())
+
+
 def _latent_pool(latent_pages, latent_scale, dev):
     """(num_pages, page_size, block) of a bf16 latent pool (block 0), or of an 8-bit
     one with its scales."""
+    dtype = torch.bfloat16 if latent_scale is None else E4M3
+    if (isinstance(latent_pages, torch.Tensor) and latent_pages.dtype is dtype and latent_pages.dim() == 3
+            and latent_pages.get_device() == dev.index and latent_pages.is_contiguous()):
+        P, PS, L = latent_pages.shape  # (as below, in one pass while all is well)
+        if L == MLA_LATENT:
+            if latent_scale is None:
+                return P, PS, 0
+            if _fine(latent_scale, E8M0, dev.index, (P, PS)):
+                return P, PS, 1
     _require(latent_pages, "latent_pages", torch.bfloat16 if latent_scale is None else E4M3, dev, 3)
     P, PS, L = latent_pages.shape
     if L != MLA_LATENT:
@@ -1480,6 +1495,11 @@ def _latent_pool(latent_pages, latent_scale, dev):
 
 def _latent_rows(t, name, dev, N, width):
     """The row stride of a [N, width] bf16 operand whose rows may be strided."""
+    if (N > 1 and isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.get_device() == dev.index
+            and t.shape == (N, width)):  # (as below, in one pass while all is well)
+        stride, unit = t.stride()
+        if unit == 1:
+            return stride
     _require(t, name, torch.bfloat16, dev, 2, contiguous=False)
     if t.shape != (N, width) or (N > 0 and t.stride(1) != 1):
         raise ValueError(f"{name} must be [{N}, {width}] with unit last stride "
@@ -1500,22 +1520,29 @@ def latent_rope_append(c, pe, q_pe, positions, inv_freq, slots, latent_pages, la
     another in a call.  A slot outside the pool (-1) writes nothing; slots must
     differ.  adjacent and factor as rope()'s.  Returns q_out [N, H, 64]."""
     dev = _gpu(c, "c")
-    _require(q_pe, "q_pe", torch.bfloat16, dev, 3, contiguous=False)
+    idx = dev.index
+    if not (isinstance(q_pe, torch.Tensor) and q_pe.dtype is torch.bfloat16 and q_pe.get_device() == idx
+            and q_pe.dim() == 3):
+        _require(q_pe, "q_pe", torch.bfloat16, dev, 3, contiguous=False)
     N, H, W = q_pe.shape
     c_stride, pe_stride = _latent_rows(c, "c", dev, N, MLA_C), _latent_rows(pe, "pe", dev, N, MLA_PE)
-    if W != MLA_PE or H == 0 or (N > 0 and q_pe.stride(2) != 1):
+    q_stride, q_head, unit = q_pe.stride()
+    if W != MLA_PE or H == 0 or (N > 0 and unit != 1):
         raise ValueError(f"q_pe must be [{N}, H, {MLA_PE}] with unit last stride (got {tuple(q_pe.shape)}, "
                          f"strides {q_pe.stride()})")
-    q_head = q_pe.stride(1) if H > 1 else MLA_PE
-    q_stride = q_pe.stride(0) if N > 1 else H * q_head
-    _require(positions, "positions", torch.int32, dev, 1)
-    _require(slots, "slots", torch.int32, dev, 1)
-    _require(inv_freq, "inv_freq", torch.float32, dev, 1)
-    if positions.shape[0] != N or slots.shape[0] != N or inv_freq.shape[0] != MLA_PE // 2:
+    if H == 1:
+        q_head = MLA_PE
+    if N <= 1:
+        q_stride = H * q_head
+    if not (_fine(positions, torch.int32, idx, (N,)) and _fine(slots, torch.int32, idx, (N,))
+            and _fine(inv_freq, torch.float32, idx, (MLA_PE // 2,))):
+        _require(positions, "positions", torch.int32, dev, 1)
+        _require(slots, "slots", torch.int32, dev, 1)
+        _require(inv_freq, "inv_freq", torch.float32, dev, 1)
         raise ValueError(f"positions and slots must be [{N}] and inv_freq [{MLA_PE // 2}]")
     P, PS, block = _latent_pool(latent_pages, latent_scale, dev)
     f32 = 0
-    if norm_weight is not None:
+    if norm_weight is not None and not _fine(norm_weight, torch.bfloat16, idx, (MLA_C,)):
         f32 = int(isinstance(norm_weight, torch.Tensor) and norm_weight.dtype == torch.float32)
         _require(norm_weight, "norm_weight", torch.float32 if f32 else torch.bfloat16, dev, 1)
         if norm_weight.shape[0] != MLA_C:
@@ -1546,20 +1573,22 @@ def latent_gather(latent_pages, page_table, cu_rows, n_rows, start=None, latent_
     dev = _gpu(latent_pages, "latent_pages")
     P, PS, block = _latent_pool(latent_pages, latent_scale, dev)
     _require(page_table, "page_table", torch.int32, dev, 2)
-    _require(cu_rows, "cu_rows", torch.int32, dev, 1)
     B, N = page_table.shape[0], int(n_rows)
-    if cu_rows.shape[0] != B + 1 or N < 0:
+    if N < 0 or not _fine(cu_rows, torch.int32, dev.index, (B + 1,)):
+        _require(cu_rows, "cu_rows", torch.int32, dev, 1)
         raise ValueError("cu_rows must be [B + 1] for page_table's B rows, and n_rows >= 0")
-    if start is not None:
+    if start is not None and not _fine(start, torch.int32, dev.index, (B,)):
         _require(start, "start", torch.int32, dev, 1)
-        if start.shape[0] != B:
-            raise ValueError("start must be [B]")
+        raise ValueError("start must be [B]")
+    c_stride, pe_stride = MLA_C, MLA_PE
     if c_out is None:
         c_out = torch.empty((N, MLA_C), dtype=torch.bfloat16, device=dev)
+    else:
+        c_stride = _latent_rows(c_out, "c_out", dev, N, MLA_C)
     if pe_out is None:
         pe_out = torch.empty((N, MLA_PE), dtype=torch.bfloat16, device=dev)
-    c_stride = _latent_rows(c_out, "c_out", dev, N, MLA_C)
-    pe_stride = _latent_rows(pe_out, "pe_out", dev, N, MLA_PE)
+    else:
+        pe_stride = _latent_rows(pe_out, "pe_out", dev, N, MLA_PE)
     if N == 0 or B == 0:
         return c_out, pe_out
     _run("ws_latent_gather", dev, _ptr(latent_pages), _ptr(latent_scale), block, _ptr(page_table),
@@ -1623,8 +1652,8 @@ def _mla8_decode(name, dtype, q_nope, q_pe, latent_pages, latent_scale, page_tab
         raise TypeError("latent_scale must be a tensor")
     P, PS, block = _latent_pool(latent_pages, latent_scale, dev)
     B, H = _latent_queries(q_nope, q_pe, page_table, dev)
-    _require(gpu_len, "gpu_len", torch.int32, dev, 1)
-    if page_table.shape[0] != B or gpu_len.shape[0] != B:
+    if page_table.shape[0] != B or not _fine(gpu_len, torch.int32, dev.index, (B,)):
+        _require(gpu_len, "gpu_len", torch.int32, dev, 1)
         raise ValueError("page_table/gpu_len batch mismatch")
     out, lse = _latent_out(out, lse, B, H, dtype, dev, name="out" if dtype == torch.float32 else "out_bf16")
     if B == 0:
@@ -1667,10 +1696,10 @@ def mla_prompt(q_nope, q_pe, latent_pages, page_table, kv_len, cu_new, scale, ma
     dev = _gpu(q_nope, "q_nope")
     P, PS, block = _latent_pool(latent_pages, latent_scale, dev)
     N, H = _latent_queries(q_nope, q_pe, page_table, dev)
-    _require(kv_len, "kv_len", torch.int32, dev, 1)
-    _require(cu_new, "cu_new", torch.int32, dev, 1)
     B = page_table.shape[0]
-    if kv_len.shape[0] != B or cu_new.shape[0] != B + 1:
+    if not (_fine(kv_len, torch.int32, dev.index, (B,)) and _fine(cu_new, torch.int32, dev.index, (B + 1,))):
+        _require(kv_len, "kv_len", torch.int32, dev, 1)
+        _require(cu_new, "cu_new", torch.int32, dev, 1)
         raise ValueError("kv_len must be [B] and cu_new [B + 1] for page_table's B rows")
     dtype = out_dtype if out is None else getattr(out, "dtype", None)
     if dtype not in (torch.bfloat16, torch.float32):
