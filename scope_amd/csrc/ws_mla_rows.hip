@@ -45,6 +45,22 @@ constexpr int kRowsTile = 128;       // rows of a tile, 32 a wave (mla_few_kerne
 constexpr int kRowsMaxSplits = 256;  // of a tile
 constexpr int kRowsMinShare = 4;     // blocks of a split, at the least
 
+// Division by a number that the host knows: n / d = n m >> s for 0 <= n < 2^31, with 2^k the
+// least power of two >= d, m = floor(2^(31 + k) / d) + 1 (2^31 for d = 1) and s = 31 + k: m d
+// exceeds 2^s by at most d <= 2^k, which n < 2^31 keeps below a unit of the quotient.  A
+// division by a variable takes some 40 instructions, a quarter of a workgroup's start.
+struct Divisor {
+  uint32_t m, s;
+};
+static Divisor divisor(uint32_t d) {
+  uint32_t k = 0;
+  while ((1ull << k) < d) ++k;
+  return Divisor{d == 1 ? 1u << 31 : (uint32_t)((1ull << (31 + k)) / d + 1), 31 + k};
+}
+__device__ __forceinline__ int quotient(int n, const Divisor& d) {
+  return (int)(((unsigned long long)(unsigned)n * d.m) >> d.s);
+}
+
 struct RowsParams {
   const uint16_t* q_nope;
   const uint16_t* q_pe;
@@ -65,7 +81,9 @@ struct RowsParams {
   bool join_shared;
   int pieces;     // room for them
   int piece_rows;
-  int tile;       // rows of a tile
+  int tile;       // rows of a tile (a power of two)
+  int tile_log2;
+  Divisor by_H, by_page;
   float scale_log2;  // > 0
   uint32_t q_sign;   // 0x80008000 where the caller's scale is negative
 };
@@ -85,7 +103,7 @@ __device__ __forceinline__ RowsSeq rows_seq(const RowsParams& p, int b) {
     s.n = min(max(p.cu_new[b + 1], s.c0), p.N) - s.c0;
   }
   s.len = p.kv_len[b];
-  s.tiles = (s.n * p.H + p.tile - 1) / p.tile;
+  s.tiles = (int)((unsigned)(s.n * p.H + p.tile - 1) >> p.tile_log2);
   s.blocks = len_ok(s.len, 0, p.cap) ? (s.len + 31) / 32 : 0;
   return s;
 }
@@ -99,8 +117,7 @@ struct RowsPlace {
 };
 
 // Wave sums and maxima of the ROCm device library (DPP sequences; every lane active).
-extern "C" __device__ unsigned long long __ockl_wfred_add_u64(unsigned long long);
-extern "C" __device__ int __ockl_wfred_max_i32(int);
+extern "C" __device__ float __ockl_wfred_add_f32(float);
 
 // Item `at` of the list of all tiles' splits (TILES: of the split tiles): where the items do
 // not fit the chip at once, longest sequences first (up to 64 of them), their last tile first.  A tile has one split for every M of
@@ -130,15 +147,15 @@ __device__ __forceinline__ RowsPlace rows_place_n(const RowsParams& p, int at) {
   const int mine = PER > 0 ? PER : max(min(per, p.B - b0), 0);
   float rM = 0.f;
   if (p.n_splits == 0) {
-    unsigned long long sum = 0;
+    float sum = 0.f;
     int tiles = 0;
 #pragma unroll 4
     for (int k = 0; k < mine; ++k) {
       const RowsSeq s = seq(k);
-      sum += (unsigned long long)s.tiles * (unsigned)s.blocks;
+      sum = fmaf((float)s.tiles, (float)s.blocks, sum);  // (the same in every kernel)
       tiles += s.tiles;
     }
-    const float total = (float)__ockl_wfred_add_u64(sum);
+    const float total = __ockl_wfred_add_f32(sum);
     auto blocks_at = [&](int places) {
       return (int)fminf(ceilf(fmaxf(total * __builtin_amdgcn_rcpf((float)max(places, 1)), (float)kRowsMinShare)),
                         1e9f);
@@ -185,9 +202,13 @@ __device__ __forceinline__ RowsPlace rows_place_n(const RowsParams& p, int at) {
   int from = lane;  // the lane whose sequences stand at this lane's place in the list
   if (!TILES && PER == 1 && !p.fit && p.B > 1) {  // (splits that fit once are alike)
     int rank = 0;
-    for (int j = 0; j < p.B; ++j) {
-      const int other = __builtin_amdgcn_readlane(key, j);
-      rank += other > key || (other == key && j < lane) ? 1 : 0;
+    const int mark = lane < p.B ? key : -1;  // (no sequence: behind the others)
+    for (int j0 = 0; j0 < p.B; j0 += 8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int other = __builtin_amdgcn_readlane(mark, j0 + j);
+        rank += other > mark || (other == mark && j0 + j < lane) ? 1 : 0;
+      }
     }
     if (lane >= p.B) rank = lane;
     from = __builtin_amdgcn_ds_permute(4 * rank, lane);
@@ -276,6 +297,7 @@ struct RowsRing {
   static constexpr int kQuery = kScales + (F8 ? 4 * 2 * 256 : 0);
   static constexpr int kLds = kQuery + (F8 ? 256 * 16 : 0);
 };
+static_assert(kRowsTile == 1 << 7, "tile_log2");
 static_assert(RowsRing<true>::kLds <= 160 * 1024 - 64 && RowsRing<false>::kLds <= 160 * 1024 - 64, "LDS");
 static_assert(RowsRing<true>::kScales >= kRowsTile * 65 * 16, "the queries are staged in the tiles");
 
@@ -369,8 +391,9 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, RowsWork& w) {
   w.len_good = len_ok(pl.len, 0, p.cap);
   w.first_pos = pl.len - pl.n;  // position of the sequence's first query
   // tokens that the tile's first row and its last one see
-  w.lim_lo = w.first_pos + w.row0 / p.H + 1;
-  const int lim_hi = w.len_good ? max(w.first_pos + (w.row0 + w.here - 1) / p.H + 1, 0) : 0;
+  w.lim_lo = w.first_pos + quotient(w.row0, p.by_H) + 1;
+  const int lim_hi =
+      w.len_good ? max(w.first_pos + quotient(w.row0 + w.here - 1, p.by_H) + 1, 0) : 0;
   const int nb = (lim_hi + 31) / 32;
   // (nb split / splits without 64 bits: splits is at most kRowsMaxSplits)
   const unsigned each = (unsigned)nb / (unsigned)pl.splits, rest = (unsigned)nb - each * (unsigned)pl.splits;
@@ -414,14 +437,13 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   const int lane = tid & 63;
   const int n32 = lane & 31;  // row of the wave (QK B, PV B, output) or token (A operands)
   const int j2 = lane >> 5;
-  const int H = p.H;
   RowsWork w;
   if (!rows_work(p, w)) return;
   if (tid == 0) s_redo = 0;  // read after the ring's barriers
   const int nblk = w.nblk, t_begin = w.t_begin, t_end = w.t_end, here = w.here;
   const int rows = min(max(here - 32 * wave, 0), 32);  // this wave's
   // the tokens that the lane's row sees (past the rows: the last one again)
-  const int lim_lane = w.first_pos + min(w.row0 + 32 * wave + n32, w.R_all - 1) / H + 1;
+  const int lim_lane = w.first_pos + quotient(min(w.row0 + 32 * wave + n32, w.R_all - 1), p.by_H) + 1;
 
   const uint32_t lds0 =
       (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem);
@@ -466,12 +488,12 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   };
   auto set_pids = [&](int raw) __attribute__((always_inline)) {
     const int t0 = first_tok();
-    const int page = t0 / p.page_size;
+    const int page = quotient(t0, p.by_page);
     const int pid = clamp_page(raw, p.num_pages);
     m_tok = (pid * p.page_size + (t0 - page * p.page_size)) | (raw == pid ? 0 : (int)0x80000000u);
   };
-  auto fetch_pids = [&]() __attribute__((always_inline)) { set_pids(pt[first_tok() / p.page_size]); };
-  int raw_pid = pt[first_tok() / p.page_size];
+  auto fetch_pids = [&]() __attribute__((always_inline)) { set_pids(pt[quotient(first_tok(), p.by_page)]); };
+  int raw_pid = pt[quotient(first_tok(), p.by_page)];
 
   // Q^T of this wave's rows, through LDS a 1 KB row an instruction (row slots of 65 chunks):
   // k-step u holds columns 16 u + 8 j2 .. + 8.
@@ -965,7 +987,7 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
   if (!rows_work(p, w)) return;
   const int t_begin = w.t_begin, t_end = w.t_end, here = w.here;
   const int nblk = max((w.nblk - wave + 3) >> 2, 0);  // this wave's
-  const int lim_lane = w.first_pos + min(w.row0 + n32, w.R_all - 1) / p.H + 1;
+  const int lim_lane = w.first_pos + quotient(min(w.row0 + n32, w.R_all - 1), p.by_H) + 1;
   const uint32_t lds0 = (uint32_t)uniform(
       (int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem + kFewWave * wave));
   char* const mem = s_mem + kFewWave * wave;
@@ -997,7 +1019,7 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
   };
   auto set_pids = [&](int raw) __attribute__((always_inline)) {
     const int t0 = first_tok();
-    const int page = t0 / p.page_size;
+    const int page = quotient(t0, p.by_page);
     const int pid = clamp_page(raw, p.num_pages);
     m_tok = (pid * p.page_size + (t0 - page * p.page_size)) | (raw == pid ? 0 : (int)0x80000000u);
   };
@@ -1006,7 +1028,7 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
   auto issue = [&](int i) __attribute__((always_inline)) {
     if (i - pid_base >= 64) {
       pid_base += 64;
-      set_pids(pt[first_tok() / p.page_size]);
+      set_pids(pt[quotient(first_tok(), p.by_page)]);
     }
     const int tok_raw = __builtin_amdgcn_readlane(m_tok, i - pid_base);
     const uint32_t bit = 1u << (i & 1);
@@ -1030,7 +1052,7 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
   // eight behind them, as a 16-byte read of the latents delivers them.
   u32x4 qb[36];
   if (nblk > 0) {
-    int raw_pid = pt[first_tok() / p.page_size];
+    int raw_pid = pt[quotient(first_tok(), p.by_page)];
     const uint16_t* qrow0 = p.q_nope + w.g_row0 * kRowsC;
 #pragma clang loop unroll(disable)
     for (int h = 0; h < here; ++h)
@@ -1165,7 +1187,7 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
     if (nblk == 0) break;
     if (pid_base != 0) {
       pid_base = 0;
-      set_pids(pt[first_tok() / p.page_size]);
+      set_pids(pt[quotient(first_tok(), p.by_page)]);
     }
     issue(0);
     if (nblk > 1) issue(1);
@@ -1501,6 +1523,9 @@ static int rows_run(const char* name, const uint16_t* q_nope, const uint16_t* q_
   p.pieces = (int)pl.pieces;
   p.piece_rows = pl.piece_rows;
   p.tile = pl.tile;
+  p.tile_log2 = pl.few ? 5 : 7;
+  p.by_H = divisor((uint32_t)H);
+  p.by_page = divisor((uint32_t)page_size);
   p.join_shared = pl.pieces >= 12 * pl.tiles;
   // the smallest normal float for 0: every finite score then rounds to the same
   // probability, and masked tokens stay -inf
@@ -1517,6 +1542,7 @@ static int rows_run(const char* name, const uint16_t* q_nope, const uint16_t* q_
     p.latent = copy;
     p.page_table = table;
     p.page_size = p.cap = pl.pad;  // (a length past max_len, which the call rules out, is NaN)
+    p.by_page = divisor((uint32_t)pl.pad);
     p.max_pages = 1;
     p.num_pages = B;
   }
