@@ -33,8 +33,11 @@ constexpr int kLatW = kLatC + kLatPe;
 constexpr int kLatPairs = kLatPe / 2;
 constexpr int kLatTokens = 4;  // most tokens of a workgroup, one a wave
 // With a scale for several tokens: waves of a workgroup, tokens a wave takes at a time (in
-// registers between the two looks at them), the most tokens whose runs a workgroup looks for,
-// and the workgroups of a call where it takes more than one (two a CU fit at a time).
+// registers between the two looks at them), and the tokens whose runs a workgroup looks for: as
+// many as leave kRunGroups workgroups (one for each token: 780 tokens 10.7 us instead of 8.1,
+// 1200 15.5 instead of 10.3; 384 to 1024 workgroups are alike on average), up to kRunWindow or, with scales of 32 tokens and more, twice
+// that (16000 tokens of 4 sequences: 29.7 us instead of 34; with scales of 2 tokens 132 instead
+// of 116).
 constexpr int kRunWaves = 8;
 constexpr int kRunTokens = 4;
 constexpr int kRunChunk = kRunWaves * kRunTokens;
@@ -432,7 +435,8 @@ struct GatherParams {
 constexpr int kGatherRows = 32;   // most rows of a workgroup
 constexpr int kGatherParts = 36;  // 16-column parts of a row
 
-// A workgroup takes p.rows rows: their places first (a thread a row, the sequence by bisection
+// A workgroup takes p.rows rows (8, or 32 once those fill the chip: 4000 rows of 8 bits 4.6 and
+// 5.5 us, 36000 16.5 and 14.4; 16000 of bf16 9.6 and 8.6): their places first (a thread a row, the sequence by bisection
 // over cu in LDS), then 16 columns a thread.
 template <bool F8>
 __global__ __launch_bounds__(256) void latent_gather_kernel(const GatherParams p) {
@@ -582,11 +586,13 @@ extern "C" int ws_latent_rope_append(const uint16_t* c, int64_t c_stride, const 
   p.N = N;
   p.H = H;
   p.num_slots = num_pages * page_size;
-  // a token a workgroup while there are few, four once those fill the chip
+  // A token a workgroup while there are few, four (with runs: eight) once those fill the chip
+  // (1024 tokens, 16 heads: 4.1 and 4.2 us, 4096: 8.0 and 7.4, with runs 18.6 and 12.9; 1024
+  // tokens of 128 heads: 8.6 and 10.5).
   const bool runs = latent_scale && p.block_log2 > 0;
   p.tokens = N < 2048 ? 1 : runs ? kRunTurns : kLatTokens;
   const int turn_groups = (N + p.tokens - 1) / p.tokens;
-  p.window = std::min(std::max(N / kRunGroups, 1), kRunWindow);
+  p.window = std::min((N + kRunGroups - 1) / kRunGroups, p.block_log2 >= 5 ? 2 * kRunWindow : kRunWindow);
   p.run_groups = runs ? (N + p.window - 1) / p.window : 0;
   const long long grid = (long long)turn_groups + p.run_groups;
   const int threads = runs ? 64 * kRunWaves : 256;
