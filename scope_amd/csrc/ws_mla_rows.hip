@@ -934,13 +934,15 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   }
 }
 
-// 8-bit pages under few rows (at most 32 of a sequence, on average): a tile is one wave's 32
-// rows, the four waves take every fourth block of its tokens each, and their sums meet in LDS
-// at the end.  With 16 rows the products are small beside the loads, so what counts is that
-// each wave keeps a block on its way while it works on another, without a barrier: a block
-// takes a wave about 5000 cycles, the HBM 4 x 1900.  The latents are widened where they are
+// 8-bit pages under few rows (kFewRows): a tile is one wave's 32 rows, the four waves take
+// every fourth block of its tokens each, and their sums meet in LDS at the end.  With 16 rows
+// the products are small beside the loads, so what counts is that each wave keeps a block on
+// its way while it works on another, without a barrier: a block takes a wave 5200 cycles,
+// 1300 of the CU, the HBM some 2000 of its share.  The latents are widened where they are
 // read: the scores' operand by its token's scale, the values' operand as it is, with the
-// scale on the token's probability.
+// scale on the token's probability.  Bound by HBM in long batches (16 sequences of 3000 to
+// 32768 tokens, 16 heads: 193 MB in 41 us, 4.7 TB/s), by one chain of loads, a block and the
+// merge in short ones (one of 8192: 11.8 us).
 constexpr int kFewTile = 32;
 constexpr int kFewDma = 19;  // 1 KB load instructions of a block, and one for the scales
 constexpr int kFewSlot = 1024 * kFewDma;
@@ -1400,6 +1402,15 @@ __global__ __launch_bounds__(256) void latent_widen_kernel(const RowsParams p, u
 constexpr int kWidenTiles = 12;
 constexpr size_t kWidenBytes = 256u << 20;
 
+// Rows of a sequence, on average, up to which 8-bit pages are read by mla_few_kernel, and
+// with few tokens up to a whole tile of the other kernel's, for the shorter start and end
+// (mla_rows_kernel and mla_few_kernel, with the join, us: 16 sequences of 3000 to 32768 tokens, 16
+// heads 83 and 50, 40 heads 88 and 79, 32 of 64 heads 183 and 134, 128 heads 202 and 273; one of
+// 4000 tokens, 16 heads 21 and 16, 128 heads 24.6 and 19.3; 4 of 8000, 128 heads 34 and 28.6; 60
+// of 500 to 2000 54.5 and 48.2, 140 of 500 to 4000 137 and 160).
+constexpr int kFewRows = 64;
+constexpr long long kFewTokens = 1 << 17;
+
 struct RowsPlan {
   long long tiles, grid, pieces, joins;
   size_t copy;  // bytes of the widened latents (0: none)
@@ -1410,7 +1421,9 @@ struct RowsPlan {
 // decode: one token a sequence
 static RowsPlan rows_plan(int N, int B, int H, bool decode, bool fp8, int max_len, int n_splits) {
   RowsPlan r;
-  r.few = fp8 && (long long)N * H <= (long long)kFewTile * B;
+  const long long rows = (long long)N * H;
+  r.few = fp8 && (rows <= (long long)kFewRows * B ||
+                  (rows <= (long long)kRowsTile * B && (long long)B * max_len <= kFewTokens));
   r.tile = r.few ? kFewTile : kRowsTile;
   const long long each = (H + r.tile - 1) / r.tile;
   r.tiles = decode ? B * each : std::min((long long)N * H / r.tile + B, (long long)N * each);

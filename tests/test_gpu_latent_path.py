@@ -570,6 +570,61 @@ def test_decode8_at_a_long_capacity(B):
     R.check(lse, want_l, tol_l, "lse")
 
 
+FAR = (1 << 17) + 64  # a max_len from which few rows over 8-bit pages run in tiles of 128
+
+
+def wide_table(table, page):
+    return np.concatenate([table, np.full((table.shape[0], FAR // page + 1 - table.shape[1]), -1, np.int32)], 1)
+
+
+@pytest.mark.parametrize("H, block, lens, splits", [
+    (65, 1, [200, 1, 7], 0), (100, 64, [31, 64, 0, 65], 3), (128, 32, [500, 33], 1), (130, 1, [140], 0),
+    (128, 1, [2090], 1), (72, 64, [4200, 3], 1)])
+def test_decode8_tiles_of_128_rows(H, block, lens, splits):
+    page = 64
+    table, P, cpu = L.pools(lens, page, 8, block, H + len(lens))
+    qn, qp = queries(len(lens), H, 9)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, None, page, block, SCALE, pieces=splits != 1)
+    args = (qn.to(DEV), qp.to(DEV), *dev(cpu), ints(wide_table(table, page)), ints(lens), SCALE, FAR, splits)
+    out, lse = ops.mla8_decode_partial(*args)
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
+    o16, l16 = ops.mla8_decode_full(*args)
+    R.check(o16, want_o, tol_o + want_o.abs() * 2.0 ** -8, "bf16 out")
+    R.check(l16, want_l, tol_l, "lse")
+
+
+@pytest.mark.parametrize("H, lens, new, scale, sigma, what", [
+    (16, [300, 90], [7, 5], SCALE, 1.0, None), (20, [200], [4], -0.1, 1.0, None), (2, [90], [40], 0.0, 1.0, None),
+    (1, [300], [100], 1.0, 4.0, None), (16, [400], [6], 0.125, 1.0, "token"), (2, [200], [60], 0.125, 1.0, "token"),
+    (16, [200], [6], 0.125, 1.0, "scale"), (2, [2130], [60], SCALE, 1.0, "page")])
+def test_prompt_tiles_of_128_rows_over_8_bits(H, lens, new, scale, sigma, what):
+    """Scale signs, scores that climb out of the first block's headroom, NaN tokens and scales,
+    a bad page in a later window of ids."""
+    page, block, T, n = 32, 4, lens[0], new[0]
+    splits = 1 if what == "page" or sigma > 1 else 0
+    table, P, (pool, sc) = L.pools(lens, page, 8, block, 12, sigma=max(sigma / 2, 1.0))
+    qn, qp = queries(sum(new), H, 1, sigma)
+    at = {"token": T - n // 2 - 1, "scale": (T - 1) // block * block, "page": 2090 // page * page}.get(what, T)
+    pid, off = int(table[0, min(at, T - 1) // page]), at % page
+    if what == "token":
+        pool.view(torch.uint8)[pid, off, 300] = 0x7f
+    elif what == "scale":
+        sc.view(torch.uint8)[pid, off // block] = 255
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, (pool, sc), table, lens, new, page, block, scale,
+                                               pieces=splits != 1)
+    if what == "page":
+        table[0, at // page] = P
+    out, lse = prompt_on(qn, qp, (pool, sc), wide_table(table, page), lens, new, scale, max_len=FAR, n_splits=splits)
+    clean = np.arange(sum(new))
+    clean = clean[(clean >= n) | (clean + T - n < at)]
+    assert (what is None) == (len(clean) == sum(new)) and len(clean) > 0
+    R.check(out[clean], want_o[clean], tol_o[clean], "out")
+    R.check(lse[clean], want_l[clean], tol_l[clean], "lse")
+    gone = np.setdiff1d(np.arange(sum(new)), clean)
+    assert bool(out[gone].isnan().all()) and bool(lse[gone].isnan().all())
+
+
 @pytest.mark.parametrize("bits", (16, 8))
 def test_pools_past_4_gib(bits):
     """The same pages at the far end of a pool of more than 2^32 bytes: the same bits."""
