@@ -16,8 +16,11 @@
 // ws_latent_gather reads ranges of tokens back as bf16 rows (e4m3 times a power of two is a
 // bf16 number: exact).
 //
-// All of it is bound by HBM or, for a decode step's few tokens, by the launch and one chain
-// of loads.
+// All of it is bound by HBM or, for a decode step's few tokens, by the launch and one chain of
+// loads: 32 tokens into 8-bit pages 3.9 us; 16100 tokens of 16 heads into bf16 pages 17.7 us
+// (103 MB: 5.9 TB/s, the rate of a copy); 4651 into 8 bits with a scale for 32 tokens 12.9 us (32
+// MB; two runs of tokens one after the other in some workgroup); 29700 tokens read back from 8
+// bits 11.8 us (51 MB), 7700 in 150 ranges from bf16 6.0 us (18 MB).
 #include <math.h>
 
 #include <algorithm>
@@ -287,8 +290,9 @@ __device__ __forceinline__ void run_put(const LatentParams& p, int tok, int n, c
 // With a scale for several tokens, a workgroup takes the run of tokens from tok on whose
 // slots lie in one block, if tok is the run's first: the block's tokens follow one another in
 // a call, so nobody else writes the block.  Two looks at the tokens: their largest magnitude,
-// then their values (up to kRunChunk tokens from the registers, more from the cache again).  (A wave for every fourth token, one at a time, and read again: 4651 tokens to
-// blocks of 32 53.7 us.)
+// then their values (up to kRunChunk tokens from the registers, more from the cache again).  (A
+// wave for every fourth token, one at a time, and read again: 4651 tokens to blocks of 32 53.7
+// us.)
 //
 // at: the lane of the run's first token in `slots`, which holds the slots of tokens base +
 // lane (-1 outside the call).

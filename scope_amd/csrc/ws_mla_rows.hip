@@ -25,8 +25,9 @@
 //
 // The scores stay with bf16 products.  gfx950's scaled 8-bit products take e4m3 latents and
 // a query split into two e4m3 halves without any widening, at the same rate, but add up
-// their 64 terms in some 17 bits below the largest one, not in fp32: an lse off by 4e-5, a
-// hundred times this kernel's (2700 against 2900 cycles a step).
+// their 64 terms in some 17 bits below the largest one, not in fp32: an lse off by 4e-5
+// instead of 3e-6 (4000 new tokens of 4 sequences, 16 heads, behind 500 to 8000 8-bit
+// tokens: 614 us; 667 with the widening in the steps, 579 + 10 over a widened copy).
 #include <math.h>
 
 #include <algorithm>
@@ -120,11 +121,11 @@ struct RowsPlace {
 extern "C" __device__ float __ockl_wfred_add_f32(float);
 
 // Item `at` of the list of all tiles' splits (TILES: of the split tiles): where the items do
-// not fit the chip at once, longest sequences first (up to 64 of them), their last tile first.  A tile has one split for every M of
-// its sequence's blocks, M the batch's blocks over `fill` workgroups; where the tiles alone
-// are fewer than those, M is the least of four between that and the blocks over `fill` less
-// the tiles at which all items fit (the last one fits for sure: a split more than M's
-// quotient for every tile).  Every kernel of a call finds the same.  Every lane must call
+// not fit the chip at once, longest sequences first (up to 64 of them), their last tile
+// first.  A tile has one split for every M of its sequence's blocks, M the batch's blocks
+// over `fill` workgroups; where the tiles alone are fewer than those, M is the least of four
+// between that and the blocks over `fill` less the tiles at which all items fit (the last
+// one fits for sure: a split more than M's quotient for every tile).  Every kernel of a call finds the same.  Every lane must call
 // it; the result is uniform.  PER: sequences of a lane (0: any number, in a loop that reads
 // them again; they are not split to fit).
 template <bool TILES, int PER>
@@ -278,8 +279,9 @@ __device__ __forceinline__ RowsPlace rows_place(const RowsParams& p, int at) {
 // 8 bits: three, and per wave two slots for its eight rows of a block as they are in the
 // pages, 36 chunks of 16 bytes each, and the rows' scales, loaded four blocks ahead.  Lane l has
 // chunks l / 8 + 8 i (i < 5; past the 36th the last one) of row l % 8: one scale a lane, one
-// address and constant steps on either side, and 16 lanes' writes into the tile meet 16
-// chunk slots mod 16.
+// address and constant steps on either side.  (8 lanes' writes into the tile meet 4 chunk
+// slots mod 8, twice each, a fifth of the LDS cycles; chunks (l / 8) ^ (l % 2) + 8 i meet 8
+// and took as many cycles.)
 constexpr int kRowsTileBytes = 16 * kWideTileAlloc;
 constexpr int kRawRows = 8;             // of a wave
 constexpr int kRawDma = 5;              // load instructions, and one for the scales
@@ -424,6 +426,15 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, RowsWork& w) {
   return false;
 }
 
+// Bound by the matrix units with the power they may draw, and the instructions that feed them
+// (a wave alone on its SIMD, 512 registers): a step of 32 tokens and 128 rows is 68 products of
+// 32 x 32 x 16 a wave, 2176 cycles of the matrix unit, and takes 3100 over bf16 tiles, 4000 with
+// 8-bit blocks widened in it (some 100 instructions more).  8192 tokens of a prompt, 16
+// heads: 955 us, 1.22 PFLOP/s of the products the rows need (744 us on zeros, where power does
+// not bind).  4000 tokens in 4 chunks over 8-bit pages: 579 us, 1.13 PFLOP/s.  4 tokens of 16
+// heads each behind 4000 to 32000: 40 us, 4.0 TB/s; 24 prompts up to 600 tokens of 20 heads 76
+// us; decode of 128 heads, 8 sequences of 16000 to 32768 8-bit tokens: 65 us, 0.8 PFLOP/s.
+// Around its steps a workgroup spends 3 us before its first product and 4 us behind the last.
 template <bool F8>
 __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   using R = RowsRing<F8>;
@@ -1267,7 +1278,10 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
 // Combines the pieces of the tiles that were split: a wave a row, or (p.join_shared: many
 // pieces a tile, on average) a workgroup a row, each wave a quarter of the pieces.  A lane has
 // eight columns.  (Without shared rows a workgroup takes kJoinRows: in a call whose tiles
-// fill the chip hardly any is split, and every workgroup looks for its tile first.)
+// fill the chip hardly any is split, and every workgroup looks for its tile first.)  A launch,
+// the look for the tile and one chain of loads, 5 us; 8 tiles of 128 rows in 32 pieces each, 34 MB,
+// 9.7 us.  Shared rows for 12 pieces a tile and more: 16 tiles of 16 pieces 50 us with the
+// attention and 64 with a wave a row, 24 prompts of 2 or 3 pieces 88 and 69.
 constexpr int kJoinRows = 16;
 struct JoinAcc {
   float m, sum;
@@ -1366,7 +1380,8 @@ __global__ __launch_bounds__(256) void mla_rows_join_kernel(const RowsParams p) 
 }
 
 // Every sequence's tokens from 8-bit pages as bf16 rows [b][pad], one page a sequence (table:
-// its id), for prompts whose tiles read them many times.  Tokens in a bad page are NaN.
+// its id), for prompts whose tiles read them many times.  Tokens in a bad page are NaN.  Bound by
+// HBM: 20500 tokens, 35 MB, 9.8 us.
 constexpr int kWidenTokens = 32;  // of a workgroup
 __global__ __launch_bounds__(256) void latent_widen_kernel(const RowsParams p, uint16_t* copy,
                                                            int32_t* table, int pad) {
