@@ -663,7 +663,8 @@ int ws_latent_rope_append(const uint16_t* c, int64_t c_stride, const uint16_t* p
  * Tokens of the latent pages (ws_latent_rope_append's pools) as bf16 rows: row r, cu_rows[b]
  * <= r < cu_rows[b + 1] (cu_rows [B + 1] non-decreasing), is token start[b] + r - cu_rows[b]
  * of sequence b (start NULL: 0), its 512 columns to c_out + r * c_stride and its 64 rotary ones
- * to pe_out + r * pe_stride (strides in elements, multiples of 8); exact from 8-bit pages.
+ * to pe_out + r * pe_stride (strides in elements, multiples of 8); exact from 8-bit pages
+ * (down to bf16's least step, 2^-133).
  * Rows outside [cu_rows[0], cu_rows[B]) and past N are not written.  A token outside the
  * capacity or in a page with an id outside the pool gives a row of NaN.
  * The reference reads its dense buffers in place (system/deepseek.py:194-202).

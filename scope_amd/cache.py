@@ -660,8 +660,8 @@ class MlaRequestPartition(_RequestPages):
         """The step's tokens, q_nope [N, H, 512] and q_pe [N, H, 64] turned, over the pages:
         (out [N, H, 512] in out_dtype (fp32 or bf16), lse [N, H]), which merges with a host
         partial as the other partitions' (ops.lse_merge).  One token of every sequence
-        runs the decode kernels where there is one for the pages and the output,
-        anything else the prompt kernel."""
+        runs the decode kernels where there is one for the pages, the output and the
+        sizes, anything else the prompt kernel."""
         step = self._step()
         if q_nope.dim() != 3 or q_nope.shape[0] != step.slots.shape[0]:
             raise ValueError(f"q_nope must hold the step's {step.slots.shape[0]} tokens "
@@ -674,7 +674,9 @@ class MlaRequestPartition(_RequestPages):
             decode = ops.mla8_decode_partial if out_dtype == torch.float32 else ops.mla8_decode_full
             return decode(q_nope, q_pe, self.latent[layer], self.scale[layer], self.page_table, self.len_dev,
                           scale, max_len)
-        if single and self.batch and out_dtype == torch.float32 and H % 16 == 0 and self.batch * H // 16 <= 2048:
+        groups = self.batch * H // 16  # (mla_decode_partial's rows; its block index ends at 2^31)
+        if (single and self.batch and out_dtype == torch.float32 and H % 16 == 0 and groups <= 2048
+                and groups * ((max_len + 32) // 32) < 1 << 19):
             if q_pe.shape != (self.batch, H, ops.MLA_PE) or not (q_nope.is_contiguous() and q_pe.is_contiguous()):
                 raise ValueError(f"q_pe must be [{self.batch}, {H}, {ops.MLA_PE}], and both queries contiguous")
             out, lse = ops.mla_decode_partial(q_nope.view(-1, q_nope.shape[2]), q_pe.view(-1, ops.MLA_PE),

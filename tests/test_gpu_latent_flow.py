@@ -64,6 +64,26 @@ def attention(q, n_new, kv, scale):
     return res
 
 
+@pytest.mark.parametrize("B, H, long", [(130, 16, 131008), (3, 48, 2000)])
+def test_single_tokens_of_many_long_sequences(B, H, long):
+    """Single tokens over bf16 pages with fp32 outputs, at and past the block index range of
+    the decode kernel."""
+    part = MlaRequestPartition(1, B, 1 << 17, 64, num_pages=long // 64 + 2 * B)
+    part.latent.normal_(generator=torch.Generator(device=DEV).manual_seed(B))
+    n = [3] * B
+    n[1] = long
+    part.begin(n)
+    part.begin([1] * B)
+    qn, qp = bf16_randn((B, H, C), 5), bf16_randn((B, H, PE), 6)
+    out, lse = part.attend(0, qn.to(DEV), qp.to(DEV), 0.05)
+    pool, table = part.latent[0].cpu(), part.page_table.cpu()
+    for b in (0, 1, B - 1):
+        kv = L.rows_of(pool, None, table[b], n[b] + 1, 64, 1)
+        want_o, want_l, tol_o, tol_l = L.attend(torch.cat([qn, qp], -1).double()[b:b + 1], kv, [n[b] + 1], 0.05, True)
+        R.check(out[b:b + 1], want_o, tol_o, f"out of {b}")
+        R.check(lse[b:b + 1], want_l, tol_l, f"lse of {b}")
+
+
 @pytest.mark.parametrize("bits, block, H", [(16, 1, 16), (8, 1, 16), (8, 32, 20), (16, 1, 5), (8, 8, 40)])
 def test_requests_through_the_partition(bits, block, H):
     """Prompts, a chunk beside single tokens, single tokens, then a sequence that ends and

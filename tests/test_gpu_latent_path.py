@@ -161,6 +161,41 @@ def test_append_blocks(block, page, calls):
     assert rose >= 2 or block == 2  # (some block did rise)
 
 
+@pytest.mark.parametrize("block, n_new", [(64, [9000, 1, 8000, 40, 9001]), (32, [13000] + [31] * 40), (4, [13001, 5])])
+def test_append_many_runs(block, n_new):
+    """Enough tokens that a workgroup looks for runs among many."""
+    page, N = 64, sum(n_new)
+    cols = -(-max(n_new) // page)
+    P = sum(-(-n // page) for n in n_new)
+    ids, table = np.random.default_rng(block).permutation(P), np.zeros((len(n_new), cols), np.int64)
+    at = 0
+    for b, n in enumerate(n_new):
+        k = -(-n // page)
+        table[b, :k] = ids[at:at + k]
+        at += k
+    seq = np.repeat(np.arange(len(n_new)), n_new)
+    tok = np.concatenate([np.arange(n) for n in n_new])
+    slots = table[seq, tok // page] * page + tok % page
+    c, pe = bf16_randn((N, C), 1, 2.0), bf16_randn((N, PE), 2, 2.0)
+    pool, scale = fresh(P, page, 8, block)
+    ops.latent_rope_append(c.to(DEV), pe.to(DEV), torch.zeros((N, 1, PE), dtype=torch.bfloat16, device=DEV),
+                           torch.zeros(N, dtype=torch.int32, device=DEV), torch.ones(32, device=DEV), ints(slots),
+                           pool, scale)  # (position 0: nothing turns, so all of it is exact)
+    x = torch.cat([c, pe], 1).float()
+    group = torch.from_numpy(slots // block)
+    top = torch.zeros(P * page // block).scatter_reduce_(0, group, x.abs().amax(1), "amax")
+    e = torch.frexp(top / 448)
+    byte = e.exponent - (e.mantissa == 0.5).int() + 127  # the least power of two >= top / 448
+    used = torch.unique(group)
+    got_s = scale.view(torch.uint8).cpu().view(-1)
+    assert torch.equal(got_s[used].int(), byte[used])
+    want = torch.ldexp(x, 127 - byte[group][:, None]).to(R.E4M3).float()
+    assert torch.equal(pool.view(torch.uint8).cpu().view(-1, W)[slots].view(R.E4M3).float(), want)
+    spare = torch.ones(P * page, dtype=torch.bool)
+    spare[slots] = False
+    assert bool((pool.view(torch.uint8).cpu().view(-1, W)[spare] == 0x31).all())
+
+
 @pytest.mark.parametrize("block", (1, 32))
 def test_append_odd_rows(block):
     """Rows of zeros, of very small and large values, and with an infinity or a NaN, which
@@ -261,6 +296,26 @@ def test_gather_nan_scale():
     bad = torch.zeros(40, dtype=torch.bool)
     bad[16:24] = True
     assert torch.equal(c.isnan().all(1).cpu(), bad) and torch.equal(pe.isnan().any(1).cpu(), bad)
+
+
+def test_gather_every_code_at_every_scale():
+    """All 256 codes under the scales 2^-126 to 2^127: the product to the nearest bf16, which
+    it is but where it falls below 2^-133 or leaves the range."""
+    page, n = 32, 254
+    table, P, (pool, sc) = L.pools([n], page, 8, 1, 4)
+    codes = (torch.arange(n)[:, None] * 37 + torch.arange(W)[None]).to(torch.uint8)
+    for t in range(n):
+        pid, off = int(table[0, t // page]), t % page
+        pool.view(torch.uint8)[pid, off] = codes[t]
+        sc.view(torch.uint8)[pid, off] = t + 1
+    c, pe = ops.latent_gather(pool.to(DEV), ints(table), ints([0, n]), n, latent_scale=sc.to(DEV))
+    want = (codes.view(R.E4M3).double() * 2.0 ** (torch.arange(n).double()[:, None] - 126)).float().to(torch.bfloat16)
+    got = torch.cat([c, pe], 1).cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+    low = codes[0].view(R.E4M3).double().nan_to_num(0.0) * 2.0 ** -126
+    assert bool((want[0].double().nan_to_num(0.0) != low).any())  # (so it is rounded there)
+    assert torch.equal(want[2:100].double().nan_to_num(0.0),
+                       (codes.view(R.E4M3).double() * 2.0 ** (torch.arange(n).double()[:, None] - 126))[2:100].nan_to_num(0.0))
 
 
 # ---------------------------------------------------------------------------
@@ -578,7 +633,7 @@ def wide_table(table, page):
 
 
 @pytest.mark.parametrize("H, block, lens, splits", [
-    (65, 1, [200, 1, 7], 0), (100, 64, [31, 64, 0, 65], 3), (128, 32, [500, 33], 1), (130, 1, [140], 0),
+    (1024, 1, [40, 200], 0), (65, 1, [200, 1, 7], 0), (100, 64, [31, 64, 0, 65], 3), (128, 32, [500, 33], 1), (130, 1, [140], 0),
     (128, 1, [2090], 1), (72, 64, [4200, 3], 1)])
 def test_decode8_tiles_of_128_rows(H, block, lens, splits):
     page = 64
