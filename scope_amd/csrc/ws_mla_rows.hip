@@ -543,6 +543,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     const char* sb;
     const uint8_t* ss;
     uint32_t wbase, last, lim;  // (8 bits, lim: the block's last row)
+    uint32_t off;               // (8 bits: the lane's first chunk, from instruction 0 on)
   };
   auto issue_begin = [&](int k) __attribute__((always_inline)) {
     const int kc = min(k, nblk - 1);
@@ -572,13 +573,16 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     asm volatile("" : "+s"(d.wbase), "+s"(d.last));
     return d;
   };
-  auto dma_one = [&](const Dma& d, int i) __attribute__((always_inline)) {
+  auto dma_one = [&](Dma& d, int i) __attribute__((always_inline)) {
     if constexpr (F8) {
       int l = lane;
       asm volatile("" : "+v"(l));  // (recomputed at each use)
       const uint32_t row = min((uint32_t)(kRawRows * wave + (l & 7)), d.lim);
-      if (i < kRawDma)
-        rows_dma16(row * kRow + 16 * min(8 * i + (l >> 3), 35), d.sb, d.wbase, 1024 * i);
+      if (i == 0) d.off = row * kRow + 16 * (l >> 3);
+      if (i < kRawDma - 1)
+        rows_dma16(d.off + 128 * i, d.sb, d.wbase, 1024 * i);
+      else if (i < kRawDma)
+        rows_dma16(d.off + 128 * i - 16 * max((l >> 3) - 3, 0), d.sb, d.wbase, 1024 * i);
       else
         rows_dma1(row >> p.block_log2, d.ss, d.last);
     } else {
@@ -590,7 +594,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     }
   };
   auto issue = [&](int k) __attribute__((always_inline)) {
-    const Dma d = issue_begin(k);
+    Dma d = issue_begin(k);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) dma_one(d, i);
   };
@@ -759,7 +763,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     else wide_wait_barrier<kPer>();
     if (__builtin_expect(odd, 0)) clean(kk);
     if constexpr (F8) rows_wait<kPer>();  // block kk + 2's loads
-    const Dma d = issue_begin(kk + (F8 ? 4 : 3));
+    Dma d = issue_begin(kk + (F8 ? 4 : 3));
     const uint32_t to = lds0 + (uint32_t)tile_of(kk + 2) * kRowsTileBytes + offp[0];
     f32x16 sc;
     constexpr int kLead = F8 ? 3 : 4;  // links that an operand is read ahead
