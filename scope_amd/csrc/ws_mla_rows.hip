@@ -367,6 +367,13 @@ __device__ __forceinline__ void rows_store(char* dst, int row_bytes, const uint3
     *(u32x4*)(dst + (size_t)h * row_bytes + col_byte) = *(const u32x4*)(src + h * 260);
 }
 
+// Whether a row's reference does not serve its largest score: that climbed out of the
+// headroom, or lies far below, as it can where every score of the row's first block is -inf
+// and the reference is 0 (a reference that is a score is no larger than the largest).
+__device__ __forceinline__ bool reference_off(float top, float m_run) {
+  return top > m_run + kWideHeadroomLog2 || (top < m_run - kWideHeadroomLog2 && top != neg_inf());
+}
+
 // What a bf16 pair holds of infinities and NaN: their halves' bits, all set.
 __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
   const uint32_t hit = (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15;
@@ -888,14 +895,14 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     }
     const float top = m_max * sx;
     // every load of the pass has landed and every wave is done with the tiles
-    const bool climbed = __builtin_amdgcn_ballot_w64(top > m_run + kWideHeadroomLog2) != 0;
-    if (rows > 0 && climbed && lane == 0) s_redo = 1;
+    const bool off = __builtin_amdgcn_ballot_w64(reference_off(top, m_run)) != 0;
+    if (rows > 0 && off && lane == 0) s_redo = 1;
     wide_wait_barrier<0>();
     const bool redo = s_redo != 0;
     wide_wait_barrier<0>();  // every wave has read s_redo
     if (tid == 0) s_redo = 0;
     if (pass > 0 || !redo) break;
-    // scores climbed out of the reference's headroom: again, from the rows' largest
+    // scores out of the reference's reach: again, from the rows' largest
     m_run = top == neg_inf() ? 0.f : top;
   }
 
@@ -1220,7 +1227,7 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
     pair_xor32(m_max, lo, hi);
     m_max = fmaxf(lo, hi);
     const float top = m_max * sx;
-    if (pass > 0 || __builtin_amdgcn_ballot_w64(top > m_run + kWideHeadroomLog2) == 0) break;
+    if (pass > 0 || __builtin_amdgcn_ballot_w64(reference_off(top, m_run)) == 0) break;
     m_run = top == neg_inf() ? 0.f : top;
   }
 

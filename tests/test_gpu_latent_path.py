@@ -760,3 +760,35 @@ def test_refused_tensors():
         with pytest.raises(err, match=says):
             ops.mla_prompt(**{**dict(q_nope=qn, q_pe=q, latent_pages=pool, page_table=t, kv_len=n, cu_new=cu, scale=1.0,
                                      max_len=3), **kw})
+
+
+@pytest.mark.parametrize("bits, far", [(16, False), (8, False), (8, True)])
+@pytest.mark.parametrize("n, H, splits", [(3, 4, 1), (40, 4, 1), (3, 4, 2)])
+def test_prompt_first_blocks_of_infinite_scores(bits, far, n, H, splits):
+    """Every score of the first 40 tokens is -inf (over 8-bit pages by a product past fp32's
+    range), the others' lie far below 0: the first block gives the softmax no reference, and
+    the others are what counts."""
+    T, page, lead, scale = 150, 64, 40, 0.1
+    table, P, (pool, sc) = L.pools([T], page, bits, 1, 23)
+    raw = pool if bits == 16 else pool.view(torch.uint8)
+    for t in range(T):
+        p, o = int(table[0, t // page]), t % page
+        if bits == 16:
+            raw[p, o, C:C + 8] = math.inf if t < lead else 64.0
+        elif t < lead:
+            raw[p, o] = 0
+            raw[p, o, C:C + 8] = 0x77  # 240, at a scale of 2^120
+            sc.view(torch.uint8)[p, o] = 247
+        else:
+            raw[p, o, C:C + 8] = 0x78  # 256
+            sc.view(torch.uint8)[p, o] = 125
+    qn, qp = queries(n, H, 5)
+    qp[..., :8] = -16.0
+    rows = L.rows_of(pool, sc, table[0], T, page)
+    vis = [T - n + i + 1 - lead for i in range(n)]
+    want_o, want_l, tol_o, tol_l = L.attend(torch.cat([qn, qp], -1).double(), rows[lead:], vis, scale, splits != 1)
+    assert float(want_l.max()) < -300
+    out, lse = prompt_on(qn, qp, (pool, sc), wide_table(table, page) if far else table, [T], [n], scale,
+                         max_len=FAR if far else None, n_splits=splits)
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
