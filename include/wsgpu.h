@@ -709,7 +709,8 @@ int ws_mla8_decode_full(const uint16_t* q_nope, const uint16_t* q_pe,
  * mergeable with a host partial (ws_lse_merge).  Rows outside [cu_new[0], cu_new[B]) are
  * not written.  A row that sees a token in a page with an id outside the pool is NaN, and
  * so is every row of a sequence whose length is outside [0, capacity]; an infinity or a NaN
- * in a token changes only the rows that see it.
+ * in a token changes only the rows that see it (under a score of -inf, of weight 0, its own
+ * column of theirs alone).
  * n_splits, max_len and the workspace (ws_mla_prompt_plan; fp8: whether the pages are
  * 8-bit) as ws_mla8_decode_partial's.
  * The reference runs prompts through its framework's attention on expanded keys and values

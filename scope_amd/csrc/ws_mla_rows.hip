@@ -450,6 +450,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   constexpr int kPer = F8 ? kRawDma + 1 : kWideDmaPerWave;  // a wave's load instructions of a block
   __shared__ __attribute__((aligned(1024))) char s_mem[R::kLds];
   __shared__ int s_redo;
+  __shared__ int s_odd[2];  // by a block's parity: its tile is to be cleaned (soft_x)
   const int tid = threadIdx.x;
   const int wave = uniform(tid >> 6);
   const int lane = tid & 63;
@@ -457,7 +458,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   const int j2 = lane >> 5;
   RowsWork w;
   if (!rows_work(p, w)) return;
-  if (tid == 0) s_redo = 0;  // read after the ring's barriers
+  if (tid == 0) s_redo = s_odd[0] = s_odd[1] = 0;  // read after the ring's barriers
   const int nblk = w.nblk, t_begin = w.t_begin, t_end = w.t_end, here = w.here;
   const int rows = min(max(here - 32 * wave, 0), 32);  // this wave's
   // the tokens that the lane's row sees (past the rows: the last one again)
@@ -669,18 +670,22 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     asm volatile("" : : : "memory");
   };
   const float sx = p.scale_log2;
+  // Whether the tile's first row does not see all of block kb, or its page id is bad (alike in
+  // the four waves).
+  auto masked = [&](int kb) __attribute__((always_inline)) {
+    return t_begin + 32 * kb + 32 > w.lim_lo || ((bad_bits >> (kb & 31)) & 1) != 0;
+  };
   // The scores of block kb in the log2 domain less the reference (xa: the first 16 tokens',
-  // xh: the others').  In the blocks that the tile's first row does not see whole, a score
-  // that a row does not see is -inf, and an infinity or a NaN in a token shows in its
-  // score: a row that sees it is NaN, and where a row of the wave does not, the result is
-  // true and the tile is cleaned before its values are taken.
+  // xh: the others').  In a masked block a score that a row does not see is -inf, and an
+  // infinity or a NaN in a token shows in its score: where a row of the wave does not see
+  // it, the tile is cleaned before its values are taken.  Returns whether the block is masked.
   auto soft_x = [&](int kb, const f32x16& sc, float (&xa)[8], float (&xh)[8], bool first)
       __attribute__((always_inline)) {
     const int t0 = t_begin + 32 * kb;
     f32x16 v = sc;
-    bool odd = false;
-    const bool bad_page = (bad_bits >> (kb & 31)) & 1;
-    if (t0 + 32 > w.lim_lo || bad_page) {
+    const bool look = masked(kb);
+    if (look) {
+      const bool bad_page = (bad_bits >> (kb & 31)) & 1;
       int l = lane;  // recomputed here rather than kept live
       asm volatile("" : "+v"(l));
       const int lim = lim_lane - t0 - 4 * (l >> 5);
@@ -688,12 +693,10 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const bool seen = 8 * (i >> 2) + (i & 3) < lim;
-        const bool finite = __builtin_fabsf(v[i]) < __builtin_inff();
-        hidden |= !seen && !finite;
-        const float x = bad_page || !finite ? qnan() : v[i];
-        v[i] = seen ? x : neg_inf();
+        hidden |= !seen && !(__builtin_fabsf(v[i]) < __builtin_inff());
+        v[i] = !seen ? neg_inf() : bad_page ? qnan() : v[i];
       }
-      odd = __builtin_amdgcn_ballot_w64(hidden) != 0;
+      if (__builtin_amdgcn_ballot_w64(hidden) != 0) s_odd[kb & 1] = 1;
     }
     float r = max3(v[0], v[1], v[2]);
 #pragma unroll
@@ -712,7 +715,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
       xa[i] = __builtin_fmaf(v[i], sx, nm);
       xh[i] = __builtin_fmaf(v[8 + i], sx, nm);
     }
-    return odd;
+    return look;
   };
   // One dword of a k-step's P^T (two exp2), its probabilities added to the row sum as rounded
   auto soft_p = [&](float (&xs)[8], u32x4& pbs, int dd) __attribute__((always_inline)) {
@@ -744,31 +747,67 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     }
     soft_s(xa, xh);
   };
-  // Takes the infinities and NaN out of block kk's tile, where some token that a row of the
-  // wave does not see holds one (0 * inf would bring it into that row).  Behind the barrier
-  // at which every wave has its scores of the tile; a row that sees one is NaN by its score
-  // (soft_x), whatever it finds in the tile.
-  auto clean = [&](int kk) __attribute__((always_inline)) {
-    u32x4* tile = s_tile + tile_of(kk) * kTileChunks;
+  // NaN into the columns of a row's sums in which block kk's tile has an infinity or a NaN of
+  // a token that the row sees: what the values' product would add (its score is not finite,
+  // so its weight is 0 or NaN).  A product of 2^127 there and 2^127 where a token is seen goes
+  // past fp32's range, and its opposite after it leaves NaN.  (8-bit pages hold NaN besides
+  // numbers, which a row that sees it has from its score.)
+  auto mark = [&](int kk) __attribute__((always_inline)) {
+    const uint32_t vt = vbase(tile_of(kk));
+    const int lim = lim_lane - (t_begin + 32 * kk) - 4 * j2;
 #pragma clang loop unroll(disable)
-    for (int c = lane; c < kTileChunks; c += 64) {
-      u32x4 x = tile[c];
+    for (int s = 0; s < 2; ++s) {
+      u32x4 vis;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int t = 16 * s + 8 * (d >> 1) + 2 * (d & 1);  // soft_x's tokens 8 s + 2 d and the next
+        vis[d] = (t < lim ? 0x7f00u : 0u) | (t + 1 < lim ? 0x7f000000u : 0u);
+      }
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        u32x4 x = vread(vt + 16 * kWideRowsS * s, c), y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t at = nonfinite_halves(x[e]);
+          x[e] = at & 0x7f007f00u;
+          y[e] = at & 0xff00ff00u;
+        }
+        pv_mfma(x, vis, c);
+        pv_mfma(y, vis, c);
+      }
+    }
+  };
+  // Takes the infinities and NaN out of block kk's tile, where a token that some row of the
+  // workgroup does not see holds one (0 * inf would bring it into that row); rows that see it
+  // have it from mark.  (look: the block is masked.)  All waves call it behind the barrier at which each has its scores of
+  // the tile; a wave that is ahead notes the other parity.
+  auto clean = [&](int kk, bool look) __attribute__((always_inline)) {
+    if (!look || __builtin_expect(uniform(s_odd[kk & 1]) == 0, 1)) return;
+    int k = kk, first = tid;
+    asm volatile("" : "+s"(k), "+v"(first));  // (nothing of this is kept from step to step)
+    if (!F8 && rows > 0) mark(k);
+    wide_lds_barrier();  // every wave has read the note and the tile
+    if (first == 0) s_odd[k & 1] = 0;
+    const uint32_t tile = lds0 + (uint32_t)tile_of(k) * kRowsTileBytes;
+#pragma clang loop unroll(disable)
+    for (int c = first; c < kTileChunks; c += 256) {
+      u32x4 x = rows_lds_b128(tile + 16 * c);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] &= ~nonfinite_halves(x[e]);
-      tile[c] = x;
+      rows_lds_put(tile + 16 * c, x);
     }
-    wide_lds_wait();
+    wide_lds_barrier();
   };
 
   // Step kk of the ring (ws_mla_wide.h): block kk + 1's scores with block kk's values'
   // product between their links, the loads over them (bf16: block kk + 3's; 8 bits: block kk
   // + 4's, behind the widening of this wave's part of block kk + 2), and the softmax of
   // block kk + 1 beside the last products.
-  auto step = [&](int kk, float (&xa)[8], float (&xh)[8], bool& odd) __attribute__((always_inline)) {
+  auto step = [&](int kk, float (&xa)[8], float (&xh)[8], bool& look) __attribute__((always_inline)) {
     const int tp = tile_of(kk), tq = tile_of(kk + 1);
     if constexpr (F8) wide_lds_barrier();
     else wide_wait_barrier<kPer>();
-    if (__builtin_expect(odd, 0)) clean(kk);
+    clean(kk, look);
     if constexpr (F8) rows_wait<kPer>();  // block kk + 2's loads
     Dma d = issue_begin(kk + (F8 ? 4 : 3));
     const uint32_t to = lds0 + (uint32_t)tile_of(kk + 2) * kRowsTileBytes + offp[0];
@@ -809,7 +848,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
       if (m == 26) {
         __builtin_amdgcn_sched_barrier(0);
         qk_settle_short(sc);
-        odd = soft_x(kk + 1, sc, xa, xh, false);
+        look = soft_x(kk + 1, sc, xa, xh, false);
       }
       if (m + 3 < 32) va[(m + 3) & 3] = vread(vt, m + 3);
       pv_mfma(va[m & 3], pb[1], m);
@@ -852,7 +891,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     }
     if (rows > 0) {
       float xa[8], xh[8];
-      bool odd;
+      bool look;
       {
         f32x16 sc;
         u32x4 kr[5];
@@ -865,28 +904,31 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
           qk_link(sc, kr[u % 5], u, last);
         }
         qk_settle(sc);
-        odd = soft_x(0, sc, xa, xh, true);
+        look = soft_x(0, sc, xa, xh, true);
       }
 #pragma clang loop unroll(disable)
-      for (int k = 0; k + 1 < nblk; ++k) step(k, xa, xh, odd);
+      for (int k = 0; k + 1 < nblk; ++k) step(k, xa, xh, look);
       wide_lds_barrier();  // every wave has its scores of the last tile
-      if (__builtin_expect(odd, 0)) clean(nblk - 1);
+      clean(nblk - 1, look);
       values(nblk - 1, xa, xh);
     } else {  // the ring's waits, barriers and loads alone
 #pragma clang loop unroll(disable)
       for (int k = 0; k + 1 < nblk; ++k) {
         if constexpr (F8) {
           wide_lds_barrier();
+          clean(k, masked(k));
           rows_wait<kPer>();
           widen_block(k + 2);
           wide_lds_wait();
           issue(k + 4);
         } else {
           wide_wait_barrier<kPer>();
+          clean(k, masked(k));
           issue(k + 3);
         }
       }
       wide_lds_barrier();
+      clean(nblk - 1, masked(nblk - 1));
     }
     {  // the row's largest score (both its lanes)
       float lo, hi;
@@ -913,13 +955,16 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
   const float l_tot = lo + hi;
   const float inv_l = s_tot == 0.f ? 0.f : 1.f / l_tot;
   const float lse_v = s_tot == 0.f ? neg_inf() : (m_run + __log2f(s_tot)) * kLn2;
-  if (j2 == 0 && n32 < rows) {
-    const size_t at = w.o_row0 + 32 * wave + n32;
+  int el = lane;  // (what the end takes of the lane is spilled around the loop otherwise)
+  asm volatile("" : "+v"(el));
+  const int en = el & 31, ej = el >> 5;
+  if (ej == 0 && en < rows) {
+    const size_t at = w.o_row0 + 32 * wave + en;
     if (w.piece) p.part_lse[at] = lse_v;
     else if (p.lse) p.lse[at] = lse_v;
   }
   // The outputs leave through LDS, 1 KB a store instruction: accumulator ct value i is
-  // column 32 ct + 8 (i / 4) + 4 j2 + i % 4.
+  // column 32 ct + 8 (i / 4) + 4 ej + i % 4.
   uint32_t* stage = (uint32_t*)s_mem + (size_t)(32 * wave) * 260;
   if (rows == 0) return;
   uint16_t* to16 = w.piece ? p.part_out : p.out_bf16;
@@ -928,12 +973,12 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
     for (int ct = 0; ct < 16; ++ct)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *(uint2*)(stage + n32 * 260 + 16 * ct + 4 * q + 2 * j2) =
+        *(uint2*)(stage + en * 260 + 16 * ct + 4 * q + 2 * ej) =
             make_uint2(pack_bf16x2(acc[ct][4 * q] * inv_l, acc[ct][4 * q + 1] * inv_l),
                        pack_bf16x2(acc[ct][4 * q + 2] * inv_l, acc[ct][4 * q + 3] * inv_l));
     wide_lds_wait();
-    rows_store((char*)(to16 + (w.o_row0 + 32 * wave) * kRowsC), kRowsC * 2, stage + 4 * lane,
-               16 * lane, rows);
+    rows_store((char*)(to16 + (w.o_row0 + 32 * wave) * kRowsC), kRowsC * 2, stage + 4 * el,
+               16 * el, rows);
     wide_lds_wait();
   }
   if (!w.piece && p.out_f32) {
@@ -945,12 +990,12 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int ct = 8 * hc + c8;
-          *(float4*)(stage + n32 * 260 + 32 * c8 + 8 * q + 4 * j2) =
+          *(float4*)(stage + en * 260 + 32 * c8 + 8 * q + 4 * ej) =
               make_float4(acc[ct][4 * q] * inv_l, acc[ct][4 * q + 1] * inv_l,
                           acc[ct][4 * q + 2] * inv_l, acc[ct][4 * q + 3] * inv_l);
         }
       wide_lds_wait();
-      rows_store(dst, kRowsC * 4, stage + 4 * lane, 1024 * hc + 16 * lane, rows);
+      rows_store(dst, kRowsC * 4, stage + 4 * el, 1024 * hc + 16 * el, rows);
       wide_lds_wait();  // the next half overwrites the rows
     }
   }
@@ -1138,10 +1183,8 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const bool seen = 8 * (e >> 2) + (e & 3) < lim;
-        const bool finite = __builtin_fabsf(v[e]) < __builtin_inff();
-        hidden |= !seen && !finite;
-        const float x = bad_page || !finite ? qnan() : v[e];
-        v[e] = seen ? x : neg_inf();
+        hidden |= !seen && !(__builtin_fabsf(v[e]) < __builtin_inff());
+        v[e] = !seen ? neg_inf() : bad_page ? qnan() : v[e];
       }
       odd = __builtin_amdgcn_ballot_w64(hidden) != 0;
     }

@@ -792,3 +792,44 @@ def test_prompt_first_blocks_of_infinite_scores(bits, far, n, H, splits):
                          max_len=FAR if far else None, n_splits=splits)
     R.check(out, want_o, tol_o, "out")
     R.check(lse, want_l, tol_l, "lse")
+
+
+def without_token(q, rows, at, vis, scale, pieces):
+    """attend() of queries for which token `at` has the weight 0: that token left out."""
+    kept = torch.cat([rows[:at], rows[at + 1:]])
+    return L.attend(q, kept, [v - (v > at) for v in vis], scale, pieces)
+
+
+@pytest.mark.parametrize("H, n, splits", [(2, 60, 1), (2, 60, 2), (1, 100, 0), (16, 20, 1), (16, 4, 0)])
+@pytest.mark.parametrize("column, value", [(5, math.inf), (511, -math.inf), (570, math.inf), (570, -math.inf)])
+@pytest.mark.parametrize("place", ("seen whole", "masked early", "masked", "last"))
+def test_prompt_infinite_scores(H, n, splits, column, value, place):
+    """An infinity in a token's latent, under queries whose score of it is +inf in some rows
+    and -inf in others.  -inf has the weight 0, wherever the row's tile ends: the row is what
+    it is without the token, but for the token's own column (0 * inf).  +inf leaves nothing of
+    the row, and rows that do not see the token are as if it were not there."""
+    T, page = 200, 64
+    at = {"seen whole": 20, "masked early": T - n + 1, "masked": T - n // 2 - 1, "last": T - 2}[place]
+    table, P, (pool, _) = L.pools([T], page, 16, 1, 17)
+    rows = L.rows_of(pool, None, table[0], T, page)
+    pool[int(table[0, at // page]), at % page, column] = value
+    qn, qp = queries(n, H, 5)
+    sign = torch.where(torch.rand((n, H), generator=torch.Generator().manual_seed(n)) < 0.6, -1.0, 1.0)
+    sign.view(-1)[-2:] = torch.tensor([1.0, -1.0])  # (both, whatever sees the token)
+    size = sign * (1 if value > 0 else -1)  # score: sign * inf
+    (qn if column < C else qp)[..., column if column < C else column - C] = size.to(torch.bfloat16)
+    out, lse = prompt_on(qn, qp, (pool, None), table, [T], [n], 0.125, n_splits=splits)
+    out, lse = out.cpu(), lse.cpu()
+    q = torch.cat([qn, qp], -1).double()
+    vis = [T - n + i + 1 for i in range(n)]
+    sees = torch.tensor(vis)[:, None] > at
+    want_o, want_l, tol_o, tol_l = without_token(q, rows, at, vis, 0.125, splits != 1)
+    gone, zero = sees & (sign > 0), sees & (sign < 0)
+    assert bool(gone.any()) and bool(zero.any())
+    assert bool(out[gone].isnan().all()) and not bool(lse[gone].isfinite().any())
+    if column < C:
+        assert bool(out[zero][:, column].isnan().all())
+        out[..., column][zero] = want_o[..., column][zero].float()
+    fine = ~gone
+    R.check(out[fine], want_o[fine], tol_o[fine], "out")
+    R.check(lse[fine], want_l[fine], tol_l[fine], "lse")
