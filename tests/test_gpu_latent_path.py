@@ -833,3 +833,34 @@ def test_prompt_infinite_scores(H, n, splits, column, value, place):
     fine = ~gone
     R.check(out[fine], want_o[fine], tol_o[fine], "out")
     R.check(lse[fine], want_l[fine], tol_l[fine], "lse")
+
+
+def test_prompt_copy_of_idle_sequences():
+    """Prompts of many tiles over 8-bit pages beside sequences without new tokens: the
+    widened copy takes the latents of those that have some, and no others."""
+    lens, new, page, H = [300, 5000, 290, 400, 0], [200, 0, 150, 1, 0], 32, 24
+    N, B, max_len = sum(new), len(lens), max(lens)
+    assert N * H >= 12 * 128 * B
+    table, P, cpu = L.pools(lens, page, 8, 4, 6)
+    pool, sc = dev(cpu)
+    qn, qp = queries(N, H, 3)
+    dqn, dqp, t, l, cu = qn.to(DEV), qp.to(DEV), ints(table), ints(lens), ints(np.concatenate([[0], np.cumsum(new)]))
+    _, size = ops.mla_prompt_plan(N, B, H, max_len, fp8=True)
+    pad = -(-max_len // 32) * 32
+    ws = torch.full((size,), 0xa5, dtype=torch.uint8, device=DEV)
+    out, lse = torch.empty((N, H, C), device=DEV), torch.empty((N, H), device=DEV)
+    assert ops.lib().ws_mla_prompt(
+        dqn.data_ptr(), dqp.data_ptr(), pool.data_ptr(), sc.data_ptr(), t.data_ptr(), l.data_ptr(), cu.data_ptr(), N, B, H,
+        page, table.shape[1], P, 4, max_len, 0, SCALE, None, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), size,
+        torch.cuda.current_stream().cuda_stream) == 0
+    rows = ws[size - B * pad * 2 * W:].view(B, pad, 2 * W).cpu()
+    for b, n in enumerate(new):
+        want = L.rows_of(*cpu, table[b], lens[b], page, 4)
+        if n:
+            assert torch.equal(rows[b, :lens[b]].contiguous().view(torch.bfloat16).double(), want), b
+            assert bool((rows[b, lens[b]:] == 0xa5).all()), b
+        else:
+            assert bool((rows[b] == 0xa5).all()), f"sequence {b} has no rows that read its copy"
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, new, page, 4, SCALE)
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
