@@ -689,14 +689,15 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
       int l = lane;  // recomputed here rather than kept live
       asm volatile("" : "+v"(l));
       const int lim = lim_lane - t0 - 4 * (l >> 5);
-      bool hidden = false;
+      const float bad = bad_page ? qnan() : 0.f;
+      float hidden = 0.f;  // NaN: a score that is not seen is not finite
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const bool seen = 8 * (i >> 2) + (i & 3) < lim;
-        hidden |= !seen && !(__builtin_fabsf(v[i]) < __builtin_inff());
-        v[i] = !seen ? neg_inf() : bad_page ? qnan() : v[i];
+        hidden = __builtin_fmaf(seen ? 0.f : v[i], 0.f, hidden);
+        v[i] = seen ? v[i] + bad : neg_inf();
       }
-      if (__builtin_amdgcn_ballot_w64(hidden) != 0) s_odd[kb & 1] = 1;
+      if (__builtin_amdgcn_ballot_w64(hidden != hidden) != 0) s_odd[kb & 1] = 1;
     }
     float r = max3(v[0], v[1], v[2]);
 #pragma unroll
