@@ -340,9 +340,13 @@ int ws_attn_append_decode_partial(const uint16_t* q, const uint16_t* k_new,
  * 64 sequences); other calls plan each group of 16 heads as a sequence of its
  * own over the shared latent.  A sequence's new latent is written once.
  * Outputs out: [B*H][512] fp32 normalised, lse: [B*H] fp32.
+ * ws_mla_decode_fits: 1 if the call takes a batch of B sequences of up to max_len tokens
+ * under H heads, 0 if it would refuse it (B * H / 16 up to 2048, and fewer than 2^19 blocks of
+ * 32 tokens over all plan sequences at max_len).
  * Replaces the GPU partial of _mla_compressed_forward
  * (system/deepseek.py:364-392; also roofline/bench_rstar_revalidate_ds2.py:74-86).
  */
+int ws_mla_decode_fits(int B, int H, int max_len);
 int ws_mla_decode_partial(const uint16_t* q_nope, const uint16_t* q_pe,
                           const uint16_t* latent_pages,
                           const int32_t* page_table, const int32_t* gpu_len,

@@ -674,9 +674,10 @@ class MlaRequestPartition(_RequestPages):
             decode = ops.mla8_decode_partial if out_dtype == torch.float32 else ops.mla8_decode_full
             return decode(q_nope, q_pe, self.latent[layer], self.scale[layer], self.page_table, self.len_dev,
                           scale, max_len)
-        groups = self.batch * H // 16  # (mla_decode_partial's rows; its block index ends at 2^31)
-        if (single and self.batch and out_dtype == torch.float32 and H % 16 == 0 and groups <= 2048
-                and groups * ((max_len + 32) // 32) < 1 << 19):
+        # (decode and prompt kernel, us: 32 sequences of 8192 tokens, 16 heads 59 and 69; 64 of 32768,
+        # 128 heads 579 and 590; 4 of 32768, 64 heads 78 and 46)
+        if (single and self.batch and out_dtype == torch.float32
+                and ops.mla_decode_fits(self.batch, H, max_len)):
             if q_pe.shape != (self.batch, H, ops.MLA_PE) or not (q_nope.is_contiguous() and q_pe.is_contiguous()):
                 raise ValueError(f"q_pe must be [{self.batch}, {H}, {ops.MLA_PE}], and both queries contiguous")
             out, lse = ops.mla_decode_partial(q_nope.view(-1, q_nope.shape[2]), q_pe.view(-1, ops.MLA_PE),

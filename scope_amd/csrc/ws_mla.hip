@@ -423,6 +423,15 @@ int mla_workgroups(int n_workgroups, int B, int max_len) {
   return std::min(n, kMaxSplits);
 }
 
+// Head counts and batches that the kernels take, and lengths whose block numbers hold: the
+// plan's products of a split's number (up to 4096) and the blocks of all plan sequences.
+static bool mla_batch_ok(int B, int H) {
+  return B >= 0 && H >= kMlaH && H % kMlaH == 0 && (long long)B * (H / kMlaH) <= kMaxSeqs;
+}
+static bool mla_blocks_ok(int plan_seqs, int max_len) {
+  return (long long)plan_seqs * (((long long)max_len + 32) / 32) * 4096 < (1LL << 31);
+}
+
 static int mla_launch(const uint16_t* q_nope, const uint16_t* q_pe,
                       const uint16_t* c_new, long long c_stride, const uint16_t* pe_new,
                       long long pe_stride, uint16_t* latent_pages,
@@ -434,7 +443,7 @@ static int mla_launch(const uint16_t* q_nope, const uint16_t* q_pe,
   if (!q_nope || !q_pe || !latent_pages || !page_table || !len_in || !out || !lse)
     return set_error(WS_EINVAL, "%s: null pointer", name);
   // H = 16 ng: each 16-head group is its own plan sequence over the shared latent
-  if (B < 0 || H < kMlaH || H % kMlaH || (long long)B * (H / kMlaH) > kMaxSeqs)
+  if (!mla_batch_ok(B, H))
     return set_error(WS_EINVAL,
                      "%s: B=%d H=%d unsupported (H a multiple of 16, B * H / 16 <= %d)", name, B,
                      H, kMaxSeqs);
@@ -462,7 +471,7 @@ static int mla_launch(const uint16_t* q_nope, const uint16_t* q_pe,
   if (B == 0) return WS_OK;
   const int Bv = lay.plan_seqs;  // plan sequences (sequence, head group)
   const int hp = lay.piece_heads;
-  if ((long long)Bv * ((max_len + 32) / 32) * 4096 >= (1LL << 31))
+  if (!mla_blocks_ok(Bv, max_len))
     return set_error(WS_EINVAL, "%s: %d sequences of %d tokens exceed the block index range",
                      name, Bv, max_len);
   if ((long long)num_pages * page_size >= (1LL << 31))  // bit 31 marks bad page ids
@@ -522,6 +531,10 @@ static int mla_launch(const uint16_t* q_nope, const uint16_t* q_pe,
 }  // namespace ws
 
 using namespace ws;
+
+extern "C" int ws_mla_decode_fits(int B, int H, int max_len) {
+  return mla_batch_ok(B, H) && max_len >= 0 && mla_blocks_ok(mla_layout(B, H).plan_seqs, max_len);
+}
 
 extern "C" int ws_mla_decode_partial(const uint16_t* q_nope, const uint16_t* q_pe,
                                      const uint16_t* latent_pages,

@@ -41,6 +41,7 @@ EXPORTS = (
     "ws_attn_decode_plan",
     "ws_gqa_decode_partial",
     "ws_gqa_append_decode_partial",
+    "ws_mla_decode_fits",
     "ws_mla_decode_partial",
     "ws_mla_append_decode_partial",
     "ws_gqa_append_decode_split",
@@ -200,6 +201,8 @@ def lib() -> ctypes.CDLL:
                                             f32, vp, vp, vp, vp] + [i32] * 5 + [vp]
         L.ws_latent_gather.restype = i32
         L.ws_latent_gather.argtypes = [vp, vp, i32, vp, vp, vp, vp, i64, vp, i64] + [i32] * 5 + [vp]
+        L.ws_mla_decode_fits.restype = i32
+        L.ws_mla_decode_fits.argtypes = [i32] * 3
         L.ws_mla8_decode_plan.restype = i32
         L.ws_mla8_decode_plan.argtypes = [i32] * 4 + [ctypes.POINTER(i32), ctypes.POINTER(sz)]
         for fn in (L.ws_mla8_decode_partial, L.ws_mla8_decode_full):
@@ -576,6 +579,12 @@ def attn_decode_partial(q, k_pages, v_pages, page_table, gpu_len, scale, max_len
         _ptr(q), _ptr(k_new), _ptr(v_new), _ptr(k_pages), _ptr(v_pages), _ptr(page_table),
         _ptr(gpu_len), _ptr(len_out), *tail), "ws_attn_append_decode_partial")
     return out, lse
+
+
+def mla_decode_fits(batch: int, H: int, max_len: int) -> bool:
+    """Whether mla_decode_partial takes `batch` sequences of up to max_len tokens under H heads
+    (ws_mla_decode_fits)."""
+    return bool(lib().ws_mla_decode_fits(batch, H, max_len))
 
 
 def mla_decode_partial(q_nope, q_pe, latent_pages, page_table, gpu_len, scale, max_len,

@@ -348,3 +348,31 @@ def test_partition_knows_its_device():
     part = MlaRequestPartition(1, 2, 128, 32, device="cuda")
     assert part.device == part.page_table.device and part.device.index is not None
     assert part.latent.device == part.device
+
+
+@pytest.mark.parametrize("B, H, long, decodes", [
+    (64, 128, 40000, True), (64, 128, 32 * 8191 - 2, True), (64, 128, 32 * 8191 - 1, False), (130, 16, 32 * 4032 - 1, False),
+    (32, 32, 32 * 16000, True)])
+def test_single_tokens_run_decode_as_far_as_it_goes(B, H, long, decodes, monkeypatch):
+    """Single tokens over bf16 pages with fp32 outputs run the decode kernel up to the sizes it
+    takes (a sequence of 128 heads counts once there), and the prompt kernel past them."""
+    ran = []
+    for name in ("mla_decode_partial", "mla_prompt"):
+        real = getattr(ops, name)
+        monkeypatch.setattr(ops, name, lambda *a, _r=real, _n=name, **k: ran.append(_n) or _r(*a, **k))
+    part = MlaRequestPartition(1, B, 1 << 19, 64, num_pages=long // 64 + 2 * B)
+    part.latent.normal_(generator=torch.Generator(device=DEV).manual_seed(B))
+    n = [3] * B
+    n[1] = long
+    part.begin(n)
+    part.begin([1] * B)
+    qn, qp = bf16_randn((B, H, C), 5), bf16_randn((B, H, PE), 6)
+    out, lse = part.attend(0, qn.to(DEV), qp.to(DEV), 0.05)
+    assert ran == ["mla_decode_partial" if decodes else "mla_prompt"]
+    pool, table, heads = part.latent[0].cpu(), part.page_table.cpu(), [0, H // 2 + 1, H - 1]
+    q = torch.cat([qn, qp], -1).double()[:, heads]
+    for b in (0, 1, B - 1):
+        kv = L.rows_of(pool, None, table[b], n[b] + 1, 64, 1)
+        want_o, want_l, tol_o, tol_l = L.attend(q[b:b + 1], kv, [n[b] + 1], 0.05, True)
+        R.check(out[b:b + 1, heads], want_o, tol_o, f"out of {b}")
+        R.check(lse[b:b + 1, heads], want_l, tol_l, f"lse of {b}")

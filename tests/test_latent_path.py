@@ -162,3 +162,27 @@ def test_exponent_rule():
     assert [L.exponent(x) for x in (448.0, 449.0, 0.0, 2.0 ** -130, 3e38, 1.75 * 2.0 ** -118)] == \
         [0, 1, -126, -126, math.ceil(math.log2(3e38 / 448)), -126]
     assert R.E8M0 == ops.E8M0 and np.isfinite(L.exponent(1e-40))
+
+
+@pytest.mark.parametrize("B, H, most", [
+    (1, 16, (1 << 24) - 33), (130, 16, 32 * 4032 - 1), (3, 48, 32 * ((1 << 19) // 9) - 1), (64, 128, 32 * 8191 - 1),
+    (65, 128, 32 * 8065 - 1), (32, 32, 32 * 16383 - 1), (31, 32, 32 * 8456 - 1), (256, 128, 32 * 2047 - 1)])
+def test_decode_fits_is_what_the_launch_takes(B, H, most):
+    """The query beside the launch's own check, at the longest sequences that it takes and
+    one token past them: 128 heads (and 32 to 112 from 1024 rows on) count sequences, other
+    calls groups of 16 heads."""
+    def launch(n):
+        pages = n // 64 + 1
+        return ops.lib().ws_mla_decode_partial(FAKE, FAKE, FAKE, FAKE, FAKE, B, H, 64, pages, 4, n, 0, 1.0, FAKE, FAKE,
+                                               None, 0, None)
+    for n, fits in ((most, True), (most + 1, False), (100, True)):
+        assert ops.mla_decode_fits(B, H, n) is fits
+        assert launch(n) == (-3 if fits else -1) and ("workspace" if fits else "block index range") in err()
+    assert not ops.mla_decode_fits(B, H, -1)
+
+
+def test_decode_fits_batches():
+    assert ops.mla_decode_fits(2048, 16, 100) and not ops.mla_decode_fits(2049, 16, 100)
+    assert ops.mla_decode_fits(256, 128, 100) and not ops.mla_decode_fits(257, 128, 100)
+    assert not any(ops.mla_decode_fits(1, H, 100) for H in (0, -16, 8, 20, 100))
+    assert ops.mla_decode_fits(0, 16, 100) and not ops.mla_decode_fits(-1, 16, 100)
