@@ -595,10 +595,11 @@ extern "C" int ws_latent_rope_append(const uint16_t* c, int64_t c_stride, const 
   // tokens of 128 heads: 8.6 and 10.5).
   const bool runs = latent_scale && p.block_log2 > 0;
   p.tokens = N < 2048 ? 1 : runs ? kRunTurns : kLatTokens;
-  const int turn_groups = (N + p.tokens - 1) / p.tokens;
-  p.window = std::min((N + kRunGroups - 1) / kRunGroups, p.block_log2 >= 5 ? 2 * kRunWindow : kRunWindow);
-  p.run_groups = runs ? (N + p.window - 1) / p.window : 0;
-  const long long grid = (long long)turn_groups + p.run_groups;
+  const long long n = N;  // (sums past 32 bits)
+  p.window = (int)std::min<long long>((n + kRunGroups - 1) / kRunGroups,
+                                      p.block_log2 >= 5 ? 2 * kRunWindow : kRunWindow);
+  p.run_groups = runs ? (int)((n + p.window - 1) / p.window) : 0;
+  const long long grid = (n + p.tokens - 1) / p.tokens + p.run_groups;
   const int threads = runs ? 64 * kRunWaves : 256;
   if (grid * threads >= (1LL << 32))
     return set_error(WS_EINVAL, "%s: %d tokens exceed the launch grid", name, N);
@@ -644,7 +645,10 @@ extern "C" int ws_latent_gather(const void* latent_pages, const uint8_t* latent_
   p.num_pages = num_pages;
   p.cap = (int)std::min<long long>((long long)page_size * max_pages, 0x7fffffffLL);
   p.rows = N >= 8192 ? kGatherRows : 8;
-  const dim3 g((unsigned)((N + p.rows - 1) / p.rows)), b(256);
+  const long long groups = ((long long)N + p.rows - 1) / p.rows;
+  if (groups * 256 >= (1LL << 32))
+    return set_error(WS_EINVAL, "%s: %d rows exceed the launch grid", name, N);
+  const dim3 g((unsigned)groups), b(256);
   hipStream_t s = (hipStream_t)stream;
   if (latent_scale)
     hipLaunchKernelGGL(latent_gather_kernel<true>, g, b, 0, s, p);

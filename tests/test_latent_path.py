@@ -186,3 +186,12 @@ def test_decode_fits_batches():
     assert ops.mla_decode_fits(256, 128, 100) and not ops.mla_decode_fits(257, 128, 100)
     assert not any(ops.mla_decode_fits(1, H, 100) for H in (0, -16, 8, 20, 100))
     assert ops.mla_decode_fits(0, 16, 100) and not ops.mla_decode_fits(-1, 16, 100)
+
+
+@pytest.mark.parametrize("N", (1 << 30, (1 << 31) - 800, (1 << 31) - 1))
+@pytest.mark.parametrize("block", (0, 1, 32))
+def test_tokens_past_the_launch_grid(N, block):
+    """Counts up to the largest 32-bit number are refused, not wrapped around."""
+    scale = FAKE if block else None
+    assert append(N=N, H=1, qs=64, scale=scale, block=block) == -1 and "launch grid" in err()
+    assert gather(N=N, scale=scale, block=block) == -1 and "launch grid" in err()
