@@ -647,9 +647,9 @@ int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void* v_pages,
  * for every scale_block slots (latent_scale [num_pages][page_size / scale_block]; scale_block
  * a power of two that divides page_size) for 2^(byte - 127), the least power of two >= 2^-126
  * with max|x| <= 448 times it over the block's tokens.  With scale_block > 1 the tokens of a
- * block follow one another in a call, and slots of the block below the call's lowest hold
- * tokens from before: the scale is no less than theirs, and where it rises their values
- * are rounded again.  An infinity or a NaN becomes NaN in its place and has no part in the
+ * block follow one another in a call (between them none of another block or without a slot),
+ * and slots of the block below the call's lowest hold tokens from before: the scale is no less
+ * than theirs, and where it rises their values are rounded again.  An infinity or a NaN becomes NaN in its place and has no part in the
  * scale.
  * The reference computes the norm and the rotation in the model library and copies the
  * result into dense host and GPU buffers (system/deepseek.py:251, 171-192).

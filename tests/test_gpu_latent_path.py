@@ -864,3 +864,46 @@ def test_prompt_copy_of_idle_sequences():
     want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, new, page, 4, SCALE)
     R.check(out, want_o, tol_o, "out")
     R.check(lse, want_l, tol_l, "lse")
+
+
+def test_max_len_picks_the_kernel_not_the_result():
+    """The same call at its longest sequence's length and at the row's capacity (a captured
+    step's): other kernels run, and each result is within its bounds."""
+    page, cap = 64, 1 << 17
+    wide = lambda t: np.concatenate([t, np.full((t.shape[0], cap // page - t.shape[1]), -1, np.int32)], 1)
+    lens, H = [300, 70], 100  # (more than 64 rows a sequence)
+    table, P, cpu = L.pools(lens, page, 8, 1, 3)
+    qn, qp = queries(2, H, 9)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, None, page, 1, SCALE)
+    for max_len in (300, cap):
+        out, lse = ops.mla8_decode_partial(qn.to(DEV), qp.to(DEV), *dev(cpu), ints(wide(table)), ints(lens), SCALE, max_len)
+        R.check(out, want_o, tol_o, f"decode at {max_len}")
+        R.check(lse, want_l, tol_l, f"decode's lse at {max_len}")
+    lens, new, H = [300, 200], [180, 150], 20  # (12 tiles of rows a sequence: a widened copy, where it fits)
+    table, P, cpu = L.pools(lens, page, 8, 32, 4)
+    N = sum(new)
+    copied = [ops.mla_prompt_plan(N, 2, H, m, 1, fp8=True)[1] > ops.mla_prompt_plan(N, 2, H, m, 1)[1] for m in (300, cap)]
+    assert copied == [True, False]
+    qn, qp = queries(N, H, 9)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, new, page, 32, SCALE)
+    for max_len in (300, cap):
+        out, lse = prompt_on(qn, qp, cpu, wide(table), lens, new, SCALE, max_len=max_len)
+        R.check(out, want_o, tol_o, f"prompt at {max_len}")
+        R.check(lse, want_l, tol_l, f"prompt's lse at {max_len}")
+
+
+@pytest.mark.parametrize("bits, block", [(16, 1), (8, 1), (8, 64)])
+@pytest.mark.parametrize("H, chunk", [(16, 130), (5, 300)])
+def test_one_chunk_beside_single_tokens(bits, block, H, chunk):
+    """A step of continuous batching: one chunk among single tokens and sequences without any,
+    every row of it."""
+    page, rng = 64, np.random.default_rng(chunk)
+    lens, new = rng.integers(1, 700, 30), np.ones(30, np.int64)
+    lens[11], new[11] = chunk + 333, chunk
+    new[[4, 29]] = 0
+    table, P, cpu = L.pools(lens, page, bits, block, 8)
+    qn, qp = queries(int(new.sum()), H, 9)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, new, page, block, SCALE)
+    out, lse = prompt_on(qn, qp, cpu, table, lens, new, SCALE, max_len=int(max(lens)))
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
