@@ -1335,9 +1335,13 @@ __global__ __launch_bounds__(256) void mla_few_kernel(const RowsParams p) {
 // eight columns.  (Without shared rows a workgroup takes kJoinRows: in a call whose tiles
 // fill the chip hardly any is split, and every workgroup looks for its tile first.)  A launch,
 // the look for the tile and one chain of loads, 5 us; 8 tiles of 128 rows in 32 pieces each, 34 MB,
-// 9.7 us.  Shared rows for 12 pieces a tile and more: 16 tiles of 16 pieces 50 us with the
-// attention and 64 with a wave a row, 24 prompts of 2 or 3 pieces 88 and 69.
+// 9.7 us.  Shared rows for kJoinShared pieces a tile and more, over the fewest tiles that the
+// call's rows can make: 16 tiles of 16 pieces 50 us with the attention and 64 with a wave a row, 24
+// prompts of 2 or 3 pieces 88 and 69.  (Over the most tiles, a sequence more for each, 8 x 4
+// drafted tokens of 16 heads over 4000 to 32000 8-bit tokens took 54 us instead of 40.5, 20 x 7 of
+// 4 heads over bf16 54 instead of 45; 12 x 10 of 16 heads, 24 tiles for 15, 56 instead of 58.)
 constexpr int kJoinRows = 16;
+constexpr int kJoinShared = 12;
 struct JoinAcc {
   float m, sum;
   float a[8];
@@ -1476,7 +1480,8 @@ constexpr size_t kWidenBytes = 256u << 20;
 
 // Rows of a sequence, on average, up to which 8-bit pages are read by mla_few_kernel, and
 // with few tokens up to a whole tile of the other kernel's, for the shorter start and end
-// (mla_rows_kernel and mla_few_kernel, with the join, us: 16 sequences of 3000 to 32768 tokens, 16
+// (mla_rows_kernel and mla_few_kernel, with the join, us: 8 x 4 drafted tokens of 16 heads over
+// 4000 to 32000 49 and 40.5, 16 x 4 92 and 75.5; decode of 16 sequences of 3000 to 32768 tokens, 16
 // heads 83 and 50, 40 heads 88 and 79, 32 of 64 heads 183 and 134, 128 heads 202 and 273; one of
 // 4000 tokens, 16 heads 21 and 16, 128 heads 24.6 and 19.3; 4 of 8000, 128 heads 34 and 28.6; 60
 // of 500 to 2000 54.5 and 48.2, 140 of 500 to 4000 137 and 160).
@@ -1488,7 +1493,7 @@ struct RowsPlan {
   size_t copy;  // bytes of the widened latents (0: none)
   int pad;      // tokens of a sequence there
   int fill, piece_rows, tile;
-  bool fit, few;
+  bool fit, few, join_shared;
 };
 // decode: one token a sequence
 static RowsPlan rows_plan(int N, int B, int H, bool decode, bool fp8, int max_len, int n_splits) {
@@ -1520,6 +1525,9 @@ static RowsPlan rows_plan(int N, int B, int H, bool decode, bool fp8, int max_le
     r.grid = r.fit ? r.fill : r.tiles + r.pieces;
     r.joins = std::min<long long>(r.tiles, r.fill);
   }
+  // pieces a tile: of the tiles that there are at the least (r.tiles is the most)
+  const long long least = std::max(((long long)N * H + r.tile - 1) / r.tile, (long long)std::min(N, B));
+  r.join_shared = n_splits > 1 ? n_splits >= kJoinShared : r.pieces >= kJoinShared * (decode ? r.tiles : least);
   return r;
 }
 // The workspace: the pieces' lse and outputs, the copy's table and rows.
@@ -1612,7 +1620,7 @@ static int rows_run(const char* name, const uint16_t* q_nope, const uint16_t* q_
   p.tile_log2 = pl.few ? 5 : 7;
   p.by_H = divisor((uint32_t)H);
   p.by_page = divisor((uint32_t)page_size);
-  p.join_shared = pl.pieces >= 12 * pl.tiles;
+  p.join_shared = pl.join_shared;
   // the smallest normal float for 0: every finite score then rounds to the same
   // probability, and masked tokens stay -inf
   p.scale_log2 = std::max((scale < 0.f ? -scale : scale) * kLog2e, 1.17549435e-38f);

@@ -907,3 +907,19 @@ def test_one_chunk_beside_single_tokens(bits, block, H, chunk):
     out, lse = prompt_on(qn, qp, cpu, table, lens, new, SCALE, max_len=int(max(lens)))
     R.check(out, want_o, tol_o, "out")
     R.check(lse, want_l, tol_l, "lse")
+
+
+@pytest.mark.parametrize("bits, B, H, n", [(8, 8, 16, 4), (8, 12, 16, 3), (16, 20, 4, 7), (8, 16, 16, 2)])
+def test_prompt_joins_of_few_tiles(bits, B, H, n):
+    """Drafted tokens whose rows fill their tiles, split far: the pieces of a row are joined by a
+    workgroup."""
+    page, rng = 64, np.random.default_rng(B)
+    lens = [int(x) for x in rng.integers(600, 3000, B)]
+    table, P, cpu = L.pools(lens, page, bits, 1, B)
+    qn, qp = queries(B * n, H, 9)
+    want_o, want_l, tol_o, tol_l = L.attention(qn, qp, cpu, table, lens, [n] * B, page, 1, SCALE)
+    out, lse = prompt_on(qn, qp, cpu, table, lens, [n] * B, SCALE)
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
+    again, _ = prompt_on(qn, qp, cpu, table, lens, [n] * B, SCALE)
+    assert torch.equal(again, out)
