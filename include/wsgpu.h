@@ -642,7 +642,8 @@ int ws_gqa_prompt(const uint16_t* q, const void* k_pages, const void* v_pages,
  * Slots must differ.  R turns pair i of 32 by positions[t] * inv_freq[i], columns (i, i + 32)
  * or (2 i, 2 i + 1) with adjacent != 0, times factor, as ws_rope; q_out [N][H][64] is R of
  * q_pe (token stride q_stride, head stride q_head_stride, in elements as c's and pe's
- * strides: multiples of 8), and may be q_pe itself where that is contiguous.
+ * strides: multiples of 8; a token's heads lie ahead of the next token's), and may be q_pe itself
+ * where that is contiguous.
  * latent_scale == NULL: bf16 pages.  Otherwise 8-bit pages: e4m3 values, and an e8m0 byte
  * for every scale_block slots (latent_scale [num_pages][page_size / scale_block]; scale_block
  * a power of two that divides page_size) for 2^(byte - 127), the least power of two >= 2^-126

@@ -16,11 +16,13 @@
 // ws_latent_gather reads ranges of tokens back as bf16 rows (e4m3 times a power of two is a
 // bf16 number: exact).
 //
-// All of it is bound by HBM or, for a decode step's few tokens, by the launch and one chain of
-// loads: 32 tokens into 8-bit pages 3.9 us; 16100 tokens of 16 heads into bf16 pages 17.7 us
-// (103 MB: 5.9 TB/s, the rate of a copy); 4651 into 8 bits with a scale for 32 tokens 12.9 us (32
-// MB; two runs of tokens one after the other in some workgroup); 29700 tokens read back from 8
-// bits 11.8 us (51 MB), 7700 in 150 ranges from bf16 6.0 us (18 MB).
+// With a scale for one token, in bf16 and back, all of it is bound by HBM or, for a decode step's
+// few tokens, by the launch and one chain of loads: 32 tokens into 8-bit pages 3.9 us; 16100 tokens
+// of 16 heads into bf16 pages 21.8 us (103 MB: 4.7 TB/s, where a copy of 1 GiB has 5.1; 17.4 over
+// pages that the last cache holds); 29700 tokens read back from 8 bits 11.4 us (51 MB), 7700 in 150
+// ranges from bf16 5.9 us (18 MB).  With a scale for several tokens the runs bound it, two of them
+// one after the other in some workgroup, each a chain of loads: 4651 tokens to blocks of 32 12.6 us
+// (32 MB, 2.5 TB/s), 16000 29.7 (3.1 TB/s).
 #include <math.h>
 
 #include <algorithm>

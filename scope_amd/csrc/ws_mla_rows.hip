@@ -27,7 +27,7 @@
 // a query split into two e4m3 halves without any widening, at the same rate, but add up
 // their 64 terms in some 17 bits below the largest one, not in fp32: an lse off by 4e-5
 // instead of 3e-6 (4000 new tokens of 4 sequences, 16 heads, behind 500 to 8000 8-bit
-// tokens: 614 us; 667 with the widening in the steps, 579 + 10 over a widened copy).
+// tokens: 614 us; 667 with the widening in the steps, 554 + 10 over a widened copy).
 #include <math.h>
 
 #include <algorithm>
@@ -44,7 +44,10 @@ constexpr int kRowsC = 512;
 constexpr int kRowsPe = 64;
 constexpr int kRowsTile = 128;       // rows of a tile, 32 a wave (mla_few_kernel: 32)
 constexpr int kRowsMaxSplits = 256;  // of a tile
-constexpr int kRowsMinShare = 4;     // blocks of a split, at the least
+// Blocks of a split, at the least (2, 4 and 8, us: decode of one sequence of 2048 tokens 15.9, 15.7
+// and 17.7, of 8 of 1000 16.3, 16.0 and 17.5, a prompt of 128 tokens 27.9, 16.5 and 16.5; 16 tokens
+// behind 1000 21.5, 23.0 and 27.1).
+constexpr int kRowsMinShare = 4;
 
 // Division by a number that the host knows: n / d = n m >> s for 0 <= n < 2^31, with 2^k the
 // least power of two >= d, m = floor(2^(31 + k) / d) + 1 (2^31 for d = 1) and s = 31 + k: m d
@@ -437,10 +440,10 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, RowsWork& w) {
 // (a wave alone on its SIMD, 512 registers): a step of 32 tokens and 128 rows is 68 products of
 // 32 x 32 x 16 a wave, 2176 cycles of the matrix unit, and takes 3100 over bf16 tiles, 4000 with
 // 8-bit blocks widened in it (some 100 instructions more).  8192 tokens of a prompt, 16
-// heads: 955 us, 1.22 PFLOP/s of the products the rows need (744 us on zeros, where power does
-// not bind).  4000 tokens in 4 chunks over 8-bit pages: 579 us, 1.13 PFLOP/s.  4 tokens of 16
-// heads each behind 4000 to 32000: 40 us, 4.0 TB/s; 24 prompts up to 600 tokens of 20 heads 76
-// us; decode of 128 heads, 8 sequences of 16000 to 32768 8-bit tokens: 65 us, 0.8 PFLOP/s.
+// heads: 949 us, 1.23 PFLOP/s of the products the rows need (744 us on zeros, where power does
+// not bind).  4000 tokens in 4 chunks over 8-bit pages: 558 us, 1.18 PFLOP/s.  4 tokens of 16
+// heads each behind 4000 to 32000: 43 us, 3.7 TB/s; 24 prompts up to 600 tokens of 20 heads 78
+// us; decode of 128 heads, 8 sequences of 16000 to 32768 8-bit tokens: 63 us, 0.8 PFLOP/s.
 // Around its steps a workgroup spends 3 us before its first product and 4 us behind the last.
 template <bool F8>
 __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
@@ -1009,7 +1012,7 @@ __global__ __launch_bounds__(256) void mla_rows_kernel(const RowsParams p) {
 // 1300 of the CU, the HBM some 2000 of its share.  The latents are widened where they are
 // read: the scores' operand by its token's scale, the values' operand as it is, with the
 // scale on the token's probability.  Bound by HBM in long batches (16 sequences of 3000 to
-// 32768 tokens, 16 heads: 193 MB in 41 us, 4.7 TB/s), by one chain of loads, a block and the
+// 32768 tokens, 16 heads: 193 MB in 46 us, 4.2 TB/s), by one chain of loads, a block and the
 // merge in short ones (one of 8192: 11.8 us).
 constexpr int kFewTile = 32;
 constexpr int kFewDma = 19;  // 1 KB load instructions of a block, and one for the scales
@@ -1440,8 +1443,9 @@ __global__ __launch_bounds__(256) void mla_rows_join_kernel(const RowsParams p) 
 
 // The tokens of every sequence that has rows, from 8-bit pages, as bf16 rows [b][pad], one page a
 // sequence (table: its id), for prompts whose tiles read them many times.  Tokens in a bad page
-// are NaN.  Bound by HBM: 20500 tokens, 35 MB, 9.8 us.  (A chunk of 2400 tokens of 16 heads beside
-// 23 idle sequences, 8000 tokens each: 609 us, and 669 with the idle ones' tokens too.)
+// are NaN.  Bound by HBM: 20500 tokens, 35 MB, 13.8 us (9.8 where the last cache holds the pages).
+// (A chunk of 2400 tokens of 16 heads beside 23 idle sequences, 8000 tokens each: 609 us, and 669
+// with the idle ones' tokens too.)
 constexpr int kWidenTokens = 32;  // of a workgroup
 __global__ __launch_bounds__(256) void latent_widen_kernel(const RowsParams p, uint16_t* copy,
                                                            int32_t* table, int pad) {

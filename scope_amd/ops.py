@@ -1520,8 +1520,9 @@ def latent_rope_append(c, pe, q_pe, positions, inv_freq, slots, latent_pages, la
                        norm_weight=None, eps=1e-6, adjacent=False, factor=1.0, q_out=None):
     """A forward step's latents into their pages, and the heads' q_pe turned with them
     (ws_latent_rope_append).  c [N, 512] and pe [N, 64] (rows may be strided: parts of
-    the down projection's output), q_pe [N, H, 64] (tokens and heads may be strided:
-    a part of every head's query); positions [N] int32, inv_freq [32] fp32.  Token t's
+    the down projection's output), q_pe [N, H, 64] (tokens and heads may be strided,
+    a token's heads ahead of the next token's: a part of every head's query); positions
+    [N] int32, inv_freq [32] fp32.  Token t's
     latent, c through an RMS norm with norm_weight [512] (bf16 or fp32; None: as it is)
     and pe turned by its position, goes to slot slots[t] (pages_extend), in bf16 or, with
     latent_scale, in 8 bits: e4m3 with one power of two per block of tokens.  A block
