@@ -923,3 +923,27 @@ def test_prompt_joins_of_few_tiles(bits, B, H, n):
     R.check(lse, want_l, tol_l, "lse")
     again, _ = prompt_on(qn, qp, cpu, table, lens, [n] * B, SCALE)
     assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("H, n, splits", [(2, 60, 1), (1, 100, 2), (16, 4, 1)])
+@pytest.mark.parametrize("column", (5, 570))
+def test_prompt_infinite_scores_in_two_passes(H, n, splits, column):
+    """The same with scores that climb out of the first block's headroom: the second pass
+    cleans and marks its tiles anew."""
+    T, page = 300, 32
+    table, P, (pool, _) = L.pools([T], page, 16, 1, 12, sigma=2.0)
+    rows = L.rows_of(pool, None, table[0], T, page)
+    qn, qp = queries(n, H, 1, 4.0)
+    at = T - n // 2 - 1
+    pool[int(table[0, at // page]), at % page, column] = -math.inf
+    (qn if column < C else qp)[..., column % C] = 1.0  # every score of it is -inf
+    out, lse = prompt_on(qn, qp, (pool, None), table, [T], [n], 1.0, n_splits=splits)
+    out, lse = out.cpu(), lse.cpu()
+    q, vis = torch.cat([qn, qp], -1).double(), [T - n + i + 1 for i in range(n)]
+    want_o, want_l, tol_o, tol_l = without_token(q, rows, at, vis, 1.0, splits != 1)
+    if column < C:
+        sees = torch.tensor(vis) > at
+        assert bool(out[sees][..., column].isnan().all())
+        out[sees, :, column] = want_o[sees, :, column].float()
+    R.check(out, want_o, tol_o, "out")
+    R.check(lse, want_l, tol_l, "lse")
